@@ -400,6 +400,103 @@ int lbfq_blasst_attend_bf16(const uint16_t* q, const uint16_t* k, const uint16_t
                             float sm_scale, int mode, const float* final_max, const uint8_t* keep, float* out,
                             float* dropped, int64_t* p_counts, double* p_sqerr, lbfq_stream_t stream);
 
+/* ---- Q/K norm and rotation ---------------------------------------------------
+ * (No counterpart in the reference, as all entries up to the measurement probes.)
+ * Each head's row x of D values: n = x w / sqrt(mean(x^2) + eps), and the first
+ * `rot` columns of n rotated in pairs by the angles of the row's position,
+ * columns (2i, 2i + 1) or, halves = 1, (i, i + rot / 2).  fp32 throughout, one
+ * rounding.  Element strides; rows contiguous and 16-byte aligned.  A negative
+ * position is not rotated, one past the table comes out as NaN. */
+typedef struct {
+  const void* q; const void* k; int dtype; /* (B, S, Hq, D), (B, S, Hk, D)     */
+  int64_t B, S, Hq, Hk, D;                 /* D in {64, 128}                    */
+  int64_t q_b, q_s, q_h, k_b, k_s, k_h;
+  const void* q_weight; int q_weight_dtype; /* (D) or NULL for ones            */
+  const void* k_weight; int k_weight_dtype;
+  const float* cos; const float* sin;      /* (table_len, rot / 2) contiguous   */
+  int64_t table_len; int rot;              /* a multiple of 16, at most D       */
+  const void* positions; int positions_i64; /* int32 / int64, or NULL: row s is at s */
+  int64_t pos_b, pos_s;
+  float eps; int halves;
+  void* q_out; void* k_out;                /* contiguous (forward)              */
+} lbfq_qk_norm_params;
+
+int lbfq_qk_norm_rope(const lbfq_qk_norm_params* p, lbfq_stream_t stream);
+
+/* Backward: gradients dyq / dyk of q_out / k_out to dq / dk (contiguous, of
+ * `dtype`) and to the weights (of their dtypes; NULL: not wanted).  partial:
+ * fp32 workspace of lbfq_qk_norm_rope_bwd_rows(p) * 2 * D, NULL if no weight's
+ * gradient is wanted.  The order of every sum is fixed. */
+typedef struct {
+  const void* dyq; const void* dyk;
+  int64_t dyq_b, dyq_s, dyq_h, dyk_b, dyk_s, dyk_h;
+  void* dq; void* dk;
+  void* dq_weight; void* dk_weight;
+  float* partial;
+} lbfq_qk_norm_grads;
+
+int64_t lbfq_qk_norm_rope_bwd_rows(const lbfq_qk_norm_params* p);
+int lbfq_qk_norm_rope_bwd(const lbfq_qk_norm_params* p, const lbfq_qk_norm_grads* g, lbfq_stream_t stream);
+
+/* ---- quantised paged K/V cache -------------------------------------------------
+ * Codes (num_pages, H, page, D) E4M3 and scales (num_pages, H, page, D / 32)
+ * E8M0 of K and of V, contiguous and 16-byte aligned, page = 2^page_shift
+ * tokens (16 .. 1024); the format of LBFQ_Q_MX_QK with 32 columns a scale.
+ * write: rows k[t], v[t] (fp32, fp16 or bf16) to slot slots[t] = page id * page
+ * + row; a slot outside the cache is skipped; slots must differ. */
+typedef struct {
+  const void* k; const void* v; int dtype;
+  int64_t T, H, D;
+  int64_t k_t, k_h, v_t, v_h;              /* element strides, 16-byte multiples */
+  const int64_t* slots;                    /* (T)                               */
+  uint8_t* k_codes; uint8_t* k_scale; uint8_t* v_codes; uint8_t* v_scale;
+  int64_t num_pages; int page_shift;
+} lbfq_kv_write_params;
+
+int lbfq_kv_write(const lbfq_kv_write_params* p, lbfq_stream_t stream);
+
+/* read: dtype(code * 2^e) of the first max_len tokens of each sequence, k_out and
+ * v_out (B, max_len, H, D) contiguous; rows from seq_lens[b] on, and rows whose
+ * page id lies outside the cache, are zero. */
+typedef struct {
+  const uint8_t* k_codes; const uint8_t* k_scale; const uint8_t* v_codes; const uint8_t* v_scale;
+  int64_t num_pages; int page_shift;
+  int64_t B, H, D, max_len;
+  const int32_t* block_table; int64_t table_stride, table_cols; /* (B, table_cols) */
+  const int32_t* seq_lens;                 /* (B)                               */
+  void* k_out; void* v_out; int dtype;
+} lbfq_kv_read_params;
+
+int lbfq_kv_read(const lbfq_kv_read_params* p, lbfq_stream_t stream);
+
+/* Attention of new tokens over the cache.  Sequence b: queries query_starts[b] ..
+ * query_starts[b + 1] of q (T, Hq, D), the last tokens of its seq_lens[b] cached
+ * ones.  causal: query i sees keys up to its own position seq_len - n + i; window
+ * w > 0: only keys above position - w.  Key head h serves query heads
+ * h Hq / Hk ...  Rows that see nothing are 0, lse (natural log, (T, Hq)) -inf.
+ * Keys on pages outside the cache are not seen.  max_query_len sizes the grid
+ * (0: T); more queries than that are still right.  Rows that no sequence has:
+ * lse -inf, out 0 with fill_rest, else left as they are.  workspace:
+ * lbfq_paged_attention_workspace_bytes(p), 16-byte aligned, used by this call alone. */
+typedef struct {
+  const void* q; int dtype;                /* bf16 or fp16, the output's too    */
+  int64_t T, Hq, Hk, D, B;
+  int64_t q_t, q_h;
+  const uint8_t* k_codes; const uint8_t* k_scale; const uint8_t* v_codes; const uint8_t* v_scale;
+  int64_t num_pages; int page_shift;
+  const int32_t* block_table; int64_t table_stride, table_cols;
+  const int32_t* seq_lens; const int32_t* query_starts; /* (B), (B + 1)         */
+  int64_t max_query_len;
+  float sm_scale; int causal; int64_t window;
+  void* out; int64_t out_t, out_h;
+  float* lse;                              /* or NULL                           */
+  int fill_rest;
+  void* workspace; int64_t workspace_bytes;
+} lbfq_paged_params;
+
+int64_t lbfq_paged_attention_workspace_bytes(const lbfq_paged_params* p);
+int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t stream);
+
 /* ---- measurement probe ----------------------------------------------------- */
 /* HBM streaming probe (no counterpart in the reference: it measures the
  * ceiling the prepass is held against).  mode 0 reads `bytes` from src

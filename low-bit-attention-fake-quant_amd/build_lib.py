@@ -47,6 +47,9 @@ UNITS = {
     "lbfq_attn_b128_p1.hip": ATTN_FLAGS,
     "lbfq_attn_b128_p2.hip": ATTN_FLAGS,
     "lbfq_sdpa.hip": ["-ffp-contract=off"],
+    "lbfq_qknorm.hip": ["-ffp-contract=off"],
+    "lbfq_kvcache.hip": ["-ffp-contract=off"],
+    "lbfq_paged.hip": ["-ffp-contract=off"],
 }
 
 

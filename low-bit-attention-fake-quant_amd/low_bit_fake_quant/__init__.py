@@ -2,7 +2,9 @@
 
 Drop-in for the reference package ``low_bit_fake_quant`` (its
 ``__init__.py:3-60`` exports): same names, signatures and semantics, with
-every kernel a hand-written HIP kernel in ``liblbfq_hip.so``.
+every kernel a hand-written HIP kernel in ``liblbfq_hip.so``.  Beside it stand
+the operators of a model that keeps K and V in a quantised paged cache
+(``qk_norm``, ``kv_cache``).
 """
 
 from .attention import (
@@ -21,8 +23,10 @@ from .kmeans import (
     q_kmeans_reorder,
     v_kmeans_reorder,
 )
+from .kv_cache import PagedKVCache, empty_kv_cache, paged_attention, read_kv_cache, write_kv_cache
 from .pipeline import PreparedQKV, prepare_qkv
 from .preprocess import group_mean_q, smooth_k, smooth_v_per_block
+from .qk_norm import qk_norm_rope, rotary_table
 from .quant import (
     fp8_block_dequant,
     fp8_block_quant,
@@ -37,6 +41,7 @@ from .quant import (
 __all__ = [
     "FakeQuantArtifacts",
     "KMeansReorderResult",
+    "PagedKVCache",
     "PreparedQKV",
     "PreprocessCache",
     "QuantConfig",
@@ -62,4 +67,10 @@ __all__ = [
     "v_kmeans_reorder",
     "reference_attention",
     "smooth_k",
+    "empty_kv_cache",
+    "paged_attention",
+    "qk_norm_rope",
+    "read_kv_cache",
+    "rotary_table",
+    "write_kv_cache",
 ]

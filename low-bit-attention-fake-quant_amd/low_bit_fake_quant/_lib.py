@@ -147,6 +147,72 @@ class SdpaParams(ctypes.Structure):
     ]
 
 
+class QkNormParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("dtype", _i32),
+        ("B", _i64), ("S", _i64), ("Hq", _i64), ("Hk", _i64), ("D", _i64),
+        ("q_b", _i64), ("q_s", _i64), ("q_h", _i64), ("k_b", _i64), ("k_s", _i64), ("k_h", _i64),
+        ("q_weight", _vp), ("q_weight_dtype", _i32),
+        ("k_weight", _vp), ("k_weight_dtype", _i32),
+        ("cos", _vp), ("sin", _vp),
+        ("table_len", _i64), ("rot", _i32),
+        ("positions", _vp), ("positions_i64", _i32),
+        ("pos_b", _i64), ("pos_s", _i64),
+        ("eps", _f32), ("halves", _i32),
+        ("q_out", _vp), ("k_out", _vp),
+    ]
+
+
+class QkNormGrads(ctypes.Structure):
+    _fields_ = [
+        ("dyq", _vp), ("dyk", _vp),
+        ("dyq_b", _i64), ("dyq_s", _i64), ("dyq_h", _i64), ("dyk_b", _i64), ("dyk_s", _i64), ("dyk_h", _i64),
+        ("dq", _vp), ("dk", _vp),
+        ("dq_weight", _vp), ("dk_weight", _vp),
+        ("partial", _vp),
+    ]
+
+
+class KvWriteParams(ctypes.Structure):
+    _fields_ = [
+        ("k", _vp), ("v", _vp), ("dtype", _i32),
+        ("T", _i64), ("H", _i64), ("D", _i64),
+        ("k_t", _i64), ("k_h", _i64), ("v_t", _i64), ("v_h", _i64),
+        ("slots", _vp),
+        ("k_codes", _vp), ("k_scale", _vp), ("v_codes", _vp), ("v_scale", _vp),
+        ("num_pages", _i64), ("page_shift", _i32),
+    ]
+
+
+class KvReadParams(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", _vp), ("k_scale", _vp), ("v_codes", _vp), ("v_scale", _vp),
+        ("num_pages", _i64), ("page_shift", _i32),
+        ("B", _i64), ("H", _i64), ("D", _i64), ("max_len", _i64),
+        ("block_table", _vp), ("table_stride", _i64), ("table_cols", _i64),
+        ("seq_lens", _vp),
+        ("k_out", _vp), ("v_out", _vp), ("dtype", _i32),
+    ]
+
+
+class PagedParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("dtype", _i32),
+        ("T", _i64), ("Hq", _i64), ("Hk", _i64), ("D", _i64), ("B", _i64),
+        ("q_t", _i64), ("q_h", _i64),
+        ("k_codes", _vp), ("k_scale", _vp), ("v_codes", _vp), ("v_scale", _vp),
+        ("num_pages", _i64), ("page_shift", _i32),
+        ("block_table", _vp), ("table_stride", _i64), ("table_cols", _i64),
+        ("seq_lens", _vp), ("query_starts", _vp),
+        ("max_query_len", _i64),
+        ("sm_scale", _f32), ("causal", _i32), ("window", _i64),
+        ("out", _vp), ("out_t", _i64), ("out_h", _i64),
+        ("lse", _vp),
+        ("fill_rest", _i32),
+        ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "lbfq_last_error": (ctypes.c_char_p, []),
@@ -182,6 +248,13 @@ _SIGS = {
     "lbfq_blasst_attend": (_i32, [ctypes.POINTER(BlasstAttendParams), _vp]),
     "lbfq_sdpa_dequant": (_i32, [ctypes.POINTER(SdpaDequantParams), _vp]),
     "lbfq_sdpa_fwd": (_i32, [ctypes.POINTER(SdpaParams), _vp]),
+    "lbfq_qk_norm_rope": (_i32, [ctypes.POINTER(QkNormParams), _vp]),
+    "lbfq_qk_norm_rope_bwd_rows": (_i64, [ctypes.POINTER(QkNormParams)]),
+    "lbfq_qk_norm_rope_bwd": (_i32, [ctypes.POINTER(QkNormParams), ctypes.POINTER(QkNormGrads), _vp]),
+    "lbfq_kv_write": (_i32, [ctypes.POINTER(KvWriteParams), _vp]),
+    "lbfq_kv_read": (_i32, [ctypes.POINTER(KvReadParams), _vp]),
+    "lbfq_paged_attention_workspace_bytes": (_i64, [ctypes.POINTER(PagedParams)]),
+    "lbfq_paged_attention": (_i32, [ctypes.POINTER(PagedParams), _vp]),
     "lbfq_hbm_stream": (_i32, [_i32, _vp, _vp, _i64, _i32, _vp, _vp]),
     "lbfq_issue_probe": (_i32, [_i32, _i32, _i32, _vp, _vp, _vp]),
     "lbfq_selftest_cvt_fp8": (_i32, [_vp, _i64, _vp, _vp]),
