@@ -264,6 +264,7 @@ _SIGS = {
 EXPORTED = tuple(_SIGS)
 
 _lib = None
+_gpu_seen = False  # asking torch again costs 0.5 us a call
 
 
 class HipLibraryError(RuntimeError):
@@ -272,9 +273,11 @@ class HipLibraryError(RuntimeError):
 
 def load(require_gpu: bool = True):
     """Load the library (cached).  Raises if it is absent or no GPU is visible."""
-    global _lib
-    if require_gpu and not torch.cuda.is_available():
-        raise HipLibraryError("low_bit_fake_quant needs a ROCm GPU: torch.cuda.is_available() is False")
+    global _lib, _gpu_seen
+    if require_gpu and not _gpu_seen:
+        if not torch.cuda.is_available():
+            raise HipLibraryError("low_bit_fake_quant needs a ROCm GPU: torch.cuda.is_available() is False")
+        _gpu_seen = True
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise HipLibraryError(
