@@ -92,10 +92,20 @@ __device__ __forceinline__ void store8(void* base, int64_t i, const float (&v)[8
   }
 }
 
+// v of the lane that DPP pattern CTRL names, within the lane's row of 16
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+// The sum over a row's 16 or 8 lanes, in each of them: partners at distance 1, 2
+// (quad_perm), then the mirror images of halves (row_half_mirror) and rows (row_mirror).
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v) {
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) v += __shfl_xor(v, o, 64);
+  v += dpp<0xB1>(v);
+  v += dpp<0x4E>(v);
+  v += dpp<0x141>(v);
+  if constexpr (LPR == 16) v += dpp<0x140>(v);
   return v;
 }
 
@@ -161,9 +171,21 @@ __device__ __forceinline__ void turn(const Turn& u, float (&v)[8]) {
   for (int k = 0; k < 8; ++k) v[k] = fmaf(v[k], u.c[k], o[k] * (BACK ? -u.s[k] : u.s[k]));
 }
 
+// A lane's eight weights (ones without any); a weight vector may start anywhere.
 __device__ __forceinline__ void load_weight(const void* w, int dt, int d0, float (&v)[8]) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = w ? load_as_f32(w, d0 + k, dt) : 1.0f;
+  for (int k = 0; k < 8; ++k) v[k] = 1.0f;
+  if (!w) return;
+  if (reinterpret_cast<uint64_t>(w) & 15) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = load_as_f32(w, d0 + k, dt);
+  } else if (dt == kF32) {
+    widen<kF32>(load_raw<kF32>(w, d0), v);
+  } else if (dt == kBF16) {
+    widen<kBF16>(load_raw<kBF16>(w, d0), v);
+  } else {
+    widen<kF16>(load_raw<kF16>(w, d0), v);
+  }
 }
 
 template <int DT, int D, bool HALVES>
@@ -171,42 +193,41 @@ __global__ void __launch_bounds__(256) qk_norm_kernel(const Args a) {
   constexpr int LPR = D / 8, RPW = 64 / LPR, U = 4;
   const lbfq_qk_norm_params& p = a.p;
   const int lane = threadIdx.x & 63, sub = lane / LPR, d0 = 8 * (lane % LPR);
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (unit >= a.units) return;
-  const int64_t tok = unit / a.per_token;
-  const int g0 = static_cast<int>(unit - tok * a.per_token) * a.stretch;
-  const int g1 = g0 + a.stretch < a.groups ? g0 + a.stretch : a.groups;
-  const int64_t b = tok / p.S, t = tok - b * p.S;
   const int Hq = static_cast<int>(p.Hq), H = Hq + static_cast<int>(p.Hk);
   float wq[8], wk[8];
   load_weight(p.q_weight, p.q_weight_dtype, d0, wq);
   load_weight(p.k_weight, p.k_weight_dtype, d0, wk);
-  const Turn u = make_turn<LPR, HALVES>(p, b, t, lane);
-  const int64_t qin = b * p.q_b + t * p.q_s + d0, kin = b * p.k_b + t * p.k_s + d0;
-  for (int g = g0; g < g1; g += U) {
-    Raw<DT> raw[U];
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+       unit < a.units; unit += static_cast<int64_t>(gridDim.x) * 4) {
+    const int64_t tok = unit / a.per_token;
+    const int g0 = static_cast<int>(unit - tok * a.per_token) * a.stretch;
+    const int g1 = g0 + a.stretch < a.groups ? g0 + a.stretch : a.groups;
+    const int64_t b = tok / p.S, t = tok - b * p.S;
+    const int64_t qin = b * p.q_b + t * p.q_s + d0, kin = b * p.k_b + t * p.k_s + d0;
+    const Turn u = make_turn<LPR, HALVES>(p, b, t, lane);
+    for (int g = g0; g < g1; g += U) {
+      Raw<DT> raw[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      int h = (g + i) * RPW + sub;
-      h = h < H ? h : H - 1;  // every lane takes part in the row sums; rows past the last are not stored
-      raw[i] = h < Hq ? load_raw<DT>(p.q, qin + h * p.q_h) : load_raw<DT>(p.k, kin + (h - Hq) * p.k_h);
-    }
+      for (int i = 0; i < U; ++i) {
+        int h = (g + i) * RPW + sub;
+        h = h < H ? h : H - 1;  // every lane takes part in the row sums; rows past the last are not stored
+        raw[i] = load_raw<DT>(h < Hq ? p.q : p.k, h < Hq ? qin + h * p.q_h : kin + (h - Hq) * p.k_h);
+      }
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (g + i >= g1) break;
-      const int h = (g + i) * RPW + sub;
-      const bool isq = h < Hq;
-      float x[8], ss = 0.0f;
-      widen<DT>(raw[i], x);
+      for (int i = 0; i < U; ++i) {
+        if (g + i >= g1) break;
+        const int h = (g + i) * RPW + sub;
+        const bool isq = h < Hq;
+        float x[8], ss = 0.0f;
+        widen<DT>(raw[i], x);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
-      const float r = __builtin_amdgcn_rsqf(fmaf(row_sum<LPR>(ss), 1.0f / D, p.eps));
+        for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
+        const float r = __builtin_amdgcn_rsqf(fmaf(row_sum<LPR>(ss), 1.0f / D, p.eps));
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = x[k] * r * (isq ? wq[k] : wk[k]);
-      turn<HALVES, false>(u, x);
-      if (h < H) {
-        if (isq) store8<DT>(p.q_out, (tok * p.Hq + h) * D + d0, x);
-        else store8<DT>(p.k_out, (tok * p.Hk + h - Hq) * D + d0, x);
+        for (int k = 0; k < 8; ++k) x[k] = x[k] * r * (isq ? wq[k] : wk[k]);
+        turn<HALVES, false>(u, x);
+        if (h < H)
+          store8<DT>(isq ? p.q_out : p.k_out, (isq ? tok * p.Hq + h : tok * p.Hk + h - Hq) * D + d0, x);
       }
     }
   }
@@ -244,13 +265,9 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(const GradArgs ga) {
       for (int i = 0; i < U; ++i) {
         int h = (g + i) * RPW + sub;
         h = h < H ? h : H - 1;
-        if (h < Hq) {
-          rx[i] = load_raw<DT>(p.q, qin + h * p.q_h);
-          ry[i] = load_raw<DT>(gr.dyq, gq + h * gr.dyq_h);
-        } else {
-          rx[i] = load_raw<DT>(p.k, kin + (h - Hq) * p.k_h);
-          ry[i] = load_raw<DT>(gr.dyk, gk + (h - Hq) * gr.dyk_h);
-        }
+        const bool isq = h < Hq;
+        rx[i] = load_raw<DT>(isq ? p.q : p.k, isq ? qin + h * p.q_h : kin + (h - Hq) * p.k_h);
+        ry[i] = load_raw<DT>(isq ? gr.dyq : gr.dyk, isq ? gq + h * gr.dyq_h : gk + (h - Hq) * gr.dyk_h);
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
@@ -350,20 +367,25 @@ int check(const char* who, const lbfq_qk_norm_params* p) {
   return 0;
 }
 
-// A wave takes all heads of a token once there are tokens for 8192 waves (the
-// cos, sin and weight loads are then shared by the most rows); below that, one
-// group of heads, so that a few tokens reach many CUs.
+// A wave takes all heads of a token (cos, sin and the division of its index serve
+// the most rows) where there are 4096 tokens; of fewer, so many stretches of
+// each that there are that many waves.
 void plan(const lbfq_qk_norm_params* p, Args& a) {
   a.p = *p;
   const int rpw = p->D == 128 ? 4 : 8;
   a.groups = static_cast<int>((p->Hq + p->Hk + rpw - 1) / rpw);
   const int64_t tokens = p->B * p->S;
-  a.stretch = tokens >= 8192 ? a.groups : 1;
+  int64_t per = (4096 + tokens - 1) / tokens;
+  per = per < a.groups ? per : a.groups;
+  a.stretch = static_cast<int>((a.groups + per - 1) / per);
   a.per_token = (a.groups + a.stretch - 1) / a.stretch;
   a.units = tokens * a.per_token;
 }
 
-constexpr int64_t kGradGroups = 1024;  // workgroups of a backward: four per CU
+// Workgroups of a launch, at most.  Forward: a wave per token up to 32768 of them (us for 32760 tokens x 24 heads x 128
+// bf16, 1024 / 2048 / 4096 / 8192 workgroups: 89 / 92 / 84 / 80).  Backward: four per CU, whose weight sums the second
+// launch adds up (8002 tokens x 40 heads, 512 / 1024 / 2048: 65 + 4, 47 + 5, 48 + 10 us).
+constexpr int64_t kForwardGroups = 8192, kGradGroups = 1024;
 
 }  // namespace
 
@@ -388,9 +410,8 @@ extern "C" int lbfq_qk_norm_rope(const lbfq_qk_norm_params* p, lbfq_stream_t str
   Args a{};
   plan(p, a);
   const int64_t wgs = (a.units + 3) / 4;
-  LBFQ_CHECK_ARG(wgs < (int64_t{1} << 31), "lbfq_qk_norm_rope: problem too large");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(wgs));
+  const dim3 grid(static_cast<unsigned>(wgs < kForwardGroups ? wgs : kForwardGroups));
   LBFQ_QKN_DT(qk_norm_kernel, grid, a);
   LBFQ_LAUNCH_CHECK("lbfq_qk_norm_rope");
   return 0;
