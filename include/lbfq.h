@@ -441,7 +441,8 @@ int lbfq_qk_norm_rope_bwd(const lbfq_qk_norm_params* p, const lbfq_qk_norm_grads
 /* ---- quantised paged K/V cache -------------------------------------------------
  * Codes (num_pages, H, page, D) E4M3 and scales (num_pages, H, page, D / 32)
  * E8M0 of K and of V, contiguous and 16-byte aligned, page = 2^page_shift
- * tokens (16 .. 1024); the format of LBFQ_Q_MX_QK with 32 columns a scale.
+ * tokens (16 .. 1024); the format of LBFQ_Q_MX_QK with 32 columns a scale,
+ * scales at most 2^119 (infinities are held as 448 * 2^119).
  * write: rows k[t], v[t] (fp32, fp16 or bf16) to slot slots[t] = page id * page
  * + row; a slot outside the cache is skipped; slots must differ. */
 typedef struct {

@@ -5,7 +5,9 @@
 // of D/32 bytes, (pages, H, page, D/32): what attention reads of a head is one
 // stretch.  The format is the package's MXFP8 for Q and K (lbfq_rowtile,
 // LBFQ_Q_MX_QK, 32 columns a scale), the same codes and scales bit for bit:
-//   e = ceil(log2(max(amax, 1e-4) / 448)),  code = e4m3(x 2^-e).
+//   e = ceil(log2(max(amax, 1e-4) / 448)),  code = e4m3(x 2^-e),
+// but for e <= 119: from 2^128 on (where the value would be infinite) the largest is kept instead, 448 2^119.  The cache
+// then holds finite values only, and a key that a row does not see adds 0 times something finite to it.
 //
 // Both directions are bound by memory.  D/8 lanes hold a row, eight values each;
 // a workgroup takes 64 consecutive tokens of one head of K or of V, so that the
@@ -85,7 +87,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const lbfq_kv_write_param
     for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[i][k]));
     m = fmaxf(m, __shfl_xor(m, 1, 64));
     m = fmaxf(m, __shfl_xor(m, 2, 64));
-    const float sc = mx_scale_from_amax(fmaxf(m, kAmaxFloor));
+    const float sc = fminf(mx_scale_from_amax(fmaxf(m, kAmaxFloor)), 0x1p119f);
     const float inv = 1.0f / sc;  // exact: 2^-e
     float q[8];
 #pragma unroll

@@ -1,3 +1,4 @@
+#include <type_traits>
 // Attention of new tokens over the quantised paged K/V cache (lbfq_kv_write):
 //
 //   O_i = sum_j p_ij V_j / sum_j p_ij,  p_ij = exp(sm_scale q_i . K_j - m_i)
@@ -23,14 +24,14 @@
 // holds code * 2^e exactly (four significant bits); fp16 queries are two bf16
 // terms (eleven bits, exact); P is two bf16 terms (16 bits).
 //
-// chunk (more rows).  A workgroup of NW waves has 32 NW rows; 64-key tiles are
-// read once, converted to 16 bits and staged in LDS, double-buffered, one
-// barrier a tile.  V is fp16 times a power of two (2^(7 - E), E the largest
-// scale exponent so far, so that the largest code lands at 57344): exact unless
-// a block's scale is 2^25 below the largest, and then off by 2^-40 of the largest
-// V.  So P can be fp16: 11 bits, where bf16's 8 would cost as much as the output's
-// own rounding.  K is bf16 (exact) for bf16 queries, and for fp16 ones fp16 with the
-// tile's own E.
+// chunk (more rows, 32x32x16 MFMA).  A workgroup's four waves have 32 rows each; 64-key tiles are read once,
+// converted to 16 bits and staged in LDS, one barrier a tile.  Bound by VALU issue: a wave and tile take 32 MFMAs of 32
+// cycles and about 290 VALU instructions, 32 of them exponentials of eight cycles, so the loop runs the next tile's
+// scores and this one's P V beside the softmax and the conversion, in an order fixed here.  V goes through fp16, times
+// one power of two for the workgroup's part of the keys: every value that fits is exact, and a part whose scales lie too
+// far apart for that takes a slower loop with V in bf16 and P in two bf16 terms.  So P can be fp16: 11 bits, where
+// bf16's 8 would cost as much as the output's own rounding.  K is bf16 (exact) for bf16 queries, and for fp16 ones fp16
+// under the same rule.  4680 tokens over 32760 keys, 12 heads of 128, all seen: 1.16 ms, 812 TFLOP/s.
 #include "lbfq_common.h"
 #include "../../include/lbfq.h"
 
@@ -45,6 +46,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -54,7 +57,9 @@ struct Args {
   int G;          // query heads of a key head
   int tiles;      // row tiles of a sequence that the grid has
   int splits;     // parts of the keys
+  int least;      // key tiles of a part, at least
   int64_t main;   // workgroups that attend (the others fill)
+  uint32_t combos;  // sequences x key heads x parts
   float sml2;     // sm_scale * log2(e)
   float2* ml;     // (splits, T * Hq): maximum (log2 units) and sum of a part
   float* acc;     // (splits, T * Hq, D)
@@ -145,6 +150,20 @@ __device__ __forceinline__ uint32_t pack_dt(float a, float b) {
   else return pack_f16(a, b);
 }
 
+// Eight fp16 values as two bf16 terms each: eight bits and the other three, exact
+__device__ __forceinline__ void split_f16(const uint4& x, uint4& hi, uint4& lo) {
+  const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+  uint32_t h[4], r[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float a = f16_bits_to_f32(static_cast<uint16_t>(in[e])), b = f16_bits_to_f32(static_cast<uint16_t>(in[e] >> 16));
+    h[e] = pack_bf16(a, b);
+    r[e] = pack_bf16(a - __uint_as_float(h[e] << 16), b - __uint_as_float(h[e] & 0xffff0000u));
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(r[0], r[1], r[2], r[3]);
+}
+
 // Two codes of a word (HI: the upper two) times 2^e as 16-bit values; sc: 2^e as fp32.
 template <bool HI>
 __device__ __forceinline__ uint32_t cvt_bf16(uint32_t w, float sc) {
@@ -169,7 +188,7 @@ __device__ __forceinline__ v16f mfma32_f16(const uint4& a, const uint4& b, const
 
 // lse of a row (natural logarithm) from its maximum in log2 units and its sum
 __device__ __forceinline__ float row_lse(float m, float l) {
-  return l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+  return l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // ---- decode ------------------------------------------------------------------
@@ -185,24 +204,38 @@ struct Tile {
   bool ok[2];               // the page is there
 };
 
-template <int D>
-__device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int32_t* table, int kvh, int kb, int n,
-                                          int g, Tile<D>& x) {
-  constexpr int NB = D / 16;
+// The page ids of the two halves of a tile (-1: none); the same in every lane.
+__device__ __forceinline__ void load_pages(const lbfq_paged_params& p, const int32_t* table, int kb, int (&page)[2]) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int key = kb + 16 * t, idx = key >> p.page_shift;
-    int page = idx < p.table_cols ? table[idx] : -1;
-    x.ok[t] = page >= 0 && page < p.num_pages;
-    page = x.ok[t] ? page : 0;
-    const int64_t row = ((static_cast<int64_t>(page) * p.Hk + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
-    const uint8_t* kr = p.k_codes + (row + n) * D + 16 * g;
+    const int idx = (kb + 16 * t) >> p.page_shift;
+    page[t] = idx < p.table_cols ? table[idx] : -1;
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int (&pages)[2], int kvh, int kb, int n,
+                                          int g, Tile<D>& x) {
+  constexpr int NB = D / 16;
+  int64_t row[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    x.ok[t] = pages[t] >= 0 && pages[t] < p.num_pages;
+    const int page = x.ok[t] ? pages[t] : 0;
+    row[t] = ((static_cast<int64_t>(page) * p.Hk + kvh) << p.page_shift) + ((kb + 16 * t) & ((1 << p.page_shift) - 1));
+    const uint8_t* kr = p.k_codes + row[t] * D + (n * D + 16 * g);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) x.k[t][c] = *reinterpret_cast<const uint4*>(kr + 64 * c);
-    const uint8_t* vr = p.v_codes + (row + 4 * g) * D + NB * n;
+    const uint8_t* ks = p.k_scale + row[t] * (D / 32) + n * (D / 32);
+    if constexpr (D == 128) x.ks[t] = *reinterpret_cast<const uint32_t*>(ks);
+    else x.ks[t] = *reinterpret_cast<const uint16_t*>(ks);
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const uint8_t* vr = p.v_codes + row[t] * D + (4 * g * D + NB * n);
+    const uint8_t* vs = p.v_scale + row[t] * (D / 32) + 4 * g * (D / 32);
     if constexpr (D == 128) {
-      x.ks[t] = *reinterpret_cast<const uint32_t*>(p.k_scale + (row + n) * 4);
-      const uint4 s = *reinterpret_cast<const uint4*>(p.v_scale + (row + 4 * g) * 4);
+      const uint4 s = *reinterpret_cast<const uint4*>(vs);
       x.vs[t][0] = s.x; x.vs[t][1] = s.y; x.vs[t][2] = s.z; x.vs[t][3] = s.w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -210,8 +243,7 @@ __device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int3
         x.v[t][i][0] = v.x; x.v[t][i][1] = v.y;
       }
     } else {
-      x.ks[t] = *reinterpret_cast<const uint16_t*>(p.k_scale + (row + n) * 2);
-      const uint2 s = *reinterpret_cast<const uint2*>(p.v_scale + (row + 4 * g) * 2);
+      const uint2 s = *reinterpret_cast<const uint2*>(vs);
       x.vs[t][0] = s.x; x.vs[t][1] = s.y;
 #pragma unroll
       for (int i = 0; i < 4; ++i) x.v[t][i][0] = *reinterpret_cast<const uint32_t*>(vr + i * D);
@@ -220,7 +252,7 @@ __device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int3
 }
 
 template <int DT, int D>
-__global__ void __launch_bounds__(256) paged_decode_kernel(const Args a) {
+__global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
   constexpr int NC = D / 64, NB = D / 16, NW = 4;
   const lbfq_paged_params& p = a.p;
   if (static_cast<int64_t>(blockIdx.x) >= a.main) {
@@ -260,17 +292,7 @@ __global__ void __launch_bounds__(256) paged_decode_kernel(const Args a) {
           if constexpr (DT == kBF16) {
             q[c][u] = w;
           } else {
-            const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-            uint32_t hi2[4], lo2[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = f16_bits_to_f32(static_cast<uint16_t>(in[e]));
-              const float y = f16_bits_to_f32(static_cast<uint16_t>(in[e] >> 16));
-              hi2[e] = pack_bf16(x, y);
-              lo2[e] = pack_bf16(x - __uint_as_float(hi2[e] << 16), y - __uint_as_float(hi2[e] & 0xffff0000u));
-            }
-            q[c][u] = make_uint4(hi2[0], hi2[1], hi2[2], hi2[3]);
-            q2[c][u] = make_uint4(lo2[0], lo2[1], lo2[2], lo2[3]);
+            split_f16(w, q[c][u], q2[c][u]);
           }
         }
     }
@@ -282,15 +304,17 @@ __global__ void __launch_bounds__(256) paged_decode_kernel(const Args a) {
     float m = -INFINITY, l = 0.0f;
 
     const int kt0 = lo / 32, nt = hi > lo ? (hi + 31) / 32 - kt0 : 0;
-    const int per = (nt + a.splits - 1) / a.splits;
+    int per = (nt + a.splits - 1) / a.splits;
+    per = per > a.least ? per : a.least;
     const int begin = kt0 + split * per;
     const int end = begin + per < kt0 + nt ? begin + per : kt0 + nt;
-    Tile<D> x;
-    if (begin + wave < end) load_tile<D>(p, table, kvh, 32 * (begin + wave), n, g, x);
+    int pages[2];
+    load_pages(p, table, 32 * (begin + wave), pages);
     for (int kt = begin + wave; kt < end; kt += NW) {
       const int kb = 32 * kt;
-      Tile<D> nx;
-      if (kt + NW < end) load_tile<D>(p, table, kvh, 32 * (kt + NW), n, g, nx);
+      Tile<D> x;
+      load_tile<D>(p, pages, kvh, kb, n, g, x);
+      load_pages(p, table, 32 * (kt + NW), pages);
       // S^T: lane (n, g) has query n, keys 16 t + 4 g + i
       float sc[2][4];
 #pragma unroll
@@ -384,7 +408,6 @@ __global__ void __launch_bounds__(256) paged_decode_kernel(const Args a) {
         acc[nb] = mfma16_bf16(va, pb, acc[nb]);
         acc[nb] = mfma16_bf16(va, pc, acc[nb]);
       }
-      x = nx;
     }
     // join the waves
     l = add_x32(add_x16(l));
@@ -466,43 +489,38 @@ struct Lds {
 // then of consecutive keys, eight at a time.
 __device__ __forceinline__ int key_of(int i) { return (i & 0x13) | ((i & 4) << 1) | ((i & 8) >> 1); }
 
-// The largest byte of v over the wave, the same in every lane.
-__device__ __forceinline__ int wave_max_byte(uint32_t v) {
-  uint32_t x = v & 0xffu, y = (v >> 8) & 0xffu;
-  x = x > y ? x : y;
-  y = (v >> 16) & 0xffu;
-  x = x > y ? x : y;
-  y = v >> 24;
-  x = x > y ? x : y;
-#define LBFQ_ROR(c)                                                                                             \
-  do {                                                                                                          \
-    y = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), c, 0xf, 0xf, true));                \
-    x = x > y ? x : y;                                                                                          \
-  } while (0)
-  LBFQ_ROR(0x128);  // row_ror:8, 4, 2, 1
-  LBFQ_ROR(0x124);
-  LBFQ_ROR(0x122);
-  LBFQ_ROR(0x121);
-#undef LBFQ_ROR
-  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  x = r[0] > r[1] ? r[0] : r[1];
-  const auto r2 = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  x = r2[0] > r2[1] ? r2[0] : r2[1];
-  return __builtin_amdgcn_readfirstlane(x);
+// Largest (low half) and 255 - smallest (high half) of the scale bytes so far and of word v.
+__device__ __forceinline__ uint32_t span_join(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <int N>  // N bytes of v
+__device__ __forceinline__ uint32_t span_add(uint32_t span, uint32_t v) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t b = (v >> (8 * i)) & 0xffu;
+    span = span_join(span, b | ((255u - b) << 16));
+  }
+  return span;
 }
 
-// 2^(byte - E + 7) as fp32 (0 far below)
-__device__ __forceinline__ float rel_scale(uint32_t byte, int E) {
-  const int e = static_cast<int>(byte) - E + 134;
-  return __uint_as_float(static_cast<uint32_t>(e < 0 ? 0 : e) << 23);
-}
+// What the values of a part's K or V are multiplied by, 2^(134 - E), on their way to fp16, so that the largest
+// code lands at 57344.  The smallest one, 2^-9, with a scale 2^-22 of the largest is then fp16's smallest step: within
+// that span every value is exact.  A part whose scales are further apart is `wide`: bf16, as they are.
+constexpr int kSpan = 22;
+struct Unit {
+  int E;
+  bool wide;
+};
 
-template <int DT, int D, int NW>
-__global__ void __launch_bounds__(NW * 64, 2) paged_chunk_kernel(const Args a) {
-  constexpr int NT = NW * 64, NKS = D / 16, NDB = D / 32, CH = D / 32;
-  constexpr int KT = 64 * CH, VT = 8 * (D / 4);     // threads that K and V take, 32 codes each
-  constexpr bool BOTH = NT < KT + VT;               // every thread does both
-  static_assert(BOTH ? NT == KT && NT == VT : true, "a tile's threads");
+template <int DT, int D>
+__global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
+  constexpr int NW = 4, QB = 32 * NW, NT = 64 * NW;
+  constexpr int NKS = D / 16, NDB = D / 32, CH = D / 32;
+  constexpr int KC = 64 * D / NT;  // K codes of a thread
+  constexpr int KT = D / KC;       // threads of a key's row
+  constexpr int VK = KC / 4;       // V keys of a thread, four columns each
+  constexpr int WKEYS = 64 / NW;   // keys that a wave stages
+  static_assert(WKEYS == 16 || WKEYS == 8, "one page a wave");
   using L = Lds<D>;
   const lbfq_paged_params& p = a.p;
   if (static_cast<int64_t>(blockIdx.x) >= a.main) {
@@ -510,259 +528,511 @@ __global__ void __launch_bounds__(NW * 64, 2) paged_chunk_kernel(const Args a) {
     return;
   }
   __shared__ __align__(16) uint8_t lds[2 * L::BUF];
-  // Workgroups go to the eight XCDs in turn: neighbours in `id` are on one
-  // XCD, so the row tiles of a head share that XCD's L2.
-  int64_t id = blockIdx.x;
-  {
-    const int64_t q8 = a.main / 8, r8 = a.main % 8, x = id % 8;
-    id = x * q8 + (x < r8 ? x : r8) + id / 8;
-  }
-  // the last rows first: under a causal mask they take longest
-  const int tile0 = a.tiles - 1 - static_cast<int>(id % a.tiles);
-  int64_t rest = id / a.tiles;
-  const int split = static_cast<int>(rest % a.splits);
-  rest /= a.splits;
-  const int kvh = static_cast<int>(rest % p.Hk);
-  const int64_t b = rest / p.Hk;
+  // Workgroups go to the eight XCDs in turn.  Pieces of eight neighbouring row tiles are dealt to them whole, so that
+  // those that read the same keys share an L2; the pieces of all heads and parts (`combos`) with the last rows first,
+  // which take longest under a causal mask, and turned by one XCD from round to round, so that none has all of a kind.
+  const uint32_t round = blockIdx.x / 64, piece = round * 8 + (blockIdx.x + round) % 8, combos = a.combos;
+  const int tile0 = a.tiles - 1 - static_cast<int>(piece / combos * 8 + blockIdx.x / 8 % 8);
+  if (tile0 < 0) return;
+  uint32_t rest = piece % combos;
+  const int split = static_cast<int>(rest % static_cast<uint32_t>(a.splits));
+  rest /= static_cast<uint32_t>(a.splits);
+  const int Hk = static_cast<int>(p.Hk);
+  const int kvh = static_cast<int>(rest % static_cast<uint32_t>(Hk));
+  const int b = static_cast<int>(rest / static_cast<uint32_t>(Hk));
   const Seq s = sequence(p, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 31, g = lane >> 5;
   const int32_t* table = p.block_table + b * p.table_stride;
-  const int64_t R = p.T * p.Hq, rows = static_cast<int64_t>(s.n) * a.G;
-  constexpr int QB = 32 * NW;
-  const bool krole = BOTH || tid < KT, vrole = BOTH || (tid >= KT && tid < KT + VT);
-  const int kid = tid, vid = BOTH ? tid : tid - KT;
-  const int kkey = kid / CH, kch = kid % CH;          // K: a key's 32 columns
-  const int vkg = vid / (D / 4), vdq = vid % (D / 4);  // V: eight keys by four columns
+  const int cols = static_cast<int>(p.table_cols), num_pages = static_cast<int>(p.num_pages);
+  const int shift = p.page_shift, pmask = (1 << p.page_shift) - 1;
+  const int64_t R = p.T * p.Hq;
+  const int G = a.G;
+  const int rows = s.n * G;  // below 2^30: the host checks T * Hq
+  // Staging: wave w takes keys WKEYS w .. of a tile, which lie in one page.
+  const int kkey = lane / KT, kq = lane % KT;           // K: key kkey of the wave's, columns KC kq ..
+  const int vkg = lane / (D / 4), vdq = lane % (D / 4);  // V: keys VK vkg .. of the wave's, columns 4 vdq ..
+  static_assert(64 / KT == WKEYS && 64 / (D / 4) * VK == WKEYS, "a wave's keys");
+  const uint32_t koff = kkey * D + KC * kq, ksoff = kkey * CH + KC * kq / 32;
+  const uint32_t voff = VK * vkg * D + 4 * vdq, vsoff = VK * vkg * CH;
 
-  for (int64_t r0 = static_cast<int64_t>(tile0) * QB; r0 < rows; r0 += static_cast<int64_t>(a.tiles) * QB) {
-    const int64_t rw = r0 + wave * 32;
-    const int64_t rr = rw + li < rows ? rw + li : rows - 1;
-    const int qi = static_cast<int>(rr / a.G), h = kvh * a.G + static_cast<int>(rr % a.G);
+  // The page of key `key` (the same in every lane), or -1.
+  auto page_of = [&](int key) {
+    const int idx = key >> shift;
+    const int page = idx < cols ? table[idx] : -1;
+    return page >= 0 && page < num_pages ? page : -1;
+  };
+  auto row_of = [&](int page, int key) -> int64_t {
+    return (static_cast<int64_t>(page * Hk + kvh) << shift) + (key & pmask);
+  };
+
+  for (int r0 = tile0 * QB; r0 < rows; r0 += a.tiles * QB) {
+    const int rw = r0 + wave * 32;
+    const int rr = rw + li < rows ? rw + li : rows - 1;
+    const int qi = rr / G, h = kvh * G + (rr - qi * G);
     const int lo_r = s.lo(qi), hi_r = s.hi(qi);
-    const int first = static_cast<int>(r0 / a.G);
-    const int last = static_cast<int>(((r0 + QB < rows ? r0 + QB : rows) - 1) / a.G);
-    const int lo = s.lo(first), hi = s.hi(last);
-    // the same of the wave's rows
-    const int64_t w0 = rw < rows ? rw : rows - 1, w1 = rw + 31 < rows ? rw + 31 : rows - 1;
-    const int wf = __builtin_amdgcn_readfirstlane(static_cast<int>(w0 / a.G));
-    const int wl = __builtin_amdgcn_readfirstlane(static_cast<int>(w1 / a.G));
-    const int wlo = s.lo(wf), whi = rw < rows ? s.hi(wl) : 0, wlo_all = s.lo(wl), whi_all = s.hi(wf);
+    const int first = r0 / G, last = ((r0 + QB < rows ? r0 + QB : rows) - 1) / G;
+    const int lo = s.lo(first), hi = s.hi(last);  // keys that some row of the workgroup sees
+    const int wf = __builtin_amdgcn_readfirstlane((rw < rows ? rw : rows - 1) / G);
+    const int wl = __builtin_amdgcn_readfirstlane((rw + 31 < rows ? rw + 31 : rows - 1) / G);
+    const int wlo = s.lo(wf), whi = rw < rows ? s.hi(wl) : 0;  // that some row of the wave sees
+    const int lo_all = s.lo(wl), hi_all = s.hi(wf);            // that every row of the wave sees
 
-    uint4 q[NKS];
-    {
-      const uint16_t* qr = reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 8 * g;
-#pragma unroll
-      for (int k = 0; k < NKS; ++k) q[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
-    }
+    const int kt0 = lo / 64, nt = hi > lo ? (hi + 63) / 64 - kt0 : 0;
+    int per = (nt + a.splits - 1) / a.splits;
+    per = per > a.least ? per : a.least;
+    const int begin = kt0 + split * per;
+    const int end = begin + per < kt0 + nt ? begin + per : kt0 + nt;
+
     v16f acc[NDB];
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[db][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;
-
-    const int kt0 = lo / 64, nt = hi > lo ? (hi + 63) / 64 - kt0 : 0;
-    const int per = (nt + a.splits - 1) / a.splits;
-    const int begin = kt0 + split * per;
-    const int end = begin + per < kt0 + nt ? begin + per : kt0 + nt;
-
-    // staging registers of the next tile
-    uint4 kc[2];
-    uint32_t kse = 127, vc[8], vse[8 * CH / 4], vw = 0, kw = 0;
-    bool vok = false;
-    // exponents (bytes) of the tile in LDS and of acc; from 2^-63 on, so that no factor made of them underflows
-    int E = 64, Ek = 64, Eacc = 64;
-
-    auto row_of = [&](int key, bool& ok) -> int64_t {
-      const int idx = key >> p.page_shift;
-      int page = idx < p.table_cols ? table[idx] : -1;
-      ok = page >= 0 && page < p.num_pages;
-      page = ok ? page : 0;
-      return ((static_cast<int64_t>(page) * p.Hk + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
-    };
-    auto stage_load = [&](int kt) {
-      const int kb = 64 * kt;
-      if (krole) {
-        bool ok;
-        const int64_t row = row_of(kb + kkey, ok);
-        const uint4* src = reinterpret_cast<const uint4*>(p.k_codes + row * D + 32 * kch);
-        kc[0] = src[0];
-        kc[1] = src[1];
-        kse = p.k_scale[row * CH + kch];
-      }
-      if (vrole) {
-        const int64_t row = row_of(kb + 8 * vkg, vok);
-        const uint8_t* src = p.v_codes + row * D + 4 * vdq;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) vc[j] = *reinterpret_cast<const uint32_t*>(src + j * D);
-#pragma unroll
-        for (int c = 0; c < 8 * CH / 16; ++c) {
-          const uint4 w = reinterpret_cast<const uint4*>(p.v_scale + row * CH)[c];
-          vse[4 * c] = w.x; vse[4 * c + 1] = w.y; vse[4 * c + 2] = w.z; vse[4 * c + 3] = w.w;
-        }
-      }
+    Unit uv{134, false}, uk{134, false};
+    if (begin < end) {
+      // The span of the part's scales, over the keys that some row sees: four keys a thread and pass.
       {
-        bool ok;
-        const int64_t row = row_of(kb + lane, ok);
-        ok = ok && kb + lane >= lo && kb + lane < hi;
-        if constexpr (CH == 4) vw = *reinterpret_cast<const uint32_t*>(p.v_scale + row * CH);
-        else vw = *reinterpret_cast<const uint16_t*>(p.v_scale + row * CH);
-        vw = ok ? vw : 0;
-        if constexpr (DT == kF16) {
-          if constexpr (CH == 4) kw = *reinterpret_cast<const uint32_t*>(p.k_scale + row * CH);
-          else kw = *reinterpret_cast<const uint16_t*>(p.k_scale + row * CH);
-          kw = ok ? kw : 0;
-        }
-      }
-    };
-    auto stage_store = [&](int kt, uint8_t* buf) {
-      const int kb = 64 * kt;
-      const int t = wave_max_byte(vw);
-      E = t > E ? t : E;
-      if constexpr (DT == kF16) {
-        Ek = wave_max_byte(kw);
-        Ek = Ek > 64 ? Ek : 64;
-      }
-      if (krole) {
-        const uint32_t w[8] = {kc[0].x, kc[0].y, kc[0].z, kc[0].w, kc[1].x, kc[1].y, kc[1].z, kc[1].w};
-        uint32_t o[16];
-        const float e = DT == kF16 ? rel_scale(kse, Ek) : __uint_as_float(kse << 23);
+        uint32_t sv = 0, sk = 0;
+        const int k1 = 64 * end < hi ? 64 * end : hi;
+        for (int key = 64 * begin + 4 * tid; key < k1; key += 4 * NT) {
+          if (key + 4 <= lo) continue;
+          const int idx = key >> shift;
+          const int page = idx < cols ? table[idx] : -1;
+          if (page < 0 || page >= num_pages) continue;
+          const int64_t row = row_of(page, key);
+          const bool whole = key >= lo && key + 4 <= k1;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          o[2 * k] = DT == kF16 ? cvt_f16<false>(w[k], e) : cvt_bf16<false>(w[k], e);
-          o[2 * k + 1] = DT == kF16 ? cvt_f16<true>(w[k], e) : cvt_bf16<true>(w[k], e);
-        }
-        uint4* dst = reinterpret_cast<uint4*>(buf + kkey * L::KP + 64 * kch);
+          for (int c = 0; c < CH; ++c) {
+            uint32_t x = reinterpret_cast<const uint32_t*>(p.v_scale + row * CH)[c];
+            uint32_t y = DT == kF16 ? reinterpret_cast<const uint32_t*>(p.k_scale + row * CH)[c] : 0u;
+            if (whole) {
+              sv = span_add<4>(sv, x);
+              if constexpr (DT == kF16) sk = span_add<4>(sk, y);
+            } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) dst[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-      }
-      if (vrole) {
-        const bool edge = kb < lo || kb + 64 > hi;
-        uint32_t o[8][2];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t by;
-          if constexpr (CH == 4) by = vse[j] >> (8 * (vdq / 8));
-          else by = vse[j / 2] >> (16 * (j & 1) + 8 * (vdq / 8));
-          by &= 0xffu;
-          uint32_t w = vc[j];
-          const int key = kb + 8 * vkg + j;
-          if (!vok || (edge && (key < lo || key >= hi))) {  // never seen: nothing of it may reach the product
-            w = 0;
-            by = 1;
+              for (int i = 0; i < 4; ++i) {
+                const int ki = key + (4 * c + i) / CH;
+                if (ki < lo || ki >= k1) continue;
+                sv = span_add<1>(sv, x >> (8 * i));
+                if constexpr (DT == kF16) sk = span_add<1>(sk, y >> (8 * i));
+              }
+            }
           }
-          const float e = rel_scale(by, E);
-          o[j][0] = cvt_f16<false>(w, e);
-          o[j][1] = cvt_f16<true>(w, e);
+        }
+        uint32_t* red = reinterpret_cast<uint32_t*>(lds);
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) {
+          sv = span_join(sv, __shfl_xor(sv, i, 64));
+          if constexpr (DT == kF16) sk = span_join(sk, __shfl_xor(sk, i, 64));
+        }
+        if (lane == 0) {
+          red[wave] = sv;
+          red[NW + wave] = sk;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          sv = span_join(sv, red[w]);
+          sk = span_join(sk, red[NW + w]);
+        }
+        __syncthreads();
+        auto unit = [&](uint32_t x) {
+          x = __builtin_amdgcn_readfirstlane(x);
+          Unit u;
+          u.E = static_cast<int>(x & 0xffu);
+          u.wide = u.E - (255 - static_cast<int>(x >> 16)) > kSpan;
+          if (u.wide || x == 0) u.E = 134;
+          return u;
+        };
+        uv = unit(sv);
+        if constexpr (DT == kF16) uk = unit(sk);
+      }
+      uint4 q[NKS];
+      {
+        const uint16_t* qr = reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 8 * g;
+#pragma unroll
+        for (int k = 0; k < NKS; ++k) q[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
+      }
+      const float c = DT == kF16 ? ldexpf(a.sml2, uk.E - 134) : a.sml2;
+      const uint32_t kadd = static_cast<uint32_t>(134 - uk.E) << 23, vadd = static_cast<uint32_t>(134 - uv.E) << 23;
+
+      // Staging registers: codes and scales of a K tile and of a V tile.
+      uint32_t kc[KC / 4], kse, vc[VK], vse[VK * CH / 4];
+      auto load_k = [&](int kt, int page) {
+        const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
+        const uint8_t* ks = p.k_codes + row * D;
+        const uint8_t* kss = p.k_scale + row * CH;
+#pragma unroll
+        for (int i = 0; i < KC / 16; ++i) {
+          const uint4 w = *reinterpret_cast<const uint4*>(ks + koff + 16 * i);
+          kc[4 * i] = w.x; kc[4 * i + 1] = w.y; kc[4 * i + 2] = w.z; kc[4 * i + 3] = w.w;
+        }
+        kse = kss[ksoff];
+      };
+      auto load_v = [&](int kt, int page) {
+        const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
+        const uint8_t* vs = p.v_codes + row * D;
+        const uint8_t* vss = p.v_scale + row * CH;
+#pragma unroll
+        for (int j = 0; j < VK; ++j) vc[j] = *reinterpret_cast<const uint32_t*>(vs + voff + j * D);
+        if constexpr (VK * CH == 32) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint4 w = reinterpret_cast<const uint4*>(vss + vsoff)[i];
+            vse[4 * i] = w.x; vse[4 * i + 1] = w.y; vse[4 * i + 2] = w.z; vse[4 * i + 3] = w.w;
+          }
+        } else if constexpr (VK * CH == 16) {
+          const uint4 w = *reinterpret_cast<const uint4*>(vss + vsoff);
+          vse[0] = w.x; vse[1] = w.y; vse[2] = w.z; vse[3] = w.w;
+        } else if constexpr (VK * CH == 8) {
+          const uint2 w = *reinterpret_cast<const uint2*>(vss + vsoff);
+          vse[0] = w.x; vse[1] = w.y;
+        } else {
+          vse[0] = *reinterpret_cast<const uint32_t*>(vss + vsoff);
+        }
+      };
+      // Keys that no row sees, or that are not there: nothing of them may reach a product.
+      auto clear_k = [&](int kt, int page) {
+        const int key0 = 64 * kt + WKEYS * wave;
+        if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
+        if (page < 0 || key0 + kkey < lo || key0 + kkey >= hi) {
+#pragma unroll
+          for (int i = 0; i < KC / 4; ++i) kc[i] = 0;
+          kse = static_cast<uint32_t>(uk.E);
+        }
+      };
+      auto clear_v = [&](int kt, int page) {
+        const int key0 = 64 * kt + WKEYS * wave;
+        if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
+        const uint32_t fill = static_cast<uint32_t>(uv.E) * 0x01010101u;
+#pragma unroll
+        for (int j = 0; j < VK; ++j)
+          if (const int key = key0 + VK * vkg + j; page < 0 || key < lo || key >= hi) {
+            vc[j] = 0;
+            if constexpr (CH == 4) vse[j] = fill;
+            else vse[j / 2] = (vse[j / 2] & (j & 1 ? 0x0000ffffu : 0xffff0000u)) | (fill & (j & 1 ? 0xffff0000u : 0xffffu));
+          }
+      };
+      // registers -> LDS, as fp16 in the part's unit or (WIDE, and K for bf16 queries) as bf16
+      auto store_k = [&](uint8_t* buf, auto WIDE) {
+        constexpr bool f16 = DT == kF16 && !WIDE;
+        uint32_t o[KC / 2];
+        const float sc = __uint_as_float((kse << 23) + (f16 ? kadd : 0u));
+#pragma unroll
+        for (int k = 0; k < KC / 4; ++k) {
+          o[2 * k] = f16 ? cvt_f16<false>(kc[k], sc) : cvt_bf16<false>(kc[k], sc);
+          o[2 * k + 1] = f16 ? cvt_f16<true>(kc[k], sc) : cvt_bf16<true>(kc[k], sc);
+        }
+        uint4* dst = reinterpret_cast<uint4*>(buf + (WKEYS * wave + kkey) * L::KP + 2 * KC * kq);
+#pragma unroll
+        for (int k = 0; k < KC / 8; ++k) dst[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+      };
+      auto store_v = [&](uint8_t* buf, auto WIDE) {
+        uint32_t o[VK][2];
+#pragma unroll
+        for (int j = 0; j < VK; ++j) {
+          uint32_t by;
+          if constexpr (CH == 4) by = __builtin_amdgcn_ubfe(vse[j], 8 * (vdq / 8), 8);
+          else by = __builtin_amdgcn_ubfe(vse[j / 2], 16 * (j & 1) + 8 * (vdq / 8), 8);
+          const float sc = __uint_as_float((by << 23) + (WIDE ? 0u : vadd));
+          o[j][0] = WIDE ? cvt_bf16<false>(vc[j], sc) : cvt_f16<false>(vc[j], sc);
+          o[j][1] = WIDE ? cvt_bf16<true>(vc[j], sc) : cvt_f16<true>(vc[j], sc);
         }
         // column 4 dq + c is V^T row c D/4 + dq, so that neighbouring lanes write neighbouring rows
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t sel = c & 1 ? 0x07060302u : 0x05040100u;
-          uint32_t w[4];
+        for (int cc = 0; cc < 4; ++cc) {
+          const uint32_t sel = cc & 1 ? 0x07060302u : 0x05040100u;
+          uint32_t w[VK / 2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = __builtin_amdgcn_perm(o[2 * j + 1][c / 2], o[2 * j][c / 2], sel);
-          *reinterpret_cast<uint4*>(buf + L::KBYTES + (c * (D / 4) + vdq) * L::VP + 16 * vkg) =
-              make_uint4(w[0], w[1], w[2], w[3]);
+          for (int j = 0; j < VK / 2; ++j) w[j] = __builtin_amdgcn_perm(o[2 * j + 1][cc / 2], o[2 * j][cc / 2], sel);
+          uint8_t* dst = buf + L::KBYTES + (cc * (D / 4) + vdq) * L::VP + 2 * (WKEYS * wave + VK * vkg);
+          if constexpr (VK == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+          else if constexpr (VK == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+          else *reinterpret_cast<uint32_t*>(dst) = w[0];
         }
-      }
-    };
-
-    if (begin < end) {
-      stage_load(begin);
-      stage_store(begin, lds);
-    }
-    __syncthreads();
-    for (int kt = begin; kt < end; ++kt) {
-      const uint8_t* buf = lds + ((kt - begin) & 1) * L::BUF;
-      const int kb = 64 * kt;
-      const int Et = E, Ekt = Ek;
-      if (kt + 1 < end) stage_load(kt + 1);
-      if (kb < whi && kb + 64 > wlo) {
-        v16f sc[2];
+      };
+      // The same in eight pieces each, narrow
+      struct Staged {
+        uint32_t k[KC / 2], v[VK][2];
+      };
+      auto k_piece = [&](Staged& st, int i, uint8_t* buf) {
+        constexpr int W = KC >= 32 ? KC / 32 : 1;
+        const float sc = __uint_as_float((kse << 23) + (DT == kF16 ? kadd : 0u));
 #pragma unroll
-        for (int bl = 0; bl < 2; ++bl) {
-          const uint8_t* kr = buf + (32 * bl + key_of(li)) * L::KP + 16 * g;
+        for (int e = 0; e < W; ++e) {
+          const int k = i * W + e;
+          if (k >= KC / 4) continue;
+          st.k[2 * k] = DT == kF16 ? cvt_f16<false>(kc[k], sc) : cvt_bf16<false>(kc[k], sc);
+          st.k[2 * k + 1] = DT == kF16 ? cvt_f16<true>(kc[k], sc) : cvt_bf16<true>(kc[k], sc);
+          if (k & 1)
+            *reinterpret_cast<uint4*>(buf + (WKEYS * wave + kkey) * L::KP + 2 * KC * kq + 8 * (k - 1)) =
+                make_uint4(st.k[2 * k - 2], st.k[2 * k - 1], st.k[2 * k], st.k[2 * k + 1]);
+        }
+      };
+      auto v_piece = [&](Staged& st, int i, uint8_t* buf) {
+        constexpr int W = VK >= 4 ? VK / 4 : 1;  // keys in each of the first four pieces, then a column in each
+        if (i < 4) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sc[bl][r] = 0.0f;
+          for (int e = 0; e < W; ++e) {
+            const int j = i * W + e;
+            if (j >= VK) continue;
+            uint32_t by;
+            if constexpr (CH == 4) by = __builtin_amdgcn_ubfe(vse[j], 8 * (vdq / 8), 8);
+            else by = __builtin_amdgcn_ubfe(vse[j / 2], 16 * (j & 1) + 8 * (vdq / 8), 8);
+            const float sc = __uint_as_float((by << 23) + vadd);
+            st.v[j][0] = cvt_f16<false>(vc[j], sc);
+            st.v[j][1] = cvt_f16<true>(vc[j], sc);
+          }
+        } else {
+          const int cc = i - 4;
+          const uint32_t sel = cc & 1 ? 0x07060302u : 0x05040100u;
+          uint32_t w[VK / 2];
 #pragma unroll
-          for (int k = 0; k < NKS; ++k) {
-            const uint4 kop = *reinterpret_cast<const uint4*>(kr + 32 * k);
-            if constexpr (DT == kBF16) sc[bl] = mfma32_bf16(kop, q[k], sc[bl]);
-            else sc[bl] = mfma32_f16(kop, q[k], sc[bl]);
+          for (int j = 0; j < VK / 2; ++j) w[j] = __builtin_amdgcn_perm(st.v[2 * j + 1][cc / 2], st.v[2 * j][cc / 2], sel);
+          uint8_t* dst = buf + L::KBYTES + (cc * (D / 4) + vdq) * L::VP + 2 * (WKEYS * wave + VK * vkg);
+          if constexpr (VK == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+          else if constexpr (VK == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+          else *reinterpret_cast<uint32_t*>(dst) = w[0];
+        }
+      };
+      // S^T of 32 keys: register r is key 32 bl + 16 (r / 8) + 8 g + r % 8 of the tile in buf
+      auto scores = [&](const uint8_t* buf, int bl, v16f& sc, auto WIDE) {
+        const uint8_t* kr = buf + (32 * bl + key_of(li)) * L::KP + 16 * g;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NKS; ++k) {
+          const uint4 kop = *reinterpret_cast<const uint4*>(kr + 32 * k);
+          if constexpr (DT == kF16 && WIDE) {  // bf16 keys, the query's eleven bits in two bf16 terms
+            uint4 qh, ql;
+            split_f16(q[k], qh, ql);
+            sc = mfma32_bf16(kop, qh, sc);
+            sc = mfma32_bf16(kop, ql, sc);
+          } else if constexpr (DT == kBF16) {
+            sc = mfma32_bf16(kop, q[k], sc);
+          } else {
+            sc = mfma32_f16(kop, q[k], sc);
           }
         }
-        // register r of block bl is key kb + 32 bl + 16 (r / 8) + 8 g + r % 8
-        bool whole = kb >= wlo_all && kb + 64 <= whi_all;
-        uint32_t pages = 0xfu;  // of the tile's four groups of 16 keys, those whose page is there
-        {
-          bool ok = true;
-          if (lane < 4) {
-            const int idx = (kb + 16 * lane) >> p.page_shift;
-            const int page = idx < p.table_cols ? table[idx] : -1;
-            ok = page >= 0 && page < p.num_pages;
+      };
+      // The tile's scores masked where a row does not see the key, the row's maximum brought up to date (and with it the
+      // sums so far); returns the maximum in use.
+      auto settle = [&](int kb, uint32_t here, v16f& s0, v16f& s1) -> float {
+        if (!(kb >= lo_all && kb + 64 <= hi_all && here == 0xfu)) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = kb + 16 * (r >> 3) + 8 * g + (r & 7);
+            if (key < lo_r || key >= hi_r || !((here >> (r >> 3)) & 1u)) s0[r] = -INFINITY;
+            if (key + 32 < lo_r || key + 32 >= hi_r || !((here >> (2 + (r >> 3))) & 1u)) s1[r] = -INFINITY;
           }
-          pages = static_cast<uint32_t>(__ballot(ok)) & 0xfu;
-          whole = whole && pages == 0xfu;
         }
-        if (!whole) {
-#pragma unroll
-          for (int bl = 0; bl < 2; ++bl)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int key = kb + 32 * bl + 16 * (r >> 3) + 8 * g + (r & 7);
-              if (key < lo_r || key >= hi_r || !((pages >> (2 * bl + (r >> 3))) & 1u)) sc[bl][r] = -INFINITY;
-            }
-        }
-        const float c = DT == kF16 ? a.sml2 * ldexpf(1.0f, Ekt - 134) : a.sml2;
         float mx = -INFINITY;
 #pragma unroll
-        for (int bl = 0; bl < 2; ++bl)
-#pragma unroll
-          for (int r = 0; r < 16; r += 2) mx = fmaxf(mx, fmaxf(sc[bl][r], sc[bl][r + 1]));
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(s0[r], s1[r]));
         mx = max_x32(mx) * c;
         // p may grow to 2^8 past the maximum in use before that is moved (fp16 holds 65504)
-        if (__any(mx > m + 8.0f) || Et != Eacc) {
+        if (__any(mx > m + 8.0f)) {
           const float mn = fmaxf(m, mx);
           const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-          const float ae = al * ldexpf(1.0f, Eacc - Et);
           m = mn;
           l *= al;
-          Eacc = Et;
 #pragma unroll
           for (int db = 0; db < NDB; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[db][r] *= ae;
+            for (int r = 0; r < 16; ++r) acc[db][r] *= al;
         }
-        const float ms = m == -INFINITY ? 0.0f : m;
+        return m == -INFINITY ? 0.0f : m;
+      };
+
+      // A mask bit for each group of 16 keys of the tile: its page is there.
+      auto pages_there = [&](int kt) {
+        bool ok = true;
+        if (lane < 4) {
+          const int idx = (64 * kt + 16 * lane) >> shift;
+          const int pg = idx < cols ? table[idx] : -1;
+          ok = pg >= 0 && pg < num_pages;
+        }
+        return static_cast<uint32_t>(__ballot(ok)) & 0xfu;
+      };
+
+      auto page_at = [&](int kt) { return page_of(64 * kt + WKEYS * wave); };  // of the wave's keys: a scalar
+      if (uv.wide || uk.wide) {
+        // Rare (see Unit), and plain: one tile after the other.
+        for (int kt = begin; kt < end; ++kt) {
+          const int page = page_at(kt);
+          load_k(kt, page);
+          load_v(kt, page);
+          clear_k(kt, page);
+          clear_v(kt, page);
+          if (uk.wide) store_k(lds, std::true_type{});
+          else store_k(lds, std::false_type{});
+          if (uv.wide) store_v(lds, std::true_type{});
+          else store_v(lds, std::false_type{});
+          __syncthreads();
+          v16f sc[2];
 #pragma unroll
-        for (int bl = 0; bl < 2; ++bl)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int r = 8 * j + 2 * k;
-              const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[bl][r], c, -ms));
-              const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[bl][r + 1], c, -ms));
-              l += p0 + p1;
-              w[k] = pack_f16(p0, p1);
-            }
-            const uint4 pb = make_uint4(w[0], w[1], w[2], w[3]);
-            const uint8_t* vr = buf + L::KBYTES + li * L::VP + 16 * g + 32 * (2 * bl + j);
-#pragma unroll
-            for (int db = 0; db < NDB; ++db)
-              acc[db] = mfma32_f16(*reinterpret_cast<const uint4*>(vr + 32 * db * L::VP), pb, acc[db]);
+          for (int bl = 0; bl < 2; ++bl) {
+            if (uk.wide) scores(lds, bl, sc[bl], std::true_type{});
+            else scores(lds, bl, sc[bl], std::false_type{});
           }
+          const float ms = settle(64 * kt, pages_there(kt), sc[0], sc[1]);
+#pragma unroll
+          for (int bl = 0; bl < 2; ++bl)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint8_t* vr = lds + L::KBYTES + li * L::VP + 16 * g + 32 * (2 * bl + j);
+              float x[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                x[k] = __builtin_amdgcn_exp2f(fmaf(sc[bl][8 * j + k], c, -ms));
+                l += x[k];
+              }
+              uint32_t w[4], w2[4];
+              if (uv.wide) {  // V is bf16 as it is: P in two bf16 terms (16 bits)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  w[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+                  w2[k] = pack_bf16(x[2 * k] - __uint_as_float(w[k] << 16),
+                                    x[2 * k + 1] - __uint_as_float(w[k] & 0xffff0000u));
+                }
+#pragma unroll
+                for (int db = 0; db < NDB; ++db) {
+                  const uint4 va = *reinterpret_cast<const uint4*>(vr + 32 * db * L::VP);
+                  acc[db] = mfma32_bf16(va, make_uint4(w[0], w[1], w[2], w[3]), acc[db]);
+                  acc[db] = mfma32_bf16(va, make_uint4(w2[0], w2[1], w2[2], w2[3]), acc[db]);
+                }
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = pack_f16(x[2 * k], x[2 * k + 1]);
+#pragma unroll
+                for (int db = 0; db < NDB; ++db)
+                  acc[db] = mfma32_f16(*reinterpret_cast<const uint4*>(vr + 32 * db * L::VP),
+                                       make_uint4(w[0], w[1], w[2], w[3]), acc[db]);
+              }
+            }
+          __syncthreads();
+        }
+      } else {
+        constexpr std::false_type kNarrow{};
+        uint8_t* const buf0 = lds;
+        uint8_t* const buf1 = lds + L::BUF;
+        auto upto = [&](int kt) { return kt < end ? kt : end - 1; };  // steps past the end repeat it, unused
+        // The pages and masks of the tiles on the way: of V's registers, of K's, of the next K; of the scores' tile and
+        // the two after it.
+        int pv = page_at(begin), pk, pn;
+        load_k(begin, pv);
+        clear_k(begin, pv);
+        store_k(buf0, kNarrow);
+        pk = page_at(upto(begin + 1));
+        load_v(begin, pv);
+        load_k(upto(begin + 1), pk);
+        clear_v(begin, pv);
+        clear_k(upto(begin + 1), pk);
+        store_v(buf0, kNarrow);
+        store_k(buf1, kNarrow);
+        pv = pk;
+        pk = page_at(upto(begin + 2));
+        pn = page_at(upto(begin + 3));
+        load_v(upto(begin + 1), pv);
+        load_k(upto(begin + 2), pk);
+        uint32_t here0 = pages_there(begin), here1 = pages_there(upto(begin + 1)), here2 = pages_there(upto(begin + 2));
+        __syncthreads();
+        v16f sa, sb, sc_;
+        scores(buf0, 0, sa, kNarrow);
+        scores(buf0, 1, sb, kNarrow);
+        __syncthreads();  // the first step puts another K tile there
+        // Tile kt: its scores are in s0 and s1; the next tile's go to s2 and, when s0 is used up, s0 (three blocks for what
+        // would be four).  In LDS: K of kt + 1 (nxt), V of kt (cur).  In the staging registers: K of kt + 2, V of kt + 1.
+        auto step = [&](int kt, uint8_t* cur, uint8_t* nxt, v16f& s0, v16f& s1, v16f& s2) {
+          // The step's products in order: of each half of the tile the next tile's scores (NKS products) and this one's
+          // two quarters of P V (NDB each).  Their LDS operands are read kAhead products ahead, and each product is
+          // followed by a piece of what the VALU has to do meanwhile: the softmax of the half beside the scores, the
+          // conversion of the staged K (first half) or V tile (second) beside P V.  The order is fixed here; left to the
+          // compiler, every read was next to its product.
+          constexpr int HALF = NKS + 2 * NDB, kAhead = 5;
+          uint4 ring[kAhead];
+          const uint8_t* const kr = nxt + key_of(li) * L::KP + 16 * g;
+          const uint8_t* const vr = cur + L::KBYTES + li * L::VP + 16 * g;
+          auto fetch = [&](int n) {
+            if (n >= 2 * HALF) return;
+            const int bl = n / HALF, i = n % HALF;
+            const uint8_t* src = i < NKS ? kr + 32 * bl * L::KP + 32 * i
+                                         : vr + 32 * ((i - NKS) % NDB) * L::VP + 32 * (2 * bl + (i - NKS) / NDB);
+            ring[n % kAhead] = *reinterpret_cast<const uint4*>(src);
+          };
+#pragma unroll
+          for (int n = 0; n < kAhead; ++n) fetch(n);
+          const float ms = settle(64 * kt, here0, s0, s1);
+          clear_k(upto(kt + 2), pk);
+          clear_v(upto(kt + 1), pv);
+          Staged st;
+#pragma unroll
+          for (int bl = 0; bl < 2; ++bl) {
+            uint32_t w[8];
+            v16f& sc = bl == 0 ? s0 : s1;
+            v16f& sn = bl == 0 ? s2 : s0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sn[r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) {
+              const int n = bl * HALF + i;
+              const uint4 x = ring[n % kAhead];
+              if (i < NKS) {
+                sn = DT == kBF16 ? mfma32_bf16(x, q[i], sn) : mfma32_f16(x, q[i], sn);
+                fetch(n + kAhead);
+#pragma unroll
+                for (int e = 0; e < 8 / NKS; ++e) {
+                  const int k = i * (8 / NKS) + e;
+                  const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k], c, -ms));
+                  const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k + 1], c, -ms));
+                  l += p0 + p1;
+                  w[k] = pack_f16(p0, p1);
+                }
+              } else {
+                const int j = (i - NKS) / NDB, db = (i - NKS) % NDB;
+                acc[db] = mfma32_f16(x, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]), acc[db]);
+                fetch(n + kAhead);
+#pragma unroll
+                for (int e = 0; e < 4 / NDB; ++e) {
+                  const int k = (i - NKS) * (4 / NDB) + e;  // 0 .. 7
+                  if (bl == 0) k_piece(st, k, cur);
+                  else v_piece(st, k, nxt);
+                }
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+          pv = pk;
+          pk = pn;
+          load_v(upto(kt + 2), pv);
+          load_k(upto(kt + 3), pk);
+          pn = page_at(upto(kt + 4));
+          here0 = here1;
+          here1 = here2;
+          here2 = pages_there(upto(kt + 3));
+          __syncthreads();
+        };
+        // (two LDS buffers and three blocks of scores: the order comes round after six steps)
+        for (int kt = begin; kt < end;) {
+          step(kt, buf0, buf1, sa, sb, sc_);
+          if (++kt >= end) break;
+          step(kt, buf1, buf0, sc_, sa, sb);
+          if (++kt >= end) break;
+          step(kt, buf0, buf1, sb, sc_, sa);
+          if (++kt >= end) break;
+          step(kt, buf1, buf0, sa, sb, sc_);
+          if (++kt >= end) break;
+          step(kt, buf0, buf1, sc_, sa, sb);
+          if (++kt >= end) break;
+          step(kt, buf1, buf0, sb, sc_, sa);
+          ++kt;
+        }
       }
-      if (kt + 1 < end) stage_store(kt + 1, lds + ((kt + 1 - begin) & 1) * L::BUF);
-      __syncthreads();
+      l = add_x32(l);
     }
-    // V^T row x = c D/4 + dq holds column 4 dq + c.  Row 32 db + 8 (r / 4) + 4 g + r % 4 is lane (li, g)'s register r
-    // of acc[db].
-    l = add_x32(l);
-    const float back = ldexpf(1.0f, Eacc - 134);
+    const float back = ldexpf(1.0f, uv.E - 134);
     if (rw + li < rows) {
       const int64_t tok = s.start + qi;
       const bool one = a.splits == 1;
@@ -771,68 +1041,44 @@ __global__ void __launch_bounds__(NW * 64, 2) paged_chunk_kernel(const Args a) {
       if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
       if (!one && g == 0) a.ml[at] = make_float2(m, l);
       if (one || l > 0.0f) {
-        if constexpr (D == 128) {
-          // c = db, dq = 8 (r / 4) + 4 g + r % 4: four consecutive columns from the four blocks
+        // Register r of acc[db] is V^T row 32 db + 8 (r / 4) + 4 g + r % 4 = c D/4 + dq, column 4 dq + c: for piece i
+        // the columns 32 i + 16 g + 4 k + c.  D = 128: c = db, r = 4 i + k; D = 64: c = 2 db + r / 8, r % 8 = 4 i + k.
 #pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            const int col = 32 * r4 + 16 * g;
-            float o[16];
+        for (int i = 0; i < NDB; ++i) {
+          const int col = 32 * i + 16 * g;
+          float o[16];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
-              for (int db = 0; db < NDB; ++db) o[4 * k + db] = acc[db][4 * r4 + k] * f;
-            if (one) {
-              uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col);
-              dst[0] = make_uint4(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]), pack_dt<DT>(o[4], o[5]),
-                                  pack_dt<DT>(o[6], o[7]));
-              dst[1] = make_uint4(pack_dt<DT>(o[8], o[9]), pack_dt<DT>(o[10], o[11]), pack_dt<DT>(o[12], o[13]),
-                                  pack_dt<DT>(o[14], o[15]));
-            } else {
-              float4* dst = reinterpret_cast<float4*>(a.acc + at * D + col);
+            for (int cc = 0; cc < 4; ++cc)
+              o[4 * k + cc] = (D == 128 ? acc[cc % NDB][4 * i + k] : acc[cc / 2][8 * (cc & 1) + 4 * (i & 1) + k]) * f;
+          if (one) {
+            uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col);
+            dst[0] = make_uint4(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]), pack_dt<DT>(o[4], o[5]),
+                                pack_dt<DT>(o[6], o[7]));
+            dst[1] = make_uint4(pack_dt<DT>(o[8], o[9]), pack_dt<DT>(o[10], o[11]), pack_dt<DT>(o[12], o[13]),
+                                pack_dt<DT>(o[14], o[15]));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(a.acc + at * D + col);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-            }
+            for (int k = 0; k < 4; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
-        } else {
-          // D = 64: row x = 16 c + dq; block db holds c = 2 db (r < 8) and 2 db + 1, dq = 8 ((r / 4) % 2) + 4 g + r % 4
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-            {
-              const int col = 32 * half + 16 * g;
-              float o[16];
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[4 * k + c] = acc[c / 2][8 * (c & 1) + 4 * half + k] * f;
-              if (one) {
-                uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col);
-                dst[0] = make_uint4(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]), pack_dt<DT>(o[4], o[5]),
-                                    pack_dt<DT>(o[6], o[7]));
-                dst[1] = make_uint4(pack_dt<DT>(o[8], o[9]), pack_dt<DT>(o[10], o[11]), pack_dt<DT>(o[12], o[13]),
-                                    pack_dt<DT>(o[14], o[15]));
-              } else {
-                float4* dst = reinterpret_cast<float4*>(a.acc + at * D + col);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-              }
-            }
         }
       }
     }
-    __syncthreads();
+    __syncthreads();  // the next rows use the same LDS
   }
 }
 
 // ---- joining the parts of the keys ---------------------------------------------
 
-// A wave per row: 2^(m_s - M) weights of the parts, summed in their order.
+// A wave per row: the parts' maxima and sums one to a lane (there are at most
+// 64), then their outputs with weights 2^(m_s - M), summed in the parts' order.
 template <int DT, int D>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
+__global__ void __launch_bounds__(64) paged_combine_kernel(const Args a) {
   const lbfq_paged_params& p = a.p;
-  const int64_t R = p.T * p.Hq;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= R) return;
-  const int lane = threadIdx.x & 63;
+  const int64_t R = p.T * p.Hq, row = blockIdx.x;
+  const int lane = threadIdx.x;
   const int64_t tok = row / p.Hq;
   const int h = static_cast<int>(row - tok * p.Hq);
   uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + lane * (D / 64);
@@ -841,14 +1087,31 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
 #pragma unroll
   for (int k = 0; k < D / 64; ++k) o[k] = 0.0f;
   if (mine) {
-    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.ml[s * R + row].x);
-    for (int s = 0; s < a.splits; ++s) {
-      const float2 x = a.ml[s * R + row];
-      if (!(x.y > 0.0f)) continue;  // nothing in this part (its sums were not written)
-      const float f = __builtin_amdgcn_exp2f(x.x - M);
-      l = fmaf(x.y, f, l);
+    float2 x = make_float2(-INFINITY, 0.0f);
+    if (lane < a.splits) x = a.ml[lane * R + row];
+    const bool some = x.y > 0.0f;  // else nothing in this part, and its outputs were not written
+    M = some ? x.x : -INFINITY;
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k) o[k] = fmaf(a.acc[(s * R + row) * D + lane * (D / 64) + k], f, o[k]);
+    for (int i = 1; i < 64; i <<= 1) M = fmaxf(M, __shfl_xor(M, i, 64));
+    const float f = some ? __builtin_amdgcn_exp2f(x.x - M) : 0.0f;
+    l = some ? x.y * f : 0.0f;
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) l += __shfl_xor(l, i, 64);
+    const float* src = a.acc + row * D + lane * (D / 64);
+    for (int s0 = 0; s0 < a.splits; s0 += 8) {
+      float y[8][D / 64];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int s = s0 + i < a.splits ? s0 + i : a.splits - 1;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) y[i][k] = src[s * R * D + k];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (s0 + i) & 63));
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) o[k] = s0 + i < a.splits && w > 0.0f ? fmaf(y[i][k], w, o[k]) : o[k];
+      }
     }
   }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
@@ -863,11 +1126,19 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
 
 struct Plan {
   bool decode;
-  int tiles, splits;
+  int tiles, splits, least;
 };
 
 constexpr int kDecodeRows = 16;
 
+// The keys are split where the row tiles alone are fewer workgroups than the chip wants.  The lengths are on the device:
+// the rule goes by the table's width, and a sequence whose part would have fewer than `least` tiles uses fewer parts.
+//
+// decode: 2048 workgroups (eight per CU, three at a time), parts of 256 keys at least.  48 sequences of 8000 to 16000
+// keys, 8 key heads, us: 1024 / 2048 / 4096 / 8192 workgroups 262 / 242 / 242 / 273.
+// chunk: one sequence's parts are all alike, so the 512 that run at a time are enough (64 tokens over 20000 keys, 32 / 8
+// heads: 85 us, with 1024 workgroups 104; 512 tokens: 226 and 255).  Several have unequal lengths, and more workgroups
+// even them out (four of up to 509 tokens and 9001 keys, 512 / 1024 / 2048 / 4096: 106 / 85 / 75 / 91).
 Plan plan(const lbfq_paged_params* p) {
   Plan x;
   const int64_t G = p->Hq / p->Hk;
@@ -878,11 +1149,12 @@ Plan plan(const lbfq_paged_params* p) {
   x.tiles = static_cast<int>((rows + tile - 1) / tile);
   const int64_t wgs = x.tiles * p->Hk * p->B;
   const int64_t keys = p->table_cols << p->page_shift;
-  const int64_t want = x.decode ? 2048 : 512, least = x.decode ? 256 : 512;
+  const int64_t want = x.decode || p->B > 1 ? 2048 : 512, least = x.decode ? 256 : 512;
   int64_t s = want / wgs;
   if (s > keys / least) s = keys / least;
-  if (s > 64) s = 64;
+  if (s > 64) s = 64;  // a lane each in the combine kernel
   x.splits = s < 1 ? 1 : static_cast<int>(s);
+  x.least = static_cast<int>(least / (x.decode ? 32 : 64));
   return x;
 }
 
@@ -902,7 +1174,7 @@ int check(const lbfq_paged_params* p) {
   LBFQ_CHECK_ARG(p->T > 0 && p->B > 0 && p->T < (int64_t{1} << 30) && p->B < (int64_t{1} << 30),
                  "%s: bad number of tokens or sequences", who);
   LBFQ_CHECK_ARG(p->page_shift >= 4 && p->page_shift <= 10, "%s: pages hold 16 to 1024 tokens, a power of two", who);
-  LBFQ_CHECK_ARG(p->num_pages > 0 && p->num_pages < (int64_t{1} << 31), "%s: bad number of pages", who);
+  LBFQ_CHECK_ARG(p->num_pages > 0 && p->num_pages * p->Hk < (int64_t{1} << 31), "%s: bad number of pages", who);
   LBFQ_CHECK_ARG(p->table_cols > 0 && (p->table_cols << p->page_shift) <= (int64_t{1} << 30) &&
                      p->table_cols < (int64_t{1} << 30) && p->table_stride >= 0,
                  "%s: bad block table", who);
@@ -934,6 +1206,7 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   a.G = static_cast<int>(p->Hq / p->Hk);
   a.tiles = x.tiles;
   a.splits = x.splits;
+  a.least = x.least;
   a.sml2 = p->sm_scale * kLog2e;
   const int64_t R = p->T * p->Hq;
   if (x.splits > 1) {
@@ -942,8 +1215,11 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
     a.acc = static_cast<float*>(p->workspace);
     a.ml = reinterpret_cast<float2*>(a.acc + x.splits * R * p->D);
   }
-  LBFQ_CHECK_ARG(p->B < (int64_t{1} << 30) / (p->Hk * x.splits) / x.tiles, "lbfq_paged_attention: problem too large");
+  LBFQ_CHECK_ARG(R < (int64_t{1} << 30), "lbfq_paged_attention: problem too large");
+  LBFQ_CHECK_ARG(p->B < (int64_t{1} << 30) / (p->Hk * x.splits) / (x.tiles + 7), "lbfq_paged_attention: problem too large");
   a.main = p->B * p->Hk * x.tiles * x.splits;
+  a.combos = static_cast<uint32_t>(p->B * p->Hk * x.splits);
+  if (!x.decode) a.main = (static_cast<int64_t>((x.tiles + 7) / 8) * a.combos + 7) / 8 * 64;
   // rows that no sequence has: the combine kernel sees every row, otherwise some workgroups more
   const int64_t fill = (p->fill_rest || p->lse) && x.splits == 1 ? 8 : 0;
   const dim3 grid(static_cast<unsigned>(a.main + fill));
@@ -956,15 +1232,16 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
     else if (d128) hipLaunchKernelGGL((paged_decode_kernel<kF16, 128>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((paged_decode_kernel<kF16, 64>), grid, block, 0, st, a);
   } else {
-    const dim3 block(256);
-    if (bf && d128) hipLaunchKernelGGL((paged_chunk_kernel<kBF16, 128, 4>), grid, block, 0, st, a);
-    else if (bf) hipLaunchKernelGGL((paged_chunk_kernel<kBF16, 64, 4>), grid, block, 0, st, a);
-    else if (d128) hipLaunchKernelGGL((paged_chunk_kernel<kF16, 128, 4>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((paged_chunk_kernel<kF16, 64, 4>), grid, block, 0, st, a);
+#define LBFQ_PC(DT, DD) hipLaunchKernelGGL((paged_chunk_kernel<DT, DD>), grid, dim3(256), 0, st, a)
+    if (bf && d128) LBFQ_PC(kBF16, 128);
+    else if (bf) LBFQ_PC(kBF16, 64);
+    else if (d128) LBFQ_PC(kF16, 128);
+    else LBFQ_PC(kF16, 64);
+#undef LBFQ_PC
   }
   LBFQ_LAUNCH_CHECK("lbfq_paged_attention");
   if (x.splits > 1) {
-    const dim3 gc(static_cast<unsigned>((R + 3) / 4)), block(256);
+    const dim3 gc(static_cast<unsigned>(R)), block(64);
     if (bf && d128) hipLaunchKernelGGL((paged_combine_kernel<kBF16, 128>), gc, block, 0, st, a);
     else if (bf) hipLaunchKernelGGL((paged_combine_kernel<kBF16, 64>), gc, block, 0, st, a);
     else if (d128) hipLaunchKernelGGL((paged_combine_kernel<kF16, 128>), gc, block, 0, st, a);

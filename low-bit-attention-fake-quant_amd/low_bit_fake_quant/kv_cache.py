@@ -1,8 +1,8 @@
 """A quantised paged K/V cache and attention over it, on gfx950.
 
 The cache holds K and V in the package's MXFP8 format (E4M3 codes, one E8M0
-scale per 32 columns of a row: ``quant.mxfp8_qk_quant`` bit for bit), in pages
-that sequences take as they grow.  ``write_kv_cache`` quantises new rows into
+scale per 32 columns of a row: ``quant.mxfp8_qk_quant`` bit for bit below 3e38),
+in pages that sequences take as they grow.  ``write_kv_cache`` quantises new rows into
 it, ``paged_attention`` attends over it (one token of each sequence, or a chunk),
 ``read_kv_cache`` gives the values back, e.g. for ``fake_quant_attention``.
 
@@ -110,10 +110,11 @@ def write_kv_cache(k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, slots:
     outside the cache (-1 for padding) is skipped.  The slots of one call must
     differ: what one that is named twice holds afterwards is not defined.
 
-    Per 32 columns the scale is 2^ceil(log2(max(amax, 1e-4) / 448)) and the codes
-    round to nearest, ties to even.  As with the package's other quantisers, a NaN
-    leaves its block's scale alone and becomes -448 * scale, and an infinity
-    becomes +-448 * 2^127.
+    Per 32 columns the scale is 2^ceil(log2(max(amax, 1e-4) / 448)), at most 2^119,
+    and the codes round to nearest, ties to even.  As with the package's other
+    quantisers, a NaN leaves its block's scale alone and becomes -448 * scale.  An
+    infinity, or anything past 448 * 2^119 = 3e38, is held as that: the cache's
+    values are finite, and what a query does not see cannot reach its result.
     """
     n, h, page, d, index = _check_cache(cache)
     shape = k.shape
@@ -212,8 +213,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Ten
     log of each row's sum of exponentials, fp32 (T, Hq), -inf for a row that sees
     nothing.
 
-    Scores, softmax and sums are fp32 on exact products of codes and queries; P is
-    rounded to at least 11 bits for the second product, the result once.
+    Scores, softmax and sums are fp32 on exact products of cached values and
+    queries; P is rounded to at least 11 bits for the second product, the result
+    once.
     """
     n, hk, page, d, index = _check_cache(cache)
     shape = q.shape

@@ -116,9 +116,14 @@ def attend(q, cache, table, lens, starts, *, causal=True, window=None, sm_scale=
 
 
 def check(got, want, tol, what):
+    """Each value within its bound.  Rounding to nearest gives infinity from half a step
+    past the type's largest value on (fp16: 65504 + 16); a value whose bound reaches
+    that far may come out as that infinity."""
+    top = torch.finfo(got.dtype).max
+    over = want.abs() + tol >= top * (1 + torch.finfo(got.dtype).eps / 4)
     got = got.double()
     assert not torch.isnan(got).any(), f"{what}: NaN"
-    bad = ~((got == want) | ((got - want).abs() <= tol))
+    bad = ~((got == want) | ((got - want).abs() <= tol) | (over & (got == torch.sign(want) * math.inf)))
     assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} outside, first at "
                            f"{tuple(int(i) for i in bad.nonzero()[0])}: {got[bad][0].item()} for {want[bad][0].item()} "
                            f"(bound {tol.expand_as(want)[bad][0].item():.3g})")

@@ -68,8 +68,8 @@ def test_written_rows_equal_the_quantiser_and_the_definition(gpu, T, h, d, page,
         assert torch.equal(c[rest], b[rest]) and torch.equal(s[rest], bs[rest])
 
 
-def test_zero_nan_and_infinite_rows_are_written_as_the_quantiser_does(gpu):
-    from low_bit_fake_quant import empty_kv_cache, mxfp8_qk_quant, write_kv_cache
+def test_zero_nan_and_infinite_rows(gpu):
+    from low_bit_fake_quant import empty_kv_cache, mxfp8_qk_quant, read_kv_cache, write_kv_cache
     x = cpu_randn(6, 2, 128, seed=4, dtype=torch.float32)
     x[0] = 0
     x[1, :, 5] = math.nan
@@ -81,10 +81,14 @@ def test_zero_nan_and_infinite_rows_are_written_as_the_quantiser_does(gpu):
     cache = empty_kv_cache(1, 16, 2, 128, device=gpu)
     write_kv_cache(x, -x, cache, torch.arange(6, device=gpu))
     for i, t in ((0, x), (2, -x)):
-        codes, sc = mxfp8_qk_quant(t[None])
+        # infinities are held as the largest finite value, 448 * 2^119
+        codes, sc = mxfp8_qk_quant(t.clamp(-448 * 2.0 ** 119, 448 * 2.0 ** 119)[None])
         assert torch.equal(cache[i].view(torch.uint8)[0, :, :6].transpose(0, 1), codes[0].view(torch.uint8))
         assert torch.equal(torch.exp2(cache[i + 1][0, :, :6].transpose(0, 1).double() - 127), sc[0].double())
-        assert not torch.isnan(cache[i].float()).any()  # no call writes a NaN code
+    k, v = read_kv_cache(cache, torch.zeros(1, 1, dtype=torch.int32, device=gpu),
+                         torch.tensor([6], dtype=torch.int32, device=gpu), 6, dtype=torch.float32)
+    assert torch.isfinite(k).all() and torch.isfinite(v).all()
+    assert (k[0, 2, :, 40] == 448 * 2.0 ** 119).all() and (k[0, 3, :, 70] == -448 * 2.0 ** 119).all()
 
 
 @pytest.mark.parametrize("layout", ["packed", "head_major", "unaligned", "expanded", "last_strided"])

@@ -150,6 +150,46 @@ def test_nan_codes_that_no_row_sees(gpu, n):
                                                        window=40)) if i in (0, 2)], "window")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("n", [2, 4, 40])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan"), 3e38, 1e20])
+def test_huge_and_not_finite_keys_and_values_in_masked_places(gpu, bad, n, dtype):
+    """The last token's K and V hold infinities, NaN or huge values: the queries
+    before it do not see it, and their results are what they are without it."""
+    from low_bit_fake_quant import paged_attention, write_kv_cache
+    q, cache, table, lens, starts = problem(gpu, lens=[130, 75], counts=[n, n], dtype=dtype, garbage=False)
+    run = lambda: paged_attention(q, cache, table, lens, starts, max_query_len=n, return_lse=True)  # noqa: E731
+    out, lse = run()
+    x = torch.ones(2, 2, 128, device=gpu)
+    x[:, :, ::3] = bad
+    slots = torch.tensor([int(table[b, (L - 1) // 16]) * 16 + (L - 1) % 16 for b, L in enumerate((130, 75))], device=gpu)
+    write_kv_cache(x, x, cache, slots)
+    got, gl = run()
+    want, wlse, tol, ltol = ref.attend(q, cache, table, lens, starts)
+    before = [i for i in range(2 * n) if i % n != n - 1]
+    ref.check(got[before], want[before], tol[before], "before")
+    ref.check(gl[before], wlse[before], ltol[before], "before lse")
+    ref.check(out[before], want[before], tol[before], "without")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [1, 40])
+def test_scales_of_k_and_v_further_apart_than_fp16_reaches(gpu, n, d, dtype):
+    """K rows over 2^-30 ... 2^3 and V rows over 2^-40 ... 2^20, and either alone: the
+    chunk kernel's loop for such parts, for K, for V and for both."""
+    from low_bit_fake_quant import write_kv_cache
+    for kspan, vspan in (((-30, 3), (0, 0)), ((0, 0), (-40, 20)), ((-30, 3), (-40, 20))):
+        args = problem(gpu, lens=[150, 90], counts=[n, n], d=d, dtype=dtype, garbage=False)
+        g = torch.Generator().manual_seed(5)
+        for b, L in enumerate((150, 90)):
+            k, v = (torch.randn(L, 2, d, generator=g) * torch.exp2(torch.randint(*(s[0], s[1] + 1), (L, 1, 1), generator=g).float())
+                    for s in (kspan, vspan))
+            at = torch.arange(L)
+            write_kv_cache(k.to(gpu), v.to(gpu), args[1], (args[2].cpu().long()[b, at // 16] * 16 + at % 16).to(gpu))
+        run_and_check(args, f"K 2^{kspan} V 2^{vspan}", hint=n)
+
+
 @pytest.mark.parametrize("n", [1, 40])
 @pytest.mark.parametrize("span", [(-3, 3), (-30, 30), (8, 14), (-20, -12)])
 def test_values_of_very_different_sizes(gpu, n, span):
