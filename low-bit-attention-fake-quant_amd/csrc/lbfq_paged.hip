@@ -222,7 +222,7 @@ __device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int 
   for (int t = 0; t < 2; ++t) {
     x.ok[t] = pages[t] >= 0 && pages[t] < p.num_pages;
     const int page = x.ok[t] ? pages[t] : 0;
-    row[t] = ((static_cast<int64_t>(page) * p.Hk + kvh) << p.page_shift) + ((kb + 16 * t) & ((1 << p.page_shift) - 1));
+    row[t] = (static_cast<int64_t>(page * static_cast<int>(p.Hk) + kvh) << p.page_shift) + ((kb + 16 * t) & ((1 << p.page_shift) - 1));
     const uint8_t* kr = p.k_codes + row[t] * D + (n * D + 16 * g);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) x.k[t][c] = *reinterpret_cast<const uint4*>(kr + 64 * c);
@@ -261,24 +261,27 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
   }
   __shared__ __align__(16) float acc_s[NW][16][D + 4];
   __shared__ float m_s[NW][16], l_s[NW][16];
-  const int split = static_cast<int>(blockIdx.x % a.splits);
-  int64_t rest = blockIdx.x / a.splits;
-  const int kvh = static_cast<int>(rest % p.Hk);
-  rest /= p.Hk;
-  const int tile0 = static_cast<int>(rest % a.tiles);
-  const int64_t b = rest / a.tiles;
+  // 32-bit indices: the divisions of 64-bit ones were most of this kernel's code and a fifth of a small call's time
+  const uint32_t splits = static_cast<uint32_t>(a.splits), Hk = static_cast<uint32_t>(p.Hk);
+  const int split = static_cast<int>(blockIdx.x % splits);
+  uint32_t rest = blockIdx.x / splits;
+  const int kvh = static_cast<int>(rest % Hk);
+  rest /= Hk;
+  const int tile0 = static_cast<int>(rest % static_cast<uint32_t>(a.tiles));
+  const int b = static_cast<int>(rest / static_cast<uint32_t>(a.tiles));
   const Seq s = sequence(p, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int32_t* table = p.block_table + b * p.table_stride;
-  const int64_t R = p.T * p.Hq, rows = static_cast<int64_t>(s.n) * a.G;
-  for (int64_t r0 = static_cast<int64_t>(tile0) * 16; r0 < rows; r0 += static_cast<int64_t>(a.tiles) * 16) {
+  const int64_t R = p.T * p.Hq;
+  const int G = a.G, rows = s.n * G;  // below 2^30: the host checks T * Hq
+  for (int r0 = tile0 * 16; r0 < rows; r0 += a.tiles * 16) {
     // this lane's query; rows past the last repeat it and are not stored
-    const int64_t rr = r0 + n < rows ? r0 + n : rows - 1;
-    const int qi = static_cast<int>(rr / a.G), h = kvh * a.G + static_cast<int>(rr % a.G);
+    const int rr = r0 + n < rows ? r0 + n : rows - 1;
+    const int qi = rr / G, h = kvh * G + (rr - qi * G);
     const int lo_r = s.lo(qi), hi_r = s.hi(qi);
-    const int first = static_cast<int>(r0 / a.G);
-    const int last = static_cast<int>(((r0 + 16 < rows ? r0 + 16 : rows) - 1) / a.G);
+    const int first = r0 / G;
+    const int last = ((r0 + 16 < rows ? r0 + 16 : rows) - 1) / G;
     const int lo = s.lo(first), hi = s.hi(last);          // keys that some row sees
     const int lo_all = s.lo(last), hi_all = s.hi(first);  // keys that every row sees
     uint4 q[NC][2], q2[DT == kF16 ? NC : 1][2];
@@ -447,9 +450,8 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
           }
           o[k] = t.x; o[k + 1] = t.y; o[k + 2] = t.z; o[k + 3] = t.w;
         }
-        const int64_t r = r0 + row;
-        const int64_t tok = s.start + r / a.G;
-        const int hh = kvh * a.G + static_cast<int>(r % a.G);
+        const int qq = (r0 + row) / G, hh = kvh * G + (r0 + row - qq * G);
+        const int64_t tok = s.start + qq;
         if (a.splits == 1) {
           const float inv = L > 0.0f ? 1.0f / L : 0.0f;
           uint32_t w[NB / 2];
@@ -1072,50 +1074,72 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
 
 // ---- joining the parts of the keys ---------------------------------------------
 
+// The largest / the sum over the wave, in every lane
+__device__ __forceinline__ float wave_max(float v) {
+#define LBFQ_ROR(c) v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), c, 0xf, 0xf, true)))
+  LBFQ_ROR(0x128);  // row_ror:8, 4, 2, 1
+  LBFQ_ROR(0x124);
+  LBFQ_ROR(0x122);
+  LBFQ_ROR(0x121);
+#undef LBFQ_ROR
+  return max_x32(max_x16(v));
+}
+__device__ __forceinline__ float wave_add(float v) {
+#define LBFQ_ROR(c) v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), c, 0xf, 0xf, true))
+  LBFQ_ROR(0x128);
+  LBFQ_ROR(0x124);
+  LBFQ_ROR(0x122);
+  LBFQ_ROR(0x121);
+#undef LBFQ_ROR
+  return add_x32(add_x16(v));
+}
+
 // A wave per row: the parts' maxima and sums one to a lane (there are at most
-// 64), then their outputs with weights 2^(m_s - M), summed in the parts' order.
+// 64), their outputs with weights 2^(m_s - M) summed in the parts' order.  All
+// latency at a few rows: the first sixteen parts are on their way before the
+// weights are known.
 template <int DT, int D>
 __global__ void __launch_bounds__(64) paged_combine_kernel(const Args a) {
+  constexpr int U = 16, DL = D / 64;
   const lbfq_paged_params& p = a.p;
-  const int64_t R = p.T * p.Hq, row = blockIdx.x;
+  const uint32_t row = blockIdx.x, Hq = static_cast<uint32_t>(p.Hq);
+  const int64_t R = p.T * p.Hq;
   const int lane = threadIdx.x;
-  const int64_t tok = row / p.Hq;
-  const int h = static_cast<int>(row - tok * p.Hq);
-  uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + lane * (D / 64);
+  const int tok = static_cast<int>(row / Hq);
+  const int h = static_cast<int>(row - tok * Hq);
+  float2 x = make_float2(-INFINITY, 0.0f);
+  if (lane < a.splits) x = a.ml[lane * R + row];
+  const float* src = a.acc + static_cast<int64_t>(row) * D + lane * DL;
+  float y[U][DL];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int s = s0 + i < a.splits ? s0 + i : a.splits - 1;
+#pragma unroll
+      for (int k = 0; k < DL; ++k) y[i][k] = src[s * R * D + k];
+    }
+  };
+  load(0);
   const bool mine = tok >= p.query_starts[0] && tok < p.query_starts[p.B];
-  float M = -INFINITY, l = 0.0f, o[D / 64];
+  const bool some = mine && x.y > 0.0f;  // else nothing in this part, and its outputs were not written
+  const float M = wave_max(some ? x.x : -INFINITY);
+  const float f = some ? __builtin_amdgcn_exp2f(x.x - M) : 0.0f;
+  const float l = wave_add(some ? x.y * f : 0.0f);
+  float o[DL];
 #pragma unroll
-  for (int k = 0; k < D / 64; ++k) o[k] = 0.0f;
-  if (mine) {
-    float2 x = make_float2(-INFINITY, 0.0f);
-    if (lane < a.splits) x = a.ml[lane * R + row];
-    const bool some = x.y > 0.0f;  // else nothing in this part, and its outputs were not written
-    M = some ? x.x : -INFINITY;
+  for (int k = 0; k < DL; ++k) o[k] = 0.0f;
+  for (int s0 = 0; s0 < a.splits; s0 += U) {
+    if (s0) load(s0);
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) M = fmaxf(M, __shfl_xor(M, i, 64));
-    const float f = some ? __builtin_amdgcn_exp2f(x.x - M) : 0.0f;
-    l = some ? x.y * f : 0.0f;
+    for (int i = 0; i < U; ++i) {
+      const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + i));
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) l += __shfl_xor(l, i, 64);
-    const float* src = a.acc + row * D + lane * (D / 64);
-    for (int s0 = 0; s0 < a.splits; s0 += 8) {
-      float y[8][D / 64];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int s = s0 + i < a.splits ? s0 + i : a.splits - 1;
-#pragma unroll
-        for (int k = 0; k < D / 64; ++k) y[i][k] = src[s * R * D + k];
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (s0 + i) & 63));
-#pragma unroll
-        for (int k = 0; k < D / 64; ++k) o[k] = s0 + i < a.splits && w > 0.0f ? fmaf(y[i][k], w, o[k]) : o[k];
-      }
+      for (int k = 0; k < DL; ++k) o[k] = w > 0.0f ? fmaf(y[i][k], w, o[k]) : o[k];  // (no lane past the parts has one)
     }
   }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   if (mine || p.fill_rest) {
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + lane * DL;
     if constexpr (D == 128) *reinterpret_cast<uint32_t*>(dst) = pack_dt<DT>(o[0] * inv, o[1] * inv);
     else *dst = static_cast<uint16_t>(pack_dt<DT>(o[0] * inv, 0.0f));
   }
@@ -1134,8 +1158,9 @@ constexpr int kDecodeRows = 16;
 // The keys are split where the row tiles alone are fewer workgroups than the chip wants.  The lengths are on the device:
 // the rule goes by the table's width, and a sequence whose part would have fewer than `least` tiles uses fewer parts.
 //
-// decode: 2048 workgroups (eight per CU, three at a time), parts of 256 keys at least.  48 sequences of 8000 to 16000
-// keys, 8 key heads, us: 1024 / 2048 / 4096 / 8192 workgroups 262 / 242 / 242 / 273.
+// decode: 1536 workgroups, twice the three per CU that run at a time, parts of 256 keys at least.  48 sequences of 8000
+// to 16000 keys, 8 key heads, us: 256 / 1536 / 2048 / 4096 / 8192 workgroups 314 / 240 / 244 / 245 / 273.  One sequence
+// of 5003 keys, parts of 128 / 256 / 512 keys: 9.4 + 6.4 (combine), 10.1 + 5.1, 13.4 + 4.2.
 // chunk: one sequence's parts are all alike, so the 512 that run at a time are enough (64 tokens over 20000 keys, 32 / 8
 // heads: 85 us, with 1024 workgroups 104; 512 tokens: 226 and 255).  Several have unequal lengths, and more workgroups
 // even them out (four of up to 509 tokens and 9001 keys, 512 / 1024 / 2048 / 4096: 106 / 85 / 75 / 91).
@@ -1149,7 +1174,7 @@ Plan plan(const lbfq_paged_params* p) {
   x.tiles = static_cast<int>((rows + tile - 1) / tile);
   const int64_t wgs = x.tiles * p->Hk * p->B;
   const int64_t keys = p->table_cols << p->page_shift;
-  const int64_t want = x.decode || p->B > 1 ? 2048 : 512, least = x.decode ? 256 : 512;
+  const int64_t want = x.decode ? 1536 : p->B > 1 ? 2048 : 512, least = x.decode ? 256 : 512;
   int64_t s = want / wgs;
   if (s > keys / least) s = keys / least;
   if (s > 64) s = 64;  // a lane each in the combine kernel

@@ -25,11 +25,27 @@ namespace {
 
 struct Args {
   lbfq_qk_norm_params p;
-  int64_t units;   // (token, stretch of head groups)
-  int per_token;   // stretches of a token
+  uint32_t units;  // (token, stretch of head groups); below 2^31
+  uint32_t per_token;  // stretches of a token
   int stretch;     // head groups of a stretch
   int groups;      // head groups of a token
 };
+
+// A unit's token and head groups (32-bit divisions: 64-bit ones are a hundred instructions each)
+struct Place {
+  uint32_t tok, b, t;
+  int g0, g1;
+};
+__device__ __forceinline__ Place place(const Args& a, uint32_t unit) {
+  Place x;
+  const uint32_t S = static_cast<uint32_t>(a.p.S);
+  x.tok = unit / a.per_token;
+  x.g0 = static_cast<int>(unit - x.tok * a.per_token) * a.stretch;
+  x.g1 = x.g0 + a.stretch < a.groups ? x.g0 + a.stretch : a.groups;
+  x.b = x.tok / S;
+  x.t = x.tok - x.b * S;
+  return x;
+}
 
 struct GradArgs {
   Args a;
@@ -197,12 +213,11 @@ __global__ void __launch_bounds__(256) qk_norm_kernel(const Args a) {
   float wq[8], wk[8];
   load_weight(p.q_weight, p.q_weight_dtype, d0, wq);
   load_weight(p.k_weight, p.k_weight_dtype, d0, wk);
-  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-       unit < a.units; unit += static_cast<int64_t>(gridDim.x) * 4) {
-    const int64_t tok = unit / a.per_token;
-    const int g0 = static_cast<int>(unit - tok * a.per_token) * a.stretch;
-    const int g1 = g0 + a.stretch < a.groups ? g0 + a.stretch : a.groups;
-    const int64_t b = tok / p.S, t = tok - b * p.S;
+  for (uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); unit < a.units;
+       unit += gridDim.x * 4) {
+    const Place pl = place(a, unit);
+    const int g0 = pl.g0, g1 = pl.g1;
+    const int64_t tok = pl.tok, b = pl.b, t = pl.t;
     const int64_t qin = b * p.q_b + t * p.q_s + d0, kin = b * p.k_b + t * p.k_s + d0;
     const Turn u = make_turn<LPR, HALVES>(p, b, t, lane);
     for (int g = g0; g < g1; g += U) {
@@ -250,12 +265,10 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(const GradArgs ga) {
   load_weight(p.k_weight, p.k_weight_dtype, d0, wk);
 #pragma unroll
   for (int k = 0; k < 8; ++k) sq[k] = sk[k] = 0.0f;
-  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + wave; unit < a.units;
-       unit += static_cast<int64_t>(gridDim.x) * 4) {
-    const int64_t tok = unit / a.per_token;
-    const int g0 = static_cast<int>(unit - tok * a.per_token) * a.stretch;
-    const int g1 = g0 + a.stretch < a.groups ? g0 + a.stretch : a.groups;
-    const int64_t b = tok / p.S, t = tok - b * p.S;
+  for (uint32_t unit = blockIdx.x * 4 + wave; unit < a.units; unit += gridDim.x * 4) {
+    const Place pl = place(a, unit);
+    const int g0 = pl.g0, g1 = pl.g1;
+    const int64_t tok = pl.tok, b = pl.b, t = pl.t;
     const Turn u = make_turn<LPR, HALVES>(p, b, t, lane);
     const int64_t qin = b * p.q_b + t * p.q_s + d0, kin = b * p.k_b + t * p.k_s + d0;
     const int64_t gq = b * gr.dyq_b + t * gr.dyq_s + d0, gk = b * gr.dyk_b + t * gr.dyk_s + d0;
@@ -351,8 +364,8 @@ int check(const char* who, const lbfq_qk_norm_params* p) {
   LBFQ_CHECK_ARG(p->D == 64 || p->D == 128, "%s: D must be 64 or 128", who);
   LBFQ_CHECK_ARG(p->dtype >= kF32 && p->dtype <= kBF16, "%s: bad dtype %d", who, p->dtype);
   LBFQ_CHECK_ARG(p->B > 0 && p->S > 0 && p->Hq > 0 && p->Hk > 0, "%s: empty problem", who);
-  LBFQ_CHECK_ARG(p->Hq + p->Hk < (1 << 20) && p->B < (int64_t{1} << 40) / p->S &&
-                     p->B * p->S < (int64_t{1} << 50) / (p->Hq + p->Hk),
+  LBFQ_CHECK_ARG(p->Hq + p->Hk < (1 << 20) && p->B < (int64_t{1} << 31) / p->S &&
+                     p->B * p->S < (int64_t{1} << 31) / ((p->Hq + p->Hk + 3) / 4),
                  "%s: problem too large", who);
   LBFQ_CHECK_ARG(p->q && p->k && p->cos && p->sin, "%s: missing tensor", who);
   LBFQ_CHECK_ARG(p->rot > 0 && p->rot <= p->D && p->rot % 16 == 0, "%s: rot must be a multiple of 16 up to D", who);
@@ -378,8 +391,8 @@ void plan(const lbfq_qk_norm_params* p, Args& a) {
   int64_t per = (4096 + tokens - 1) / tokens;
   per = per < a.groups ? per : a.groups;
   a.stretch = static_cast<int>((a.groups + per - 1) / per);
-  a.per_token = (a.groups + a.stretch - 1) / a.stretch;
-  a.units = tokens * a.per_token;
+  a.per_token = static_cast<uint32_t>((a.groups + a.stretch - 1) / a.stretch);
+  a.units = static_cast<uint32_t>(tokens * a.per_token);
 }
 
 // Workgroups of a launch, at most.  Forward: a wave per token up to 32768 of them (us for 32760 tokens x 24 heads x 128
@@ -409,7 +422,7 @@ extern "C" int lbfq_qk_norm_rope(const lbfq_qk_norm_params* p, lbfq_stream_t str
   LBFQ_CHECK_ARG(p->q_out && p->k_out, "lbfq_qk_norm_rope: missing output");
   Args a{};
   plan(p, a);
-  const int64_t wgs = (a.units + 3) / 4;
+  const int64_t wgs = (static_cast<int64_t>(a.units) + 3) / 4;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(wgs < kForwardGroups ? wgs : kForwardGroups));
   LBFQ_QKN_DT(qk_norm_kernel, grid, a);
@@ -421,7 +434,7 @@ extern "C" int64_t lbfq_qk_norm_rope_bwd_rows(const lbfq_qk_norm_params* p) {
   if (!p || p->B <= 0 || p->S <= 0 || p->Hq <= 0 || p->Hk <= 0) return 0;
   Args a{};
   plan(p, a);
-  const int64_t wgs = (a.units + 3) / 4;
+  const int64_t wgs = (static_cast<int64_t>(a.units) + 3) / 4;
   return wgs < kGradGroups ? wgs : kGradGroups;
 }
 
