@@ -49,7 +49,7 @@ UNITS = {
     "lbfq_sdpa.hip": ["-ffp-contract=off"],
     "lbfq_qknorm.hip": ["-ffp-contract=off"],
     "lbfq_kvcache.hip": ["-ffp-contract=off"],
-    "lbfq_paged.hip": ["-ffp-contract=off", "-fno-honor-nans"],
+    "lbfq_paged.hip": ["-ffp-contract=off"],
 }
 
 

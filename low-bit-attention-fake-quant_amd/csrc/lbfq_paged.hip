@@ -117,11 +117,15 @@ __device__ void fill_rest(const lbfq_paged_params& p, int64_t wg, int64_t wgs) {
   }
 }
 
+// The larger, NaN if either is: v_maximum3_f32, three operands an instruction, where fmaxf would first quiet each
+// MFMA result with an instruction of its own
+__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // v of the lanes 16 and 32 away (v_permlane16_swap / v_permlane32_swap of v with
 // itself leave it and the partner's value in the two results)
 __device__ __forceinline__ float max_x32(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  return vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float add_x32(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -129,7 +133,7 @@ __device__ __forceinline__ float add_x32(float v) {
 }
 __device__ __forceinline__ float max_x16(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  return vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float add_x16(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -186,9 +190,13 @@ __device__ __forceinline__ v16f mfma32_f16(const uint4& a, const uint4& b, const
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// lse of a row (natural logarithm) from its maximum in log2 units and its sum
+// Whether a row's sum has anything in it (a NaN has: a row whose query holds one comes out as NaN, not as empty)
+__device__ __forceinline__ bool filled(float l) { return l != 0.0f; }
+
+
+// lse of a row (natural logarithm) from what its sum is relative to, in log2 units, and the sum
 __device__ __forceinline__ float row_lse(float m, float l) {
-  return l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  return filled(l) ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
 
 // ---- decode ------------------------------------------------------------------
@@ -358,11 +366,11 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
             }
           }
       }
-      float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                       fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+      float mx = vmax(vmax(vmax(sc[0][0], sc[0][1]), vmax(sc[0][2], sc[0][3])),
+                       vmax(vmax(sc[1][0], sc[1][1]), vmax(sc[1][2], sc[1][3])));
       mx = max_x32(max_x16(mx)) * a.sml2;
       if (__any(mx > m)) {
-        const float mn = fmaxf(m, mx);
+        const float mn = vmax(m, mx);
         const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         l *= al;
@@ -421,7 +429,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
     __syncthreads();
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, m_s[w][n]);
+    for (int w = 0; w < NW; ++w) M = vmax(M, m_s[w][n]);
     const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -434,10 +442,10 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
       const int row = threadIdx.x >> 4, part = threadIdx.x & 15;
       float MM = -INFINITY, L = 0.0f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) MM = fmaxf(MM, m_s[w][row]);
+      for (int w = 0; w < NW; ++w) MM = vmax(MM, m_s[w][row]);
 #pragma unroll
       for (int w = 0; w < NW; ++w)
-        L += m_s[w][row] == -INFINITY ? 0.0f : l_s[w][row] * __builtin_amdgcn_exp2f(m_s[w][row] - MM);
+        L += filled(l_s[w][row]) ? l_s[w][row] * __builtin_amdgcn_exp2f(m_s[w][row] - MM) : 0.0f;
       if (r0 + row < rows) {
         float o[NB];
 #pragma unroll
@@ -453,7 +461,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
         const int qq = (r0 + row) / G, hh = kvh * G + (r0 + row - qq * G);
         const int64_t tok = s.start + qq;
         if (a.splits == 1) {
-          const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+          const float inv = filled(L) ? 1.0f / L : 0.0f;
           uint32_t w[NB / 2];
 #pragma unroll
           for (int k = 0; k < NB / 2; ++k) w[k] = pack_dt<DT>(o[2 * k] * inv, o[2 * k + 1] * inv);
@@ -465,7 +473,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
         } else {
           const int64_t at = split * R + tok * p.Hq + hh;
           if (part == 0) a.ml[at] = make_float2(MM, L);
-          if (L > 0.0f) {
+          if (filled(L)) {
 #pragma unroll
             for (int k = 0; k < NB; k += 4)
               *reinterpret_cast<float4*>(a.acc + at * D + part * NB + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
@@ -819,8 +827,8 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
           }
         }
       };
-      // The tile's scores masked where a row does not see the key, the row's maximum brought up to date (and with it the
-      // sums so far); returns the maximum in use.
+      // The tile's scores masked where a row does not see the key, the row's reference m brought up to date (and with it
+      // the sums so far); returns what p is relative to.
       auto settle = [&](int kb, uint32_t here, v16f& s0, v16f& s1) -> float {
         if (!(kb >= lo_all && kb + 64 <= hi_all && here == 0xfu)) {
 #pragma unroll
@@ -832,11 +840,12 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(s0[r], s1[r]));
+        for (int r = 0; r < 16; ++r) mx = vmax(mx, vmax(s0[r], s1[r]));
         mx = max_x32(mx) * c;
-        // p may grow to 2^8 past the maximum in use before that is moved (fp16 holds 65504)
-        if (__any(mx > m + 8.0f)) {
-          const float mn = fmaxf(m, mx);
+        // m is 7 below a maximum seen: p may grow to 2^15 before m is moved (fp16 holds 65504), and is a normal fp16 number,
+        // with all its 11 bits, down to 2^-21 of the row's largest.
+        if (__any(mx > m + 15.0f)) {
+          const float mn = vmax(m, mx - 7.0f);
           const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
           m = mn;
           l *= al;
@@ -1038,11 +1047,11 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
     if (rw + li < rows) {
       const int64_t tok = s.start + qi;
       const bool one = a.splits == 1;
-      const float f = one ? (l > 0.0f ? back / l : 0.0f) : back;
+      const float f = one ? (filled(l) ? back / l : 0.0f) : back;
       const int64_t at = split * R + tok * p.Hq + h;
       if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
       if (!one && g == 0) a.ml[at] = make_float2(m, l);
-      if (one || l > 0.0f) {
+      if (one || filled(l)) {
         // Register r of acc[db] is V^T row 32 db + 8 (r / 4) + 4 g + r % 4 = c D/4 + dq, column 4 dq + c: for piece i
         // the columns 32 i + 16 g + 4 k + c.  D = 128: c = db, r = 4 i + k; D = 64: c = 2 db + r / 8, r % 8 = 4 i + k.
 #pragma unroll
@@ -1076,7 +1085,7 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
 
 // The largest / the sum over the wave, in every lane
 __device__ __forceinline__ float wave_max(float v) {
-#define LBFQ_ROR(c) v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), c, 0xf, 0xf, true)))
+#define LBFQ_ROR(c) v = vmax(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), c, 0xf, 0xf, true)))
   LBFQ_ROR(0x128);  // row_ror:8, 4, 2, 1
   LBFQ_ROR(0x124);
   LBFQ_ROR(0x122);
@@ -1121,7 +1130,7 @@ __global__ void __launch_bounds__(64) paged_combine_kernel(const Args a) {
   };
   load(0);
   const bool mine = tok >= p.query_starts[0] && tok < p.query_starts[p.B];
-  const bool some = mine && x.y > 0.0f;  // else nothing in this part, and its outputs were not written
+  const bool some = mine && filled(x.y);  // else nothing in this part, and its outputs were not written
   const float M = wave_max(some ? x.x : -INFINITY);
   const float f = some ? __builtin_amdgcn_exp2f(x.x - M) : 0.0f;
   const float l = wave_add(some ? x.y * f : 0.0f);
@@ -1134,10 +1143,10 @@ __global__ void __launch_bounds__(64) paged_combine_kernel(const Args a) {
     for (int i = 0; i < U; ++i) {
       const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + i));
 #pragma unroll
-      for (int k = 0; k < DL; ++k) o[k] = w > 0.0f ? fmaf(y[i][k], w, o[k]) : o[k];  // (no lane past the parts has one)
+      for (int k = 0; k < DL; ++k) o[k] = filled(w) ? fmaf(y[i][k], w, o[k]) : o[k];  // (no lane past the parts has one)
     }
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const float inv = filled(l) ? 1.0f / l : 0.0f;
   if (mine || p.fill_rest) {
     uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + lane * DL;
     if constexpr (D == 128) *reinterpret_cast<uint32_t*>(dst) = pack_dt<DT>(o[0] * inv, o[1] * inv);
@@ -1211,7 +1220,8 @@ int check(const lbfq_paged_params* p) {
                    reinterpret_cast<uint64_t>(p->k_scale) | reinterpret_cast<uint64_t>(p->v_scale)) & 15) == 0 &&
                      ((p->q_t | p->q_h | p->out_t | p->out_h) & 7) == 0,
                  "%s: rows must be 16-byte aligned", who);
-  LBFQ_CHECK_ARG(p->sm_scale > 0.0f && p->sm_scale < INFINITY, "%s: sm_scale must be positive and finite", who);
+  // (beyond, a scale of K times sm_scale could leave fp32's range)
+  LBFQ_CHECK_ARG(p->sm_scale >= 0x1p-64f && p->sm_scale <= 0x1p15f, "%s: sm_scale must lie in 2^-64 .. 2^15", who);
   LBFQ_CHECK_ARG(p->window >= 0 && p->window <= (int64_t{1} << 30), "%s: bad window", who);
   return 0;
 }

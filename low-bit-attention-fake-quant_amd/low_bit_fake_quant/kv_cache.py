@@ -207,15 +207,15 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Ten
     nothing gives zeros.
 
     ``max_query_len``: the most new tokens of a sequence, if known; it sizes the
-    launch, and results do not depend on it.  ``sm_scale``: 1/sqrt(D) by default.
+    launch, and results do not depend on it.  ``sm_scale``: 1/sqrt(D) by default, in 2^-64 ... 2^15.
     ``out``: takes the result, rows of no sequence left as they are (in a new tensor
     they are zero); it may not overlap the inputs.  ``return_lse``: also the natural
     log of each row's sum of exponentials, fp32 (T, Hq), -inf for a row that sees
     nothing.
 
     Scores, softmax and sums are fp32 on exact products of cached values and
-    queries; P is rounded to at least 11 bits for the second product, the result
-    once.
+    queries; P is rounded for the second product, to 11 bits or more down to 2^-21
+    of the row's largest, and the result once.  A NaN in a query makes its row NaN.
     """
     n, hk, page, d, index = _check_cache(cache)
     shape = q.shape
@@ -235,8 +235,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Ten
     _check_index(seq_lens, "seq_lens", b, index, torch.int32)
     _check_index(query_starts, "query_starts", b + 1, index, torch.int32)
     sm_scale = 1.0 / math.sqrt(d) if sm_scale is None else float(sm_scale)
-    if not 0.0 < sm_scale < math.inf:
-        raise ValueError(f"sm_scale must be positive and finite; got {sm_scale}")
+    if not 2.0 ** -64 <= sm_scale <= 2.0 ** 15:
+        raise ValueError(f"sm_scale must lie in 2^-64 ... 2^15; got {sm_scale}")
     if window is not None and window <= 0:
         raise ValueError(f"window must be positive; got {window}")
     if max_query_len is not None and max_query_len < 0:

@@ -172,6 +172,36 @@ def test_huge_and_not_finite_keys_and_values_in_masked_places(gpu, bad, n, dtype
     ref.check(out[before], want[before], tol[before], "without")
 
 
+@pytest.mark.parametrize("n,L", [(1, 20), (1, 5000), (40, 100), (40, 5000)])
+def test_a_nan_in_a_query_stays_in_its_row(gpu, n, L):
+    q, cache, table, lens, starts = problem(gpu, lens=[L, L], counts=[n, n], garbage=False)
+    q[n - 1, 1, 7] = math.nan
+    q[n, 2, 100] = math.inf  # its scores are +-inf: NaN, or 0 where all are -inf, as for a row that sees nothing
+    from low_bit_fake_quant import paged_attention
+    out, lse = paged_attention(q, cache, table, lens, starts, max_query_len=n, return_lse=True)
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device=gpu)
+    bad[n - 1, 1] = bad[n, 2] = True
+    assert torch.isnan(out[n - 1, 1]).all() and torch.isnan(lse[n - 1, 1])
+    want, wlse, tol, ltol = ref.attend(torch.nan_to_num(q, 0, 0, 0), cache, table, lens, starts)
+    ref.check(out[~bad], want[~bad], tol[~bad], "others")
+    ref.check(lse[~bad], wlse[~bad], ltol[~bad], "others lse")
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_few_large_and_many_small_weights(gpu, n):
+    """One key holds half the weight, thousands share the rest, each 2^-12 and less of it."""
+    from low_bit_fake_quant import write_kv_cache
+    q, cache, table, lens, starts = problem(gpu, lens=[6000], counts=[n], garbage=False, qscale=1.0)
+    k = torch.zeros(6000, 2, 128)
+    k[0] = q[:, ::2].mean(0).sign().cpu().float()
+    q.copy_(k[0].repeat_interleave(2, 0).to(q.dtype)[None] * (12.5 / math.sqrt(128) * 0.8))
+    g = torch.Generator().manual_seed(1)
+    v = torch.randn(6000, 2, 128, generator=g)
+    at = torch.arange(6000)
+    write_kv_cache(k.to(gpu), v.to(gpu), cache, (table.cpu().long()[0, at // 16] * 16 + at % 16).to(gpu))
+    run_and_check((q, cache, table, lens, starts), "one and many", hint=n)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("n", [1, 40])
@@ -325,7 +355,7 @@ def test_refusals(gpu):
             (dict(table=table.long()), TypeError, "int32"), (dict(table=table[:, :0]), ValueError, "no columns"),
             (dict(lens=lens.long()), TypeError, "seq_lens must be"), (dict(starts=starts[:1]), ValueError, "query_starts"),
             (dict(sm_scale=0.0), ValueError, "sm_scale"), (dict(sm_scale=-1.0), ValueError, "sm_scale"),
-            (dict(sm_scale=math.nan), ValueError, "sm_scale"), (dict(window=0), ValueError, "window"),
+            (dict(sm_scale=math.nan), ValueError, "sm_scale"), (dict(sm_scale=2.0 ** 16), ValueError, "sm_scale"), (dict(window=0), ValueError, "window"),
             (dict(max_query_len=-1), ValueError, "max_query_len"), (dict(out=q[:1].clone()), ValueError, "out must be"),
             (dict(out=q[:1].expand(2, -1, -1)), ValueError, "out must have"),
             (dict(q=q.clone().requires_grad_()), ValueError, "no backward pass")):
