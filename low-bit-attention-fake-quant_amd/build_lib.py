@@ -6,7 +6,8 @@ Python package that loads it).  The prepass / k-means translation units are
 compiled with ``-ffp-contract=off`` so their arithmetic is exactly the
 documented op sequence (the CPU oracle reproduces it bit for bit); the
 attention units allow contraction and are built with -fno-honor-nans.  Packed-FP32 instructions are disabled
-for all device code.
+for all device code.  ``csrc/lbfq_torch.cpp``, host code in front of the C ABI, becomes the
+Python module ``low_bit_fake_quant/_lbfq_torch.so``.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "low_bit_fake_quant", "liblbfq_hip.so")
+TORCH_OUT = os.path.join(HERE, "low_bit_fake_quant", "_lbfq_torch.so")
 BUILD = os.path.join(HERE, "_build")
 ARCH = os.environ.get("LBFQ_ARCH", "gfx950")
 
@@ -100,10 +102,41 @@ def device_asm(obj: str) -> str:
     return os.path.join(os.path.dirname(obj), f"{base}-hip-amdgcn-amd-amdhsa-{ARCH}.s")
 
 
+def _compile_torch() -> str:
+    """Object of the torch-side host code (csrc/lbfq_torch.cpp; no device code)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    obj = os.path.join(BUILD, "lbfq_torch_host.obj")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + sysconfig.get_paths()["include"], *("-isystem" + i for i in cpp_extension.include_paths()),
+           "-c", os.path.join(CSRC, "lbfq_torch.cpp"), "-o", obj]
+    r = subprocess.run(cmd, capture_output=True, text=True, cwd=BUILD)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for lbfq_torch.cpp:\n{' '.join(cmd)}\n{r.stderr}")
+    return obj
+
+
+def _link_torch(obj: str) -> None:
+    """_lbfq_torch.so, next to the library it calls (found through $ORIGIN)."""
+    from torch.utils import cpp_extension
+    tmp = TORCH_OUT + ".tmp"
+    cmd = ["g++", "-shared", obj, "-o", tmp, "-L" + os.path.dirname(OUT), "-l:" + os.path.basename(OUT),
+           "-Wl,-rpath,$ORIGIN", "-L" + cpp_extension.TORCH_LIB_PATH, "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True, cwd=BUILD)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{r.stderr}")
+    os.replace(tmp, TORCH_OUT)
+
+
 def build(verbose: bool = True) -> str:
     os.makedirs(BUILD, exist_ok=True)
-    with cf.ThreadPoolExecutor(max_workers=min(len(UNITS), os.cpu_count() or 8)) as ex:
+    with cf.ThreadPoolExecutor(max_workers=min(len(UNITS) + 1, os.cpu_count() or 8)) as ex:
+        host = ex.submit(_compile_torch)
         objs = list(ex.map(lambda kv: _compile(*kv), UNITS.items()))
+        host = host.result()
     _check_mfma(objs)
     tmp = OUT + ".tmp"
     cmd = ["hipcc", f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
@@ -111,8 +144,9 @@ def build(verbose: bool = True) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{r.stderr}")
     os.replace(tmp, OUT)
+    _link_torch(host)
     if verbose:
-        print(f"built {OUT}", file=sys.stderr)
+        print(f"built {OUT} and {os.path.basename(TORCH_OUT)}", file=sys.stderr)
     return OUT
 
 

@@ -1108,12 +1108,14 @@ __device__ __forceinline__ float wave_add(float v) {
 // latency at a few rows: the first sixteen parts are on their way before the
 // weights are known.
 template <int DT, int D>
-__global__ void __launch_bounds__(64) paged_combine_kernel(const Args a) {
+__global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
   constexpr int U = 16, DL = D / 64;
   const lbfq_paged_params& p = a.p;
-  const uint32_t row = blockIdx.x, Hq = static_cast<uint32_t>(p.Hq);
+  const uint32_t row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t Hq = static_cast<uint32_t>(p.Hq);
   const int64_t R = p.T * p.Hq;
-  const int lane = threadIdx.x;
+  if (row >= R) return;
+  const int lane = threadIdx.x & 63;
   const int tok = static_cast<int>(row / Hq);
   const int h = static_cast<int>(row - tok * Hq);
   float2 x = make_float2(-INFINITY, 0.0f);
@@ -1122,11 +1124,11 @@ __global__ void __launch_bounds__(64) paged_combine_kernel(const Args a) {
   float y[U][DL];
   auto load = [&](int s0) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int s = s0 + i < a.splits ? s0 + i : a.splits - 1;
+    for (int i = 0; i < U; ++i)
+      if (s0 + i < a.splits) {
 #pragma unroll
-      for (int k = 0; k < DL; ++k) y[i][k] = src[s * R * D + k];
-    }
+        for (int k = 0; k < DL; ++k) y[i][k] = src[(s0 + i) * R * D + k];
+      }
   };
   load(0);
   const bool mine = tok >= p.query_starts[0] && tok < p.query_starts[p.B];
@@ -1140,11 +1142,12 @@ __global__ void __launch_bounds__(64) paged_combine_kernel(const Args a) {
   for (int s0 = 0; s0 < a.splits; s0 += U) {
     if (s0) load(s0);
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + i));
+    for (int i = 0; i < U; ++i)
+      if (s0 + i < a.splits) {
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + i));
 #pragma unroll
-      for (int k = 0; k < DL; ++k) o[k] = filled(w) ? fmaf(y[i][k], w, o[k]) : o[k];  // (no lane past the parts has one)
-    }
+        for (int k = 0; k < DL; ++k) o[k] = filled(w) ? fmaf(y[i][k], w, o[k]) : o[k];
+      }
   }
   const float inv = filled(l) ? 1.0f / l : 0.0f;
   if (mine || p.fill_rest) {
@@ -1276,7 +1279,7 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   }
   LBFQ_LAUNCH_CHECK("lbfq_paged_attention");
   if (x.splits > 1) {
-    const dim3 gc(static_cast<unsigned>(R)), block(64);
+    const dim3 gc(static_cast<unsigned>((R + 3) / 4)), block(256);
     if (bf && d128) hipLaunchKernelGGL((paged_combine_kernel<kBF16, 128>), gc, block, 0, st, a);
     else if (bf) hipLaunchKernelGGL((paged_combine_kernel<kBF16, 64>), gc, block, 0, st, a);
     else if (d128) hipLaunchKernelGGL((paged_combine_kernel<kF16, 128>), gc, block, 0, st, a);

@@ -338,20 +338,21 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(const GradArgs ga) {
   }
 }
 
-// The rows of `partial` added up in 64 bits: 64 columns by 16 slices a workgroup.
+// The rows of `partial` added up in 64 bits: 16 columns by 64 slices a workgroup
+// (1024 rows: 4.1 us; 64 columns by 16 slices, 4 workgroups: 5.4).
 __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* partial, int rows, int D, void* dwq, int dtq,
                                                           void* dwk, int dtk) {
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+  const int c = threadIdx.x & 15, slice = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
   double s = 0.0;
 #pragma unroll 8
-  for (int r = slice; r < rows; r += 16) s += partial[static_cast<int64_t>(r) * 2 * D + col];
-  __shared__ double red[16][64];
-  red[slice][threadIdx.x & 63] = s;
+  for (int r = slice; r < rows; r += 64) s += partial[static_cast<int64_t>(r) * 2 * D + col];
+  __shared__ double red[64][16];
+  red[slice][c] = s;
   __syncthreads();
   if (slice) return;
   s = 0.0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) s += red[i][threadIdx.x];
+#pragma unroll 8
+  for (int i = 0; i < 64; ++i) s += red[i][c];
   if (col < D) {
     if (dwq) store_from_f32(dwq, col, dtq, static_cast<float>(s));
   } else if (dwk) {
@@ -397,7 +398,7 @@ void plan(const lbfq_qk_norm_params* p, Args& a) {
 
 // Workgroups of a launch, at most.  Forward: a wave per token up to 32768 of them (us for 32760 tokens x 24 heads x 128
 // bf16, 1024 / 2048 / 4096 / 8192 workgroups: 89 / 92 / 84 / 80).  Backward: four per CU, whose weight sums the second
-// launch adds up (8002 tokens x 40 heads, 512 / 1024 / 2048: 65 + 4, 47 + 5, 48 + 10 us).
+// launch adds up (8002 tokens x 40 heads, 512 / 1024 / 2048: 65 + 4, 47 + 4, 48 + 10 us).
 constexpr int64_t kForwardGroups = 8192, kGradGroups = 1024;
 
 }  // namespace
@@ -457,7 +458,7 @@ extern "C" int lbfq_qk_norm_rope_bwd(const lbfq_qk_norm_params* p, const lbfq_qk
   LBFQ_QKN_DT(qk_norm_bwd_kernel, grid, ga);
   LBFQ_LAUNCH_CHECK("lbfq_qk_norm_rope_bwd");
   if (ga.g.partial) {
-    hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(static_cast<unsigned>(2 * p->D / 64)), dim3(1024), 0, st, g->partial,
+    hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(static_cast<unsigned>(2 * p->D / 16)), dim3(1024), 0, st, g->partial,
                        rows, static_cast<int>(p->D), g->dq_weight, p->q_weight_dtype, g->dk_weight, p->k_weight_dtype);
     LBFQ_LAUNCH_CHECK("lbfq_qk_norm_rope_bwd (weights)");
   }

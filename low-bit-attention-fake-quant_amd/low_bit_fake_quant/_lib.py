@@ -264,7 +264,6 @@ _SIGS = {
 EXPORTED = tuple(_SIGS)
 
 _lib = None
-_gpu_seen = False  # asking torch again costs 0.5 us a call
 
 
 class HipLibraryError(RuntimeError):
@@ -273,11 +272,9 @@ class HipLibraryError(RuntimeError):
 
 def load(require_gpu: bool = True):
     """Load the library (cached).  Raises if it is absent or no GPU is visible."""
-    global _lib, _gpu_seen
-    if require_gpu and not _gpu_seen:
-        if not torch.cuda.is_available():
-            raise HipLibraryError("low_bit_fake_quant needs a ROCm GPU: torch.cuda.is_available() is False")
-        _gpu_seen = True
+    global _lib
+    if require_gpu and not torch.cuda.is_available():
+        raise HipLibraryError("low_bit_fake_quant needs a ROCm GPU: torch.cuda.is_available() is False")
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise HipLibraryError(
@@ -289,6 +286,24 @@ def load(require_gpu: bool = True):
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+_torch_ops = None
+
+
+def torch_ops():
+    """The module ``_lbfq_torch`` (host code of the cache operators, ``csrc/lbfq_torch.cpp``)."""
+    global _torch_ops
+    if _torch_ops is None:
+        load(require_gpu=False)  # the library that it links to
+        try:
+            from . import _lbfq_torch
+        except ImportError as e:
+            raise HipLibraryError("low_bit_fake_quant._lbfq_torch is missing or does not load; build it with `python "
+                                  "low-bit-attention-fake-quant_amd/build_lib.py`") from e
+        _lbfq_torch.set_hooks(_raw_stream or (lambda i: torch.cuda.current_stream(i).cuda_stream), HipLibraryError)
+        _torch_ops = _lbfq_torch
+    return _torch_ops
 
 
 def check(rc: int, what: str) -> None:

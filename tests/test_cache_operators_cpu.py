@@ -110,6 +110,17 @@ def test_cache_entries_refuse(lib):
     assert lib.lbfq_paged_attention_workspace_bytes(None) == 0
 
 
+def test_a_missing_host_module_is_said_loudly(lib, monkeypatch):
+    import sys
+
+    from low_bit_fake_quant import _lib
+    monkeypatch.setattr(_lib, "_torch_ops", None)
+    monkeypatch.setitem(sys.modules, "low_bit_fake_quant._lbfq_torch", None)
+    monkeypatch.delattr(sys.modules["low_bit_fake_quant"], "_lbfq_torch", raising=False)
+    with pytest.raises(_lib.HipLibraryError, match="build it"):
+        _lib.torch_ops()
+
+
 def test_python_entries_refuse_cpu_tensors():
     from low_bit_fake_quant import empty_kv_cache, paged_attention, qk_norm_rope, read_kv_cache, rotary_table, write_kv_cache
     c = empty_kv_cache(2, 16, 1, 64, device="cpu")
