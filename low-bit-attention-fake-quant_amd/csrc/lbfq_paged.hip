@@ -1,4 +1,3 @@
-#include <type_traits>
 // Attention of new tokens over the quantised paged K/V cache (lbfq_kv_write):
 //
 //   O_i = sum_j p_ij V_j / sum_j p_ij,  p_ij = exp(sm_scale q_i . K_j - m_i)
@@ -32,6 +31,8 @@
 // far apart for that takes a slower loop with V in bf16 and P in two bf16 terms.  So P can be fp16: 11 bits, where
 // bf16's 8 would cost as much as the output's own rounding.  K is bf16 (exact) for bf16 queries, and for fp16 ones fp16
 // under the same rule.  4680 tokens over 32760 keys, 12 heads of 128, all seen: 1.16 ms, 812 TFLOP/s.
+#include <type_traits>
+
 #include "lbfq_common.h"
 #include "../../include/lbfq.h"
 
@@ -55,11 +56,12 @@ constexpr float kLn2 = 0.6931471805599453f;
 struct Args {
   lbfq_paged_params p;
   int G;          // query heads of a key head
-  int tiles;      // row tiles of a sequence that the grid has
   int splits;     // parts of the keys
   int least;      // key tiles of a part, at least
+  int slots;      // chunk: places for row tiles, over all sequences
+  uint32_t piece;   // chunk: neighbouring slots that go to one XCD
+  uint32_t combos;  // decode: sequences x key heads; chunk: key heads x parts
   int64_t main;   // workgroups that attend (the others fill)
-  uint32_t combos;  // sequences x key heads x parts
   float sml2;     // sm_scale * log2(e)
   float2* ml;     // (splits, T * Hq): maximum (log2 units) and sum of a part
   float* acc;     // (splits, T * Hq, D)
@@ -97,6 +99,28 @@ __device__ __forceinline__ Seq sequence(const lbfq_paged_params& p, int64_t b) {
   s.causal = p.causal != 0;
   s.window = static_cast<int>(p.window);
   return s;
+}
+
+// The chunk kernel's row tiles have 128 rows.  Sequence b has the slots from slot_of(b) up to slot_of(b + 1), one more
+// than its rows need at the most: where a tile belongs follows from query_starts alone, and hardly a workgroup comes
+// for nothing.
+constexpr int kChunkRows = 128;
+__device__ __forceinline__ int slot_of(const lbfq_paged_params& p, int G, int b) {
+  const int T = static_cast<int>(p.T), s0 = p.query_starts[b];
+  return (s0 < 0 ? 0 : s0 > T ? T : s0) * G / kChunkRows + b;
+}
+// The last sequence whose slots start at or before `slot`: 64 places looked at at a time.
+__device__ __forceinline__ int sequence_at(const lbfq_paged_params& p, int G, int slot) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  for (int n = static_cast<int>(p.B); n > 1;) {
+    const int step = (n + 63) / 64, i = lane * step;
+    const uint64_t before = __ballot(i < n && slot_of(p, G, lo + (i < n ? i : 0)) <= slot);
+    const int k = before ? 63 - __builtin_clzll(before) : 0;
+    lo += k * step;
+    n = step < n - k * step ? step : n - k * step;
+  }
+  return lo;
 }
 
 // Rows of the token dimension that no sequence has: zero (a new output), lse -inf.
@@ -270,20 +294,19 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
   __shared__ __align__(16) float acc_s[NW][16][D + 4];
   __shared__ float m_s[NW][16], l_s[NW][16];
   // 32-bit indices: the divisions of 64-bit ones were most of this kernel's code and a fifth of a small call's time
-  const uint32_t splits = static_cast<uint32_t>(a.splits), Hk = static_cast<uint32_t>(p.Hk);
-  const int split = static_cast<int>(blockIdx.x % splits);
-  uint32_t rest = blockIdx.x / splits;
-  const int kvh = static_cast<int>(rest % Hk);
-  rest /= Hk;
-  const int tile0 = static_cast<int>(rest % static_cast<uint32_t>(a.tiles));
-  const int b = static_cast<int>(rest / static_cast<uint32_t>(a.tiles));
+  // The parts come last: those behind a short sequence's end then leave the XCDs (workgroups go to them in turn) and their
+  // shader engines evenly loaded.
+  const uint32_t Hk = static_cast<uint32_t>(p.Hk);
+  const int split = static_cast<int>(blockIdx.x / a.combos);
+  const uint32_t rest = blockIdx.x % a.combos;
+  const int b = static_cast<int>(rest / Hk), kvh = static_cast<int>(rest % Hk);
   const Seq s = sequence(p, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int32_t* table = p.block_table + b * p.table_stride;
   const int64_t R = p.T * p.Hq;
   const int G = a.G, rows = s.n * G;  // below 2^30: the host checks T * Hq
-  for (int r0 = tile0 * 16; r0 < rows; r0 += a.tiles * 16) {
+  for (int r0 = 0; r0 < rows; r0 += 16) {  // once, but for more new tokens than max_query_len
     // this lane's query; rows past the last repeat it and are not stored
     const int rr = r0 + n < rows ? r0 + n : rows - 1;
     const int qi = rr / G, h = kvh * G + (rr - qi * G);
@@ -524,13 +547,13 @@ struct Unit {
 
 template <int DT, int D>
 __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
-  constexpr int NW = 4, QB = 32 * NW, NT = 64 * NW;
+  constexpr int NW = 4, QB = kChunkRows, NT = 64 * NW;
+  static_assert(QB == 32 * NW, "32 rows a wave");
   constexpr int NKS = D / 16, NDB = D / 32, CH = D / 32;
   constexpr int KC = 64 * D / NT;  // K codes of a thread
   constexpr int KT = D / KC;       // threads of a key's row
   constexpr int VK = KC / 4;       // V keys of a thread, four columns each
-  constexpr int WKEYS = 64 / NW;   // keys that a wave stages
-  static_assert(WKEYS == 16 || WKEYS == 8, "one page a wave");
+  constexpr int WKEYS = 64 / NW;   // keys that a wave stages: of one page
   using L = Lds<D>;
   const lbfq_paged_params& p = a.p;
   if (static_cast<int64_t>(blockIdx.x) >= a.main) {
@@ -538,18 +561,18 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
     return;
   }
   __shared__ __align__(16) uint8_t lds[2 * L::BUF];
-  // Workgroups go to the eight XCDs in turn.  Pieces of eight neighbouring row tiles are dealt to them whole, so that
+  // Workgroups go to the eight XCDs in turn.  Pieces of up to eight neighbouring row tiles are dealt to them whole, so that
   // those that read the same keys share an L2; the pieces of all heads and parts (`combos`) with the last rows first,
   // which take longest under a causal mask, and turned by one XCD from round to round, so that none has all of a kind.
-  const uint32_t round = blockIdx.x / 64, piece = round * 8 + (blockIdx.x + round) % 8, combos = a.combos;
-  const int tile0 = a.tiles - 1 - static_cast<int>(piece / combos * 8 + blockIdx.x / 8 % 8);
-  if (tile0 < 0) return;
-  uint32_t rest = piece % combos;
-  const int split = static_cast<int>(rest % static_cast<uint32_t>(a.splits));
-  rest /= static_cast<uint32_t>(a.splits);
-  const int Hk = static_cast<int>(p.Hk);
-  const int kvh = static_cast<int>(rest % static_cast<uint32_t>(Hk));
-  const int b = static_cast<int>(rest / static_cast<uint32_t>(Hk));
+  // (No slots in vain: where seven of eight workgroups had nothing to do, the others shared a quarter of the chip: an
+  // XCD's four shader engines take its workgroups in turn.  1024 keys, 512 heads of 128 rows: 203 us, dense 60.)
+  const uint32_t ps = a.piece, round = blockIdx.x / (8 * ps), piece = round * 8 + (blockIdx.x + round) % 8;
+  const int slot = a.slots - 1 - static_cast<int>(piece / a.combos * ps + blockIdx.x / 8 % ps);
+  if (slot < 0) return;
+  const uint32_t rest = piece % a.combos, splits = static_cast<uint32_t>(a.splits);
+  const int split = static_cast<int>(rest % splits), kvh = static_cast<int>(rest / splits);
+  const int G = a.G, Hk = static_cast<int>(p.Hk);
+  const int b = sequence_at(p, G, slot), r0 = (slot - slot_of(p, G, b)) * QB;
   const Seq s = sequence(p, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 31, g = lane >> 5;
@@ -557,8 +580,8 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
   const int cols = static_cast<int>(p.table_cols), num_pages = static_cast<int>(p.num_pages);
   const int shift = p.page_shift, pmask = (1 << p.page_shift) - 1;
   const int64_t R = p.T * p.Hq;
-  const int G = a.G;
   const int rows = s.n * G;  // below 2^30: the host checks T * Hq
+  if (r0 < 0 || r0 >= rows) return;
   // Staging: wave w takes keys WKEYS w .. of a tile, which lie in one page.
   const int kkey = lane / KT, kq = lane % KT;           // K: key kkey of the wave's, columns KC kq ..
   const int vkg = lane / (D / 4), vdq = lane % (D / 4);  // V: keys VK vkg .. of the wave's, columns 4 vdq ..
@@ -576,508 +599,465 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
     return (static_cast<int64_t>(page * Hk + kvh) << shift) + (key & pmask);
   };
 
-  for (int r0 = tile0 * QB; r0 < rows; r0 += a.tiles * QB) {
-    const int rw = r0 + wave * 32;
-    const int rr = rw + li < rows ? rw + li : rows - 1;
-    const int qi = rr / G, h = kvh * G + (rr - qi * G);
-    const int lo_r = s.lo(qi), hi_r = s.hi(qi);
-    const int first = r0 / G, last = ((r0 + QB < rows ? r0 + QB : rows) - 1) / G;
-    const int lo = s.lo(first), hi = s.hi(last);  // keys that some row of the workgroup sees
-    const int wf = __builtin_amdgcn_readfirstlane((rw < rows ? rw : rows - 1) / G);
-    const int wl = __builtin_amdgcn_readfirstlane((rw + 31 < rows ? rw + 31 : rows - 1) / G);
-    const int wlo = s.lo(wf), whi = rw < rows ? s.hi(wl) : 0;  // that some row of the wave sees
-    const int lo_all = s.lo(wl), hi_all = s.hi(wf);            // that every row of the wave sees
+  const int rw = r0 + wave * 32;
+  const int rr = rw + li < rows ? rw + li : rows - 1;
+  const int qi = rr / G, h = kvh * G + (rr - qi * G);
+  const int lo_r = s.lo(qi), hi_r = s.hi(qi);
+  const int first = r0 / G, last = ((r0 + QB < rows ? r0 + QB : rows) - 1) / G;
+  const int lo = s.lo(first), hi = s.hi(last);  // keys that some row of the workgroup sees
+  const int wf = __builtin_amdgcn_readfirstlane((rw < rows ? rw : rows - 1) / G);
+  const int wl = __builtin_amdgcn_readfirstlane((rw + 31 < rows ? rw + 31 : rows - 1) / G);
+  const int lo_all = s.lo(wl), hi_all = s.hi(wf);            // that every row of the wave sees
 
-    const int kt0 = lo / 64, nt = hi > lo ? (hi + 63) / 64 - kt0 : 0;
-    int per = (nt + a.splits - 1) / a.splits;
-    per = per > a.least ? per : a.least;
-    const int begin = kt0 + split * per;
-    const int end = begin + per < kt0 + nt ? begin + per : kt0 + nt;
+  const int kt0 = lo / 64, nt = hi > lo ? (hi + 63) / 64 - kt0 : 0;
+  int per = (nt + a.splits - 1) / a.splits;
+  per = per > a.least ? per : a.least;
+  const int begin = kt0 + split * per;
+  const int end = begin + per < kt0 + nt ? begin + per : kt0 + nt;
 
-    v16f acc[NDB];
+  v16f acc[NDB];
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
+  for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[db][r] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    Unit uv{134, false}, uk{134, false};
-    if (begin < end) {
-      // The span of the part's scales, over the keys that some row sees: four keys a thread and pass.
-      {
-        uint32_t sv = 0, sk = 0;
-        const int k1 = 64 * end < hi ? 64 * end : hi;
-        for (int key = 64 * begin + 4 * tid; key < k1; key += 4 * NT) {
-          if (key + 4 <= lo) continue;
-          const int idx = key >> shift;
-          const int page = idx < cols ? table[idx] : -1;
-          if (page < 0 || page >= num_pages) continue;
-          const int64_t row = row_of(page, key);
-          const bool whole = key >= lo && key + 4 <= k1;
+    for (int r = 0; r < 16; ++r) acc[db][r] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  Unit uv{134, false}, uk{134, false};
+  if (begin < end) {
+    uint4 q[NKS];
+    {
+      const uint16_t* qr = reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 8 * g;
 #pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            uint32_t x = reinterpret_cast<const uint32_t*>(p.v_scale + row * CH)[c];
-            uint32_t y = DT == kF16 ? reinterpret_cast<const uint32_t*>(p.k_scale + row * CH)[c] : 0u;
-            if (whole) {
-              sv = span_add<4>(sv, x);
-              if constexpr (DT == kF16) sk = span_add<4>(sk, y);
-            } else {
+      for (int k = 0; k < NKS; ++k) q[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
+    }
+    // Staging registers: codes and scales of a K tile and of a V tile.
+    struct KRegs {
+      uint32_t c[KC / 4], e;
+    } kx, ky;
+    uint32_t vc[VK], vse[VK * CH / 4];
+    auto load_k = [&](KRegs& x, int kt, int page) {
+      const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
+      const uint8_t* ks = p.k_codes + row * D;
+      const uint8_t* kss = p.k_scale + row * CH;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int ki = key + (4 * c + i) / CH;
-                if (ki < lo || ki >= k1) continue;
-                sv = span_add<1>(sv, x >> (8 * i));
-                if constexpr (DT == kF16) sk = span_add<1>(sk, y >> (8 * i));
-              }
+      for (int i = 0; i < KC / 16; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4*>(ks + koff + 16 * i);
+        x.c[4 * i] = w.x; x.c[4 * i + 1] = w.y; x.c[4 * i + 2] = w.z; x.c[4 * i + 3] = w.w;
+      }
+      x.e = kss[ksoff];
+    };
+    auto load_v = [&](int kt, int page) {
+      const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
+      const uint8_t* vs = p.v_codes + row * D;
+      const uint8_t* vss = p.v_scale + row * CH;
+#pragma unroll
+      for (int j = 0; j < VK; ++j) vc[j] = *reinterpret_cast<const uint32_t*>(vs + voff + j * D);
+      if constexpr (D == 128) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 w = reinterpret_cast<const uint4*>(vss + vsoff)[i];
+          vse[4 * i] = w.x; vse[4 * i + 1] = w.y; vse[4 * i + 2] = w.z; vse[4 * i + 3] = w.w;
+        }
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(vss + vsoff);
+        vse[0] = w.x; vse[1] = w.y;
+      }
+    };
+    auto page_at = [&](int kt) { return page_of(64 * kt + WKEYS * wave); };  // of the wave's keys: a scalar
+    auto upto = [&](int kt) { return kt < end ? kt : end - 1; };  // steps past the end repeat it, unused
+    // The first tiles are on their way while the scales are looked through.
+    const int page0 = page_at(begin), page1 = page_at(upto(begin + 1));
+    load_k(kx, begin, page0);
+    load_v(begin, page0);
+    load_k(ky, upto(begin + 1), page1);
+    // The span of the part's scales, over the keys that some row sees: four keys a thread and pass.
+    {
+      uint32_t sv = 0, sk = 0;
+      const int k1 = 64 * end < hi ? 64 * end : hi;
+      for (int key = 64 * begin + 4 * tid; key < k1; key += 4 * NT) {
+        if (key + 4 <= lo) continue;
+        const int idx = key >> shift;
+        const int page = idx < cols ? table[idx] : -1;
+        if (page < 0 || page >= num_pages) continue;
+        const int64_t row = row_of(page, key);
+        const bool whole = key >= lo && key + 4 <= k1;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          uint32_t x = reinterpret_cast<const uint32_t*>(p.v_scale + row * CH)[c];
+          uint32_t y = DT == kF16 ? reinterpret_cast<const uint32_t*>(p.k_scale + row * CH)[c] : 0u;
+          if (whole) {
+            sv = span_add<4>(sv, x);
+            if constexpr (DT == kF16) sk = span_add<4>(sk, y);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int ki = key + (4 * c + i) / CH;
+              if (ki < lo || ki >= k1) continue;
+              sv = span_add<1>(sv, x >> (8 * i));
+              if constexpr (DT == kF16) sk = span_add<1>(sk, y >> (8 * i));
             }
           }
         }
-        uint32_t* red = reinterpret_cast<uint32_t*>(lds);
-#pragma unroll
-        for (int i = 1; i < 64; i <<= 1) {
-          sv = span_join(sv, __shfl_xor(sv, i, 64));
-          if constexpr (DT == kF16) sk = span_join(sk, __shfl_xor(sk, i, 64));
-        }
-        if (lane == 0) {
-          red[wave] = sv;
-          red[NW + wave] = sk;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          sv = span_join(sv, red[w]);
-          sk = span_join(sk, red[NW + w]);
-        }
-        __syncthreads();
-        auto unit = [&](uint32_t x) {
-          x = __builtin_amdgcn_readfirstlane(x);
-          Unit u;
-          u.E = static_cast<int>(x & 0xffu);
-          u.wide = u.E - (255 - static_cast<int>(x >> 16)) > kSpan;
-          if (u.wide || x == 0) u.E = 134;
-          return u;
-        };
-        uv = unit(sv);
-        if constexpr (DT == kF16) uk = unit(sk);
       }
-      uint4 q[NKS];
-      {
-        const uint16_t* qr = reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 8 * g;
+      uint32_t* red = reinterpret_cast<uint32_t*>(lds);
 #pragma unroll
-        for (int k = 0; k < NKS; ++k) q[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
+      for (int i = 1; i < 64; i <<= 1) {
+        sv = span_join(sv, __shfl_xor(sv, i, 64));
+        if constexpr (DT == kF16) sk = span_join(sk, __shfl_xor(sk, i, 64));
       }
-      const float c = DT == kF16 ? ldexpf(a.sml2, uk.E - 134) : a.sml2;
-      const uint32_t kadd = static_cast<uint32_t>(134 - uk.E) << 23, vadd = static_cast<uint32_t>(134 - uv.E) << 23;
+      if (lane == 0) {
+        red[wave] = sv;
+        red[NW + wave] = sk;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        sv = span_join(sv, red[w]);
+        sk = span_join(sk, red[NW + w]);
+      }
+      __syncthreads();
+      auto unit = [&](uint32_t x) {
+        x = __builtin_amdgcn_readfirstlane(x);
+        Unit u;
+        u.E = static_cast<int>(x & 0xffu);
+        u.wide = u.E - (255 - static_cast<int>(x >> 16)) > kSpan;
+        if (u.wide || x == 0) u.E = 134;
+        return u;
+      };
+      uv = unit(sv);
+      if constexpr (DT == kF16) uk = unit(sk);
+    }
+    const float c = DT == kF16 ? ldexpf(a.sml2, uk.E - 134) : a.sml2;
+    const uint32_t kadd = static_cast<uint32_t>(134 - uk.E) << 23, vadd = static_cast<uint32_t>(134 - uv.E) << 23;
 
-      // Staging registers: codes and scales of a K tile and of a V tile.
-      uint32_t kc[KC / 4], kse, vc[VK], vse[VK * CH / 4];
-      auto load_k = [&](int kt, int page) {
-        const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
-        const uint8_t* ks = p.k_codes + row * D;
-        const uint8_t* kss = p.k_scale + row * CH;
+    // Keys that no row sees, or that are not there: nothing of them may reach a product.
+    auto clear_k = [&](KRegs& x, int kt, int page) {
+      const int key0 = 64 * kt + WKEYS * wave;
+      if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
+      if (page < 0 || key0 + kkey < lo || key0 + kkey >= hi) {
 #pragma unroll
-        for (int i = 0; i < KC / 16; ++i) {
-          const uint4 w = *reinterpret_cast<const uint4*>(ks + koff + 16 * i);
-          kc[4 * i] = w.x; kc[4 * i + 1] = w.y; kc[4 * i + 2] = w.z; kc[4 * i + 3] = w.w;
+        for (int i = 0; i < KC / 4; ++i) x.c[i] = 0;
+        x.e = static_cast<uint32_t>(uk.E);
+      }
+    };
+    auto clear_v = [&](int kt, int page) {
+      const int key0 = 64 * kt + WKEYS * wave;
+      if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
+      const uint32_t fill = static_cast<uint32_t>(uv.E) * 0x01010101u;
+#pragma unroll
+      for (int j = 0; j < VK; ++j)
+        if (const int key = key0 + VK * vkg + j; page < 0 || key < lo || key >= hi) {
+          vc[j] = 0;
+          if constexpr (CH == 4) vse[j] = fill;
+          else vse[j / 2] = (vse[j / 2] & (j & 1 ? 0x0000ffffu : 0xffff0000u)) | (fill & (j & 1 ? 0xffff0000u : 0xffffu));
         }
-        kse = kss[ksoff];
-      };
-      auto load_v = [&](int kt, int page) {
-        const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
-        const uint8_t* vs = p.v_codes + row * D;
-        const uint8_t* vss = p.v_scale + row * CH;
+    };
+    // Registers -> LDS, as fp16 in the part's unit or (WIDE, and K for bf16 queries) as bf16; in eight pieces each.
+    struct Staged {
+      uint32_t k[KC / 2], v[VK][2];
+    };
+    auto k_piece = [&](Staged& st, const KRegs& x, int k, uint8_t* buf, auto WIDE) {
+      if (k >= KC / 4) return;  // (D = 64 has four)
+      constexpr bool f16 = DT == kF16 && !WIDE;
+      const float sc = __uint_as_float((x.e << 23) + (f16 ? kadd : 0u));
+      st.k[2 * k] = f16 ? cvt_f16<false>(x.c[k], sc) : cvt_bf16<false>(x.c[k], sc);
+      st.k[2 * k + 1] = f16 ? cvt_f16<true>(x.c[k], sc) : cvt_bf16<true>(x.c[k], sc);
+      if (k & 1)
+        *reinterpret_cast<uint4*>(buf + (WKEYS * wave + kkey) * L::KP + 2 * KC * kq + 8 * (k - 1)) =
+            make_uint4(st.k[2 * k - 2], st.k[2 * k - 1], st.k[2 * k], st.k[2 * k + 1]);
+    };
+    auto v_piece = [&](Staged& st, int i, uint8_t* buf, auto WIDE) {
+      if (i < 4) {  // a quarter of the keys, then a column in each piece
 #pragma unroll
-        for (int j = 0; j < VK; ++j) vc[j] = *reinterpret_cast<const uint32_t*>(vs + voff + j * D);
-        if constexpr (VK * CH == 32) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint4 w = reinterpret_cast<const uint4*>(vss + vsoff)[i];
-            vse[4 * i] = w.x; vse[4 * i + 1] = w.y; vse[4 * i + 2] = w.z; vse[4 * i + 3] = w.w;
-          }
-        } else if constexpr (VK * CH == 16) {
-          const uint4 w = *reinterpret_cast<const uint4*>(vss + vsoff);
-          vse[0] = w.x; vse[1] = w.y; vse[2] = w.z; vse[3] = w.w;
-        } else if constexpr (VK * CH == 8) {
-          const uint2 w = *reinterpret_cast<const uint2*>(vss + vsoff);
-          vse[0] = w.x; vse[1] = w.y;
-        } else {
-          vse[0] = *reinterpret_cast<const uint32_t*>(vss + vsoff);
-        }
-      };
-      // Keys that no row sees, or that are not there: nothing of them may reach a product.
-      auto clear_k = [&](int kt, int page) {
-        const int key0 = 64 * kt + WKEYS * wave;
-        if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
-        if (page < 0 || key0 + kkey < lo || key0 + kkey >= hi) {
-#pragma unroll
-          for (int i = 0; i < KC / 4; ++i) kc[i] = 0;
-          kse = static_cast<uint32_t>(uk.E);
-        }
-      };
-      auto clear_v = [&](int kt, int page) {
-        const int key0 = 64 * kt + WKEYS * wave;
-        if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
-        const uint32_t fill = static_cast<uint32_t>(uv.E) * 0x01010101u;
-#pragma unroll
-        for (int j = 0; j < VK; ++j)
-          if (const int key = key0 + VK * vkg + j; page < 0 || key < lo || key >= hi) {
-            vc[j] = 0;
-            if constexpr (CH == 4) vse[j] = fill;
-            else vse[j / 2] = (vse[j / 2] & (j & 1 ? 0x0000ffffu : 0xffff0000u)) | (fill & (j & 1 ? 0xffff0000u : 0xffffu));
-          }
-      };
-      // registers -> LDS, as fp16 in the part's unit or (WIDE, and K for bf16 queries) as bf16
-      auto store_k = [&](uint8_t* buf, auto WIDE) {
-        constexpr bool f16 = DT == kF16 && !WIDE;
-        uint32_t o[KC / 2];
-        const float sc = __uint_as_float((kse << 23) + (f16 ? kadd : 0u));
-#pragma unroll
-        for (int k = 0; k < KC / 4; ++k) {
-          o[2 * k] = f16 ? cvt_f16<false>(kc[k], sc) : cvt_bf16<false>(kc[k], sc);
-          o[2 * k + 1] = f16 ? cvt_f16<true>(kc[k], sc) : cvt_bf16<true>(kc[k], sc);
-        }
-        uint4* dst = reinterpret_cast<uint4*>(buf + (WKEYS * wave + kkey) * L::KP + 2 * KC * kq);
-#pragma unroll
-        for (int k = 0; k < KC / 8; ++k) dst[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-      };
-      auto store_v = [&](uint8_t* buf, auto WIDE) {
-        uint32_t o[VK][2];
-#pragma unroll
-        for (int j = 0; j < VK; ++j) {
+        for (int j = i * (VK / 4); j < (i + 1) * (VK / 4); ++j) {
           uint32_t by;
           if constexpr (CH == 4) by = __builtin_amdgcn_ubfe(vse[j], 8 * (vdq / 8), 8);
           else by = __builtin_amdgcn_ubfe(vse[j / 2], 16 * (j & 1) + 8 * (vdq / 8), 8);
           const float sc = __uint_as_float((by << 23) + (WIDE ? 0u : vadd));
-          o[j][0] = WIDE ? cvt_bf16<false>(vc[j], sc) : cvt_f16<false>(vc[j], sc);
-          o[j][1] = WIDE ? cvt_bf16<true>(vc[j], sc) : cvt_f16<true>(vc[j], sc);
-        }
-        // column 4 dq + c is V^T row c D/4 + dq, so that neighbouring lanes write neighbouring rows
-#pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-          const uint32_t sel = cc & 1 ? 0x07060302u : 0x05040100u;
-          uint32_t w[VK / 2];
-#pragma unroll
-          for (int j = 0; j < VK / 2; ++j) w[j] = __builtin_amdgcn_perm(o[2 * j + 1][cc / 2], o[2 * j][cc / 2], sel);
-          uint8_t* dst = buf + L::KBYTES + (cc * (D / 4) + vdq) * L::VP + 2 * (WKEYS * wave + VK * vkg);
-          if constexpr (VK == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-          else if constexpr (VK == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-          else *reinterpret_cast<uint32_t*>(dst) = w[0];
-        }
-      };
-      // The same in eight pieces each, narrow
-      struct Staged {
-        uint32_t k[KC / 2], v[VK][2];
-      };
-      auto k_piece = [&](Staged& st, int i, uint8_t* buf) {
-        constexpr int W = KC >= 32 ? KC / 32 : 1;
-        const float sc = __uint_as_float((kse << 23) + (DT == kF16 ? kadd : 0u));
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const int k = i * W + e;
-          if (k >= KC / 4) continue;
-          st.k[2 * k] = DT == kF16 ? cvt_f16<false>(kc[k], sc) : cvt_bf16<false>(kc[k], sc);
-          st.k[2 * k + 1] = DT == kF16 ? cvt_f16<true>(kc[k], sc) : cvt_bf16<true>(kc[k], sc);
-          if (k & 1)
-            *reinterpret_cast<uint4*>(buf + (WKEYS * wave + kkey) * L::KP + 2 * KC * kq + 8 * (k - 1)) =
-                make_uint4(st.k[2 * k - 2], st.k[2 * k - 1], st.k[2 * k], st.k[2 * k + 1]);
-        }
-      };
-      auto v_piece = [&](Staged& st, int i, uint8_t* buf) {
-        constexpr int W = VK >= 4 ? VK / 4 : 1;  // keys in each of the first four pieces, then a column in each
-        if (i < 4) {
-#pragma unroll
-          for (int e = 0; e < W; ++e) {
-            const int j = i * W + e;
-            if (j >= VK) continue;
-            uint32_t by;
-            if constexpr (CH == 4) by = __builtin_amdgcn_ubfe(vse[j], 8 * (vdq / 8), 8);
-            else by = __builtin_amdgcn_ubfe(vse[j / 2], 16 * (j & 1) + 8 * (vdq / 8), 8);
-            const float sc = __uint_as_float((by << 23) + vadd);
-            st.v[j][0] = cvt_f16<false>(vc[j], sc);
-            st.v[j][1] = cvt_f16<true>(vc[j], sc);
-          }
-        } else {
-          const int cc = i - 4;
-          const uint32_t sel = cc & 1 ? 0x07060302u : 0x05040100u;
-          uint32_t w[VK / 2];
-#pragma unroll
-          for (int j = 0; j < VK / 2; ++j) w[j] = __builtin_amdgcn_perm(st.v[2 * j + 1][cc / 2], st.v[2 * j][cc / 2], sel);
-          uint8_t* dst = buf + L::KBYTES + (cc * (D / 4) + vdq) * L::VP + 2 * (WKEYS * wave + VK * vkg);
-          if constexpr (VK == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-          else if constexpr (VK == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-          else *reinterpret_cast<uint32_t*>(dst) = w[0];
-        }
-      };
-      // S^T of 32 keys: register r is key 32 bl + 16 (r / 8) + 8 g + r % 8 of the tile in buf
-      auto scores = [&](const uint8_t* buf, int bl, v16f& sc, auto WIDE) {
-        const uint8_t* kr = buf + (32 * bl + key_of(li)) * L::KP + 16 * g;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < NKS; ++k) {
-          const uint4 kop = *reinterpret_cast<const uint4*>(kr + 32 * k);
-          if constexpr (DT == kF16 && WIDE) {  // bf16 keys, the query's eleven bits in two bf16 terms
-            uint4 qh, ql;
-            split_f16(q[k], qh, ql);
-            sc = mfma32_bf16(kop, qh, sc);
-            sc = mfma32_bf16(kop, ql, sc);
-          } else if constexpr (DT == kBF16) {
-            sc = mfma32_bf16(kop, q[k], sc);
-          } else {
-            sc = mfma32_f16(kop, q[k], sc);
-          }
-        }
-      };
-      // The tile's scores masked where a row does not see the key, the row's reference m brought up to date (and with it
-      // the sums so far); returns what p is relative to.
-      auto settle = [&](int kb, uint32_t here, v16f& s0, v16f& s1) -> float {
-        if (!(kb >= lo_all && kb + 64 <= hi_all && here == 0xfu)) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = kb + 16 * (r >> 3) + 8 * g + (r & 7);
-            if (key < lo_r || key >= hi_r || !((here >> (r >> 3)) & 1u)) s0[r] = -INFINITY;
-            if (key + 32 < lo_r || key + 32 >= hi_r || !((here >> (2 + (r >> 3))) & 1u)) s1[r] = -INFINITY;
-          }
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = vmax(mx, vmax(s0[r], s1[r]));
-        mx = max_x32(mx) * c;
-        // m is 7 below a maximum seen: p may grow to 2^15 before m is moved (fp16 holds 65504), and is a normal fp16 number,
-        // with all its 11 bits, down to 2^-21 of the row's largest.
-        if (__any(mx > m + 15.0f)) {
-          const float mn = vmax(m, mx - 7.0f);
-          const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-          m = mn;
-          l *= al;
-#pragma unroll
-          for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[db][r] *= al;
-        }
-        return m == -INFINITY ? 0.0f : m;
-      };
-
-      // A mask bit for each group of 16 keys of the tile: its page is there.
-      auto pages_there = [&](int kt) {
-        bool ok = true;
-        if (lane < 4) {
-          const int idx = (64 * kt + 16 * lane) >> shift;
-          const int pg = idx < cols ? table[idx] : -1;
-          ok = pg >= 0 && pg < num_pages;
-        }
-        return static_cast<uint32_t>(__ballot(ok)) & 0xfu;
-      };
-
-      auto page_at = [&](int kt) { return page_of(64 * kt + WKEYS * wave); };  // of the wave's keys: a scalar
-      if (uv.wide || uk.wide) {
-        // Rare (see Unit), and plain: one tile after the other.
-        for (int kt = begin; kt < end; ++kt) {
-          const int page = page_at(kt);
-          load_k(kt, page);
-          load_v(kt, page);
-          clear_k(kt, page);
-          clear_v(kt, page);
-          if (uk.wide) store_k(lds, std::true_type{});
-          else store_k(lds, std::false_type{});
-          if (uv.wide) store_v(lds, std::true_type{});
-          else store_v(lds, std::false_type{});
-          __syncthreads();
-          v16f sc[2];
-#pragma unroll
-          for (int bl = 0; bl < 2; ++bl) {
-            if (uk.wide) scores(lds, bl, sc[bl], std::true_type{});
-            else scores(lds, bl, sc[bl], std::false_type{});
-          }
-          const float ms = settle(64 * kt, pages_there(kt), sc[0], sc[1]);
-#pragma unroll
-          for (int bl = 0; bl < 2; ++bl)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint8_t* vr = lds + L::KBYTES + li * L::VP + 16 * g + 32 * (2 * bl + j);
-              float x[8];
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                x[k] = __builtin_amdgcn_exp2f(fmaf(sc[bl][8 * j + k], c, -ms));
-                l += x[k];
-              }
-              uint32_t w[4], w2[4];
-              if (uv.wide) {  // V is bf16 as it is: P in two bf16 terms (16 bits)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  w[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
-                  w2[k] = pack_bf16(x[2 * k] - __uint_as_float(w[k] << 16),
-                                    x[2 * k + 1] - __uint_as_float(w[k] & 0xffff0000u));
-                }
-#pragma unroll
-                for (int db = 0; db < NDB; ++db) {
-                  const uint4 va = *reinterpret_cast<const uint4*>(vr + 32 * db * L::VP);
-                  acc[db] = mfma32_bf16(va, make_uint4(w[0], w[1], w[2], w[3]), acc[db]);
-                  acc[db] = mfma32_bf16(va, make_uint4(w2[0], w2[1], w2[2], w2[3]), acc[db]);
-                }
-              } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = pack_f16(x[2 * k], x[2 * k + 1]);
-#pragma unroll
-                for (int db = 0; db < NDB; ++db)
-                  acc[db] = mfma32_f16(*reinterpret_cast<const uint4*>(vr + 32 * db * L::VP),
-                                       make_uint4(w[0], w[1], w[2], w[3]), acc[db]);
-              }
-            }
-          __syncthreads();
+          st.v[j][0] = WIDE ? cvt_bf16<false>(vc[j], sc) : cvt_f16<false>(vc[j], sc);
+          st.v[j][1] = WIDE ? cvt_bf16<true>(vc[j], sc) : cvt_f16<true>(vc[j], sc);
         }
       } else {
-        constexpr std::false_type kNarrow{};
-        uint8_t* const buf0 = lds;
-        uint8_t* const buf1 = lds + L::BUF;
-        auto upto = [&](int kt) { return kt < end ? kt : end - 1; };  // steps past the end repeat it, unused
-        // The pages and masks of the tiles on the way: of V's registers, of K's, of the next K; of the scores' tile and
-        // the two after it.
-        int pv = page_at(begin), pk, pn;
-        load_k(begin, pv);
-        clear_k(begin, pv);
-        store_k(buf0, kNarrow);
-        pk = page_at(upto(begin + 1));
-        load_v(begin, pv);
-        load_k(upto(begin + 1), pk);
-        clear_v(begin, pv);
-        clear_k(upto(begin + 1), pk);
-        store_v(buf0, kNarrow);
-        store_k(buf1, kNarrow);
-        pv = pk;
-        pk = page_at(upto(begin + 2));
-        pn = page_at(upto(begin + 3));
-        load_v(upto(begin + 1), pv);
-        load_k(upto(begin + 2), pk);
-        uint32_t here0 = pages_there(begin), here1 = pages_there(upto(begin + 1)), here2 = pages_there(upto(begin + 2));
+        // column 4 dq + c is V^T row c D/4 + dq, so that neighbouring lanes write neighbouring rows
+        const int cc = i - 4;
+        const uint32_t sel = cc & 1 ? 0x07060302u : 0x05040100u;
+        uint32_t w[VK / 2];
+#pragma unroll
+        for (int j = 0; j < VK / 2; ++j) w[j] = __builtin_amdgcn_perm(st.v[2 * j + 1][cc / 2], st.v[2 * j][cc / 2], sel);
+        uint8_t* dst = buf + L::KBYTES + (cc * (D / 4) + vdq) * L::VP + 2 * (WKEYS * wave + VK * vkg);
+        if constexpr (VK == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+      }
+    };
+    auto store_k = [&](const KRegs& x, uint8_t* buf, auto WIDE) {
+      Staged st;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k_piece(st, x, i, buf, WIDE);
+    };
+    auto store_v = [&](uint8_t* buf, auto WIDE) {
+      Staged st;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v_piece(st, i, buf, WIDE);
+    };
+    // S^T of 32 keys: register r is key 32 bl + 16 (r / 8) + 8 g + r % 8 of the tile in buf
+    auto scores = [&](const uint8_t* buf, int bl, v16f& sc, auto WIDE) {
+      const uint8_t* kr = buf + (32 * bl + key_of(li)) * L::KP + 16 * g;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NKS; ++k) {
+        const uint4 kop = *reinterpret_cast<const uint4*>(kr + 32 * k);
+        if constexpr (DT == kF16 && WIDE) {  // bf16 keys, the query's eleven bits in two bf16 terms
+          uint4 qh, ql;
+          split_f16(q[k], qh, ql);
+          sc = mfma32_bf16(kop, qh, sc);
+          sc = mfma32_bf16(kop, ql, sc);
+        } else if constexpr (DT == kBF16) {
+          sc = mfma32_bf16(kop, q[k], sc);
+        } else {
+          sc = mfma32_f16(kop, q[k], sc);
+        }
+      }
+    };
+    // The tile's scores masked where a row does not see the key, the row's reference m brought up to date (and with it
+    // the sums so far); returns what p is relative to.
+    auto settle = [&](int kb, uint32_t here, v16f& s0, v16f& s1) -> float {
+      if (!(kb >= lo_all && kb + 64 <= hi_all && here == 0xfu)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = kb + 16 * (r >> 3) + 8 * g + (r & 7);
+          if (key < lo_r || key >= hi_r || !((here >> (r >> 3)) & 1u)) s0[r] = -INFINITY;
+          if (key + 32 < lo_r || key + 32 >= hi_r || !((here >> (2 + (r >> 3))) & 1u)) s1[r] = -INFINITY;
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = vmax(mx, vmax(s0[r], s1[r]));
+      mx = max_x32(mx) * c;
+      // m is 7 below a maximum seen: p may grow to 2^15 before m is moved (fp16 holds 65504), and is a normal fp16 number,
+      // with all its 11 bits, down to 2^-21 of the row's largest.
+      if (__any(mx > m + 15.0f)) {
+        const float mn = vmax(m, mx - 7.0f);
+        const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= al;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] *= al;
+      }
+      return m == -INFINITY ? 0.0f : m;
+    };
+
+    // A mask bit for each group of 16 keys of the tile: its page is there.
+    auto pages_there = [&](int kt) {
+      bool ok = true;
+      if (lane < 4) {
+        const int idx = (64 * kt + 16 * lane) >> shift;
+        const int pg = idx < cols ? table[idx] : -1;
+        ok = pg >= 0 && pg < num_pages;
+      }
+      return static_cast<uint32_t>(__ballot(ok)) & 0xfu;
+    };
+
+    if (uv.wide || uk.wide) {
+      // Rare (see Unit), and plain: one tile after the other.
+      for (int kt = begin; kt < end; ++kt) {
+        const int page = page_at(kt);
+        load_k(kx, kt, page);
+        load_v(kt, page);
+        clear_k(kx, kt, page);
+        clear_v(kt, page);
+        if (uk.wide) store_k(kx, lds, std::true_type{});
+        else store_k(kx, lds, std::false_type{});
+        if (uv.wide) store_v(lds, std::true_type{});
+        else store_v(lds, std::false_type{});
         __syncthreads();
-        v16f sa, sb, sc_;
-        scores(buf0, 0, sa, kNarrow);
-        scores(buf0, 1, sb, kNarrow);
-        __syncthreads();  // the first step puts another K tile there
-        // Tile kt: its scores are in s0 and s1; the next tile's go to s2 and, when s0 is used up, s0 (three blocks for what
-        // would be four).  In LDS: K of kt + 1 (nxt), V of kt (cur).  In the staging registers: K of kt + 2, V of kt + 1.
-        auto step = [&](int kt, uint8_t* cur, uint8_t* nxt, v16f& s0, v16f& s1, v16f& s2) {
-          // The step's products in order: of each half of the tile the next tile's scores (NKS products) and this one's
-          // two quarters of P V (NDB each).  Their LDS operands are read kAhead products ahead, and each product is
-          // followed by a piece of what the VALU has to do meanwhile: the softmax of the half beside the scores, the
-          // conversion of the staged K (first half) or V tile (second) beside P V.  The order is fixed here; left to the
-          // compiler, every read was next to its product.
-          constexpr int HALF = NKS + 2 * NDB, kAhead = 5;
-          uint4 ring[kAhead];
-          const uint8_t* const kr = nxt + key_of(li) * L::KP + 16 * g;
-          const uint8_t* const vr = cur + L::KBYTES + li * L::VP + 16 * g;
-          auto fetch = [&](int n) {
-            if (n >= 2 * HALF) return;
-            const int bl = n / HALF, i = n % HALF;
-            const uint8_t* src = i < NKS ? kr + 32 * bl * L::KP + 32 * i
-                                         : vr + 32 * ((i - NKS) % NDB) * L::VP + 32 * (2 * bl + (i - NKS) / NDB);
-            ring[n % kAhead] = *reinterpret_cast<const uint4*>(src);
-          };
+        v16f sc[2];
 #pragma unroll
-          for (int n = 0; n < kAhead; ++n) fetch(n);
-          const float ms = settle(64 * kt, here0, s0, s1);
-          clear_k(upto(kt + 2), pk);
-          clear_v(upto(kt + 1), pv);
-          Staged st;
+        for (int bl = 0; bl < 2; ++bl) {
+          if (uk.wide) scores(lds, bl, sc[bl], std::true_type{});
+          else scores(lds, bl, sc[bl], std::false_type{});
+        }
+        const float ms = settle(64 * kt, pages_there(kt), sc[0], sc[1]);
 #pragma unroll
-          for (int bl = 0; bl < 2; ++bl) {
-            uint32_t w[8];
-            v16f& sc = bl == 0 ? s0 : s1;
-            v16f& sn = bl == 0 ? s2 : s0;
+        for (int bl = 0; bl < 2; ++bl)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sn[r] = 0.0f;
+          for (int j = 0; j < 2; ++j) {
+            const uint8_t* vr = lds + L::KBYTES + li * L::VP + 16 * g + 32 * (2 * bl + j);
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < HALF; ++i) {
-              const int n = bl * HALF + i;
-              const uint4 x = ring[n % kAhead];
-              if (i < NKS) {
-                sn = DT == kBF16 ? mfma32_bf16(x, q[i], sn) : mfma32_f16(x, q[i], sn);
-                fetch(n + kAhead);
+            for (int k = 0; k < 8; ++k) {
+              x[k] = __builtin_amdgcn_exp2f(fmaf(sc[bl][8 * j + k], c, -ms));
+              l += x[k];
+            }
+            uint32_t w[4], w2[4];
+            if (uv.wide) {  // V is bf16 as it is: P in two bf16 terms (16 bits)
 #pragma unroll
-                for (int e = 0; e < 8 / NKS; ++e) {
-                  const int k = i * (8 / NKS) + e;
-                  const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k], c, -ms));
-                  const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k + 1], c, -ms));
-                  l += p0 + p1;
-                  w[k] = pack_f16(p0, p1);
-                }
-              } else {
-                const int j = (i - NKS) / NDB, db = (i - NKS) % NDB;
-                acc[db] = mfma32_f16(x, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]), acc[db]);
-                fetch(n + kAhead);
-#pragma unroll
-                for (int e = 0; e < 4 / NDB; ++e) {
-                  const int k = (i - NKS) * (4 / NDB) + e;  // 0 .. 7
-                  if (bl == 0) k_piece(st, k, cur);
-                  else v_piece(st, k, nxt);
-                }
+              for (int k = 0; k < 4; ++k) {
+                w[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+                w2[k] = pack_bf16(x[2 * k] - __uint_as_float(w[k] << 16),
+                                  x[2 * k + 1] - __uint_as_float(w[k] & 0xffff0000u));
               }
-              __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+              for (int db = 0; db < NDB; ++db) {
+                const uint4 va = *reinterpret_cast<const uint4*>(vr + 32 * db * L::VP);
+                acc[db] = mfma32_bf16(va, make_uint4(w[0], w[1], w[2], w[3]), acc[db]);
+                acc[db] = mfma32_bf16(va, make_uint4(w2[0], w2[1], w2[2], w2[3]), acc[db]);
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = pack_f16(x[2 * k], x[2 * k + 1]);
+#pragma unroll
+              for (int db = 0; db < NDB; ++db)
+                acc[db] = mfma32_f16(*reinterpret_cast<const uint4*>(vr + 32 * db * L::VP),
+                                     make_uint4(w[0], w[1], w[2], w[3]), acc[db]);
             }
           }
-          pv = pk;
-          pk = pn;
-          load_v(upto(kt + 2), pv);
-          load_k(upto(kt + 3), pk);
-          pn = page_at(upto(kt + 4));
-          here0 = here1;
-          here1 = here2;
-          here2 = pages_there(upto(kt + 3));
-          __syncthreads();
-        };
-        // (two LDS buffers and three blocks of scores: the order comes round after six steps)
-        for (int kt = begin; kt < end;) {
-          step(kt, buf0, buf1, sa, sb, sc_);
-          if (++kt >= end) break;
-          step(kt, buf1, buf0, sc_, sa, sb);
-          if (++kt >= end) break;
-          step(kt, buf0, buf1, sb, sc_, sa);
-          if (++kt >= end) break;
-          step(kt, buf1, buf0, sa, sb, sc_);
-          if (++kt >= end) break;
-          step(kt, buf0, buf1, sc_, sa, sb);
-          if (++kt >= end) break;
-          step(kt, buf1, buf0, sb, sc_, sa);
-          ++kt;
-        }
+        __syncthreads();
       }
-      l = add_x32(l);
-    }
-    const float back = ldexpf(1.0f, uv.E - 134);
-    if (rw + li < rows) {
-      const int64_t tok = s.start + qi;
-      const bool one = a.splits == 1;
-      const float f = one ? (filled(l) ? back / l : 0.0f) : back;
-      const int64_t at = split * R + tok * p.Hq + h;
-      if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
-      if (!one && g == 0) a.ml[at] = make_float2(m, l);
-      if (one || filled(l)) {
-        // Register r of acc[db] is V^T row 32 db + 8 (r / 4) + 4 g + r % 4 = c D/4 + dq, column 4 dq + c: for piece i
-        // the columns 32 i + 16 g + 4 k + c.  D = 128: c = db, r = 4 i + k; D = 64: c = 2 db + r / 8, r % 8 = 4 i + k.
+    } else {
+      constexpr std::false_type kNarrow{};
+      uint8_t* const buf0 = lds;
+      uint8_t* const buf1 = lds + L::BUF;
+      // The pages and masks of the tiles on the way: of V's registers, of K's, of the next K; of the scores' tile and
+      // the two after it.
+      int pv = page1, pk = page_at(upto(begin + 2)), pn = page_at(upto(begin + 3));
+      clear_k(kx, begin, page0);
+      clear_v(begin, page0);
+      clear_k(ky, upto(begin + 1), page1);
+      store_k(kx, buf0, kNarrow);
+      store_v(buf0, kNarrow);
+      store_k(ky, buf1, kNarrow);
+      load_v(upto(begin + 1), pv);
+      load_k(kx, upto(begin + 2), pk);
+      uint32_t here0 = pages_there(begin), here1 = pages_there(upto(begin + 1)), here2 = pages_there(upto(begin + 2));
+      __syncthreads();
+      v16f sa, sb, sc_;
+      scores(buf0, 0, sa, kNarrow);
+      scores(buf0, 1, sb, kNarrow);
+      __syncthreads();  // the first step puts another K tile there
+      // Tile kt: its scores are in s0 and s1; the next tile's go to s2 and, when s0 is used up, s0 (three blocks for what
+      // would be four).  In LDS: K of kt + 1 (nxt), V of kt (cur).  In the staging registers: K of kt + 2, V of kt + 1.
+      auto step = [&](int kt, uint8_t* cur, uint8_t* nxt, v16f& s0, v16f& s1, v16f& s2) {
+        // The step's products in order: of each half of the tile the next tile's scores (NKS products) and this one's
+        // two quarters of P V (NDB each).  Their LDS operands are read kAhead products ahead, and each product is
+        // followed by a piece of what the VALU has to do meanwhile: the softmax of the half beside the scores, the
+        // conversion of the staged K (first half) or V tile (second) beside P V.  The order is fixed here; left to the
+        // compiler, every read was next to its product.
+        constexpr int HALF = NKS + 2 * NDB, kAhead = 5;
+        uint4 ring[kAhead];
+        const uint8_t* const kr = nxt + key_of(li) * L::KP + 16 * g;
+        const uint8_t* const vr = cur + L::KBYTES + li * L::VP + 16 * g;
+        auto fetch = [&](int n) {
+          if (n >= 2 * HALF) return;
+          const int bl = n / HALF, i = n % HALF;
+          const uint8_t* src = i < NKS ? kr + 32 * bl * L::KP + 32 * i
+                                       : vr + 32 * ((i - NKS) % NDB) * L::VP + 32 * (2 * bl + (i - NKS) / NDB);
+          ring[n % kAhead] = *reinterpret_cast<const uint4*>(src);
+        };
 #pragma unroll
-        for (int i = 0; i < NDB; ++i) {
-          const int col = 32 * i + 16 * g;
-          float o[16];
+        for (int n = 0; n < kAhead; ++n) fetch(n);
+        const float ms = settle(64 * kt, here0, s0, s1);
+        clear_k(kx, upto(kt + 2), pk);
+        clear_v(upto(kt + 1), pv);
+        Staged st;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+        for (int bl = 0; bl < 2; ++bl) {
+          uint32_t w[8];
+          v16f& sc = bl == 0 ? s0 : s1;
+          v16f& sn = bl == 0 ? s2 : s0;
 #pragma unroll
-            for (int cc = 0; cc < 4; ++cc)
-              o[4 * k + cc] = (D == 128 ? acc[cc % NDB][4 * i + k] : acc[cc / 2][8 * (cc & 1) + 4 * (i & 1) + k]) * f;
-          if (one) {
-            uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col);
-            dst[0] = make_uint4(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]), pack_dt<DT>(o[4], o[5]),
-                                pack_dt<DT>(o[6], o[7]));
-            dst[1] = make_uint4(pack_dt<DT>(o[8], o[9]), pack_dt<DT>(o[10], o[11]), pack_dt<DT>(o[12], o[13]),
-                                pack_dt<DT>(o[14], o[15]));
-          } else {
-            float4* dst = reinterpret_cast<float4*>(a.acc + at * D + col);
+          for (int r = 0; r < 16; ++r) sn[r] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          for (int i = 0; i < HALF; ++i) {
+            const int n = bl * HALF + i;
+            const uint4 x = ring[n % kAhead];
+            if (i < NKS) {
+              sn = DT == kBF16 ? mfma32_bf16(x, q[i], sn) : mfma32_f16(x, q[i], sn);
+              fetch(n + kAhead);
+#pragma unroll
+              for (int e = 0; e < 8 / NKS; ++e) {
+                const int k = i * (8 / NKS) + e;
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k], c, -ms));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k + 1], c, -ms));
+                l += p0 + p1;
+                w[k] = pack_f16(p0, p1);
+              }
+            } else {
+              const int j = (i - NKS) / NDB, db = (i - NKS) % NDB;
+              acc[db] = mfma32_f16(x, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]), acc[db]);
+              fetch(n + kAhead);
+#pragma unroll
+              for (int e = 0; e < 4 / NDB; ++e) {
+                const int k = (i - NKS) * (4 / NDB) + e;  // 0 .. 7
+                if (bl == 0) k_piece(st, kx, k, cur, kNarrow);
+                else v_piece(st, k, nxt, kNarrow);
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
+        pv = pk;
+        pk = pn;
+        load_v(upto(kt + 2), pv);
+        load_k(kx, upto(kt + 3), pk);
+        pn = page_at(upto(kt + 4));
+        here0 = here1;
+        here1 = here2;
+        here2 = pages_there(upto(kt + 3));
+        __syncthreads();
+      };
+      // (two LDS buffers and three blocks of scores: the order comes round after six steps)
+      for (int kt = begin; kt < end;) {
+        step(kt, buf0, buf1, sa, sb, sc_);
+        if (++kt >= end) break;
+        step(kt, buf1, buf0, sc_, sa, sb);
+        if (++kt >= end) break;
+        step(kt, buf0, buf1, sb, sc_, sa);
+        if (++kt >= end) break;
+        step(kt, buf1, buf0, sa, sb, sc_);
+        if (++kt >= end) break;
+        step(kt, buf0, buf1, sc_, sa, sb);
+        if (++kt >= end) break;
+        step(kt, buf1, buf0, sb, sc_, sa);
+        ++kt;
       }
     }
-    __syncthreads();  // the next rows use the same LDS
+    l = add_x32(l);
+  }
+  const float back = ldexpf(1.0f, uv.E - 134);
+  if (rw + li < rows) {
+    const int64_t tok = s.start + qi;
+    const bool one = a.splits == 1;
+    const float f = one ? (filled(l) ? back / l : 0.0f) : back;
+    const int64_t at = split * R + tok * p.Hq + h;
+    if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
+    if (!one && g == 0) a.ml[at] = make_float2(m, l);
+    if (one || filled(l)) {
+      // Register r of acc[db] is V^T row 32 db + 8 (r / 4) + 4 g + r % 4 = c D/4 + dq, column 4 dq + c: for piece i
+      // the columns 32 i + 16 g + 4 k + c.  D = 128: c = db, r = 4 i + k; D = 64: c = 2 db + r / 8, r % 8 = 4 i + k.
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) {
+        const int col = 32 * i + 16 * g;
+        float o[16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int cc = 0; cc < 4; ++cc)
+            o[4 * k + cc] = (D == 128 ? acc[cc % NDB][4 * i + k] : acc[cc / 2][8 * (cc & 1) + 4 * (i & 1) + k]) * f;
+        if (one) {
+          uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col);
+          dst[0] = make_uint4(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]), pack_dt<DT>(o[4], o[5]),
+                              pack_dt<DT>(o[6], o[7]));
+          dst[1] = make_uint4(pack_dt<DT>(o[8], o[9]), pack_dt<DT>(o[10], o[11]), pack_dt<DT>(o[12], o[13]),
+                              pack_dt<DT>(o[14], o[15]));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(a.acc + at * D + col);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        }
+      }
+    }
   }
 }
 
@@ -1162,32 +1142,45 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
 
 struct Plan {
   bool decode;
-  int tiles, splits, least;
+  int splits, least;
+  int64_t slots;
 };
 
 constexpr int kDecodeRows = 16;
 
-// The keys are split where the row tiles alone are fewer workgroups than the chip wants.  The lengths are on the device:
-// the rule goes by the table's width, and a sequence whose part would have fewer than `least` tiles uses fewer parts.
+// Parts of the keys, of 192 at least in decode (one token over 5003 keys, 8 key heads, parts of 128 / 192 / 256 / 512: 12.5 /
+// 12.0 / 13.1 / 15.5 us) and 128 in chunks (100 tokens over 700 keys, 12 heads, 128 / 256 / 512: 18 / 22 / 26).  The lengths are on the device: the rule goes by the table's width, and a shorter
+// sequence's parts are shorter, or fewer.
 //
-// decode: 1536 workgroups, twice the three per CU that run at a time, parts of 256 keys at least.  48 sequences of 8000
-// to 16000 keys, 8 key heads, us: 256 / 1536 / 2048 / 4096 / 8192 workgroups 314 / 240 / 244 / 245 / 273.  One sequence
-// of 5003 keys, parts of 128 / 256 / 512 keys: 9.4 + 6.4 (combine), 10.1 + 5.1, 13.4 + 4.2.
-// chunk: one sequence's parts are all alike, so the 512 that run at a time are enough (64 tokens over 20000 keys, 32 / 8
-// heads: 85 us, with 1024 workgroups 104; 512 tokens: 226 and 255).  Several have unequal lengths, and more workgroups
-// even them out (four of up to 509 tokens and 9001 keys, 512 / 1024 / 2048 / 4096: 106 / 85 / 75 / 91).
+// decode: the 768 workgroups that run at a time at D = 128 (24 sequences of 2000 to 4000 keys, 8 key heads, 384 / 768 /
+// 1536: 50 / 38 / 43 us; 3 of up to 40000, 384 / 768 / 1152: 57 / 41 / 46).
+// chunk, one sequence: its parts are alike, so not more than the 512 that run at a time (64 tokens over 20000 keys, 32 / 8
+// heads, 256 / 512 / 624: 55 / 53 / 71 us; 512 tokens, 384 / 512 / 640: 257 / 233 / 268).
+// chunk, several: lengths differ, and rounds of more and shorter parts even them out, but each part costs some tiles' time
+// besides its own.  With w workgroups in a part, rounds w s / 512 + c of keys / (64 s) tiles + o each take the least time
+// at s^2 = keys / w * 8 c / o; c / o = 1 / 16 fits (us for 2 / 3 / 4 / 8 parts, * the rule's: 16 sequences of up to 64 tokens
+// and 2000 keys 55* / 66 / 64 / 64; 8 of 128 and 4000 84 / 68* / 84 / 84; 4 of 700 and 9001, 12 heads 166 / 133 / 147* / 145;
+// 2 of 1024 and 16000 535 / 524 / 502* / 547).
 Plan plan(const lbfq_paged_params* p) {
   Plan x;
   const int64_t G = p->Hq / p->Hk;
   const int64_t most = p->max_query_len > 0 && p->max_query_len < p->T ? p->max_query_len : p->T;
-  const int64_t rows = most * G;
-  x.decode = rows <= kDecodeRows;
-  const int64_t tile = x.decode ? 16 : 128;
-  x.tiles = static_cast<int>((rows + tile - 1) / tile);
-  const int64_t wgs = x.tiles * p->Hk * p->B;
-  const int64_t keys = p->table_cols << p->page_shift;
-  const int64_t want = x.decode ? 1536 : p->B > 1 ? 2048 : 512, least = x.decode ? 256 : 512;
-  int64_t s = want / wgs;
+  x.decode = most * G <= kDecodeRows;
+  const int64_t tiles = (p->T * G + kChunkRows - 1) / kChunkRows;
+  x.slots = tiles + p->B - 1;
+  int64_t keys = p->table_cols << p->page_shift;
+  if (p->causal && p->window && p->window + most < keys) keys = p->window + most;
+  int64_t s = 1;
+  if (x.decode) {
+    const int64_t wgs = p->B * p->Hk;
+    s = (768 + wgs / 2) / wgs;
+  } else if (p->B == 1) {
+    s = 512 / (tiles * p->Hk);
+  } else {
+    const int64_t wgs = (tiles + p->B / 2) * p->Hk;
+    while ((s + 1) * (s + 1) * wgs <= keys / 2 && s < 64) ++s;
+  }
+  const int64_t least = x.decode ? 192 : 128;
   if (s > keys / least) s = keys / least;
   if (s > 64) s = 64;  // a lane each in the combine kernel
   x.splits = s < 1 ? 1 : static_cast<int>(s);
@@ -1242,7 +1235,7 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   Args a{};
   a.p = *p;
   a.G = static_cast<int>(p->Hq / p->Hk);
-  a.tiles = x.tiles;
+  a.slots = static_cast<int>(x.slots);
   a.splits = x.splits;
   a.least = x.least;
   a.sml2 = p->sm_scale * kLog2e;
@@ -1254,10 +1247,12 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
     a.ml = reinterpret_cast<float2*>(a.acc + x.splits * R * p->D);
   }
   LBFQ_CHECK_ARG(R < (int64_t{1} << 30), "lbfq_paged_attention: problem too large");
-  LBFQ_CHECK_ARG(p->B < (int64_t{1} << 30) / (p->Hk * x.splits) / (x.tiles + 7), "lbfq_paged_attention: problem too large");
-  a.main = p->B * p->Hk * x.tiles * x.splits;
-  a.combos = static_cast<uint32_t>(p->B * p->Hk * x.splits);
-  if (!x.decode) a.main = (static_cast<int64_t>((x.tiles + 7) / 8) * a.combos + 7) / 8 * 64;
+  // (a launch has fewer than 2^32 threads)
+  const int64_t combos = (x.decode ? p->B : x.splits) * p->Hk, groups = (x.slots + 7) / 8, piece = (x.slots + groups - 1) / groups;
+  a.main = x.decode ? combos * x.splits : (groups * combos + 7) / 8 * 8 * piece;
+  LBFQ_CHECK_ARG(a.main < (1 << 24) - 8 && (x.splits == 1 || R < (1 << 26)), "lbfq_paged_attention: problem too large");
+  a.combos = static_cast<uint32_t>(combos);
+  a.piece = static_cast<uint32_t>(piece);
   // rows that no sequence has: the combine kernel sees every row, otherwise some workgroups more
   const int64_t fill = (p->fill_rest || p->lse) && x.splits == 1 ? 8 : 0;
   const dim3 grid(static_cast<unsigned>(a.main + fill));

@@ -111,6 +111,34 @@ def test_a_wide_table_and_short_sequences(gpu):
         run_and_check(args, "wide", hint=1)
 
 
+@pytest.mark.parametrize("B,most,hq,hk,d", [(70, 40, 8, 2, 128), (150, 1, 4, 2, 64), (300, 19, 3, 3, 64),
+                                            (4200, 18, 2, 1, 64)])
+def test_many_ragged_sequences(gpu, B, most, hq, hk, d):
+    """More sequences than a wave has lanes, and than 64 waves have: where each row
+    tile belongs is found in two and in three looks.  Most have one new token, some none."""
+    g = torch.Generator().manual_seed(B)
+    counts = [[0, 1, 1, most][int(i)] for i in torch.randint(0, 4, (B,), generator=g)]
+    counts[-1] = most
+    lens = [int(n) for n in torch.randint(0, 40, (B,), generator=g)]
+    args = problem(gpu, lens=lens, counts=counts, hq=hq, hk=hk, d=d, tail=2, garbage=False)
+    run_and_check(args, f"{B} sequences", hint=most)
+
+
+@pytest.mark.parametrize("n", [3, 200])
+def test_rows_before_the_first_sequence(gpu, n):
+    from low_bit_fake_quant import paged_attention
+    q, cache, table, lens, starts = problem(gpu, lens=[400, 300, 7], counts=[n, n // 2, 1], tail=9)
+    want, wl = paged_attention(q, cache, table, lens, starts, max_query_len=n, return_lse=True)
+    q2 = torch.cat([q[-5:], q[:-5]])
+    out, lse = paged_attention(q2, cache, table, lens, starts + 5, max_query_len=n, return_lse=True)
+    assert torch.equal(out[5:], want[:-5]) and torch.equal(lse[5:], wl[:-5])
+    assert not out[:5].any() and torch.isneginf(lse[:5]).all()
+    one, l1 = paged_attention(q2[:5 + n], cache, table[:1], lens[:1], starts[:2] + 5, return_lse=True)
+    ref.check(one[5:], *[x for i, x in enumerate(ref.attend(q[:n], cache, table[:1], lens[:1], starts[:2])) if i in (0, 2)],
+              "one sequence")
+    assert not one[:5].any() and torch.isneginf(l1[:5]).all()
+
+
 @pytest.mark.parametrize("n", [1, 33])
 def test_missing_pages_are_not_seen(gpu, n):
     q, cache, table, lens, starts = problem(gpu, lens=[200, 64, 40], counts=[n, n, n])
