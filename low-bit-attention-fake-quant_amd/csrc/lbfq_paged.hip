@@ -31,6 +31,8 @@
 // far apart for that takes a slower loop with V in bf16 and P in two bf16 terms.  So P can be fp16: 11 bits, where
 // bf16's 8 would cost as much as the output's own rounding.  K is bf16 (exact) for bf16 queries, and for fp16 ones fp16
 // under the same rule.  4680 tokens over 32760 keys, 12 heads of 128, all seen: 1.16 ms, 812 TFLOP/s.
+#include <algorithm>
+#include <limits>
 #include <type_traits>
 
 #include "lbfq_common.h"
@@ -1143,7 +1145,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
 struct Plan {
   bool decode;
   int splits, least;
-  int64_t slots;
+  int64_t slots, groups, piece;  // chunk: row tiles of a head (slot_of), the pieces that they come in, row tiles of a piece
 };
 
 constexpr int kDecodeRows = 16;
@@ -1154,13 +1156,16 @@ constexpr int kDecodeRows = 16;
 //
 // decode: the 768 workgroups that run at a time at D = 128 (24 sequences of 2000 to 4000 keys, 8 key heads, 384 / 768 /
 // 1536: 50 / 38 / 43 us; 3 of up to 40000, 384 / 768 / 1152: 57 / 41 / 46).
-// chunk, one sequence: its parts are alike, so not more than the 512 that run at a time (64 tokens over 20000 keys, 32 / 8
-// heads, 256 / 512 / 624: 55 / 53 / 71 us; 512 tokens, 384 / 512 / 640: 257 / 233 / 268).
-// chunk, several: lengths differ, and rounds of more and shorter parts even them out, but each part costs some tiles' time
-// besides its own.  With w workgroups in a part, rounds w s / 512 + c of keys / (64 s) tiles + o each take the least time
-// at s^2 = keys / w * 8 c / o; c / o = 1 / 16 fits (us for 2 / 3 / 4 / 8 parts, * the rule's: 16 sequences of up to 64 tokens
-// and 2000 keys 55* / 66 / 64 / 64; 8 of 128 and 4000 84 / 68* / 84 / 84; 4 of 700 and 9001, 12 heads 166 / 133 / 147* / 145;
-// 2 of 1024 and 16000 535 / 524 / 502* / 547).
+// chunk, one sequence: the parts that take the least time by a count of tiles.  A part costs the time of 12 tiles besides
+// its own (its start, and its sums written and read again), and an XCD has 64 workgroups at a time.  Row tiles that see
+// much the same keys go in whole rounds (us for 1 / 2 / 4 / 6 / 7 parts, * the rule's: 1560 tokens, 32760 keys, 40 heads
+// 2064 / 1585 / 1374 / 1356* / 1368; 700, 8000 keys, 12 heads 216 / 121 / 88 / 72* / 98).  A causal prompt's row tiles
+// differ, the longest first, and fill the rounds up; a workgroup that is left alone on its CU takes 0.7 times as long (1 /
+// 2 / 3 / 4 parts: 2500 tokens, 32 / 8 heads 91* / 127 / 144 / 158; 5000, 5 heads 145 / 94 / 74* / 85).
+// chunk, several: lengths differ, and more and shorter parts even them out.  With w workgroups in a part, w s / 512 + c
+// rounds of keys / (64 s) tiles + o each take the least time at s^2 = keys / w * 8 c / o; c / o = 1 / 12 fits (2 / 3 / 4 /
+// 5 / 8 parts: 16 sequences of up to 64 tokens and 2000 keys 55* / 66 / 64 / 64 / 64; 8 of 128 and 4000 84 / 68* / 84 / 81
+// / 84; 4 of 700 and 9001, 12 heads 166 / 133 / 147 / 138* / 145; 2 of 1024 and 16000 535 / 524 / 502 / 530* / 547).
 Plan plan(const lbfq_paged_params* p) {
   Plan x;
   const int64_t G = p->Hq / p->Hk;
@@ -1168,22 +1173,30 @@ Plan plan(const lbfq_paged_params* p) {
   x.decode = most * G <= kDecodeRows;
   const int64_t tiles = (p->T * G + kChunkRows - 1) / kChunkRows;
   x.slots = tiles + p->B - 1;
-  int64_t keys = p->table_cols << p->page_shift;
-  if (p->causal && p->window && p->window + most < keys) keys = p->window + most;
+  x.groups = (x.slots + 7) / 8;
+  x.piece = (x.slots + x.groups - 1) / x.groups;
+  int64_t keys = p->table_cols << p->page_shift;  // that a row tile may see
+  if (p->causal && p->window) keys = std::min(keys, p->window + std::min(most, kChunkRows / G + 1));
+  const int64_t least = x.decode ? 192 : 128;
+  const int64_t limit = std::min<int64_t>(keys / least, 64);  // (a lane each in the combine kernel)
   int64_t s = 1;
   if (x.decode) {
     const int64_t wgs = p->B * p->Hk;
     s = (768 + wgs / 2) / wgs;
   } else if (p->B == 1) {
-    s = 512 / (tiles * p->Hk);
+    const bool uneven = p->causal && !p->window && 2 * most > keys;
+    int64_t best = std::numeric_limits<int64_t>::max();
+    for (int64_t n = 1; n <= limit; ++n) {
+      const int64_t of_xcd = (x.groups * p->Hk * n + 7) / 8 * x.piece, longest = keys / n + 12 * 64;
+      const int64_t cost = uneven ? std::max(of_xcd * ((keys - most / 2) / n + 12 * 64), 45 * longest)
+                                  : (of_xcd + 63) / 64 * 64 * longest;
+      if (cost < best) best = cost, s = n;
+    }
   } else {
     const int64_t wgs = (tiles + p->B / 2) * p->Hk;
-    while ((s + 1) * (s + 1) * wgs <= keys / 2 && s < 64) ++s;
+    while (3 * (s + 1) * (s + 1) * wgs <= 2 * keys && s < limit) ++s;
   }
-  const int64_t least = x.decode ? 192 : 128;
-  if (s > keys / least) s = keys / least;
-  if (s > 64) s = 64;  // a lane each in the combine kernel
-  x.splits = s < 1 ? 1 : static_cast<int>(s);
+  x.splits = static_cast<int>(std::max<int64_t>(std::min(s, limit), 1));
   x.least = static_cast<int>(least / (x.decode ? 32 : 64));
   return x;
 }
@@ -1248,11 +1261,11 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   }
   LBFQ_CHECK_ARG(R < (int64_t{1} << 30), "lbfq_paged_attention: problem too large");
   // (a launch has fewer than 2^32 threads)
-  const int64_t combos = (x.decode ? p->B : x.splits) * p->Hk, groups = (x.slots + 7) / 8, piece = (x.slots + groups - 1) / groups;
-  a.main = x.decode ? combos * x.splits : (groups * combos + 7) / 8 * 8 * piece;
+  const int64_t combos = (x.decode ? p->B : x.splits) * p->Hk;
+  a.main = x.decode ? combos * x.splits : (x.groups * combos + 7) / 8 * 8 * x.piece;
   LBFQ_CHECK_ARG(a.main < (1 << 24) - 8 && (x.splits == 1 || R < (1 << 26)), "lbfq_paged_attention: problem too large");
   a.combos = static_cast<uint32_t>(combos);
-  a.piece = static_cast<uint32_t>(piece);
+  a.piece = static_cast<uint32_t>(x.piece);
   // rows that no sequence has: the combine kernel sees every row, otherwise some workgroups more
   const int64_t fill = (p->fill_rest || p->lse) && x.splits == 1 ? 8 : 0;
   const dim3 grid(static_cast<unsigned>(a.main + fill));
