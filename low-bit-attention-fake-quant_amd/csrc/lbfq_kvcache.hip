@@ -181,7 +181,7 @@ extern "C" int lbfq_kv_write(const lbfq_kv_write_params* p, lbfq_stream_t stream
   LBFQ_CHECK_ARG(((reinterpret_cast<uint64_t>(p->k) | reinterpret_cast<uint64_t>(p->v)) & 15) == 0,
                  "lbfq_kv_write: rows must be 16-byte aligned");
   const int64_t wgs = (p->T + kRows - 1) / kRows * 2 * p->H;
-  LBFQ_CHECK_ARG(wgs < (int64_t{1} << 31), "lbfq_kv_write: problem too large");
+  LBFQ_CHECK_ARG(wgs < (int64_t{1} << 24), "lbfq_kv_write: problem too large");  // (a launch has fewer than 2^32 threads)
   const dim3 grid(static_cast<unsigned>(wgs)), block(256);
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define LBFQ_KW(DT)                                                                           \
@@ -208,7 +208,7 @@ extern "C" int lbfq_kv_read(const lbfq_kv_read_params* p, lbfq_stream_t stream) 
                  "lbfq_kv_read: missing tensor");
   LBFQ_CHECK_ARG(p->table_cols >= 0 && p->table_cols < (int64_t{1} << 40), "lbfq_kv_read: bad block table");
   const int64_t blocks = (p->max_len + kRows - 1) / kRows;
-  LBFQ_CHECK_ARG(p->B < (int64_t{1} << 31) / (blocks * 2 * p->H), "lbfq_kv_read: problem too large");
+  LBFQ_CHECK_ARG(p->B < (int64_t{1} << 24) / (blocks * 2 * p->H), "lbfq_kv_read: problem too large");
   const dim3 grid(static_cast<unsigned>(p->B * blocks * 2 * p->H)), block(256);
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define LBFQ_KR(DT)                                                                                                    \

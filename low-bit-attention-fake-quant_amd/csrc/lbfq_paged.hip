@@ -1207,7 +1207,7 @@ int64_t workspace(const lbfq_paged_params* p, const Plan& x) {
   return x.splits * R * (static_cast<int64_t>(sizeof(float2)) + p->D * 4) + 16;
 }
 
-int check(const lbfq_paged_params* p) {
+int check_sizes(const lbfq_paged_params* p) {
   const char* who = "lbfq_paged_attention";
   LBFQ_CHECK_ARG(p, "%s: null params", who);
   LBFQ_CHECK_ARG(p->D == 64 || p->D == 128, "%s: D must be 64 or 128", who);
@@ -1217,10 +1217,17 @@ int check(const lbfq_paged_params* p) {
   LBFQ_CHECK_ARG(p->T > 0 && p->B > 0 && p->T < (int64_t{1} << 30) && p->B < (int64_t{1} << 30),
                  "%s: bad number of tokens or sequences", who);
   LBFQ_CHECK_ARG(p->page_shift >= 4 && p->page_shift <= 10, "%s: pages hold 16 to 1024 tokens, a power of two", who);
-  LBFQ_CHECK_ARG(p->num_pages > 0 && p->num_pages * p->Hk < (int64_t{1} << 31), "%s: bad number of pages", who);
-  LBFQ_CHECK_ARG(p->table_cols > 0 && (p->table_cols << p->page_shift) <= (int64_t{1} << 30) &&
-                     p->table_cols < (int64_t{1} << 30) && p->table_stride >= 0,
+  LBFQ_CHECK_ARG(p->T * p->Hq < (int64_t{1} << 30), "%s: problem too large", who);
+  LBFQ_CHECK_ARG(p->num_pages > 0 && p->num_pages < (int64_t{1} << 31) / p->Hk, "%s: bad number of pages", who);
+  LBFQ_CHECK_ARG(p->table_cols > 0 && p->table_cols <= (int64_t{1} << 30) >> p->page_shift && p->table_stride >= 0,
                  "%s: bad block table", who);
+  LBFQ_CHECK_ARG(p->window >= 0 && p->window <= (int64_t{1} << 30), "%s: bad window", who);
+  return 0;
+}
+
+int check(const lbfq_paged_params* p) {
+  const char* who = "lbfq_paged_attention";
+  if (int rc = check_sizes(p)) return rc;
   LBFQ_CHECK_ARG(p->q && p->out && p->block_table && p->seq_lens && p->query_starts && p->k_codes && p->k_scale &&
                      p->v_codes && p->v_scale,
                  "%s: missing tensor", who);
@@ -1231,14 +1238,13 @@ int check(const lbfq_paged_params* p) {
                  "%s: rows must be 16-byte aligned", who);
   // (beyond, a scale of K times sm_scale could leave fp32's range)
   LBFQ_CHECK_ARG(p->sm_scale >= 0x1p-64f && p->sm_scale <= 0x1p15f, "%s: sm_scale must lie in 2^-64 .. 2^15", who);
-  LBFQ_CHECK_ARG(p->window >= 0 && p->window <= (int64_t{1} << 30), "%s: bad window", who);
   return 0;
 }
 
 }  // namespace
 
 extern "C" int64_t lbfq_paged_attention_workspace_bytes(const lbfq_paged_params* p) {
-  if (!p || p->Hk <= 0 || p->Hq <= 0 || p->T <= 0 || p->B <= 0 || p->table_cols <= 0) return 0;
+  if (check_sizes(p)) return 0;
   return workspace(p, plan(p));
 }
 
@@ -1259,7 +1265,6 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
     a.acc = static_cast<float*>(p->workspace);
     a.ml = reinterpret_cast<float2*>(a.acc + x.splits * R * p->D);
   }
-  LBFQ_CHECK_ARG(R < (int64_t{1} << 30), "lbfq_paged_attention: problem too large");
   // (a launch has fewer than 2^32 threads)
   const int64_t combos = (x.decode ? p->B : x.splits) * p->Hk;
   a.main = x.decode ? combos * x.splits : (x.groups * combos + 7) / 8 * 8 * x.piece;

@@ -385,6 +385,7 @@ std::tuple<Tensor, OptTensor> attention(const Tensor& q_, const Tensor& kc, cons
     bool distinct = rows_16b(*out_);
     for (int64_t i = 0; i < 2; ++i) distinct = distinct && (out_->size(i) <= 1 || out_->stride(i) != 0);
     if (!distinct) bad_value("out must have contiguous, distinct rows that start on 16-byte boundaries");
+    if (at::GradMode::is_enabled() && out_->requires_grad()) refuse_grad("paged_attention");
   }
   On dev(q_);
   const Tensor out = out_ ? *out_ : at::empty(q_.sizes(), q_.options());
@@ -422,12 +423,21 @@ std::tuple<Tensor, OptTensor> attention(const Tensor& q_, const Tensor& kc, cons
     p.workspace_bytes = need;
   }
   check_rc(lbfq_paged_attention(&p, stream(q)), "lbfq_paged_attention");
+  if (out_ && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();  // written in place: autograd is to know
   return {out, lse};
 }
 
 }  // namespace
 
 PYBIND11_MODULE(_lbfq_torch, m) {
+  // (of pybind's own it would be a plain RuntimeError)
+  py::register_local_exception_translator([](std::exception_ptr e) {
+    try {
+      if (e) std::rethrow_exception(e);
+    } catch (const c10::OutOfMemoryError& x) {
+      PyErr_SetString(py::module_::import("torch").attr("OutOfMemoryError").ptr(), x.what_without_backtrace());
+    }
+  });
   m.def("set_hooks", [](py::object stream, py::object error) {
     stream_of = new py::object(std::move(stream));
     library_error = new py::object(std::move(error));

@@ -108,6 +108,22 @@ def test_cache_entries_refuse(lib):
     a.workspace, a.workspace_bytes = FAKE, need - 1
     assert lib.lbfq_paged_attention(ctypes.byref(a), None) == -1 and b"workspace" in lib.lbfq_last_error()
     assert lib.lbfq_paged_attention_workspace_bytes(None) == 0
+    # sizes that the launch refuses need none, and are not divided by
+    a.window = 5
+    for name, bad in (("Hq", 1), ("Hk", 0), ("T", 1 << 62), ("T", 1 << 29), ("B", 0), ("table_cols", 1 << 62), ("page_shift", 60),
+                      ("num_pages", 1 << 62)):
+        old = getattr(a, name)
+        setattr(a, name, bad)
+        assert lib.lbfq_paged_attention_workspace_bytes(ctypes.byref(a)) == 0, name
+        assert lib.lbfq_paged_attention(ctypes.byref(a), None) == -1, name
+        setattr(a, name, old)
+    assert lib.lbfq_paged_attention_workspace_bytes(ctypes.byref(a)) >= 0
+    # more workgroups than a launch may have
+    a.window, a.B, a.T, a.max_query_len, a.Hk, a.Hq = 0, 1 << 23, 1 << 23, 1, 2, 4
+    assert lib.lbfq_paged_attention(ctypes.byref(a), None) == -1 and b"too large" in lib.lbfq_last_error()
+    for p, fn in ((w, lib.lbfq_kv_write), (r, lib.lbfq_kv_read)):
+        p.T = p.B = 1 << 29
+        assert fn(ctypes.byref(p), None) == -1 and b"too large" in lib.lbfq_last_error()
 
 
 def test_a_missing_host_module_is_said_loudly(lib, monkeypatch):

@@ -386,9 +386,31 @@ def test_refusals(gpu):
             (dict(sm_scale=math.nan), ValueError, "sm_scale"), (dict(sm_scale=2.0 ** 16), ValueError, "sm_scale"), (dict(window=0), ValueError, "window"),
             (dict(max_query_len=-1), ValueError, "max_query_len"), (dict(out=q[:1].clone()), ValueError, "out must be"),
             (dict(out=q[:1].expand(2, -1, -1)), ValueError, "out must have"),
-            (dict(q=q.clone().requires_grad_()), ValueError, "no backward pass")):
+            (dict(q=q.clone().requires_grad_()), ValueError, "no backward pass"),
+            (dict(out=q.clone().requires_grad_()), ValueError, "no backward pass")):
         with pytest.raises(err, match=msg):
             call(**kw)
     assert paged_attention(q[:0], cache, table, lens, starts * 0).shape == (0, 4, 128)
     o, l = paged_attention(q, cache, table[:0], lens[:0], starts[:1], return_lse=True)
     assert not o.any() and torch.isneginf(l).all()
+
+
+def test_an_output_that_autograd_has_saved(gpu):
+    """Writing into `out` counts as a change in place: a backward pass that needs the old values says so."""
+    from low_bit_fake_quant import paged_attention
+    args = problem(gpu, lens=[20], counts=[2])
+    out = torch.zeros_like(args[0])
+    w = torch.ones_like(out, requires_grad=True)
+    y = (out * w).sum()
+    paged_attention(*args, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        paged_attention(*args, out=torch.zeros_like(args[0]))
+
+
+def test_out_of_memory_is_torchs_error(gpu):
+    from low_bit_fake_quant import read_kv_cache
+    _, cache, table, lens, _ = problem(gpu, lens=[20], counts=[1])
+    with pytest.raises(torch.OutOfMemoryError):
+        read_kv_cache(cache, table, lens, 1 << 34, dtype=torch.float32)
