@@ -2,12 +2,13 @@
 // arguments, allocations and parameter structs, in front of the C entries.
 //
 // A call on a few tokens is bound by this part.  In Python with ctypes it took 14
-// us for qk_norm_rope and 9.5 for write_kv_cache; the
-// same here takes 5.6 and 3.9.  Kernels stay behind the C ABI (include/lbfq.h), in
+// us for qk_norm_rope and 9.5 for write_kv_cache; here 5.6 and 3.9.  Kernels stay behind the C ABI (include/lbfq.h), in
 // liblbfq_hip.so, which this module links to.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -20,6 +21,8 @@
 namespace py = pybind11;
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 namespace {
 
@@ -238,6 +241,57 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> norm_backward(const Tensor& q, 
   return {dq, dk, dqw, dkw};
 }
 
+// The two as one differentiable operator.  (As a torch.autograd.Function in Python a training step on a few tokens took
+// 100 us, as this 78: most of the rest is torch handing it to its own thread.)
+struct NormFunction : torch::autograd::Function<NormFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& qw,
+                               const OptTensor& kw, const Tensor& cos, const Tensor& sin, const OptTensor& positions,
+                               double eps, const std::string& pairs) {
+    ctx->save_for_backward({q, k, qw.value_or(Tensor()), kw.value_or(Tensor()), cos, sin, positions.value_or(Tensor())});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["pairs"] = pairs;
+    const auto [yq, yk] = norm_forward(q, k, qw, kw, cos, sin, positions, eps, pairs);
+    return {yq, yk};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    const py::gil_scoped_acquire gil;  // (the engine's threads come without it; stream() and errors need it)
+    const variable_list x = ctx->get_saved_variables();
+    const auto given = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    const OptTensor qw = given(x[2]), kw = given(x[3]);
+    // (an input that was not given has no edge)
+    const bool want_qw = qw && ctx->needs_input_grad(2), want_kw = kw && ctx->needs_input_grad(qw ? 3 : 2);
+    const bool again = at::GradMode::is_enabled();
+    variable_list g;
+    {
+      const at::AutoGradMode off(false);
+      auto [dq, dk, dqw, dkw] = norm_backward(x[0], x[1], qw, kw, x[4], x[5], given(x[6]), ctx->saved_data["eps"].toDouble(),
+                                              ctx->saved_data["pairs"].toStringRef(), dy[0], dy[1], want_qw, want_kw);
+      g = {dq, dk, dqw.value_or(Tensor()), dkw.value_or(Tensor())};
+    }
+    if (again) {  // create_graph: whoever differentiates these is told
+      for (Tensor& t : g)
+        if (t.defined()) t = t.detach().set_requires_grad(true);
+      g = torch::autograd::DelayedError("qk_norm_rope has no second derivative", 4)(std::move(g));
+    }
+    g.resize(9);
+    return g;
+  }
+};
+
+std::tuple<Tensor, Tensor> norm(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& cos,
+                                const Tensor& sin, const OptTensor& positions, double eps, const std::string& pairs) {
+  if (at::GradMode::is_enabled()) {
+    if (cos.requires_grad() || sin.requires_grad())
+      bad_value("qk_norm_rope has no gradient for cos and sin; detach them");
+    if (q.requires_grad() || k.requires_grad() || (qw && qw->requires_grad()) || (kw && kw->requires_grad())) {
+      const variable_list y = NormFunction::apply(q, k, qw, kw, cos, sin, positions, eps, pairs);
+      return {y[0], y[1]};
+    }
+  }
+  return norm_forward(q, k, qw, kw, cos, sin, positions, eps, pairs);
+}
+
 // ---- the cache ---------------------------------------------------------------------
 
 struct Cache {
@@ -442,8 +496,7 @@ PYBIND11_MODULE(_lbfq_torch, m) {
     stream_of = new py::object(std::move(stream));
     library_error = new py::object(std::move(error));
   });
-  m.def("qk_norm_rope", &norm_forward);
-  m.def("qk_norm_rope_backward", &norm_backward);
+  m.def("qk_norm_rope", &norm);
   m.def("write_kv_cache", &kv_write);
   m.def("read_kv_cache", &kv_read);
   m.def("paged_attention", &attention);

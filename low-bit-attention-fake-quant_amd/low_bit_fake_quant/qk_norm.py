@@ -23,22 +23,6 @@ def rotary_table(length: int, rot: int, theta: float = 10000.0, *, device=None) 
     return a.cos().float(), a.sin().float()
 
 
-class _QkNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, pairs):
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.eps, ctx.pairs = eps, pairs
-        return _lib.torch_ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, pairs)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dyq, dyk):
-        want = ctx.needs_input_grad
-        dq, dk, dqw, dkw = _lib.torch_ops().qk_norm_rope_backward(*ctx.saved_tensors, ctx.eps, ctx.pairs, dyq, dyk,
-                                                                  want[2], want[3])
-        return dq if want[0] else None, dk if want[1] else None, dqw, dkw, None, None, None, None, None
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
                  cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None, *, eps: float = 1e-6,
                  pairs: str = "adjacent") -> tuple[torch.Tensor, torch.Tensor]:
@@ -58,15 +42,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     rotated (padding); one past the table comes out as NaN.
 
     Arithmetic is fp32 with one rounding at the end.  Gradients reach q, k and the
-    weights (``cos`` and ``sin`` take none); the weights' sums have a fixed order.
+    weights (``cos`` and ``sin`` take none); the weights' sums have a fixed order.  A
+    second derivative is refused.
     Returns new contiguous tensors of the inputs' shapes and dtype.
     """
-    if torch.is_grad_enabled():
-        if cos.requires_grad or sin.requires_grad:
-            raise ValueError("qk_norm_rope has no gradient for cos and sin; detach them")
-        if q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad) or (
-                k_weight is not None and k_weight.requires_grad):
-            return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, pairs)
     return _lib.torch_ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, pairs)
 
 

@@ -176,6 +176,44 @@ def test_only_what_is_asked_for(gpu):
         assert not qk_norm_rope(x, k, w, wk, cos, sin, pos)[0].requires_grad
 
 
+def test_a_second_derivative_is_refused(gpu):
+    from low_bit_fake_quant import qk_norm_rope
+    q, k, wq, _, cos, sin, pos = case(gpu, 1, 6, 4, 4, 64, torch.float32)
+    q.requires_grad_()
+    wq.requires_grad_()
+    yq, yk = qk_norm_rope(q, k, wq, None, cos, sin, pos)
+    (plain,) = torch.autograd.grad(yq.square().sum() + yk.sum(), q, retain_graph=True)
+    (g,) = torch.autograd.grad(yq.square().sum() + yk.sum(), q, create_graph=True)
+    assert torch.equal(g, plain)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        g.sum().backward()
+
+
+def test_backward_on_a_side_stream_and_in_threads(gpu):
+    """The backward pass runs on the forward's stream, in autograd's own thread, from several callers at once."""
+    import threading
+    args = case(gpu, 2, 300, 6, 2, 128, torch.bfloat16)
+    dq, dk = torch.ones_like(args[0]), torch.ones_like(args[1])
+    want = gradients(args, dq, dk)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream(device=gpu)
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = gradients(args, dq, dk)
+                s.synchronize()
+                bad.extend(i for i, (a, b) in enumerate(zip(got, want)) if not torch.equal(a, b))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_padding_positions_and_positions_past_the_table(gpu):
     from low_bit_fake_quant import qk_norm_rope
     q, k, wq, wk, cos, sin, pos = case(gpu, 1, 5, 2, 2, 64, torch.float32, rot=32)
