@@ -591,12 +591,6 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
   const uint32_t koff = kkey * D + KC * kq, ksoff = kkey * CH + KC * kq / 32;
   const uint32_t voff = VK * vkg * D + 4 * vdq, vsoff = VK * vkg * CH;
 
-  // The page of key `key` (the same in every lane), or -1.
-  auto page_of = [&](int key) {
-    const int idx = key >> shift;
-    const int page = idx < cols ? table[idx] : -1;
-    return page >= 0 && page < num_pages ? page : -1;
-  };
   auto row_of = [&](int page, int key) -> int64_t {
     return (static_cast<int64_t>(page * Hk + kvh) << shift) + (key & pmask);
   };
@@ -664,10 +658,25 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
         vse[0] = w.x; vse[1] = w.y;
       }
     };
-    auto page_at = [&](int kt) { return page_of(64 * kt + WKEYS * wave); };  // of the wave's keys: a scalar
     auto upto = [&](int kt) { return kt < end ? kt : end - 1; };  // steps past the end repeat it, unused
+    // Page ids of the tiles from kt on: lane 4 i + w has that of tile kt + i's keys 16 w .., which wave w stages.  One load,
+    // so one wait; looked up where they are needed, each id cost the time of a trip to memory (4680 tokens over 32760 keys,
+    // 12 heads: 1.16 ms, so 1.10).
+    auto group_of = [&](int kt) { return (64 * upto(kt + (lane >> 2 & 3)) + 16 * (lane & 3)) >> shift; };
+    auto look = [&](int kt) {
+      const int idx = group_of(kt);
+      return table[idx < cols ? idx : cols - 1];
+    };
+    auto there = [&](int kt, int id) -> uint32_t {  // a bit per lane: the page is there
+      return static_cast<uint32_t>(__ballot(group_of(kt) < cols && id >= 0 && id < num_pages));
+    };
+    auto page_in = [&](int id, uint32_t mask, int i) {  // of tile kt + i's keys of this wave, or -1; a scalar
+      return mask >> (4 * i + wave) & 1u ? __builtin_amdgcn_readlane(id, 4 * i + wave) : -1;
+    };
     // The first tiles are on their way while the scales are looked through.
-    const int page0 = page_at(begin), page1 = page_at(upto(begin + 1));
+    const int ids = look(begin);
+    const uint32_t mask = there(begin, ids);
+    const int page0 = page_in(ids, mask, 0), page1 = page_in(ids, mask, 1);
     load_k(kx, begin, page0);
     load_v(begin, page0);
     load_k(ky, upto(begin + 1), page1);
@@ -850,21 +859,12 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
       return m == -INFINITY ? 0.0f : m;
     };
 
-    // A mask bit for each group of 16 keys of the tile: its page is there.
-    auto pages_there = [&](int kt) {
-      bool ok = true;
-      if (lane < 4) {
-        const int idx = (64 * kt + 16 * lane) >> shift;
-        const int pg = idx < cols ? table[idx] : -1;
-        ok = pg >= 0 && pg < num_pages;
-      }
-      return static_cast<uint32_t>(__ballot(ok)) & 0xfu;
-    };
-
     if (uv.wide || uk.wide) {
       // Rare (see Unit), and plain: one tile after the other.
       for (int kt = begin; kt < end; ++kt) {
-        const int page = page_at(kt);
+        const int id = look(kt);
+        const uint32_t here = there(kt, id);
+        const int page = page_in(id, here, 0);
         load_k(kx, kt, page);
         load_v(kt, page);
         clear_k(kx, kt, page);
@@ -880,7 +880,7 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
           if (uk.wide) scores(lds, bl, sc[bl], std::true_type{});
           else scores(lds, bl, sc[bl], std::false_type{});
         }
-        const float ms = settle(64 * kt, pages_there(kt), sc[0], sc[1]);
+        const float ms = settle(64 * kt, here & 0xfu, sc[0], sc[1]);
 #pragma unroll
         for (int bl = 0; bl < 2; ++bl)
 #pragma unroll
@@ -922,8 +922,8 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
       uint8_t* const buf0 = lds;
       uint8_t* const buf1 = lds + L::BUF;
       // The pages and masks of the tiles on the way: of V's registers, of K's, of the next K; of the scores' tile and
-      // the two after it.
-      int pv = page1, pk = page_at(upto(begin + 2)), pn = page_at(upto(begin + 3));
+      // the three after it.
+      int pv = page1, pk = page_in(ids, mask, 2), pn = page_in(ids, mask, 3);
       clear_k(kx, begin, page0);
       clear_v(begin, page0);
       clear_k(ky, upto(begin + 1), page1);
@@ -932,7 +932,7 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
       store_k(ky, buf1, kNarrow);
       load_v(upto(begin + 1), pv);
       load_k(kx, upto(begin + 2), pk);
-      uint32_t here0 = pages_there(begin), here1 = pages_there(upto(begin + 1)), here2 = pages_there(upto(begin + 2));
+      uint32_t here0 = mask & 0xfu, here1 = mask >> 4 & 0xfu, here2 = mask >> 8 & 0xfu, here3 = mask >> 12 & 0xfu;
       __syncthreads();
       v16f sa, sb, sc_;
       scores(buf0, 0, sa, kNarrow);
@@ -947,6 +947,7 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
         // conversion of the staged K (first half) or V tile (second) beside P V.  The order is fixed here; left to the
         // compiler, every read was next to its product.
         constexpr int HALF = NKS + 2 * NDB, kAhead = 5;
+        const int id = look(kt + 4);  // back by the end of the step
         uint4 ring[kAhead];
         const uint8_t* const kr = nxt + key_of(li) * L::KP + 16 * g;
         const uint8_t* const vr = cur + L::KBYTES + li * L::VP + 16 * g;
@@ -1003,10 +1004,12 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
         pk = pn;
         load_v(upto(kt + 2), pv);
         load_k(kx, upto(kt + 3), pk);
-        pn = page_at(upto(kt + 4));
+        const uint32_t mask = there(kt + 4, id);
+        pn = page_in(id, mask, 0);
         here0 = here1;
         here1 = here2;
-        here2 = pages_there(upto(kt + 3));
+        here2 = here3;
+        here3 = mask & 0xfu;
         __syncthreads();
       };
       // (two LDS buffers and three blocks of scores: the order comes round after six steps)
