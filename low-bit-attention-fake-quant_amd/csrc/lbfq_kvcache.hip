@@ -6,12 +6,18 @@
 // stretch.  The format is the package's MXFP8 for Q and K (lbfq_rowtile,
 // LBFQ_Q_MX_QK, 32 columns a scale), the same codes and scales bit for bit:
 //   e = ceil(log2(max(amax, 1e-4) / 448)),  code = e4m3(x 2^-e),
-// but for e <= 119: from 2^128 on (where the value would be infinite) the largest is kept instead, 448 2^119.  The cache
-// then holds finite values only, and a key that a row does not see adds 0 times something finite to it.
+// but for e <= 119: from 2^128 on (where the value would be infinite) the largest
+// is kept instead, 448 2^119.  The cache then holds finite values only, and a key
+// that a row does not see adds 0 times something finite to it.
 //
 // Both directions are bound by memory.  D/8 lanes hold a row, eight values each;
 // a workgroup takes 64 consecutive tokens of one head of K or of V, so that the
-// scales of its rows, four bytes each, fill whole lines from one workgroup.
+// scales of its rows, four bytes each, fill whole lines from one workgroup, and a
+// thread's rows (four at D = 128) are all on their way before the first is used.
+// Writing 32760 tokens x 40 heads x 128 from bf16: 196 us, 5.2 TB/s of bytes read
+// and written (a copy of 1 GiB reaches 5.1 to 5.5).  Reading 8 sequences of up to
+// 16384 x 8 heads to bf16: 147 us, 4.7 TB/s (what only writes reaches 5.3).  A few
+// tokens: 3.0 and 4.6 us, a launch's own time.
 #include "lbfq_common.h"
 #include "../../include/lbfq.h"
 

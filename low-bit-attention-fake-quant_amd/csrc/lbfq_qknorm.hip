@@ -15,7 +15,9 @@
 // Bound by memory: D/8 lanes hold a row, eight values each (one 16-byte load of
 // 16-bit data), so a wave covers four (D = 128) or eight (D = 64) heads of one
 // token.  The heads of Q and K of a token are one list; a wave walks a stretch of
-// it with the rotation's cos and sin and both weights in registers.
+// it with the rotation's cos and sin and both weights in registers.  32760 tokens x
+// 24 heads x 128 bf16: 80 us, 5.0 TB/s (a copy of 1 GiB: 5.1 to 5.5).  Backward, 8002
+// tokens x 40 heads x 128: 48 + 4 us, 5.1 TB/s.  A few tokens: 3.9 us.
 #include "lbfq_common.h"
 #include "../../include/lbfq.h"
 
