@@ -1068,59 +1068,72 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
 
 // ---- joining the parts of the keys ---------------------------------------------
 
-// The largest / the sum over the wave, in every lane
-__device__ __forceinline__ float wave_max(float v) {
+// The largest / the sum over a row's 16 or 64 lanes, in every one of them
+template <int LPR>
+__device__ __forceinline__ float lanes_max(float v) {
 #define LBFQ_ROR(c) v = vmax(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), c, 0xf, 0xf, true)))
   LBFQ_ROR(0x128);  // row_ror:8, 4, 2, 1
   LBFQ_ROR(0x124);
   LBFQ_ROR(0x122);
   LBFQ_ROR(0x121);
 #undef LBFQ_ROR
-  return max_x32(max_x16(v));
+  return LPR == 64 ? max_x32(max_x16(v)) : v;
 }
-__device__ __forceinline__ float wave_add(float v) {
+template <int LPR>
+__device__ __forceinline__ float lanes_add(float v) {
 #define LBFQ_ROR(c) v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), c, 0xf, 0xf, true))
   LBFQ_ROR(0x128);
   LBFQ_ROR(0x124);
   LBFQ_ROR(0x122);
   LBFQ_ROR(0x121);
 #undef LBFQ_ROR
-  return add_x32(add_x16(v));
+  return LPR == 64 ? add_x32(add_x16(v)) : v;
 }
 
-// A wave per row: the parts' maxima and sums one to a lane (there are at most
-// 64), their outputs with weights 2^(m_s - M) summed in the parts' order.  All
-// latency at a few rows: the first sixteen parts are on their way before the
-// weights are known.
-template <int DT, int D>
+// LPR lanes a row, at least as many as parts: the parts' maxima and sums one to a lane, their outputs with weights
+// 2^(m_s - M) summed in the parts' order.  At a few rows it is all latency: the first parts are on their way before the
+// weights are known.  16 lanes for up to 16 parts of 4096 rows or more, which wide loads serve better than many waves (with
+// 64 lanes -> 16, us of the whole call: 29000 rows of 64, 3 parts 62.7 -> 57.7; 16000 of 128, 2 parts 50.9 -> 48.4; but 1200
+// of 128, 5 parts 16.5 -> 16.8, and 32, 7 parts 9.8 -> 10.0), else 64.
+template <int DT, int D, int LPR>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
-  constexpr int U = 16, DL = D / 64;
+  constexpr int U = LPR == 16 ? 8 : 16, DL = D / LPR, RPW = 64 / LPR;
   const lbfq_paged_params& p = a.p;
-  const uint32_t row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t Hq = static_cast<uint32_t>(p.Hq);
-  const int64_t R = p.T * p.Hq;
-  if (row >= R) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, sub = lane / LPR, li = lane % LPR;
+  const uint32_t wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t Hq = static_cast<uint32_t>(p.Hq), R = static_cast<uint32_t>(p.T * p.Hq);  // below 2^30
+  if (wave * RPW >= R) return;
+  const bool there = wave * RPW + sub < R;  // rows past the last repeat it and are not stored
+  const uint32_t row = there ? wave * RPW + sub : R - 1;
   const int tok = static_cast<int>(row / Hq);
   const int h = static_cast<int>(row - tok * Hq);
   float2 x = make_float2(-INFINITY, 0.0f);
-  if (lane < a.splits) x = a.ml[lane * R + row];
-  const float* src = a.acc + static_cast<int64_t>(row) * D + lane * DL;
+  if (li < a.splits) x = a.ml[static_cast<int64_t>(li) * R + row];
+  const float* src = a.acc + static_cast<int64_t>(row) * D + li * DL;
   float y[U][DL];
   auto load = [&](int s0) {
 #pragma unroll
     for (int i = 0; i < U; ++i)
       if (s0 + i < a.splits) {
+        const float* from = src + static_cast<int64_t>(s0 + i) * R * D;
+        if constexpr (DL % 4 == 0) {
 #pragma unroll
-        for (int k = 0; k < DL; ++k) y[i][k] = src[(s0 + i) * R * D + k];
+          for (int k = 0; k < DL; k += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(from + k);
+            y[i][k] = v.x; y[i][k + 1] = v.y; y[i][k + 2] = v.z; y[i][k + 3] = v.w;
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < DL; ++k) y[i][k] = from[k];
+        }
       }
   };
   load(0);
   const bool mine = tok >= p.query_starts[0] && tok < p.query_starts[p.B];
   const bool some = mine && filled(x.y);  // else nothing in this part, and its outputs were not written
-  const float M = wave_max(some ? x.x : -INFINITY);
+  const float M = lanes_max<LPR>(some ? x.x : -INFINITY);
   const float f = some ? __builtin_amdgcn_exp2f(x.x - M) : 0.0f;
-  const float l = wave_add(some ? x.y * f : 0.0f);
+  const float l = lanes_add<LPR>(some ? x.y * f : 0.0f);
   float o[DL];
 #pragma unroll
   for (int k = 0; k < DL; ++k) o[k] = 0.0f;
@@ -1129,18 +1142,29 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
 #pragma unroll
     for (int i = 0; i < U; ++i)
       if (s0 + i < a.splits) {
-        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + i));
+        float w;
+        if constexpr (LPR == 64) w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s0 + i));
+        else w = __shfl(f, sub * LPR + s0 + i, 64);
 #pragma unroll
         for (int k = 0; k < DL; ++k) o[k] = filled(w) ? fmaf(y[i][k], w, o[k]) : o[k];
       }
   }
+  if (!there) return;
   const float inv = filled(l) ? 1.0f / l : 0.0f;
   if (mine || p.fill_rest) {
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + lane * DL;
-    if constexpr (D == 128) *reinterpret_cast<uint32_t*>(dst) = pack_dt<DT>(o[0] * inv, o[1] * inv);
-    else *dst = static_cast<uint16_t>(pack_dt<DT>(o[0] * inv, 0.0f));
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + li * DL;
+    if constexpr (DL == 1) {
+      *dst = static_cast<uint16_t>(pack_dt<DT>(o[0] * inv, 0.0f));
+    } else {
+      uint32_t w[DL / 2];
+#pragma unroll
+      for (int k = 0; k < DL / 2; ++k) w[k] = pack_dt<DT>(o[2 * k] * inv, o[2 * k + 1] * inv);
+      if constexpr (DL == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      else if constexpr (DL == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(dst) = w[0];
+    }
   }
-  if (p.lse && lane == 0) p.lse[row] = row_lse(M, l);
+  if (p.lse && li == 0) p.lse[row] = row_lse(M, l);
 }
 
 // ---- host --------------------------------------------------------------------
@@ -1295,11 +1319,19 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   }
   LBFQ_LAUNCH_CHECK("lbfq_paged_attention");
   if (x.splits > 1) {
-    const dim3 gc(static_cast<unsigned>((R + 3) / 4)), block(256);
-    if (bf && d128) hipLaunchKernelGGL((paged_combine_kernel<kBF16, 128>), gc, block, 0, st, a);
-    else if (bf) hipLaunchKernelGGL((paged_combine_kernel<kBF16, 64>), gc, block, 0, st, a);
-    else if (d128) hipLaunchKernelGGL((paged_combine_kernel<kF16, 128>), gc, block, 0, st, a);
-    else hipLaunchKernelGGL((paged_combine_kernel<kF16, 64>), gc, block, 0, st, a);
+    const bool narrow = x.splits <= 16 && R >= 4096;
+    const int64_t per = narrow ? 16 : 4;  // rows of a workgroup
+    const dim3 gc(static_cast<unsigned>((R + per - 1) / per)), block(256);
+#define LBFQ_PJ(DT, DD)                                                                               \
+  do {                                                                                                \
+    if (narrow) hipLaunchKernelGGL((paged_combine_kernel<DT, DD, 16>), gc, block, 0, st, a);          \
+    else hipLaunchKernelGGL((paged_combine_kernel<DT, DD, 64>), gc, block, 0, st, a);                 \
+  } while (0)
+    if (bf && d128) LBFQ_PJ(kBF16, 128);
+    else if (bf) LBFQ_PJ(kBF16, 64);
+    else if (d128) LBFQ_PJ(kF16, 128);
+    else LBFQ_PJ(kF16, 64);
+#undef LBFQ_PJ
     LBFQ_LAUNCH_CHECK("lbfq_paged_attention (combine)");
   }
   return 0;

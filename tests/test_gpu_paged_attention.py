@@ -124,6 +124,16 @@ def test_many_ragged_sequences(gpu, B, most, hq, hk, d):
     run_and_check(args, f"{B} sequences", hint=most)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_rows_of_few_parts(gpu, d, dtype):
+    """Thousands of rows whose keys are split: several rows to a wave of the kernel that joins the parts."""
+    args = problem(gpu, lens=[5000, 3100, 40], counts=[601, 300, 50], hq=6, hk=2, d=d, dtype=dtype, page=64, tail=2,
+                   garbage=False)
+    run_and_check(args, "joined", hint=601)
+    run_and_check(args, "joined, no hint, window", window=900)
+
+
 @pytest.mark.parametrize("n", [3, 200])
 def test_rows_before_the_first_sequence(gpu, n):
     from low_bit_fake_quant import paged_attention

@@ -172,6 +172,10 @@ def test_only_what_is_asked_for(gpu):
     w = wq.detach().clone().requires_grad_()
     (g,) = torch.autograd.grad(qk_norm_rope(q, k, w, None, cos, sin, pos)[0], w, q)
     assert torch.equal(g, all_[2])
+    zero = gradients((q, k, wq, wk, cos, sin, pos), torch.zeros_like(q), k)
+    w = wk.detach().clone().requires_grad_()
+    (g,) = torch.autograd.grad(qk_norm_rope(q, k, None, w, cos, sin, pos)[1], w, k)  # the first weight is not given
+    assert torch.equal(g, zero[3])
     with torch.no_grad():
         assert not qk_norm_rope(x, k, w, wk, cos, sin, pos)[0].requires_grad
 
