@@ -984,6 +984,7 @@ __global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k], c, -ms));
                 const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k + 1], c, -ms));
                 l += p0 + p1;
+                asm volatile("" : "+v"(l));  // here: else all 32 are added up at the step's end, and wait in registers
                 w[k] = pack_f16(p0, p1);
               }
             } else {
