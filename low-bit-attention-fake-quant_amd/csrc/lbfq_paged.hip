@@ -547,8 +547,12 @@ struct Unit {
   bool wide;
 };
 
+// Workgroups of a CU: three where the registers do for that, at the price of a few that go to memory (1560 tokens over 32760
+// keys, 40 heads of 64, bf16: 818 us with two, 765 with three; fp16 queries need more of them: 745 with two, 1075).
+constexpr int chunk_groups(int dt, int64_t d) { return d == 64 && dt == kBF16 ? 3 : 2; }
+
 template <int DT, int D>
-__global__ void __launch_bounds__(256, 2) paged_chunk_kernel(const Args a) {
+__global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(const Args a) {
   constexpr int NW = 4, QB = kChunkRows, NT = 64 * NW;
   static_assert(QB == 32 * NW, "32 rows a wave");
   constexpr int NKS = D / 16, NDB = D / 32, CH = D / 32;
@@ -1185,13 +1189,13 @@ constexpr int kDecodeRows = 16;
 // decode: the 768 workgroups that run at a time at D = 128 (24 sequences of 2000 to 4000 keys, 8 key heads, 384 / 768 /
 // 1536: 50 / 38 / 43 us; 3 of up to 40000, 384 / 768 / 1152: 57 / 41 / 46).
 // chunk, one sequence: the parts that take the least time by a count of tiles.  A part costs the time of 12 tiles besides
-// its own (its start, and its sums written and read again), and an XCD has 64 workgroups at a time.  Row tiles that see
+// its own (its start, and its sums written and read again), and an XCD has two (or three) workgroups a CU at a time.  Row tiles that see
 // much the same keys go in whole rounds (us for 1 / 2 / 4 / 6 / 7 parts, * the rule's: 1560 tokens, 32760 keys, 40 heads
 // 2064 / 1585 / 1374 / 1356* / 1368; 700, 8000 keys, 12 heads 216 / 121 / 88 / 72* / 98).  A causal prompt's row tiles
 // differ, the longest first, and fill the rounds up; a workgroup that is left alone on its CU takes 0.7 times as long (1 /
 // 2 / 3 / 4 parts: 2500 tokens, 32 / 8 heads 91* / 127 / 144 / 158; 5000, 5 heads 145 / 94 / 74* / 85).
-// chunk, several: lengths differ, and more and shorter parts even them out.  With w workgroups in a part, w s / 512 + c
-// rounds of keys / (64 s) tiles + o each take the least time at s^2 = keys / w * 8 c / o; c / o = 1 / 12 fits (2 / 3 / 4 /
+// chunk, several: lengths differ, and more and shorter parts even them out.  With w workgroups in a part, w s / (8 places) + c
+// rounds of keys / (64 s) tiles + o each take the least time at s^2 = keys / w * places / 8 * c / o; c / o = 1 / 12 fits (2 / 3 / 4 /
 // 5 / 8 parts: 16 sequences of up to 64 tokens and 2000 keys 55* / 66 / 64 / 64 / 64; 8 of 128 and 4000 84 / 68* / 84 / 81
 // / 84; 4 of 700 and 9001, 12 heads 166 / 133 / 147 / 138* / 145; 2 of 1024 and 16000 535 / 524 / 502 / 530* / 547).
 Plan plan(const lbfq_paged_params* p) {
@@ -1207,6 +1211,7 @@ Plan plan(const lbfq_paged_params* p) {
   if (p->causal && p->window) keys = std::min(keys, p->window + std::min(most, kChunkRows / G + 1));
   const int64_t least = x.decode ? 192 : 128;
   const int64_t limit = std::min<int64_t>(keys / least, 64);  // (a lane each in the combine kernel)
+  const int64_t places = 32 * chunk_groups(p->dtype, p->D);  // for workgroups on an XCD
   int64_t s = 1;
   if (x.decode) {
     const int64_t wgs = p->B * p->Hk;
@@ -1217,12 +1222,12 @@ Plan plan(const lbfq_paged_params* p) {
     for (int64_t n = 1; n <= limit; ++n) {
       const int64_t of_xcd = (x.groups * p->Hk * n + 7) / 8 * x.piece, longest = keys / n + 12 * 64;
       const int64_t cost = uneven ? std::max(of_xcd * ((keys - most / 2) / n + 12 * 64), 45 * longest)
-                                  : (of_xcd + 63) / 64 * 64 * longest;
+                                  : (of_xcd + places - 1) / places * places * longest;
       if (cost < best) best = cost, s = n;
     }
   } else {
     const int64_t wgs = (tiles + p->B / 2) * p->Hk;
-    while (3 * (s + 1) * (s + 1) * wgs <= 2 * keys && s < limit) ++s;
+    while (96 * (s + 1) * (s + 1) * wgs <= places * keys && s < limit) ++s;
   }
   x.splits = static_cast<int>(std::max<int64_t>(std::min(s, limit), 1));
   x.least = static_cast<int>(least / (x.decode ? 32 : 64));
