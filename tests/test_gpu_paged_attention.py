@@ -333,6 +333,26 @@ def test_graph_replays_two_graphs_and_streams(gpu, n, L):
             assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1]), rep
 
 
+@pytest.mark.parametrize("n,L", [(4, 700), (90, 700)])
+def test_a_replay_with_other_chunk_lengths(gpu, n, L):
+    """The split of the tokens over the sequences is read on the device: a captured call follows it."""
+    from low_bit_fake_quant import paged_attention
+    a = problem(gpu, lens=[L, L // 2, L], counts=[n, n, n], hq=8, seed=3, garbage=False)
+    call = lambda: paged_attention(*a, max_query_len=3 * n, return_lse=True)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = call()
+    for starts in ((0, n, 2 * n, 3 * n), (0, 0, 3 * n, 3 * n), (0, 1, 2, 3 * n - 1), (1, 2 * n, 2 * n, 2 * n + 1)):
+        a[4].copy_(torch.tensor(starts, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        want = call()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), starts
+        ref.check(got[0], *[x for i, x in enumerate(ref.attend(*a)) if i in (0, 2)], str(starts))
+
+
 def test_repeated_calls_give_the_same_bits(gpu):
     from low_bit_fake_quant import paged_attention
     for n, L in ((1, 6000), (64, 2000), (500, 500)):
