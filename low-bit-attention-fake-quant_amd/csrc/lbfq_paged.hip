@@ -256,7 +256,8 @@ __device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int 
   for (int t = 0; t < 2; ++t) {
     x.ok[t] = pages[t] >= 0 && pages[t] < p.num_pages;
     const int page = x.ok[t] ? pages[t] : 0;
-    row[t] = (static_cast<int64_t>(page * static_cast<int>(p.Hk) + kvh) << p.page_shift) + ((kb + 16 * t) & ((1 << p.page_shift) - 1));
+    row[t] = (static_cast<int64_t>(page * static_cast<int>(p.Hk) + kvh) << p.page_shift) +
+             ((kb + 16 * t) & ((1 << p.page_shift) - 1));
     const uint8_t* kr = p.k_codes + row[t] * D + (n * D + 16 * g);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) x.k[t][c] = *reinterpret_cast<const uint4*>(kr + 64 * c);
@@ -1183,21 +1184,22 @@ struct Plan {
 constexpr int kDecodeRows = 16;
 
 // Parts of the keys, of 192 at least in decode (one token over 5003 keys, 8 key heads, parts of 128 / 192 / 256 / 512: 12.5 /
-// 12.0 / 13.1 / 15.5 us) and 128 in chunks (100 tokens over 700 keys, 12 heads, 128 / 256 / 512: 18 / 22 / 26).  The lengths are on the device: the rule goes by the table's width, and a shorter
-// sequence's parts are shorter, or fewer.
+// 11.9 / 12.8 / 15.3 us) and 128 in chunks (100 tokens over 700 keys, 12 heads, 128 / 256 / 512: 16 / 20 / 23).  The lengths
+// are on the device: the rule goes by the table's width, and a shorter sequence's parts are shorter, or fewer.
 //
 // decode: the 768 workgroups that run at a time at D = 128 (24 sequences of 2000 to 4000 keys, 8 key heads, 384 / 768 /
-// 1536: 50 / 38 / 43 us; 3 of up to 40000, 384 / 768 / 1152: 57 / 41 / 46).
+// 1536: 51 / 39 / 44 us; 3 of up to 40000, 384 / 768 / 1152: 57 / 41 / 46).
 // chunk, one sequence: the parts that take the least time by a count of tiles.  A part costs the time of 12 tiles besides
-// its own (its start, and its sums written and read again), and an XCD has two (or three) workgroups a CU at a time.  Row tiles that see
-// much the same keys go in whole rounds (us for 1 / 2 / 4 / 6 / 7 parts, * the rule's: 1560 tokens, 32760 keys, 40 heads
-// 2064 / 1585 / 1374 / 1356* / 1368; 700, 8000 keys, 12 heads 216 / 121 / 88 / 72* / 98).  A causal prompt's row tiles
-// differ, the longest first, and fill the rounds up; a workgroup that is left alone on its CU takes 0.7 times as long (1 /
-// 2 / 3 / 4 parts: 2500 tokens, 32 / 8 heads 91* / 127 / 144 / 158; 5000, 5 heads 145 / 94 / 74* / 85).
-// chunk, several: lengths differ, and more and shorter parts even them out.  With w workgroups in a part, w s / (8 places) + c
-// rounds of keys / (64 s) tiles + o each take the least time at s^2 = keys / w * places / 8 * c / o; c / o = 1 / 12 fits (2 / 3 / 4 /
-// 5 / 8 parts: 16 sequences of up to 64 tokens and 2000 keys 55* / 66 / 64 / 64 / 64; 8 of 128 and 4000 84 / 68* / 84 / 81
-// / 84; 4 of 700 and 9001, 12 heads 166 / 133 / 147 / 138* / 145; 2 of 1024 and 16000 535 / 524 / 502 / 530* / 547).
+// its own (its start, and its sums written and read again), and an XCD has two or three workgroups a CU at a time.  Row
+// tiles that see much the same keys go in whole rounds (us for 1 / 2 / 4 / 6 / 7 parts, * the rule's: 1560 tokens, 32760
+// keys, 40 heads 1717 / 1407 / 1295 / 1287* / 1288; 700, 8000 keys, 12 heads 168 / 96 / 81 / 68* / 86).  A causal prompt's
+// row tiles differ, the longest first, and fill the rounds up; a workgroup that is left alone on its CU takes 0.7 times as
+// long (1 / 2 / 3 / 4 parts: 2500 tokens, 32 / 8 heads 81* / 109 / 126 / 139; 5000, 5 heads 112 / 76 / 64* / 75).
+// chunk, several: lengths differ, and more and shorter parts even them out.  With w workgroups in a part, w s / (8 places)
+// + c rounds of keys / (64 s) tiles + o each take the least time at s^2 = keys / w * places / 8 * c / o; c / o = 1 / 10
+// fits (2 / 3 / 4 / 5 / 6 / 8 parts: 16 sequences of up to 64 tokens and 2000 keys 48* / 55 / 58 / 61 / 65 / 77; 8 of 128
+// and 4000 72 / 59 / 74* / 71 / 70 / 78; 4 of 700 and 9001, 12 heads 145 / 121 / 130 / 123 / 119* / 126; 2 of 1024 and
+// 16000 472 / 479 / 443 / 459* / 467 / 474).
 Plan plan(const lbfq_paged_params* p) {
   Plan x;
   const int64_t G = p->Hq / p->Hk;
@@ -1227,7 +1229,7 @@ Plan plan(const lbfq_paged_params* p) {
     }
   } else {
     const int64_t wgs = (tiles + p->B / 2) * p->Hk;
-    while (96 * (s + 1) * (s + 1) * wgs <= places * keys && s < limit) ++s;
+    while (80 * (s + 1) * (s + 1) * wgs <= places * keys && s < limit) ++s;
   }
   x.splits = static_cast<int>(std::max<int64_t>(std::min(s, limit), 1));
   x.least = static_cast<int>(least / (x.decode ? 32 : 64));
