@@ -66,7 +66,7 @@ struct Args {
   int64_t main;   // workgroups that attend (the others fill)
   float sml2;     // sm_scale * log2(e)
   float2* ml;     // (splits, T * Hq): maximum (log2 units) and sum of a part
-  float* acc;     // (splits, T * Hq, D)
+  float* acc;     // (splits, T * Hq, D): a part's average of the values
 };
 
 // One sequence, clamped to what the tensors hold.
@@ -286,6 +286,9 @@ __device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int 
   }
 }
 
+// What the decode kernel takes off a scale of V, in powers of two
+constexpr uint32_t kLess = 32;
+
 template <int DT, int D>
 __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
   constexpr int NC = D / 64, NB = D / 16, NW = 4;
@@ -428,7 +431,8 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
           uint32_t by;
           if constexpr (D == 128) by = x.vs[t][i] >> (8 * (n >> 2));
           else by = x.vs[t][i / 2] >> (16 * (i & 1) + 8 * (n >> 3));
-          const float e = __uint_as_float((by & 0xffu) << 23);
+          // times 2^-kLess: a sum of 2^30 of the largest values is then in fp32's range
+          const float e = __uint_as_float(__builtin_elementwise_sub_sat(by & 0xffu, kLess) << 23);
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
             vv[4 * t + i][2 * c] = cvt_bf16<false>(x.v[t][i][c], e);
@@ -486,8 +490,8 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
         }
         const int qq = (r0 + row) / G, hh = kvh * G + (r0 + row - qq * G);
         const int64_t tok = s.start + qq;
+        const float inv = filled(L) ? static_cast<float>(uint64_t{1} << kLess) / L : 0.0f;
         if (a.splits == 1) {
-          const float inv = filled(L) ? 1.0f / L : 0.0f;
           uint32_t w[NB / 2];
 #pragma unroll
           for (int k = 0; k < NB / 2; ++k) w[k] = pack_dt<DT>(o[2 * k] * inv, o[2 * k + 1] * inv);
@@ -502,7 +506,8 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
           if (filled(L)) {
 #pragma unroll
             for (int k = 0; k < NB; k += 4)
-              *reinterpret_cast<float4*>(a.acc + at * D + part * NB + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              *reinterpret_cast<float4*>(a.acc + at * D + part * NB + k) =
+                  make_float4(o[k] * inv, o[k + 1] * inv, o[k + 2] * inv, o[k + 3] * inv);
           }
         }
       }
@@ -542,7 +547,11 @@ __device__ __forceinline__ uint32_t span_add(uint32_t span, uint32_t v) {
 // What the values of a part's K or V are multiplied by, 2^(134 - E), on their way to fp16, so that the largest
 // code lands at 57344.  The smallest one, 2^-9, with a scale 2^-22 of the largest is then fp16's smallest step: within
 // that span every value is exact.  A part whose scales are further apart is `wide`: bf16, as they are.
+//
+// (A wide part's V is taken down by a power of two where its largest scale is past kWideTop: weights of up to 2^15 times
+// 2^30 of the largest values that are left, under 2^(kWideTop - 118), add up to less than 2^127.)
 constexpr int kSpan = 22;
+constexpr int kWideTop = 200;
 struct Unit {
   int E;
   bool wide;
@@ -731,16 +740,17 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
         sk = span_join(sk, red[NW + w]);
       }
       __syncthreads();
-      auto unit = [&](uint32_t x) {
+      auto unit = [&](uint32_t x, int wide) {
         x = __builtin_amdgcn_readfirstlane(x);
         Unit u;
         u.E = static_cast<int>(x & 0xffu);
         u.wide = u.E - (255 - static_cast<int>(x >> 16)) > kSpan;
-        if (u.wide || x == 0) u.E = 134;
+        if (u.wide) u.E = u.E > wide ? 134 + u.E - wide : 134;
+        if (x == 0) u.E = 134;
         return u;
       };
-      uv = unit(sv);
-      if constexpr (DT == kF16) uk = unit(sk);
+      uv = unit(sv, kWideTop);
+      if constexpr (DT == kF16) uk = unit(sk, 255);
     }
     const float c = DT == kF16 ? ldexpf(a.sml2, uk.E - 134) : a.sml2;
     const uint32_t kadd = static_cast<uint32_t>(134 - uk.E) << 23, vadd = static_cast<uint32_t>(134 - uv.E) << 23;
@@ -788,7 +798,8 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
           uint32_t by;
           if constexpr (CH == 4) by = __builtin_amdgcn_ubfe(vse[j], 8 * (vdq / 8), 8);
           else by = __builtin_amdgcn_ubfe(vse[j / 2], 16 * (j & 1) + 8 * (vdq / 8), 8);
-          const float sc = __uint_as_float((by << 23) + (WIDE ? 0u : vadd));
+          // (WIDE: far below the largest, a scale may be less than what is taken off)
+          const float sc = __uint_as_float(WIDE ? __builtin_elementwise_sub_sat(by << 23, 0u - vadd) : (by << 23) + vadd);
           st.v[j][0] = WIDE ? cvt_bf16<false>(vc[j], sc) : cvt_f16<false>(vc[j], sc);
           st.v[j][1] = WIDE ? cvt_bf16<true>(vc[j], sc) : cvt_f16<true>(vc[j], sc);
         }
@@ -1036,11 +1047,10 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
     }
     l = add_x32(l);
   }
-  const float back = ldexpf(1.0f, uv.E - 134);
   if (rw + li < rows) {
     const int64_t tok = s.start + qi;
     const bool one = a.splits == 1;
-    const float f = one ? (filled(l) ? back / l : 0.0f) : back;
+    const float f = filled(l) ? ldexpf(1.0f, uv.E - 134) / l : 0.0f;
     const int64_t at = split * R + tok * p.Hq + h;
     if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
     if (!one && g == 0) a.ml[at] = make_float2(m, l);
@@ -1096,8 +1106,8 @@ __device__ __forceinline__ float lanes_add(float v) {
   return LPR == 64 ? add_x32(add_x16(v)) : v;
 }
 
-// LPR lanes a row, at least as many as parts: the parts' maxima and sums one to a lane, their outputs with weights
-// 2^(m_s - M) summed in the parts' order.  At a few rows it is all latency: the first parts are on their way before the
+// LPR lanes a row, at least as many as parts: the parts' maxima and sums one to a lane, their outputs, each an average of
+// its values, summed in the parts' order with weights l_s 2^(m_s - M) / l that add up to one.  At a few rows it is all latency: the first parts are on their way before the
 // weights are known.  16 lanes for up to 16 parts of 4096 rows or more, which wide loads serve better than many waves (with
 // 64 lanes -> 16, us of the whole call: 29000 rows of 64, 3 parts 62.7 -> 57.7; 16000 of 128, 2 parts 50.9 -> 48.4; but 1200
 // of 128, 5 parts 16.5 -> 16.8, and 32, 7 parts 9.8 -> 10.0), else 64.
@@ -1138,8 +1148,9 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
   const bool mine = tok >= p.query_starts[0] && tok < p.query_starts[p.B];
   const bool some = mine && filled(x.y);  // else nothing in this part, and its outputs were not written
   const float M = lanes_max<LPR>(some ? x.x : -INFINITY);
-  const float f = some ? __builtin_amdgcn_exp2f(x.x - M) : 0.0f;
-  const float l = lanes_add<LPR>(some ? x.y * f : 0.0f);
+  const float part = some ? x.y * __builtin_amdgcn_exp2f(x.x - M) : 0.0f;
+  const float l = lanes_add<LPR>(part);
+  const float f = filled(l) ? part / l : 0.0f;
   float o[DL];
 #pragma unroll
   for (int k = 0; k < DL; ++k) o[k] = 0.0f;
@@ -1156,15 +1167,14 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
       }
   }
   if (!there) return;
-  const float inv = filled(l) ? 1.0f / l : 0.0f;
   if (mine || p.fill_rest) {
     uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + li * DL;
     if constexpr (DL == 1) {
-      *dst = static_cast<uint16_t>(pack_dt<DT>(o[0] * inv, 0.0f));
+      *dst = static_cast<uint16_t>(pack_dt<DT>(o[0], 0.0f));
     } else {
       uint32_t w[DL / 2];
 #pragma unroll
-      for (int k = 0; k < DL / 2; ++k) w[k] = pack_dt<DT>(o[2 * k] * inv, o[2 * k + 1] * inv);
+      for (int k = 0; k < DL / 2; ++k) w[k] = pack_dt<DT>(o[2 * k], o[2 * k + 1]);
       if constexpr (DL == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
       else if constexpr (DL == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
       else *reinterpret_cast<uint32_t*>(dst) = w[0];
