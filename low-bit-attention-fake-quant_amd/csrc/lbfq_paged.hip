@@ -1230,10 +1230,11 @@ Plan plan(const lbfq_paged_params* p) {
     s = (768 + wgs / 2) / wgs;
   } else if (p->B == 1) {
     const bool uneven = p->causal && !p->window && 2 * most > keys;
+    const int64_t seeing = std::min(most, keys);  // (a padded buffer has more tokens than the table has keys)
     int64_t best = std::numeric_limits<int64_t>::max();
     for (int64_t n = 1; n <= limit; ++n) {
       const int64_t of_xcd = (x.groups * p->Hk * n + 7) / 8 * x.piece, longest = keys / n + 12 * 64;
-      const int64_t cost = uneven ? std::max(of_xcd * ((keys - most / 2) / n + 12 * 64), 45 * longest)
+      const int64_t cost = uneven ? std::max(of_xcd * ((keys - seeing / 2) / n + 12 * 64), 45 * longest)
                                   : (of_xcd + places - 1) / places * places * longest;
       if (cost < best) best = cost, s = n;
     }
