@@ -1193,6 +1193,12 @@ struct Plan {
 
 constexpr int kDecodeRows = 16;
 
+// Bytes of a row in each part: its average and its maximum and sum.  Parts are not made beyond a workspace of kMostBytes (a
+// token buffer may be padded; those of calls that fill it take tens of MiB), one part needs none.  That also keeps the
+// rows of a call in parts under the 2^26 waves that may join them.
+int64_t part_bytes(const lbfq_paged_params* p) { return p->T * p->Hq * (static_cast<int64_t>(sizeof(float2)) + p->D * 4); }
+constexpr int64_t kMostBytes = (int64_t{1} << 30) - 16;
+
 // Parts of the keys, of 192 at least in decode (one token over 5003 keys, 8 key heads, parts of 128 / 192 / 256 / 512: 12.5 /
 // 11.9 / 12.8 / 15.3 us) and 128 in chunks (100 tokens over 700 keys, 12 heads, 128 / 256 / 512: 16 / 20 / 23).  The lengths
 // are on the device: the rule goes by the table's width, and a shorter sequence's parts are shorter, or fewer.
@@ -1222,7 +1228,8 @@ Plan plan(const lbfq_paged_params* p) {
   int64_t keys = p->table_cols << p->page_shift;  // that a row tile may see
   if (p->causal && p->window) keys = std::min(keys, p->window + std::min(most, kChunkRows / G + 1));
   const int64_t least = x.decode ? 192 : 128;
-  const int64_t limit = std::min<int64_t>(keys / least, 64);  // (a lane each in the combine kernel)
+  // (a lane each in the combine kernel)
+  const int64_t limit = std::min({keys / least, int64_t{64}, kMostBytes / part_bytes(p)});
   const int64_t places = 32 * chunk_groups(p->dtype, p->D);  // for workgroups on an XCD
   int64_t s = 1;
   if (x.decode) {
@@ -1248,9 +1255,7 @@ Plan plan(const lbfq_paged_params* p) {
 }
 
 int64_t workspace(const lbfq_paged_params* p, const Plan& x) {
-  if (x.splits == 1) return 0;
-  const int64_t R = p->T * p->Hq;
-  return x.splits * R * (static_cast<int64_t>(sizeof(float2)) + p->D * 4) + 16;
+  return x.splits == 1 ? 0 : x.splits * part_bytes(p) + 16;
 }
 
 int check_sizes(const lbfq_paged_params* p) {
@@ -1314,7 +1319,7 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   // (a launch has fewer than 2^32 threads)
   const int64_t combos = (x.decode ? p->B : x.splits) * p->Hk;
   a.main = x.decode ? combos * x.splits : (x.groups * combos + 7) / 8 * 8 * x.piece;
-  LBFQ_CHECK_ARG(a.main < (1 << 24) - 8 && (x.splits == 1 || R < (1 << 26)), "lbfq_paged_attention: problem too large");
+  LBFQ_CHECK_ARG(a.main < (1 << 24) - 8, "lbfq_paged_attention: problem too large");
   a.combos = static_cast<uint32_t>(combos);
   a.piece = static_cast<uint32_t>(x.piece);
   // rows that no sequence has: the combine kernel sees every row, otherwise some workgroups more

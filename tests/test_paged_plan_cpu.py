@@ -1,5 +1,6 @@
 """How many parts paged attention cuts the keys into, seen by the workspace that it asks
-for: no more where the token buffer is padded or nothing is said of its sequence's length."""
+for: no more where the token buffer is padded or nothing is said of its sequence's
+length, and none that would make a call too large."""
 
 import ctypes
 import os
@@ -7,6 +8,7 @@ import os
 import pytest
 
 FAKE = 0x1000
+GIB = 1 << 30
 
 
 @pytest.fixture
@@ -30,6 +32,23 @@ def need(lib, T, keys, *, B=1, hint=0, hq=32, hk=8, d=128, causal=1, window=0, p
 def test_a_padded_buffer_of_one_sequence_needs_no_more_parts(lib, T, keys):
     """The row tiles of the buffer fill the chip by themselves."""
     assert need(lib, T, keys) == need(lib, T, keys, hint=keys) == 0
+
+
+@pytest.mark.parametrize("causal", [0, 1])
+@pytest.mark.parametrize("B", [1, 3, 64])
+@pytest.mark.parametrize("hint", [0, 1, 4, 100])
+def test_the_workspace_is_bounded(lib, hint, B, causal):
+    for T in (B, 100, 1000, 4097, 50000, 1 << 20):
+        for keys in (64, 1024, 32768, 1 << 20):
+            for window in (0, 512):
+                assert 0 <= need(lib, T, keys, B=B, hint=hint, causal=causal, window=window) <= GIB, (T, keys, window)
+
+
+def test_calls_of_2_26_rows_and_more_are_taken_in_one_part(lib):
+    """(several parts would be refused: the launch that joins them has a wave a row)"""
+    for B, hint in ((1, 0), (1, 1), (2, 0), (5, 1)):
+        assert need(lib, 1 << 21, 1 << 20, B=B, hint=hint) == 0
+        assert need(lib, 1 << 21, 1 << 20, B=B, hint=hint, window=100) == 0
 
 
 def test_calls_that_need_parts_have_them(lib):
