@@ -1107,10 +1107,10 @@ __device__ __forceinline__ float lanes_add(float v) {
 }
 
 // LPR lanes a row, at least as many as parts: the parts' maxima and sums one to a lane, their outputs, each an average of
-// its values, summed in the parts' order with weights l_s 2^(m_s - M) / l that add up to one.  At a few rows it is all latency: the first parts are on their way before the
-// weights are known.  16 lanes for up to 16 parts of 4096 rows or more, which wide loads serve better than many waves (with
-// 64 lanes -> 16, us of the whole call: 29000 rows of 64, 3 parts 62.7 -> 57.7; 16000 of 128, 2 parts 50.9 -> 48.4; but 1200
-// of 128, 5 parts 16.5 -> 16.8, and 32, 7 parts 9.8 -> 10.0), else 64.
+// its values, summed in the parts' order with weights l_s 2^(m_s - M) / l that add up to one.  At a few rows it is all
+// latency: the first parts are on their way before the weights are known.  16 lanes for up to 16 parts of 4096 rows or
+// more, which wide loads serve better than many waves (with 64 lanes -> 16, us of the whole call: 29000 rows of 64, 3 parts
+// 62.7 -> 57.7; 16000 of 128, 2 parts 50.9 -> 48.4; but 1200 of 128, 5 parts 16.5 -> 16.8, and 32, 7 parts 9.8 -> 10.0), else 64.
 template <int DT, int D, int LPR>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
   constexpr int U = LPR == 16 ? 8 : 16, DL = D / LPR, RPW = 64 / LPR;
@@ -1212,10 +1212,13 @@ constexpr int64_t kMostBytes = (int64_t{1} << 30) - 16;
 // row tiles differ, the longest first, and fill the rounds up; a workgroup that is left alone on its CU takes 0.7 times as
 // long (1 / 2 / 3 / 4 parts: 2500 tokens, 32 / 8 heads 81* / 109 / 126 / 139; 5000, 5 heads 112 / 76 / 64* / 75).
 // chunk, several: lengths differ, and more and shorter parts even them out.  With w workgroups in a part, w s / (8 places)
-// + c rounds of keys / (64 s) tiles + o each take the least time at s^2 = keys / w * places / 8 * c / o; c / o = 1 / 10
-// fits (2 / 3 / 4 / 5 / 6 / 8 parts: 16 sequences of up to 64 tokens and 2000 keys 48* / 55 / 58 / 61 / 65 / 77; 8 of 128
-// and 4000 72 / 59 / 74* / 71 / 70 / 78; 4 of 700 and 9001, 12 heads 145 / 121 / 130 / 123 / 119* / 126; 2 of 1024 and
-// 16000 472 / 479 / 443 / 459* / 467 / 474).
+// + c rounds of keys / (64 s) tiles + o each take the least time at s^2 = keys / w * places / 8 * c / o.  c / o = 1 / 15: over
+// 25 batches of 2 to 16 sequences, up to 3000 new tokens and 20000 keys, the parts of 1 / 10, 12, 14, 15, 16 take 7.6, 5.2,
+// 6.4, 4.4 and 3.9% longer than the best of them, but 1 / 16 gives the last call named here two parts (us for 1 / 2 / 3 / 4 / 5 /
+// 6 / 8 parts, * the rule's: 16 sequences of up to 64 tokens and 2000 keys 51 / 48* / 54 / 56 / 61 / 65 / 77; 8 of 128 and 4000 90 /
+// 71 / 57* / 72 / 69 / 67 / 76; 4 of 700 and 9001, 12 heads 192 / 142 / 117 / 127 / 120* / 115 / 123; 2 of 1024 and 16000 475 /
+// 469 / 474 / 432* / 449 / 457 / 468; 2 of 300 and 5000 111 / 70 / 68 / 63* / 76 / 76 / 77; 4 of 509, fp16, window 4096 77 / 63 /
+// 53* / 52 / 58 / 58 / 66).
 Plan plan(const lbfq_paged_params* p) {
   Plan x;
   const int64_t G = p->Hq / p->Hk;
@@ -1247,7 +1250,7 @@ Plan plan(const lbfq_paged_params* p) {
     }
   } else {
     const int64_t wgs = (tiles + p->B / 2) * p->Hk;
-    while (80 * (s + 1) * (s + 1) * wgs <= places * keys && s < limit) ++s;
+    while (120 * (s + 1) * (s + 1) * wgs <= places * keys && s < limit) ++s;
   }
   x.splits = static_cast<int>(std::max<int64_t>(std::min(s, limit), 1));
   x.least = static_cast<int>(least / (x.decode ? 32 : 64));

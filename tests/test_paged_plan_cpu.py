@@ -57,3 +57,10 @@ def test_calls_that_need_parts_have_them(lib):
     assert need(lib, 1, 1 << 16, hint=1) >= 32 * row * 32
     assert need(lib, 100, 1 << 16) >= 3200 * row * 16
     assert need(lib, 2048, 1 << 16, B=2) >= 2048 * 32 * row * 2
+
+
+@pytest.mark.parametrize("B,T,keys,hq,hk,parts", [(16, 485, 2048, 32, 8, 2), (8, 477, 4032, 32, 8, 3), (2, 1421, 16000, 32, 8, 4),
+                                                  (2, 432, 5056, 32, 8, 4)])
+def test_parts_of_several_sequences_are_the_fastest(lib, B, T, keys, hq, hk, parts):
+    """(the times of 1 to 8 parts stand above the rule)"""
+    assert need(lib, T, keys, B=B, hq=hq, hk=hk) == parts * T * hq * (4 * 128 + 8) + 16
