@@ -6,12 +6,14 @@
 // liblbfq_hip.so, which this module links to.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <limits>
 #include <optional>
 #include <string>
@@ -97,6 +99,15 @@ int64_t row_stride(const Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.st
 
 bool on(const Tensor& t, int64_t index) { return t.is_cuda() && t.get_device() == index; }
 std::string cuda(int64_t index) { return "cuda:" + std::to_string(index); }
+
+// Forward mode: a dual tensor does not say requires_grad(), and an output without a tangent counts as one of zero.
+// (torch.no_grad leaves this mode on.)
+void refuse_tangent(const char* what, std::initializer_list<const Tensor*> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : inputs)
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined())
+      bad_value(std::string(what) + " has no forward-mode derivative; call it on the primal parts of its inputs");
+}
 
 // ---- Q/K norm and rotation -----------------------------------------------------
 
@@ -281,6 +292,8 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 
 std::tuple<Tensor, Tensor> norm(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& cos,
                                 const Tensor& sin, const OptTensor& positions, double eps, const std::string& pairs) {
+  const Tensor none;
+  refuse_tangent("qk_norm_rope", {&q, &k, qw ? &*qw : &none, kw ? &*kw : &none, &cos, &sin});
   if (at::GradMode::is_enabled()) {
     if (cos.requires_grad() || sin.requires_grad())
       bad_value("qk_norm_rope has no gradient for cos and sin; detach them");
@@ -368,6 +381,7 @@ void kv_write(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Tensor
   p.dtype = dtype_code(k_.scalar_type());
   const Tensor slots = index_tensor(slots_, "slots", k_.size(0), c.index, at::kLong);
   if (at::GradMode::is_enabled() && (k_.requires_grad() || v_.requires_grad())) refuse_grad("write_kv_cache");
+  refuse_tangent("write_kv_cache", {&k_, &v_});
   if (k_.size(0) == 0) return;
   On dev(k_);
   const Tensor k = aligned(k_), v = aligned(v_);
@@ -432,6 +446,7 @@ std::tuple<Tensor, OptTensor> attention(const Tensor& q_, const Tensor& kc, cons
   if (max_query_len && *max_query_len < 0)
     bad_value("max_query_len must not be negative; got " + std::to_string(*max_query_len));
   if (at::GradMode::is_enabled() && q_.requires_grad()) refuse_grad("paged_attention");
+  refuse_tangent("paged_attention", {&q_});
   if (out_) {
     if (out_->sizes() != q_.sizes() || out_->scalar_type() != q_.scalar_type() || !on(*out_, c.index))
       bad_value("out must be " + str(q_) + " " + name(q_.scalar_type()) + " on " + cuda(c.index) + "; got " + str(*out_) +
@@ -440,6 +455,7 @@ std::tuple<Tensor, OptTensor> attention(const Tensor& q_, const Tensor& kc, cons
     for (int64_t i = 0; i < 2; ++i) distinct = distinct && (out_->size(i) <= 1 || out_->stride(i) != 0);
     if (!distinct) bad_value("out must have contiguous, distinct rows that start on 16-byte boundaries");
     if (at::GradMode::is_enabled() && out_->requires_grad()) refuse_grad("paged_attention");
+    refuse_tangent("paged_attention", {&*out_});
   }
   On dev(q_);
   const Tensor out = out_ ? *out_ : at::empty(q_.sizes(), q_.options());

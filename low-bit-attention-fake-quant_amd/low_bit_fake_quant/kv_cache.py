@@ -6,8 +6,8 @@ in pages that sequences take as they grow.  ``write_kv_cache`` quantises new row
 it, ``paged_attention`` attends over it (one token of each sequence, or a chunk),
 ``read_kv_cache`` gives the values back, e.g. for ``fake_quant_attention``.
 
-These are for inference: they have no backward pass and refuse inputs that ask
-for one.  No call synchronises; all of them can be captured in a HIP graph.
+These are for inference: they have no derivative, backward or forward, and refuse inputs that
+ask for one.  No call synchronises; all of them can be captured in a HIP graph.
 Arguments are checked in ``csrc/lbfq_torch.cpp``.
 """
 

@@ -43,7 +43,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
 
     Arithmetic is fp32 with one rounding at the end.  Gradients reach q, k and the
     weights (``cos`` and ``sin`` take none); the weights' sums have a fixed order.  A
-    second derivative is refused.
+    second derivative and forward mode are refused.
     Returns new contiguous tensors of the inputs' shapes and dtype.
     """
     return _lib.torch_ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, pairs)
