@@ -305,6 +305,11 @@ std::tuple<Tensor, Tensor> norm(const Tensor& q, const Tensor& k, const OptTenso
   return norm_forward(q, k, qw, kw, cos, sin, positions, eps, pairs);
 }
 
+// A tensor was written in place: autograd is to know
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ---- the cache ---------------------------------------------------------------------
 
 struct Cache {
@@ -393,6 +398,7 @@ void kv_write(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Tensor
   p.slots = slots.data_ptr<int64_t>();
   c.set(p);
   check_rc(lbfq_kv_write(&p, stream(k)), "lbfq_kv_write");
+  for (const Tensor* t : {&kc, &ks, &vc, &vs}) written(*t);
 }
 
 std::tuple<Tensor, Tensor> kv_read(const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs,
@@ -493,7 +499,7 @@ std::tuple<Tensor, OptTensor> attention(const Tensor& q_, const Tensor& kc, cons
     p.workspace_bytes = need;
   }
   check_rc(lbfq_paged_attention(&p, stream(q)), "lbfq_paged_attention");
-  if (out_ && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();  // written in place: autograd is to know
+  if (out_) written(out);
   return {out, lse};
 }
 

@@ -60,3 +60,26 @@ def test_function_transforms_are_refused(gpu):
     for call in (lambda: torch.func.grad(f)(q), lambda: torch.func.jvp(f, (q,), (q,)), lambda: torch.func.vmap(f)(q[None])):
         with pytest.raises((RuntimeError, ValueError)):
             call()
+
+
+def test_a_cache_write_counts_as_a_change_in_place(gpu):
+    """A backward pass that needs what a cache tensor held before says so."""
+    from low_bit_fake_quant import empty_kv_cache, write_kv_cache
+    cache = empty_kv_cache(2, 16, 2, 64, device=gpu)
+    k, slots = torch.randn(3, 2, 64, device=gpu), torch.arange(3, device=gpu)
+    w = torch.ones(cache.k_scale.shape, device=gpu, requires_grad=True)
+    y = (w * cache.k_scale).sum()
+    versions = [t._version for t in cache]
+    write_kv_cache(k[:0], k[:0], cache, slots[:0])
+    assert [t._version for t in cache] == versions  # nothing written
+    write_kv_cache(k, k, cache, slots)
+    assert all(t._version > v for t, v in zip(cache, versions))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():  # tensors of that mode have no counter
+        own = empty_kv_cache(2, 16, 2, 64, device=gpu)
+        write_kv_cache(k, k, own, slots)
+        write_kv_cache(k, k, cache, slots)
+    write_kv_cache(k, k, own, slots)
+    for a, b in zip(own, cache):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
