@@ -100,6 +100,10 @@ int64_t row_stride(const Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.st
 bool on(const Tensor& t, int64_t index) { return t.is_cuda() && t.get_device() == index; }
 std::string cuda(int64_t index) { return "cuda:" + std::to_string(index); }
 
+void refuse_grad(const char* what) {
+  bad_value(std::string(what) + " has no backward pass; detach its inputs or call it under torch.no_grad()");
+}
+
 // Forward mode: a dual tensor does not say requires_grad(), and an output without a tangent counts as one of zero.
 // (torch.no_grad leaves this mode on.)
 void refuse_tangent(const char* what, std::initializer_list<const Tensor*> inputs) {
@@ -341,6 +345,11 @@ struct Cache {
     shift = __builtin_ctzll(static_cast<unsigned long long>(page));
   }
 
+  void refuse_derivatives(const char* what) const {
+    if (at::GradMode::is_enabled() && (kc.requires_grad() || vc.requires_grad())) refuse_grad(what);
+    refuse_tangent(what, {&kc, &vc});
+  }
+
   template <class P>
   void set(P& p) const {
     p.k_codes = static_cast<uint8_t*>(kc.data_ptr());
@@ -367,10 +376,6 @@ Tensor table_tensor(const Tensor& t, int64_t index) {
   return t.stride(1) == 1 ? t : t.contiguous();
 }
 
-void refuse_grad(const char* what) {
-  bad_value(std::string(what) + " has no backward pass; detach its inputs or call it under torch.no_grad()");
-}
-
 void kv_write(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs,
            const Tensor& slots_) {
   const Cache c(kc, ks, vc, vs);
@@ -386,6 +391,7 @@ void kv_write(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Tensor
   p.dtype = dtype_code(k_.scalar_type());
   const Tensor slots = index_tensor(slots_, "slots", k_.size(0), c.index, at::kLong);
   if (at::GradMode::is_enabled() && (k_.requires_grad() || v_.requires_grad())) refuse_grad("write_kv_cache");
+  c.refuse_derivatives("write_kv_cache");
   refuse_tangent("write_kv_cache", {&k_, &v_});
   if (k_.size(0) == 0) return;
   On dev(k_);
@@ -409,6 +415,7 @@ std::tuple<Tensor, Tensor> kv_read(const Tensor& kc, const Tensor& ks, const Ten
   const Tensor lens = index_tensor(seq_lens, "seq_lens", b, c.index, at::kInt);
   lbfq_kv_read_params p{};
   p.dtype = dtype_code(dtype);
+  c.refuse_derivatives("read_kv_cache");
   if (max_len < 0) bad_value("max_len must not be negative; got " + std::to_string(max_len));
   Tensor k = at::empty({b, max_len, c.heads, c.d}, kc.options().dtype(dtype)), v = at::empty_like(k);
   if (b && max_len) {
@@ -453,6 +460,7 @@ std::tuple<Tensor, OptTensor> attention(const Tensor& q_, const Tensor& kc, cons
     bad_value("max_query_len must not be negative; got " + std::to_string(*max_query_len));
   if (at::GradMode::is_enabled() && q_.requires_grad()) refuse_grad("paged_attention");
   refuse_tangent("paged_attention", {&q_});
+  c.refuse_derivatives("paged_attention");
   if (out_) {
     if (out_->sizes() != q_.sizes() || out_->scalar_type() != q_.scalar_type() || !on(*out_, c.index))
       bad_value("out must be " + str(q_) + " " + name(q_.scalar_type()) + " on " + cuda(c.index) + "; got " + str(*out_) +

@@ -83,3 +83,19 @@ def test_a_cache_write_counts_as_a_change_in_place(gpu):
     write_kv_cache(k, k, own, slots)
     for a, b in zip(own, cache):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("which", ["k_codes", "v_codes"])
+def test_a_cache_that_asks_for_a_gradient_is_refused(gpu, which):
+    from low_bit_fake_quant import paged_attention, read_kv_cache, write_kv_cache
+    q, cache, table, lens, starts = problem(gpu, lens=[20], counts=[2])
+    k, slots = torch.randn(2, 2, 128, device=gpu), torch.arange(2, device=gpu)
+    want = paged_attention(q, cache, table, lens, starts)
+    cache = cache._replace(**{which: getattr(cache, which).clone().requires_grad_()})
+    for call in (lambda: write_kv_cache(k, k, cache, slots), lambda: read_kv_cache(cache, table, lens, 20),
+                 lambda: paged_attention(q, cache, table, lens, starts)):
+        with pytest.raises(ValueError, match="no backward pass"):
+            call()
+    with torch.no_grad():
+        assert torch.equal(paged_attention(q, cache, table, lens, starts), want)
+        read_kv_cache(cache, table, lens, 20)
