@@ -17,6 +17,7 @@
 #include <limits>
 #include <optional>
 #include <string>
+#include <utility>
 
 #include "../../include/lbfq.h"
 
@@ -111,6 +112,24 @@ void refuse_tangent(const char* what, std::initializer_list<const Tensor*> input
   for (const Tensor* t : inputs)
     if (t->defined() && t->_fw_grad(/*level=*/0).defined())
       bad_value(std::string(what) + " has no forward-mode derivative; call it on the primal parts of its inputs");
+}
+
+// Whether no two of the rows of t (n0, n1, d), contiguous, share memory.  With strides s0 <= s1: rows that lie j s1 and i s0
+// from the first, i of the nearest two.  (One look where the rows of one dimension lie within a step of the other.)
+bool rows_apart(const Tensor& t) {
+  int64_t n0 = t.size(0), n1 = t.size(1), s0 = row_stride(t, 0), s1 = row_stride(t, 1);
+  const int64_t d = t.size(2);
+  if (n0 == 0 || n1 == 0) return true;
+  if (n0 == 1) std::swap(n0, n1), std::swap(s0, s1);
+  if (n0 == 1) return true;
+  if (n1 == 1) return s0 >= d;
+  if (s0 > s1) std::swap(n0, n1), std::swap(s0, s1);
+  if (s0 < d) return false;
+  for (int64_t j = 1; j < n1 && j * s1 < (n0 - 1) * s0 + d; ++j) {
+    const int64_t i = j * s1 / s0;
+    if ((i < n0 && j * s1 - i * s0 < d) || (i + 1 < n0 && (i + 1) * s0 - j * s1 < d)) return false;
+  }
+  return true;
 }
 
 // ---- Q/K norm and rotation -----------------------------------------------------
@@ -465,9 +484,8 @@ std::tuple<Tensor, OptTensor> attention(const Tensor& q_, const Tensor& kc, cons
     if (out_->sizes() != q_.sizes() || out_->scalar_type() != q_.scalar_type() || !on(*out_, c.index))
       bad_value("out must be " + str(q_) + " " + name(q_.scalar_type()) + " on " + cuda(c.index) + "; got " + str(*out_) +
                 " " + name(out_->scalar_type()) + " on " + out_->device().str());
-    bool distinct = rows_16b(*out_);
-    for (int64_t i = 0; i < 2; ++i) distinct = distinct && (out_->size(i) <= 1 || out_->stride(i) != 0);
-    if (!distinct) bad_value("out must have contiguous, distinct rows that start on 16-byte boundaries");
+    if (!rows_16b(*out_) || !rows_apart(*out_))
+      bad_value("out must have contiguous, distinct rows that start on 16-byte boundaries");
     if (at::GradMode::is_enabled() && out_->requires_grad()) refuse_grad("paged_attention");
     refuse_tangent("paged_attention", {&*out_});
   }
