@@ -333,6 +333,53 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// First byte of a tensor and the one behind its last.
+std::pair<int64_t, int64_t> extent(const Tensor& t) {
+  const int64_t at = reinterpret_cast<int64_t>(t.data_ptr());
+  int64_t n = 1;
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) == 0) return {at, at};
+    n += (t.size(i) - 1) * t.stride(i);
+  }
+  return {at, at + n * static_cast<int64_t>(t.element_size())};
+}
+
+// Whether, for some |i| < n0 and |j| < n1, i s0 + j s1 lies in (lo, hi): rows that are so far apart
+bool reached(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t lo, int64_t hi, bool both_ways) {
+  if (n0 < n1) std::swap(n0, n1), std::swap(s0, s1);
+  for (int64_t j = both_ways ? 1 - n1 : 0; j < n1; ++j) {
+    const int64_t from = both_ways ? 1 - n0 : 0, a = lo - j * s1, b = hi - j * s1;
+    if (s0 == 0) {
+      if (a < 0 && b > 0) return true;
+      continue;
+    }
+    int64_t i = a >= 0 ? a / s0 + 1 : 1 - (s0 - 1 - a) / s0;  // the least with i s0 > a
+    if (i < from) i = from;
+    if (i < n0 && i * s0 < b) return true;
+  }
+  return false;
+}
+
+// Whether a row of t (n0, n1, d) touches the bytes from x.first up to x.second.
+bool rows_touch(const Tensor& t, std::pair<int64_t, int64_t> x) {
+  const auto own = extent(t);
+  if (x.first == x.second || own.first >= x.second || x.first >= own.second) return false;
+  const int64_t e = static_cast<int64_t>(t.element_size());
+  return reached(t.size(0), row_stride(t, 0) * e, t.size(1), row_stride(t, 1) * e, x.first - own.first - t.size(2) * e,
+                 x.second - own.first, false);
+}
+
+// Whether out, whose rows are written while other rows of q are still to be read, may change those: it shares memory
+// with q, but not row by row (each is read before it is written).
+bool changes_queries(const Tensor& out, const Tensor& q) {
+  if (!rows_touch(out, extent(q))) return false;
+  for (int64_t i = 0; i < 2; ++i)
+    if (row_stride(out, i) != row_stride(q, i)) return true;
+  const int64_t e = static_cast<int64_t>(q.element_size()), row = q.size(2) * e;
+  const int64_t apart = extent(out).first - extent(q).first;
+  return apart != 0 && reached(q.size(0), row_stride(q, 0) * e, q.size(1), row_stride(q, 1) * e, apart - row, apart + row, true);
+}
+
 // ---- the cache ---------------------------------------------------------------------
 
 struct Cache {
@@ -498,7 +545,11 @@ std::tuple<Tensor, OptTensor> attention(const Tensor& q_, const Tensor& kc, cons
     if (lse) lse->fill_(-std::numeric_limits<float>::infinity());
     return {out, lse};
   }
-  const Tensor q = aligned(q_);
+  if (out_) {
+    for (const Tensor* x : {&c.kc, &c.ks, &c.vc, &c.vs, &table, &lens, &starts})
+      if (rows_touch(out, extent(*x))) bad_value("out must not share memory with the cache, block_table, seq_lens or query_starts");
+  }
+  const Tensor q = out_ && changes_queries(out, q_) ? q_.clone(at::MemoryFormat::Contiguous) : aligned(q_);
   lbfq_paged_params p{};
   p.q = q.data_ptr();
   p.dtype = dtype_code(q.scalar_type());

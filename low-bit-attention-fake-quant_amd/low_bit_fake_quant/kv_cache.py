@@ -103,7 +103,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Ten
     ``max_query_len``: the most new tokens of a sequence, if known; it sizes the
     launch; results do not depend on it beyond rounding.  ``sm_scale``: 1/sqrt(D) by default, in 2^-64 ... 2^15.
     ``out``: takes the result, rows of no sequence left as they are (in a new tensor
-    they are zero); it may not overlap the inputs.  ``return_lse``: also the natural
+    they are zero).  It may be ``q`` itself, or lie over parts of it (then q is copied
+    first); with the other inputs it shares no memory, nor do its rows overlap.  ``return_lse``: also the natural
     log of each row's sum of exponentials, fp32 (T, Hq), -inf for a row that sees
     nothing.
 
