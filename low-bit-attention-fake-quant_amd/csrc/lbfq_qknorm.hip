@@ -127,11 +127,12 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// What a lane needs of its token's rotation: c and s of its eight columns (1
-// and 0 past the rotated ones), and the lane its partners are in (HALVES).
+// What a lane needs of its token's rotation: whether its eight columns are rotated, their c and s, and the lane their
+// partners are in (HALVES).
 struct Turn {
   float c[8], s[8];
   int partner;
+  bool on;
 };
 
 template <int LPR, bool HALVES>
@@ -145,6 +146,7 @@ __device__ __forceinline__ Turn make_turn(const lbfq_qk_norm_params& p, int64_t 
   }
   Turn u;
   u.partner = lane;
+  u.on = false;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     u.c[k] = 1.0f;
@@ -153,6 +155,7 @@ __device__ __forceinline__ Turn make_turn(const lbfq_qk_norm_params& p, int64_t 
   if (d0 >= rot) return u;
   if constexpr (HALVES) u.partner = d0 < half ? lane + half / 8 : lane - half / 8;
   if (pos < 0) return u;  // padding: not rotated
+  u.on = true;
   if (pos >= p.table_len) {  // no such angle: loud, not out of bounds
 #pragma unroll
     for (int k = 0; k < 8; ++k) u.c[k] = u.s[k] = __builtin_nanf("");
@@ -186,7 +189,11 @@ __device__ __forceinline__ void turn(const Turn& u, float (&v)[8]) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) o[k] = HALVES ? __shfl(v[k], u.partner, 64) : v[k ^ 1];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = fmaf(v[k], u.c[k], o[k] * (BACK ? -u.s[k] : u.s[k]));
+  for (int k = 0; k < 8; ++k) {
+    // (a choice, not a rotation by 0: that would carry a neighbour's infinity or NaN over)
+    const float r = fmaf(v[k], u.c[k], o[k] * (BACK ? -u.s[k] : u.s[k]));
+    v[k] = u.on ? r : v[k];
+  }
 }
 
 // A lane's eight weights (ones without any); a weight vector may start anywhere.
