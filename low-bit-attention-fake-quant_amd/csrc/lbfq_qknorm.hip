@@ -127,6 +127,13 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
+// 1 / sqrt(v), v >= 0.  The instruction takes a number below the normal ones for 0.
+__device__ __forceinline__ float rsqrt_any(float v) {
+  const bool low = v < 0x1p-100f;
+  const float r = __builtin_amdgcn_rsqf(low ? v * 0x1p64f : v);
+  return low ? r * 0x1p32f : r;
+}
+
 // What a lane needs of its token's rotation: whether its eight columns are rotated, their c and s, and the lane their
 // partners are in (HALVES).
 struct Turn {
@@ -246,7 +253,7 @@ __global__ void __launch_bounds__(256) qk_norm_kernel(const Args a) {
         widen<DT>(raw[i], x);
 #pragma unroll
         for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
-        const float r = __builtin_amdgcn_rsqf(fmaf(row_sum<LPR>(ss), 1.0f / D, p.eps));
+        const float r = rsqrt_any(fmaf(row_sum<LPR>(ss), 1.0f / D, p.eps));
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = x[k] * r * (isq ? wq[k] : wk[k]);
         turn<HALVES, false>(u, x);
@@ -308,7 +315,7 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(const GradArgs ga) {
         }
         ss = row_sum<LPR>(ss);
         sx = row_sum<LPR>(sx);
-        const float r = __builtin_amdgcn_rsqf(fmaf(ss, 1.0f / D, p.eps));
+        const float r = rsqrt_any(fmaf(ss, 1.0f / D, p.eps));
         const float c = sx * (1.0f / D) * r * r;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
