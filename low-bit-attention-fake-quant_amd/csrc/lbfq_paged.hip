@@ -126,6 +126,7 @@ __device__ __forceinline__ int sequence_at(const lbfq_paged_params& p, int G, in
 }
 
 // Rows of the token dimension that no sequence has: zero (a new output), lse -inf.
+template <int D>
 __device__ void fill_rest(const lbfq_paged_params& p, int64_t wg, int64_t wgs) {
   int s0 = p.query_starts[0], s1 = p.query_starts[p.B];
   const int T = static_cast<int>(p.T);
@@ -134,9 +135,9 @@ __device__ void fill_rest(const lbfq_paged_params& p, int64_t wg, int64_t wgs) {
   const int rest = T - (s1 - s0);
   for (int64_t k = wg; k < rest; k += wgs) {
     const int64_t t = k < s0 ? k : k - s0 + s1;
-    for (int i = threadIdx.x; p.fill_rest && i < p.Hq * p.D / 2; i += blockDim.x) {
-      const int h = i / static_cast<int>(p.D / 2), d = i % static_cast<int>(p.D / 2);
-      reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + t * p.out_t + h * p.out_h)[d] = 0;
+    for (int i = threadIdx.x; p.fill_rest && i < p.Hq * (D / 8); i += blockDim.x) {
+      const int h = i / (D / 8), d = i % (D / 8);
+      reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + t * p.out_t + h * p.out_h)[d] = make_uint4(0, 0, 0, 0);
     }
     if (p.lse)
       for (int h = threadIdx.x; h < p.Hq; h += blockDim.x) p.lse[t * p.Hq + h] = -INFINITY;
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
   constexpr int NC = D / 64, NB = D / 16, NW = 4;
   const lbfq_paged_params& p = a.p;
   if (static_cast<int64_t>(blockIdx.x) >= a.main) {
-    fill_rest(p, blockIdx.x - a.main, gridDim.x - a.main);
+    fill_rest<D>(p, blockIdx.x - a.main, gridDim.x - a.main);
     return;
   }
   __shared__ __align__(16) float acc_s[NW][16][D + 4];
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
   using L = Lds<D>;
   const lbfq_paged_params& p = a.p;
   if (static_cast<int64_t>(blockIdx.x) >= a.main) {
-    fill_rest(p, blockIdx.x - a.main, gridDim.x - a.main);
+    fill_rest<D>(p, blockIdx.x - a.main, gridDim.x - a.main);
     return;
   }
   __shared__ __align__(16) uint8_t lds[2 * L::BUF];
@@ -1257,6 +1258,11 @@ Plan plan(const lbfq_paged_params* p) {
   return x;
 }
 
+// Workgroups that fill at most (a prompt of 2048 tokens in a buffer of 32048, 32 heads of 128, 128 / 256 / 512 / 1024: 119 / 101 /
+// 93 / 85 us, without the buffer 57; one token of 48 sequences in one of 30000: 83 / 47 / 37 / 37).  What they have to fill
+// is known on the device; without anything they end at once.
+constexpr int64_t kMostFill = 512;
+
 int64_t workspace(const lbfq_paged_params* p, const Plan& x) {
   return x.splits == 1 ? 0 : x.splits * part_bytes(p) + 16;
 }
@@ -1322,11 +1328,12 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   // (a launch has fewer than 2^32 threads)
   const int64_t combos = (x.decode ? p->B : x.splits) * p->Hk;
   a.main = x.decode ? combos * x.splits : (x.groups * combos + 7) / 8 * 8 * x.piece;
-  LBFQ_CHECK_ARG(a.main < (1 << 24) - 8, "lbfq_paged_attention: problem too large");
+  LBFQ_CHECK_ARG(a.main < (1 << 24) - kMostFill, "lbfq_paged_attention: problem too large");
   a.combos = static_cast<uint32_t>(combos);
   a.piece = static_cast<uint32_t>(x.piece);
-  // rows that no sequence has: the combine kernel sees every row, otherwise some workgroups more
-  const int64_t fill = (p->fill_rest || p->lse) && x.splits == 1 ? 8 : 0;
+  // rows that no sequence has: the combine kernel sees every row, otherwise some workgroups more, one for 64 KiB that the
+  // output holds
+  const int64_t fill = (p->fill_rest || p->lse) && x.splits == 1 ? std::min(R * p->D / (1 << 15) + 1, kMostFill) : 0;
   const dim3 grid(static_cast<unsigned>(a.main + fill));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool bf = p->dtype == kBF16, d128 = p->D == 128;
