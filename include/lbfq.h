@@ -475,8 +475,9 @@ int lbfq_kv_read(const lbfq_kv_read_params* p, lbfq_stream_t stream);
  * ones.  causal: query i sees keys up to its own position seq_len - n + i; window
  * w > 0: only keys above position - w.  Key head h serves query heads
  * h Hq / Hk ...  Rows that see nothing are 0, lse (natural log, (T, Hq)) -inf.
- * Keys on pages outside the cache are not seen.  max_query_len sizes the grid
- * (0: T); more queries than that are still right.  Rows that no sequence has:
+ * Keys on pages outside the cache are not seen.  max_query_len (0: T) picks the
+ * kernel and, with the table's width, the parts of the keys and so the workspace;
+ * more queries than that are still right.  out may be q.  Rows that no sequence has:
  * lse -inf, out 0 with fill_rest, else left as they are.  workspace:
  * lbfq_paged_attention_workspace_bytes(p), 16-byte aligned, used by this call alone. */
 typedef struct {

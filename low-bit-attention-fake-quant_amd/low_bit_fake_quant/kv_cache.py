@@ -27,7 +27,9 @@ class PagedKVCache(NamedTuple):
     """The tensors of a cache, contiguous, on one device.
 
     Row ``r`` of page ``p`` of head ``h`` is ``k_codes[p, h, r]``; its value is code *
-    2^(scale - 127), ``k_scale[p, h, r, c]`` for columns 32 c ... 32 c + 31.
+    2^(scale - 127), ``k_scale[p, h, r, c]`` for columns 32 c ... 32 c + 31.  A cache
+    that is not filled by ``write_kv_cache`` holds no NaN code and no scale of 255 where
+    a query looks.
     """
 
     k_codes: torch.Tensor  # (pages, H, page size, D) float8_e4m3fn
@@ -100,8 +102,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Ten
     on pages whose id lies outside the cache are not seen.  A query that sees
     nothing gives zeros.
 
-    ``max_query_len``: the most new tokens of a sequence, if known; it sizes the
-    launch; results do not depend on it beyond rounding.  ``sm_scale``: 1/sqrt(D) by default, in 2^-64 ... 2^15.
+    ``max_query_len``: the most new tokens of a sequence, if known.  It picks the kernel
+    (one token, or a chunk) and, with the table's width, the parts that the keys are
+    cut into, and so the workspace (at most 1 GiB); a sequence may hold more, and
+    results do not depend on it beyond rounding.  ``sm_scale``: 1/sqrt(D) by default, in 2^-64 ... 2^15.
     ``out``: takes the result, rows of no sequence left as they are (in a new tensor
     they are zero).  It may be ``q`` itself, or lie over parts of it (then q is copied
     first); with the other inputs it shares no memory, nor do its rows overlap.  ``return_lse``: also the natural
@@ -111,6 +115,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Ten
     Scores, softmax and sums are fp32 on exact products of cached values and
     queries; P is rounded for the second product, to 11 bits or more down to 2^-21
     of the row's largest, and the result once.  A NaN in a query makes its row NaN.
+    Averages stay finite up to the cache's largest values, 448 * 2^119.
     """
     out, lse = _lib.torch_ops().paged_attention(q, *cache, block_table, seq_lens, query_starts, max_query_len, sm_scale,
                                                 causal, window, out, return_lse)

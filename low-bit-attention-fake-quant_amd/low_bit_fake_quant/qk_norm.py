@@ -29,7 +29,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     """RMS norm of every head's row of Q and K and the rotation by its position.
 
     ``q`` is (B, S, Hq, D) and ``k`` (B, S, Hk, D), or (T, Hq, D) and (T, Hk, D),
-    with D 64 or 128, in fp32, fp16 or bf16; views of a joint projection are
+    with D 64 or 128, in fp32, fp16 or bf16 (every head by itself; a norm over all of a
+    token's heads at once is another operator); views of a joint projection are
     read where they are (rows that are not contiguous and 16-byte aligned are
     copied).  A row x becomes ``n = x * w / sqrt(mean(x^2) + eps)`` with
     ``q_weight`` / ``k_weight`` (D,) of any of these dtypes (None: ones), and the
@@ -39,7 +40,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     multiple of 16 up to D (``rotary_table``).  ``positions`` (int32 or int64, (S,)
     or (B, S); (T,) for three dimensions) picks the table's row of each token;
     without it token s takes row s.  A negative position is normalised and not
-    rotated (padding); one past the table comes out as NaN.
+    rotated (padding); one past the table comes out as NaN.  Columns that are not
+    rotated do not reach each other.
 
     Arithmetic is fp32 with one rounding at the end.  Gradients reach q, k and the
     weights (``cos`` and ``sin`` take none); the weights' sums have a fixed order.  A
