@@ -1328,12 +1328,14 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   // (a launch has fewer than 2^32 threads)
   const int64_t combos = (x.decode ? p->B : x.splits) * p->Hk;
   a.main = x.decode ? combos * x.splits : (x.groups * combos + 7) / 8 * 8 * x.piece;
-  LBFQ_CHECK_ARG(a.main < (1 << 24) - kMostFill, "lbfq_paged_attention: problem too large");
+  LBFQ_CHECK_ARG(a.main < (1 << 24) - 8, "lbfq_paged_attention: problem too large");
   a.combos = static_cast<uint32_t>(combos);
   a.piece = static_cast<uint32_t>(x.piece);
   // rows that no sequence has: the combine kernel sees every row, otherwise some workgroups more, one for 64 KiB that the
   // output holds
-  const int64_t fill = (p->fill_rest || p->lse) && x.splits == 1 ? std::min(R * p->D / (1 << 15) + 1, kMostFill) : 0;
+  const int64_t fill = (p->fill_rest || p->lse) && x.splits == 1
+                           ? std::min({R * p->D / (1 << 15) + 1, kMostFill, (1 << 24) - 1 - a.main})
+                           : 0;
   const dim3 grid(static_cast<unsigned>(a.main + fill));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool bf = p->dtype == kBF16, d128 = p->D == 128;
