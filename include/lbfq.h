@@ -442,7 +442,10 @@ int lbfq_qk_norm_rope_bwd(const lbfq_qk_norm_params* p, const lbfq_qk_norm_grads
  * Codes (num_pages, H, page, D) E4M3 and scales (num_pages, H, page, D / 32)
  * E8M0 of K and of V, contiguous and 16-byte aligned, page = 2^page_shift
  * tokens (16 .. 1024); the format of LBFQ_Q_MX_QK with 32 columns a scale,
- * scales at most 2^119 (infinities are held as 448 * 2^119).
+ * scales at most 2^119 (infinities are held as 448 * 2^119).  bits = 4 in the
+ * parameters below (0 and 8 are E4M3): codes (num_pages, H, page, D / 2), two E2M1
+ * values a byte, the even column in the low half; the scale is 2^ceil(log2(max(amax,
+ * 1e-4) / 6)), at most 2^125.
  * write: rows k[t], v[t] (fp32, fp16 or bf16) to slot slots[t] = page id * page
  * + row; a slot outside the cache is skipped; slots must differ. */
 typedef struct {
@@ -452,9 +455,33 @@ typedef struct {
   const int64_t* slots;                    /* (T)                               */
   uint8_t* k_codes; uint8_t* k_scale; uint8_t* v_codes; uint8_t* v_scale;
   int64_t num_pages; int page_shift;
+  int bits;                                /* of a code: 4, or 0 / 8            */
 } lbfq_kv_write_params;
 
 int lbfq_kv_write(const lbfq_kv_write_params* p, lbfq_stream_t stream);
+
+/* append: the first rot columns of q[t] and k[t] rotated in pairs (a, b) by the
+ * angle in row positions[t] of the tables, (a cos - b sin, a sin + b cos), pairs
+ * (2i, 2i + 1) or (halves) (i, i + rot / 2), each product and the sum rounded to
+ * fp32; q to q_out (T, Hq, D) in its dtype, k (from fp32) and v as write does it.
+ * A negative position is not rotated; at one past the table q comes out as NaN and
+ * nothing is written.  q and q_out NULL with Hq 0: only the cache. */
+typedef struct {
+  const void* q; const void* k; const void* v; int dtype;
+  int64_t T, Hq, Hk, D;
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h;    /* element strides, 16-byte multiples */
+  const float* cos; const float* sin;      /* (table_len, rot / 2), 16-byte aligned */
+  int64_t table_len; int rot;              /* a multiple of 16, up to D         */
+  const void* positions; int positions_i64; int64_t pos_t; /* (T) int32 or int64 */
+  int halves;
+  void* q_out;
+  const int64_t* slots;                    /* (T)                               */
+  uint8_t* k_codes; uint8_t* k_scale; uint8_t* v_codes; uint8_t* v_scale;
+  int64_t num_pages; int page_shift;
+  int bits;
+} lbfq_kv_append_params;
+
+int lbfq_kv_append(const lbfq_kv_append_params* p, lbfq_stream_t stream);
 
 /* read: dtype(code * 2^e) of the first max_len tokens of each sequence, k_out and
  * v_out (B, max_len, H, D) contiguous; rows from seq_lens[b] on, and rows whose
@@ -466,6 +493,7 @@ typedef struct {
   const int32_t* block_table; int64_t table_stride, table_cols; /* (B, table_cols) */
   const int32_t* seq_lens;                 /* (B)                               */
   void* k_out; void* v_out; int dtype;
+  int bits;
 } lbfq_kv_read_params;
 
 int lbfq_kv_read(const lbfq_kv_read_params* p, lbfq_stream_t stream);
@@ -494,6 +522,7 @@ typedef struct {
   float* lse;                              /* or NULL                           */
   int fill_rest;
   void* workspace; int64_t workspace_bytes;
+  int bits;
 } lbfq_paged_params;
 
 int64_t lbfq_paged_attention_workspace_bytes(const lbfq_paged_params* p);

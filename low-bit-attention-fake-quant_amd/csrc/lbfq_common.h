@@ -141,6 +141,29 @@ __device__ __forceinline__ uint32_t cvt4_e4m3(const float q[4]) {
 
 __device__ __forceinline__ float clamp448(float q) { return __builtin_amdgcn_fmed3f(q, -kFp8Max, kFp8Max); }
 
+// E2M1 (OCP FP4: 0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign).  Eight values of magnitude
+// up to 6 to codes, the first in the lowest four bits, to nearest, ties to even
+// (the hardware's rounding is a GPU test), and back.
+__device__ __forceinline__ float clamp6(float q) { return __builtin_amdgcn_fmed3f(q, -6.0f, 6.0f); }
+__device__ __forceinline__ uint32_t cvt8_e2m1(const float q[8]) {
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[0], q[1], 1.0f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[2], q[3], 1.0f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[4], q[5], 1.0f, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[6], q[7], 1.0f, 3);
+  return w;
+}
+__device__ __forceinline__ void values8_e2m1(uint32_t w, float (&v)[8]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 x[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1),
+                      __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = x[i][0];
+    v[2 * i + 1] = x[i][1];
+  }
+}
+
 // ceil(log2(r)) for positive normal fp32 r, exact from the bits.
 __device__ __forceinline__ int ceil_log2_exact(float r) {
   uint32_t u = __float_as_uint(r);

@@ -18,6 +18,8 @@
 // and written (a copy of 1 GiB reaches 5.1 to 5.5).  Reading 8 sequences of up to
 // 16384 x 8 heads to bf16: 147 us, 4.7 TB/s (what only writes reaches 5.3).  A few
 // tokens: 3.0 and 4.6 us, a launch's own time.
+#include <algorithm>
+
 #include "lbfq_common.h"
 #include "../../include/lbfq.h"
 
@@ -63,8 +65,44 @@ __device__ __forceinline__ void store8(void* base, int64_t i, const float (&v)[8
   }
 }
 
+// The 2^e of a block of 32 columns whose largest value is amax
+template <int BITS>
+__device__ __forceinline__ float block_scale(float amax) {
+  const float r = fmaxf(amax, kAmaxFloor);
+  if constexpr (BITS == 8) return fminf(mx_scale_from_amax(r), 0x1p119f);
+  // 6 = 1.5 2^2: r / 6 <= 2^(E - 2) for r = (1 + f) 2^E with 1 + f <= 1.5, from r's bits; no quotient is rounded
+  const uint32_t u = __float_as_uint(r), e = (u >> 23) - 2 + ((u & 0x7fffffu) > 0x400000u ? 1 : 0);
+  return __uint_as_float((e < 252 ? e : 252u) << 23);
+}
+
+// Row `row` of a cache tensor from the eight values that each of its lanes (lane part lp) holds.  All lanes of a wave
+// take part; `live`: whether this one's row is stored.
+template <int BITS, int D>
+__device__ __forceinline__ void encode_row(const float (&x)[8], uint8_t* codes, uint8_t* scale, int64_t row, int lp,
+                                           bool live) {
+  float m = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[k]));
+  m = fmaxf(m, __shfl_xor(m, 1, 64));
+  m = fmaxf(m, __shfl_xor(m, 2, 64));
+  const float sc = block_scale<BITS>(m);
+  const float inv = 1.0f / sc;  // exact: 2^-e
+  if (!live) return;
+  float q[8];
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) q[k] = clamp448(x[k] * inv);
+    *reinterpret_cast<uint2*>(codes + row * D + 8 * lp) = make_uint2(cvt4_e4m3(q), cvt4_e4m3(q + 4));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) q[k] = clamp6(x[k] * inv);
+    *reinterpret_cast<uint32_t*>(codes + row * (D / 2) + 4 * lp) = cvt8_e2m1(q);
+  }
+  if ((lp & 3) == 0) scale[row * (D / 32) + lp / 4] = static_cast<uint8_t>(__float_as_uint(sc) >> 23);
+}
+
 // workgroup: (which, head) fastest, then the block of tokens
-template <int DT, int D>
+template <int DT, int D, int BITS>
 __global__ void __launch_bounds__(256) kv_write_kernel(const lbfq_kv_write_params p) {
   constexpr int LPR = D / 8, RPI = 256 / LPR, U = kRows / RPI;  // rows at once, and in turn
   const int H = static_cast<int>(p.H);
@@ -88,25 +126,145 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const lbfq_kv_write_param
   }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    float m = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[i][k]));
-    m = fmaxf(m, __shfl_xor(m, 1, 64));
-    m = fmaxf(m, __shfl_xor(m, 2, 64));
-    const float sc = fminf(mx_scale_from_amax(fmaxf(m, kAmaxFloor)), 0x1p119f);
-    const float inv = 1.0f / sc;  // exact: 2^-e
-    float q[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) q[k] = clamp448(x[i][k] * inv);
-    if (slot[i] < 0 || slot[i] >= slots) continue;  // padding, or not in the cache
+    // (a slot outside the cache is padding)
     const int64_t row = ((slot[i] >> p.page_shift) * H + h) * (int64_t{1} << p.page_shift) +
                         (slot[i] & ((int64_t{1} << p.page_shift) - 1));
-    *reinterpret_cast<uint2*>(codes + row * D + 8 * lp) = make_uint2(cvt4_e4m3(q), cvt4_e4m3(q + 4));
-    if ((lp & 3) == 0) scale[row * (D / 32) + lp / 4] = static_cast<uint8_t>(__float_as_uint(sc) >> 23);
+    encode_row<BITS, D>(x[i], codes, scale, row, lp, slot[i] >= 0 && slot[i] < slots);
   }
 }
 
-template <int DT, int D>
+// ---- rotation, then into the cache
+
+// Eight values as they lie in memory
+template <int DT>
+struct Raw {
+  uint4 w[DT == kF32 ? 2 : 1];
+};
+
+template <int DT>
+__device__ __forceinline__ Raw<DT> load_raw(const void* base, int64_t i) {
+  Raw<DT> r;
+  if constexpr (DT == kF32) {
+    const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(base) + i);
+    r.w[0] = s[0];
+    r.w[1] = s[1];
+  } else {
+    r.w[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + i);
+  }
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void widen(const Raw<DT>& r, float (&x)[8]) {
+#pragma unroll
+  for (int c = 0; c < (DT == kF32 ? 2 : 1); ++c) {
+    const uint32_t w[4] = {r.w[c].x, r.w[c].y, r.w[c].z, r.w[c].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == kF32) {
+        x[4 * c + i] = __uint_as_float(w[i]);
+      } else if constexpr (DT == kBF16) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        x[2 * i] = f16_bits_to_f32(static_cast<uint16_t>(w[i]));
+        x[2 * i + 1] = f16_bits_to_f32(static_cast<uint16_t>(w[i] >> 16));
+      }
+    }
+  }
+}
+
+struct AppendArgs {
+  lbfq_kv_append_params p;
+  int stretch;          // heads that a workgroup walks
+  uint32_t stretches;   // of a block of tokens
+};
+
+// A thread keeps one token and eight columns: its cos and sin stay in registers while it walks the heads of Q, of K and
+// of V, one list.  (Head by head, each would read them again, four bytes for two of the row's.)  Every product and the
+// sum are rounded, so what is quantised is defined to the bit.
+template <int DT, int D, int BITS, bool HALVES>
+__global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
+  constexpr int LPR = D / 8, RPI = 256 / LPR, U = 4;
+  const lbfq_kv_append_params& p = a.p;
+  const int Hq = static_cast<int>(p.Hq), Hk = static_cast<int>(p.Hk), heads = Hq + 2 * Hk;
+  const int r = threadIdx.x / LPR, lp = threadIdx.x % LPR, lane = threadIdx.x & 63, d0 = 8 * lp;
+  const uint32_t block = blockIdx.x / a.stretches;
+  const int h0 = static_cast<int>(blockIdx.x - block * a.stretches) * a.stretch;
+  const int h1 = h0 + a.stretch < heads ? h0 + a.stretch : heads;
+  const int64_t t = static_cast<int64_t>(block) * RPI + r, tok = t < p.T ? t : p.T - 1;
+  const int half = p.rot / 2;
+  // the rotation of this thread's columns
+  const int64_t pos = p.positions_i64 ? reinterpret_cast<const int64_t*>(p.positions)[tok * p.pos_t]
+                                      : reinterpret_cast<const int32_t*>(p.positions)[tok * p.pos_t];
+  const bool past = pos >= p.table_len, turned = d0 < p.rot && pos >= 0;
+  int partner = lane;
+  float c[8], s[8];
+  {
+    constexpr int N = HALVES ? 8 : 4;
+    const int i0 = HALVES ? (d0 < half ? d0 : d0 - half) : d0 / 2;
+    if (HALVES && d0 < p.rot) partner = d0 < half ? lane + half / 8 : lane - half / 8;
+    float cc[N], ss[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) cc[k] = ss[k] = __builtin_nanf("");
+    if (turned && !past) {
+#pragma unroll
+      for (int k = 0; k < N; k += 4) {
+        const float4 cv = *reinterpret_cast<const float4*>(p.cos + pos * half + i0 + k);
+        const float4 sv = *reinterpret_cast<const float4*>(p.sin + pos * half + i0 + k);
+        cc[k] = cv.x; cc[k + 1] = cv.y; cc[k + 2] = cv.z; cc[k + 3] = cv.w;
+        ss[k] = sv.x; ss[k + 1] = sv.y; ss[k + 2] = sv.z; ss[k + 3] = sv.w;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      c[k] = cc[HALVES ? k : k / 2];
+      const float sn = ss[HALVES ? k : k / 2];
+      s[k] = (HALVES ? d0 < half : (k & 1) == 0) ? -sn : sn;  // the sign of the partner's term
+    }
+  }
+  const int64_t slots = p.num_pages << p.page_shift;
+  const int64_t slot = t < p.T ? p.slots[tok] : -1;
+  const bool live = slot >= 0 && slot < slots && !past;
+  const int64_t page_row = (slot >> p.page_shift) * Hk, in_page = slot & ((int64_t{1} << p.page_shift) - 1);
+  for (int h = h0; h < h1; h += U) {
+    Raw<DT> raw[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int g = h + i < h1 ? h + i : h1 - 1;
+      const bool isq = g < Hq, isk = g < Hq + Hk;
+      raw[i] = load_raw<DT>(isq ? p.q : isk ? p.k : p.v,
+                            tok * (isq ? p.q_t : isk ? p.k_t : p.v_t) +
+                                (isq ? g * p.q_h : isk ? (g - Hq) * p.k_h : (g - Hq - Hk) * p.v_h) + d0);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int g = h + i;
+      if (g >= h1) break;
+      float x[8];
+      widen<DT>(raw[i], x);
+      if (g < Hq + Hk) {
+        float o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = HALVES ? __shfl(x[k], partner, 64) : x[k ^ 1];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float y = as_f32(x[k] * c[k] + o[k] * s[k]);
+          x[k] = turned ? y : x[k];
+        }
+      }
+      if (g < Hq) {
+        if (t < p.T) store8<DT>(p.q_out, (t * Hq + g) * D + d0, x);
+      } else {
+        const bool isv = g >= Hq + Hk;
+        const int64_t row = ((page_row + g - (isv ? Hq + Hk : Hq)) << p.page_shift) + in_page;
+        encode_row<BITS, D>(x, isv ? p.v_codes : p.k_codes, isv ? p.v_scale : p.k_scale, row, lp, live);
+      }
+    }
+  }
+}
+
+template <int DT, int D, int BITS>
 __global__ void __launch_bounds__(256) kv_read_kernel(const lbfq_kv_read_params p, int blocks) {
   constexpr int LPR = D / 8, RPI = 256 / LPR, U = kRows / RPI;
   const int H = static_cast<int>(p.H);
@@ -122,7 +280,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const lbfq_kv_read_params 
   void* out = isv ? p.v_out : p.k_out;
   const int64_t cap = p.table_cols << p.page_shift;
   const int64_t len = p.seq_lens[b] < cap ? p.seq_lens[b] : cap;
-  uint2 c[U];
+  uint2 c[U];  // (4 bits: x holds all eight)
   uint32_t e[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
@@ -133,7 +291,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const lbfq_kv_read_params 
       const int page = p.block_table[b * p.table_stride + (t >> p.page_shift)];
       if (page >= 0 && page < p.num_pages) {
         const int64_t row = ((static_cast<int64_t>(page) * H + h) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
-        c[i] = *reinterpret_cast<const uint2*>(codes + row * D + 8 * lp);
+        if constexpr (BITS == 8) c[i] = *reinterpret_cast<const uint2*>(codes + row * D + 8 * lp);
+        else c[i].x = *reinterpret_cast<const uint32_t*>(codes + row * (D / 2) + 4 * lp);
         e[i] = scale[row * (D / 32) + lp / 4];
       }
     }
@@ -144,22 +303,30 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const lbfq_kv_read_params 
     if (t >= p.max_len) continue;
     const float sc = __uint_as_float(e[i] == 255 ? 0x7fc00000u : e[i] ? e[i] << 23 : 0x00400000u);
     float v[8];
-    v[0] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].x), 0);
-    v[1] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].x), 1);
-    v[2] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].x), 2);
-    v[3] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].x), 3);
-    v[4] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].y), 0);
-    v[5] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].y), 1);
-    v[6] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].y), 2);
-    v[7] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].y), 3);
+    if constexpr (BITS == 8) {
+      v[0] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].x), 0);
+      v[1] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].x), 1);
+      v[2] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].x), 2);
+      v[3] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].x), 3);
+      v[4] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].y), 0);
+      v[5] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].y), 1);
+      v[6] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].y), 2);
+      v[7] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(c[i].y), 3);
+    } else {
+      values8_e2m1(c[i].x, v);
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = as_f32(v[k] * sc);  // the fp32 product, then the one rounding
     store8<DT>(out, ((b * p.max_len + t) * H + h) * D + 8 * lp, v);
   }
 }
 
-int check_cache(const char* who, int64_t num_pages, int page_shift, int64_t H, int64_t D, const void* kc,
+// bits of a code: 4, or 8 (also as 0, what a struct of before has there)
+bool four(int bits) { return bits == 4; }
+
+int check_cache(const char* who, int bits, int64_t num_pages, int page_shift, int64_t H, int64_t D, const void* kc,
                 const void* ks, const void* vc, const void* vs) {
+  LBFQ_CHECK_ARG(bits == 0 || bits == 4 || bits == 8, "%s: codes have 4 or 8 bits", who);
   LBFQ_CHECK_ARG(D == 64 || D == 128, "%s: D must be 64 or 128", who);
   LBFQ_CHECK_ARG(page_shift >= 4 && page_shift <= 10, "%s: pages hold 16 to 1024 tokens, a power of two", who);
   LBFQ_CHECK_ARG(num_pages > 0 && num_pages < (int64_t{1} << 31), "%s: bad number of pages", who);
@@ -175,7 +342,7 @@ int check_cache(const char* who, int64_t num_pages, int page_shift, int64_t H, i
 
 extern "C" int lbfq_kv_write(const lbfq_kv_write_params* p, lbfq_stream_t stream) {
   LBFQ_CHECK_ARG(p, "lbfq_kv_write: null params");
-  if (int rc = check_cache("lbfq_kv_write", p->num_pages, p->page_shift, p->H, p->D, p->k_codes, p->k_scale,
+  if (int rc = check_cache("lbfq_kv_write", p->bits, p->num_pages, p->page_shift, p->H, p->D, p->k_codes, p->k_scale,
                            p->v_codes, p->v_scale))
     return rc;
   LBFQ_CHECK_ARG(p->dtype >= kF32 && p->dtype <= kBF16, "lbfq_kv_write: bad dtype %d", p->dtype);
@@ -190,10 +357,16 @@ extern "C" int lbfq_kv_write(const lbfq_kv_write_params* p, lbfq_stream_t stream
   LBFQ_CHECK_ARG(wgs < (int64_t{1} << 24), "lbfq_kv_write: problem too large");  // (a launch has fewer than 2^32 threads)
   const dim3 grid(static_cast<unsigned>(wgs)), block(256);
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define LBFQ_KW(DT)                                                                           \
-  do {                                                                                        \
-    if (p->D == 128) hipLaunchKernelGGL((kv_write_kernel<DT, 128>), grid, block, 0, st, *p);  \
-    else hipLaunchKernelGGL((kv_write_kernel<DT, 64>), grid, block, 0, st, *p);               \
+#define LBFQ_KW(DT)                                                                                            \
+  do {                                                                                                         \
+    if (four(p->bits)) {                                                                                       \
+      if (p->D == 128) hipLaunchKernelGGL((kv_write_kernel<DT, 128, 4>), grid, block, 0, st, *p);              \
+      else hipLaunchKernelGGL((kv_write_kernel<DT, 64, 4>), grid, block, 0, st, *p);                           \
+    } else if (p->D == 128) {                                                                                  \
+      hipLaunchKernelGGL((kv_write_kernel<DT, 128, 8>), grid, block, 0, st, *p);                               \
+    } else {                                                                                                   \
+      hipLaunchKernelGGL((kv_write_kernel<DT, 64, 8>), grid, block, 0, st, *p);                                \
+    }                                                                                                          \
   } while (0)
   if (p->dtype == kBF16) LBFQ_KW(kBF16);
   else if (p->dtype == kF16) LBFQ_KW(kF16);
@@ -203,9 +376,65 @@ extern "C" int lbfq_kv_write(const lbfq_kv_write_params* p, lbfq_stream_t stream
   return 0;
 }
 
+extern "C" int lbfq_kv_append(const lbfq_kv_append_params* p, lbfq_stream_t stream) {
+  const char* who = "lbfq_kv_append";
+  LBFQ_CHECK_ARG(p, "%s: null params", who);
+  if (int rc = check_cache(who, p->bits, p->num_pages, p->page_shift, p->Hk, p->D, p->k_codes, p->k_scale, p->v_codes,
+                           p->v_scale))
+    return rc;
+  LBFQ_CHECK_ARG(p->dtype >= kF32 && p->dtype <= kBF16, "%s: bad dtype %d", who, p->dtype);
+  LBFQ_CHECK_ARG(p->T > 0 && p->T < (int64_t{1} << 40), "%s: bad number of tokens", who);
+  LBFQ_CHECK_ARG(p->Hq >= 0 && p->Hq < (1 << 16), "%s: bad number of heads", who);
+  LBFQ_CHECK_ARG(p->k && p->v && p->slots && p->positions && (p->table_len == 0 || (p->cos && p->sin)) &&
+                     (p->Hq == 0 || (p->q && p->q_out)),
+                 "%s: missing tensor", who);
+  LBFQ_CHECK_ARG(p->rot > 0 && p->rot <= p->D && p->rot % 16 == 0, "%s: rot must be a multiple of 16 up to D", who);
+  LBFQ_CHECK_ARG(p->table_len >= 0 && p->table_len < (int64_t{1} << 40), "%s: bad table", who);
+  const int64_t s[6] = {p->q_t, p->q_h, p->k_t, p->k_h, p->v_t, p->v_h};
+  for (int64_t v : s) LBFQ_CHECK_ARG(v % (p->dtype == kF32 ? 4 : 8) == 0, "%s: rows must be 16-byte aligned", who);
+  uint64_t at = 0;
+  for (const void* x : {p->q, p->k, p->v, static_cast<const void*>(p->q_out), static_cast<const void*>(p->cos),
+                        static_cast<const void*>(p->sin)})
+    at |= reinterpret_cast<uint64_t>(x);
+  LBFQ_CHECK_ARG((at & 15) == 0, "%s: rows and tables must be 16-byte aligned", who);
+  AppendArgs a{};
+  a.p = *p;
+  const int64_t heads = p->Hq + 2 * p->Hk, per = 256 / (p->D / 8), blocks = (p->T + per - 1) / per;
+  // heads of a workgroup: as many as leave 2048 workgroups, and four at least
+  const int64_t stretches = std::max<int64_t>(1, std::min((heads + 3) / 4, (2048 + blocks - 1) / blocks));
+  a.stretch = static_cast<int>((heads + stretches - 1) / stretches + 3) / 4 * 4;
+  a.stretches = static_cast<uint32_t>((heads + a.stretch - 1) / a.stretch);
+  LBFQ_CHECK_ARG(blocks < (int64_t{1} << 24) / a.stretches, "%s: problem too large", who);
+  const dim3 grid(static_cast<unsigned>(blocks * a.stretches)), block(256);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+#define LBFQ_KA(DT, DD, BB)                                                                               \
+  do {                                                                                                    \
+    if (p->halves) hipLaunchKernelGGL((kv_append_kernel<DT, DD, BB, true>), grid, block, 0, st, a);       \
+    else hipLaunchKernelGGL((kv_append_kernel<DT, DD, BB, false>), grid, block, 0, st, a);                \
+  } while (0)
+#define LBFQ_KAD(DT)                                    \
+  do {                                                  \
+    if (four(p->bits)) {                                \
+      if (p->D == 128) LBFQ_KA(DT, 128, 4);             \
+      else LBFQ_KA(DT, 64, 4);                          \
+    } else if (p->D == 128) {                           \
+      LBFQ_KA(DT, 128, 8);                              \
+    } else {                                            \
+      LBFQ_KA(DT, 64, 8);                               \
+    }                                                   \
+  } while (0)
+  if (p->dtype == kBF16) LBFQ_KAD(kBF16);
+  else if (p->dtype == kF16) LBFQ_KAD(kF16);
+  else LBFQ_KAD(kF32);
+#undef LBFQ_KAD
+#undef LBFQ_KA
+  LBFQ_LAUNCH_CHECK("lbfq_kv_append");
+  return 0;
+}
+
 extern "C" int lbfq_kv_read(const lbfq_kv_read_params* p, lbfq_stream_t stream) {
   LBFQ_CHECK_ARG(p, "lbfq_kv_read: null params");
-  if (int rc = check_cache("lbfq_kv_read", p->num_pages, p->page_shift, p->H, p->D, p->k_codes, p->k_scale,
+  if (int rc = check_cache("lbfq_kv_read", p->bits, p->num_pages, p->page_shift, p->H, p->D, p->k_codes, p->k_scale,
                            p->v_codes, p->v_scale))
     return rc;
   LBFQ_CHECK_ARG(p->dtype >= kF32 && p->dtype <= kBF16, "lbfq_kv_read: bad dtype %d", p->dtype);
@@ -217,15 +446,23 @@ extern "C" int lbfq_kv_read(const lbfq_kv_read_params* p, lbfq_stream_t stream) 
   LBFQ_CHECK_ARG(p->B < (int64_t{1} << 24) / (blocks * 2 * p->H), "lbfq_kv_read: problem too large");
   const dim3 grid(static_cast<unsigned>(p->B * blocks * 2 * p->H)), block(256);
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define LBFQ_KR(DT)                                                                                                    \
-  do {                                                                                                                 \
-    if (p->D == 128) hipLaunchKernelGGL((kv_read_kernel<DT, 128>), grid, block, 0, st, *p, static_cast<int>(blocks));  \
-    else hipLaunchKernelGGL((kv_read_kernel<DT, 64>), grid, block, 0, st, *p, static_cast<int>(blocks));               \
+#define LBFQ_KR1(DT, DD, BB) hipLaunchKernelGGL((kv_read_kernel<DT, DD, BB>), grid, block, 0, st, *p, static_cast<int>(blocks))
+#define LBFQ_KR(DT)                                     \
+  do {                                                  \
+    if (four(p->bits)) {                                \
+      if (p->D == 128) LBFQ_KR1(DT, 128, 4);            \
+      else LBFQ_KR1(DT, 64, 4);                         \
+    } else if (p->D == 128) {                           \
+      LBFQ_KR1(DT, 128, 8);                             \
+    } else {                                            \
+      LBFQ_KR1(DT, 64, 8);                              \
+    }                                                   \
   } while (0)
   if (p->dtype == kBF16) LBFQ_KR(kBF16);
   else if (p->dtype == kF16) LBFQ_KR(kF16);
   else LBFQ_KR(kF32);
 #undef LBFQ_KR
+#undef LBFQ_KR1
   LBFQ_LAUNCH_CHECK("lbfq_kv_read");
   return 0;
 }

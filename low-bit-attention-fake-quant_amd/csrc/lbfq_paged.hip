@@ -195,14 +195,52 @@ __device__ __forceinline__ void split_f16(const uint4& x, uint4& hi, uint4& lo) 
   lo = make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// Two codes of a word (HI: the upper two) times 2^e as 16-bit values; sc: 2^e as fp32.
-template <bool HI>
-__device__ __forceinline__ uint32_t cvt_bf16(uint32_t w, float sc) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, sc, HI));
+// The pair I of the codes from w on (two in 16 bits, or in 8) times 2^e as 16-bit values; sc: 2^e as fp32.
+template <int BITS>
+__device__ __forceinline__ uint32_t cvt_bf16(const uint32_t* w, int i, float sc) {
+  if constexpr (BITS == 8) {
+    return __builtin_bit_cast(uint32_t, i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i >> 1], sc, true)
+                                              : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i >> 1], sc, false));
+  } else {
+    const uint32_t x = w[i >> 2];
+    switch (i & 3) {  // (known once the loops are unrolled)
+      case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 0));
+      case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 1));
+      case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 2));
+      default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 3));
+    }
+  }
 }
-template <bool HI>
-__device__ __forceinline__ uint32_t cvt_f16(uint32_t w, float sc) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, sc, HI));
+template <int BITS>
+__device__ __forceinline__ uint32_t cvt_f16(const uint32_t* w, int i, float sc) {
+  if constexpr (BITS == 8) {
+    return __builtin_bit_cast(uint32_t, i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i >> 1], sc, true)
+                                              : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i >> 1], sc, false));
+  } else {
+    const uint32_t x = w[i >> 2];
+    switch (i & 3) {
+      case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 0));
+      case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 1));
+      case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 2));
+      default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 3));
+    }
+  }
+}
+
+// N bytes from p on, in words
+template <int N>
+__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 16) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (N == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else if constexpr (N == 4) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  }
 }
 
 __device__ __forceinline__ v4f mfma16_bf16(const uint4& a, const uint4& b, const v4f& c) {
@@ -230,11 +268,12 @@ __device__ __forceinline__ float row_lse(float m, float l) {
 
 // A wave's 32 keys in registers: key t 16 + n of K for lane (n, g) = (lane % 16,
 // lane / 16), columns 64 c + 16 g ..; rows t 16 + 4 g + i of V, columns (D/16) n ..
-template <int D>
+template <int D, int BITS>
 struct Tile {
-  uint4 k[2][D / 64];
+  static constexpr int KW = BITS / 2, VB = D / 16 * BITS / 8, VW = (VB + 3) / 4;  // words of 16 codes, bytes and words of a V row
+  uint32_t k[2][D / 64][KW];
   uint32_t ks[2];
-  uint32_t v[2][4][D / 64];
+  uint32_t v[2][4][VW];
   uint32_t vs[2][D / 32];  // the scales of its four V rows
   bool ok[2];               // the page is there
 };
@@ -248,10 +287,11 @@ __device__ __forceinline__ void load_pages(const lbfq_paged_params& p, const int
   }
 }
 
-template <int D>
+template <int D, int BITS>
 __device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int (&pages)[2], int kvh, int kb, int n,
-                                          int g, Tile<D>& x) {
-  constexpr int NB = D / 16;
+                                          int g, Tile<D, BITS>& x) {
+  constexpr int RB = D * BITS / 8;  // bytes of a row
+  using X = Tile<D, BITS>;
   int64_t row[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -259,38 +299,24 @@ __device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int 
     const int page = x.ok[t] ? pages[t] : 0;
     row[t] = (static_cast<int64_t>(page * static_cast<int>(p.Hk) + kvh) << p.page_shift) +
              ((kb + 16 * t) & ((1 << p.page_shift) - 1));
-    const uint8_t* kr = p.k_codes + row[t] * D + (n * D + 16 * g);
+    const uint8_t* kr = p.k_codes + row[t] * RB + (n * RB + 2 * BITS * g);
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) x.k[t][c] = *reinterpret_cast<const uint4*>(kr + 64 * c);
-    const uint8_t* ks = p.k_scale + row[t] * (D / 32) + n * (D / 32);
-    if constexpr (D == 128) x.ks[t] = *reinterpret_cast<const uint32_t*>(ks);
-    else x.ks[t] = *reinterpret_cast<const uint16_t*>(ks);
+    for (int c = 0; c < D / 64; ++c) load_bytes<2 * BITS>(kr + 8 * BITS * c, x.k[t][c]);
+    load_bytes<D / 32>(p.k_scale + row[t] * (D / 32) + n * (D / 32), &x.ks[t]);
   }
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const uint8_t* vr = p.v_codes + row[t] * D + (4 * g * D + NB * n);
-    const uint8_t* vs = p.v_scale + row[t] * (D / 32) + 4 * g * (D / 32);
-    if constexpr (D == 128) {
-      const uint4 s = *reinterpret_cast<const uint4*>(vs);
-      x.vs[t][0] = s.x; x.vs[t][1] = s.y; x.vs[t][2] = s.z; x.vs[t][3] = s.w;
+    const uint8_t* vr = p.v_codes + row[t] * RB + (4 * g * RB + X::VB * n);
+    load_bytes<4 * (D / 32)>(p.v_scale + row[t] * (D / 32) + 4 * g * (D / 32), x.vs[t]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint2 v = *reinterpret_cast<const uint2*>(vr + i * D);
-        x.v[t][i][0] = v.x; x.v[t][i][1] = v.y;
-      }
-    } else {
-      const uint2 s = *reinterpret_cast<const uint2*>(vs);
-      x.vs[t][0] = s.x; x.vs[t][1] = s.y;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x.v[t][i][0] = *reinterpret_cast<const uint32_t*>(vr + i * D);
-    }
+    for (int i = 0; i < 4; ++i) load_bytes<X::VB>(vr + i * RB, x.v[t][i]);
   }
 }
 
 // What the decode kernel takes off a scale of V, in powers of two
 constexpr uint32_t kLess = 32;
 
-template <int DT, int D>
+template <int DT, int D, int BITS>
 __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
   constexpr int NC = D / 64, NB = D / 16, NW = 4;
   const lbfq_paged_params& p = a.p;
@@ -353,8 +379,8 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
     load_pages(p, table, 32 * (begin + wave), pages);
     for (int kt = begin + wave; kt < end; kt += NW) {
       const int kb = 32 * kt;
-      Tile<D> x;
-      load_tile<D>(p, pages, kvh, kb, n, g, x);
+      Tile<D, BITS> x;
+      load_tile<D, BITS>(p, pages, kvh, kb, n, g, x);
       load_pages(p, table, 32 * (kt + NW), pages);
       // S^T: lane (n, g) has query n, keys 16 t + 4 g + i
       float sc[2][4];
@@ -364,11 +390,11 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const float e = __uint_as_float(((x.ks[t] >> (16 * c + 8 * (g >> 1))) & 0xffu) << 23);
-          const uint32_t w[4] = {x.k[t][c].x, x.k[t][c].y, x.k[t][c].z, x.k[t][c].w};
-          const uint4 k0 = make_uint4(cvt_bf16<false>(w[0], e), cvt_bf16<true>(w[0], e), cvt_bf16<false>(w[1], e),
-                                      cvt_bf16<true>(w[1], e));
-          const uint4 k1 = make_uint4(cvt_bf16<false>(w[2], e), cvt_bf16<true>(w[2], e), cvt_bf16<false>(w[3], e),
-                                      cvt_bf16<true>(w[3], e));
+          const uint32_t* w = x.k[t][c];
+          const uint4 k0 = make_uint4(cvt_bf16<BITS>(w, 0, e), cvt_bf16<BITS>(w, 1, e), cvt_bf16<BITS>(w, 2, e),
+                                      cvt_bf16<BITS>(w, 3, e));
+          const uint4 k1 = make_uint4(cvt_bf16<BITS>(w, 4, e), cvt_bf16<BITS>(w, 5, e), cvt_bf16<BITS>(w, 6, e),
+                                      cvt_bf16<BITS>(w, 7, e));
           d = mfma16_bf16(k0, q[c][0], d);
           d = mfma16_bf16(k1, q[c][1], d);
           if constexpr (DT == kF16) {
@@ -389,7 +415,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
             // nothing that lies in the place of a key that no row sees may reach the product
             if (!x.ok[t] || key < lo || key >= hi) {
 #pragma unroll
-              for (int c = 0; c < NC; ++c) x.v[t][i][c] = 0;
+              for (int c = 0; c < Tile<D, BITS>::VW; ++c) x.v[t][i][c] = 0;
               // (four scale bytes of the row at D = 128, two at D = 64)
               if constexpr (D == 128) x.vs[t][i] = 0x7f7f7f7fu;
               else x.vs[t][i / 2] = (x.vs[t][i / 2] & (i & 1 ? 0x0000ffffu : 0xffff0000u)) | (i & 1 ? 0x7f7f0000u : 0x7f7fu);
@@ -435,10 +461,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
           // times 2^-kLess: a sum of 2^30 of the largest values is then in fp32's range
           const float e = __uint_as_float(__builtin_elementwise_sub_sat(by & 0xffu, kLess) << 23);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            vv[4 * t + i][2 * c] = cvt_bf16<false>(x.v[t][i][c], e);
-            vv[4 * t + i][2 * c + 1] = cvt_bf16<true>(x.v[t][i][c], e);
-          }
+          for (int c = 0; c < NB / 2; ++c) vv[4 * t + i][c] = cvt_bf16<BITS>(x.v[t][i], c, e);
         }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -551,7 +574,10 @@ __device__ __forceinline__ uint32_t span_add(uint32_t span, uint32_t v) {
 //
 // (A wide part's V is taken down by a power of two where its largest scale is past kWideTop: weights of up to 2^15 times
 // 2^30 of the largest values that are left, under 2^(kWideTop - 118), add up to less than 2^127.)
-constexpr int kSpan = 22;
+//
+// E2M1's largest code, 6, lands at 49152 with 2^(140 - E), and its smallest, 1/2, stays exact 36 powers of two below.
+constexpr int span_of(int bits) { return bits == 8 ? 22 : 36; }
+constexpr int unit_of(int bits) { return bits == 8 ? 134 : 140; }
 constexpr int kWideTop = 200;
 struct Unit {
   int E;
@@ -562,11 +588,13 @@ struct Unit {
 // keys, 40 heads of 64, bf16: 818 us with two, 765 with three; fp16 queries need more of them: 745 with two, 1075).
 constexpr int chunk_groups(int dt, int64_t d) { return d == 64 && dt == kBF16 ? 3 : 2; }
 
-template <int DT, int D>
+template <int DT, int D, int BITS>
 __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(const Args a) {
   constexpr int NW = 4, QB = kChunkRows, NT = 64 * NW;
   static_assert(QB == 32 * NW, "32 rows a wave");
   constexpr int NKS = D / 16, NDB = D / 32, CH = D / 32;
+  constexpr int RB = D * BITS / 8;  // bytes of a row
+  constexpr int kUnit = unit_of(BITS);
   constexpr int KC = 64 * D / NT;  // K codes of a thread
   constexpr int KT = D / KC;       // threads of a key's row
   constexpr int VK = KC / 4;       // V keys of a thread, four columns each
@@ -603,8 +631,8 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
   const int kkey = lane / KT, kq = lane % KT;           // K: key kkey of the wave's, columns KC kq ..
   const int vkg = lane / (D / 4), vdq = lane % (D / 4);  // V: keys VK vkg .. of the wave's, columns 4 vdq ..
   static_assert(64 / KT == WKEYS && 64 / (D / 4) * VK == WKEYS, "a wave's keys");
-  const uint32_t koff = kkey * D + KC * kq, ksoff = kkey * CH + KC * kq / 32;
-  const uint32_t voff = VK * vkg * D + 4 * vdq, vsoff = VK * vkg * CH;
+  const uint32_t koff = kkey * RB + KC * BITS / 8 * kq, ksoff = kkey * CH + KC * kq / 32;
+  const uint32_t voff = VK * vkg * RB + BITS / 2 * vdq, vsoff = VK * vkg * CH;
 
   auto row_of = [&](int page, int key) -> int64_t {
     return (static_cast<int64_t>(page * Hk + kvh) << shift) + (key & pmask);
@@ -632,7 +660,7 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[db][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;
-  Unit uv{134, false}, uk{134, false};
+  Unit uv{kUnit, false}, uk{kUnit, false};
   if (begin < end) {
     uint4 q[NKS];
     {
@@ -642,26 +670,24 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
     }
     // Staging registers: codes and scales of a K tile and of a V tile.
     struct KRegs {
-      uint32_t c[KC / 4], e;
+      uint32_t c[KC * BITS / 32], e;
     } kx, ky;
     uint32_t vc[VK], vse[VK * CH / 4];
     auto load_k = [&](KRegs& x, int kt, int page) {
       const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
-      const uint8_t* ks = p.k_codes + row * D;
+      const uint8_t* ks = p.k_codes + row * RB;
       const uint8_t* kss = p.k_scale + row * CH;
+      constexpr int N = KC * BITS / 8 < 16 ? KC * BITS / 8 : 16;
 #pragma unroll
-      for (int i = 0; i < KC / 16; ++i) {
-        const uint4 w = *reinterpret_cast<const uint4*>(ks + koff + 16 * i);
-        x.c[4 * i] = w.x; x.c[4 * i + 1] = w.y; x.c[4 * i + 2] = w.z; x.c[4 * i + 3] = w.w;
-      }
+      for (int i = 0; i < KC * BITS / 8 / N; ++i) load_bytes<N>(ks + koff + N * i, x.c + N / 4 * i);
       x.e = kss[ksoff];
     };
     auto load_v = [&](int kt, int page) {
       const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
-      const uint8_t* vs = p.v_codes + row * D;
+      const uint8_t* vs = p.v_codes + row * RB;
       const uint8_t* vss = p.v_scale + row * CH;
 #pragma unroll
-      for (int j = 0; j < VK; ++j) vc[j] = *reinterpret_cast<const uint32_t*>(vs + voff + j * D);
+      for (int j = 0; j < VK; ++j) load_bytes<BITS / 2>(vs + voff + j * RB, vc + j);
       if constexpr (D == 128) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -745,16 +771,16 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
         x = __builtin_amdgcn_readfirstlane(x);
         Unit u;
         u.E = static_cast<int>(x & 0xffu);
-        u.wide = u.E - (255 - static_cast<int>(x >> 16)) > kSpan;
-        if (u.wide) u.E = u.E > wide ? 134 + u.E - wide : 134;
-        if (x == 0) u.E = 134;
+        u.wide = u.E - (255 - static_cast<int>(x >> 16)) > span_of(BITS);
+        if (u.wide) u.E = u.E > wide ? kUnit + u.E - wide : kUnit;
+        if (x == 0) u.E = kUnit;
         return u;
       };
       uv = unit(sv, kWideTop);
       if constexpr (DT == kF16) uk = unit(sk, 255);
     }
-    const float c = DT == kF16 ? ldexpf(a.sml2, uk.E - 134) : a.sml2;
-    const uint32_t kadd = static_cast<uint32_t>(134 - uk.E) << 23, vadd = static_cast<uint32_t>(134 - uv.E) << 23;
+    const float c = DT == kF16 ? ldexpf(a.sml2, uk.E - kUnit) : a.sml2;
+    const uint32_t kadd = static_cast<uint32_t>(kUnit - uk.E) << 23, vadd = static_cast<uint32_t>(kUnit - uv.E) << 23;
 
     // Keys that no row sees, or that are not there: nothing of them may reach a product.
     auto clear_k = [&](KRegs& x, int kt, int page) {
@@ -762,7 +788,7 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
       if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
       if (page < 0 || key0 + kkey < lo || key0 + kkey >= hi) {
 #pragma unroll
-        for (int i = 0; i < KC / 4; ++i) x.c[i] = 0;
+        for (int i = 0; i < KC * BITS / 32; ++i) x.c[i] = 0;
         x.e = static_cast<uint32_t>(uk.E);
       }
     };
@@ -786,8 +812,8 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
       if (k >= KC / 4) return;  // (D = 64 has four)
       constexpr bool f16 = DT == kF16 && !WIDE;
       const float sc = __uint_as_float((x.e << 23) + (f16 ? kadd : 0u));
-      st.k[2 * k] = f16 ? cvt_f16<false>(x.c[k], sc) : cvt_bf16<false>(x.c[k], sc);
-      st.k[2 * k + 1] = f16 ? cvt_f16<true>(x.c[k], sc) : cvt_bf16<true>(x.c[k], sc);
+      st.k[2 * k] = f16 ? cvt_f16<BITS>(x.c, 2 * k, sc) : cvt_bf16<BITS>(x.c, 2 * k, sc);
+      st.k[2 * k + 1] = f16 ? cvt_f16<BITS>(x.c, 2 * k + 1, sc) : cvt_bf16<BITS>(x.c, 2 * k + 1, sc);
       if (k & 1)
         *reinterpret_cast<uint4*>(buf + (WKEYS * wave + kkey) * L::KP + 2 * KC * kq + 8 * (k - 1)) =
             make_uint4(st.k[2 * k - 2], st.k[2 * k - 1], st.k[2 * k], st.k[2 * k + 1]);
@@ -801,8 +827,8 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
           else by = __builtin_amdgcn_ubfe(vse[j / 2], 16 * (j & 1) + 8 * (vdq / 8), 8);
           // (WIDE: far below the largest, a scale may be less than what is taken off)
           const float sc = __uint_as_float(WIDE ? __builtin_elementwise_sub_sat(by << 23, 0u - vadd) : (by << 23) + vadd);
-          st.v[j][0] = WIDE ? cvt_bf16<false>(vc[j], sc) : cvt_f16<false>(vc[j], sc);
-          st.v[j][1] = WIDE ? cvt_bf16<true>(vc[j], sc) : cvt_f16<true>(vc[j], sc);
+          st.v[j][0] = WIDE ? cvt_bf16<BITS>(vc + j, 0, sc) : cvt_f16<BITS>(vc + j, 0, sc);
+          st.v[j][1] = WIDE ? cvt_bf16<BITS>(vc + j, 1, sc) : cvt_f16<BITS>(vc + j, 1, sc);
         }
       } else {
         // column 4 dq + c is V^T row c D/4 + dq, so that neighbouring lanes write neighbouring rows
@@ -1051,7 +1077,7 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
   if (rw + li < rows) {
     const int64_t tok = s.start + qi;
     const bool one = a.splits == 1;
-    const float f = filled(l) ? ldexpf(1.0f, uv.E - 134) / l : 0.0f;
+    const float f = filled(l) ? ldexpf(1.0f, uv.E - kUnit) / l : 0.0f;
     const int64_t at = split * R + tok * p.Hq + h;
     if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
     if (!one && g == 0) a.ml[at] = make_float2(m, l);
@@ -1270,6 +1296,7 @@ int64_t workspace(const lbfq_paged_params* p, const Plan& x) {
 int check_sizes(const lbfq_paged_params* p) {
   const char* who = "lbfq_paged_attention";
   LBFQ_CHECK_ARG(p, "%s: null params", who);
+  LBFQ_CHECK_ARG(p->bits == 0 || p->bits == 4 || p->bits == 8, "%s: codes have 4 or 8 bits", who);
   LBFQ_CHECK_ARG(p->D == 64 || p->D == 128, "%s: D must be 64 or 128", who);
   LBFQ_CHECK_ARG(p->dtype == kBF16 || p->dtype == kF16, "%s: queries are bf16 or fp16", who);
   LBFQ_CHECK_ARG(p->Hk > 0 && p->Hq > 0 && p->Hq % p->Hk == 0 && p->Hq < (1 << 16),
@@ -1339,20 +1366,18 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   const dim3 grid(static_cast<unsigned>(a.main + fill));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool bf = p->dtype == kBF16, d128 = p->D == 128;
-  if (x.decode) {
-    const dim3 block(256);
-    if (bf && d128) hipLaunchKernelGGL((paged_decode_kernel<kBF16, 128>), grid, block, 0, st, a);
-    else if (bf) hipLaunchKernelGGL((paged_decode_kernel<kBF16, 64>), grid, block, 0, st, a);
-    else if (d128) hipLaunchKernelGGL((paged_decode_kernel<kF16, 128>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((paged_decode_kernel<kF16, 64>), grid, block, 0, st, a);
-  } else {
-#define LBFQ_PC(DT, DD) hipLaunchKernelGGL((paged_chunk_kernel<DT, DD>), grid, dim3(256), 0, st, a)
-    if (bf && d128) LBFQ_PC(kBF16, 128);
-    else if (bf) LBFQ_PC(kBF16, 64);
-    else if (d128) LBFQ_PC(kF16, 128);
-    else LBFQ_PC(kF16, 64);
-#undef LBFQ_PC
-  }
+#define LBFQ_PA(KERNEL, BB)                                                                              \
+  do {                                                                                                   \
+    if (bf && d128) hipLaunchKernelGGL((KERNEL<kBF16, 128, BB>), grid, dim3(256), 0, st, a);             \
+    else if (bf) hipLaunchKernelGGL((KERNEL<kBF16, 64, BB>), grid, dim3(256), 0, st, a);                 \
+    else if (d128) hipLaunchKernelGGL((KERNEL<kF16, 128, BB>), grid, dim3(256), 0, st, a);               \
+    else hipLaunchKernelGGL((KERNEL<kF16, 64, BB>), grid, dim3(256), 0, st, a);                          \
+  } while (0)
+  if (x.decode && p->bits == 4) LBFQ_PA(paged_decode_kernel, 4);
+  else if (x.decode) LBFQ_PA(paged_decode_kernel, 8);
+  else if (p->bits == 4) LBFQ_PA(paged_chunk_kernel, 4);
+  else LBFQ_PA(paged_chunk_kernel, 8);
+#undef LBFQ_PA
   LBFQ_LAUNCH_CHECK("lbfq_paged_attention");
   if (x.splits > 1) {
     const bool narrow = x.splits <= 16 && R >= 4096;

@@ -51,6 +51,7 @@ std::string name(at::ScalarType t) {
     case at::kLong: return "torch.int64";
     case at::kByte: return "torch.uint8";
     case at::kFloat8_e4m3fn: return "torch.float8_e4m3fn";
+    case at::kFloat4_e2m1fn_x2: return "torch.float4_e2m1fn_x2";
     default: return std::string("torch.") + c10::toString(t);
   }
 }
@@ -150,6 +151,34 @@ void weight(const OptTensor& w, const char* what, int64_t d, int64_t index, Tens
   ptr = held.data_ptr();
 }
 
+// cos and sin (P, R/2) fp32; sets the table's length and R
+template <class P>
+void set_tables(P& p, const Tensor& cos, const Tensor& sin, int64_t index, Tensor& held_cos, Tensor& held_sin) {
+  if (cos.dim() != 2 || sin.sizes() != cos.sizes())
+    bad_value("cos and sin must be (P, R/2); got " + str(cos) + " and " + str(sin));
+  if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat)
+    bad_type("cos and sin must be float32; got " + name(cos.scalar_type()) + " and " + name(sin.scalar_type()));
+  p.table_len = cos.size(0);
+  const int64_t half = cos.size(1);
+  if (half == 0 || half % 8 || 2 * half > p.D)
+    bad_value("R must be a multiple of 16 up to D=" + std::to_string(p.D) + "; got " + std::to_string(2 * half));
+  p.rot = static_cast<int>(2 * half);
+  if (!on(cos, index) || !on(sin, index)) bad_value("cos and sin must live on " + cuda(index));
+  auto table = [](const Tensor& t) {
+    return t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t
+                                                                                  : t.clone(at::MemoryFormat::Contiguous);
+  };
+  held_cos = table(cos);
+  held_sin = table(sin);
+  p.cos = held_cos.template data_ptr<float>();
+  p.sin = held_sin.template data_ptr<float>();
+}
+
+bool halves_of(const std::string& pairs) {
+  if (pairs != "adjacent" && pairs != "halves") bad_value("pairs must be 'adjacent' or 'halves'; got '" + pairs + "'");
+  return pairs == "halves";
+}
+
 void norm_params(Norm& n, const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& cos,
                  const Tensor& sin, const OptTensor& positions, double eps, const std::string& pairs) {
   const int64_t dims = q.dim();
@@ -171,21 +200,11 @@ void norm_params(Norm& n, const Tensor& q, const Tensor& k, const OptTensor& qw,
   if (p.D != 64 && p.D != 128) bad_value("D must be 64 or 128; got " + std::to_string(p.D));
   if ((o && k.size(0) != p.B) || k.size(o) != p.S || k.size(o + 2) != p.D || p.Hq == 0 || p.Hk == 0)
     bad_value("q and k must agree in all but their heads; got " + str(q) + " and " + str(k));
-  if (pairs != "adjacent" && pairs != "halves") bad_value("pairs must be 'adjacent' or 'halves'; got '" + pairs + "'");
-  p.halves = pairs == "halves";
+  p.halves = halves_of(pairs);
   if (!(eps >= 0.0 && eps <= std::numeric_limits<float>::max()))
     bad_value("eps must be finite and not negative; got " + std::to_string(eps));
   p.eps = static_cast<float>(eps);
-  if (cos.dim() != 2 || sin.sizes() != cos.sizes())
-    bad_value("cos and sin must be (P, R/2); got " + str(cos) + " and " + str(sin));
-  if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat)
-    bad_type("cos and sin must be float32; got " + name(cos.scalar_type()) + " and " + name(sin.scalar_type()));
-  p.table_len = cos.size(0);
-  const int64_t half = cos.size(1);
-  if (half == 0 || half % 8 || 2 * half > p.D)
-    bad_value("R must be a multiple of 16 up to D=" + std::to_string(p.D) + "; got " + std::to_string(2 * half));
-  p.rot = static_cast<int>(2 * half);
-  if (!on(cos, index) || !on(sin, index)) bad_value("cos and sin must live on " + cuda(index));
+  set_tables(p, cos, sin, index, n.cos, n.sin);
   if (!positions) {
     if (p.S > p.table_len)
       bad_value("the table has " + std::to_string(p.table_len) + " positions, q has " + std::to_string(p.S));
@@ -205,14 +224,6 @@ void norm_params(Norm& n, const Tensor& q, const Tensor& k, const OptTensor& qw,
   }
   weight(qw, "q_weight", p.D, index, n.qw, p.q_weight, p.q_weight_dtype);
   weight(kw, "k_weight", p.D, index, n.kw, p.k_weight, p.k_weight_dtype);
-  auto table = [](const Tensor& t) {
-    return t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t
-                                                                                  : t.clone(at::MemoryFormat::Contiguous);
-  };
-  n.cos = table(cos);
-  n.sin = table(sin);
-  p.cos = n.cos.data_ptr<float>();
-  p.sin = n.sin.data_ptr<float>();
   n.q = aligned(q);
   n.k = aligned(k);
   p.q = n.q.data_ptr();
@@ -385,11 +396,13 @@ bool changes_queries(const Tensor& out, const Tensor& q) {
 struct Cache {
   const Tensor &kc, &ks, &vc, &vs;
   int64_t pages, heads, page, d, index;
-  int shift;
+  int shift, bits;
 
   Cache(const Tensor& kc_, const Tensor& ks_, const Tensor& vc_, const Tensor& vs_) : kc(kc_), ks(ks_), vc(vc_), vs(vs_) {
     if (kc.dim() != 4) bad_value("cache codes must be (pages, H, page size, D); got " + str(kc));
-    pages = kc.size(0); heads = kc.size(1); page = kc.size(2); d = kc.size(3);
+    bits = kc.scalar_type() == at::kFloat4_e2m1fn_x2 ? 4 : 8;
+    pages = kc.size(0); heads = kc.size(1); page = kc.size(2);
+    d = bits == 4 ? 2 * kc.size(3) : kc.size(3);  // (two 4-bit codes are one element)
     if (d != 64 && d != 128) bad_value("cache D must be 64 or 128; got " + std::to_string(d));
     if (page < 16 || page > 1024 || (page & (page - 1)))
       bad_value("cache page size must be a power of two from 16 to 1024; got " + std::to_string(page));
@@ -398,10 +411,10 @@ struct Cache {
     if (vc.sizes() != kc.sizes() || ks.sizes() != want || vs.sizes() != want)
       bad_value("cache tensors must be codes " + str(kc) + " and scales " + str(want) + "; got " + str(vc) + ", " + str(ks) +
                 " and " + str(vs));
-    if (kc.scalar_type() != at::kFloat8_e4m3fn || vc.scalar_type() != at::kFloat8_e4m3fn || ks.scalar_type() != at::kByte ||
-        vs.scalar_type() != at::kByte)
-      bad_type("cache codes must be float8_e4m3fn and scales uint8; got " + name(kc.scalar_type()) + ", " +
-               name(vc.scalar_type()) + ", " + name(ks.scalar_type()) + " and " + name(vs.scalar_type()));
+    if ((kc.scalar_type() != at::kFloat8_e4m3fn && bits == 8) || vc.scalar_type() != kc.scalar_type() ||
+        ks.scalar_type() != at::kByte || vs.scalar_type() != at::kByte)
+      bad_type("cache codes must both be float8_e4m3fn or float4_e2m1fn_x2 and scales uint8; got " + name(kc.scalar_type()) +
+               ", " + name(vc.scalar_type()) + ", " + name(ks.scalar_type()) + " and " + name(vs.scalar_type()));
     if (!kc.is_cuda() || !on(ks, kc.get_device()) || !on(vc, kc.get_device()) || !on(vs, kc.get_device()))
       bad_value("cache tensors must live on one CUDA device");
     if (!kc.is_contiguous() || !ks.is_contiguous() || !vc.is_contiguous() || !vs.is_contiguous())
@@ -424,6 +437,11 @@ struct Cache {
     p.v_scale = static_cast<uint8_t*>(vs.data_ptr());
     p.num_pages = pages;
     p.page_shift = shift;
+    p.bits = bits;
+  }
+
+  void written() const {
+    for (const Tensor* t : {&kc, &ks, &vc, &vs}) ::written(*t);
   }
 };
 
@@ -442,17 +460,21 @@ Tensor table_tensor(const Tensor& t, int64_t index) {
   return t.stride(1) == 1 ? t : t.contiguous();
 }
 
+// k and v: (T, the cache's heads, D), of one dtype, where the cache is
+void check_rows(const Cache& c, const Tensor& k, const Tensor& v) {
+  if (k.dim() != 3 || k.size(1) != c.heads || k.size(2) != c.d || v.sizes() != k.sizes())
+    bad_value("k and v must be (T, " + std::to_string(c.heads) + ", " + std::to_string(c.d) + "); got " + str(k) + " and " +
+              str(v));
+  if (!on(k, c.index) || !on(v, c.index))
+    bad_value("k and v must live on the cache's " + cuda(c.index) + "; got " + k.device().str() + " and " + v.device().str());
+  if (v.scalar_type() != k.scalar_type())
+    bad_type("k and v must have one dtype; got " + name(k.scalar_type()) + " and " + name(v.scalar_type()));
+}
+
 void kv_write(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs,
            const Tensor& slots_) {
   const Cache c(kc, ks, vc, vs);
-  if (k_.dim() != 3 || k_.size(1) != c.heads || k_.size(2) != c.d || v_.sizes() != k_.sizes())
-    bad_value("k and v must be (T, " + std::to_string(c.heads) + ", " + std::to_string(c.d) + "); got " + str(k_) + " and " +
-              str(v_));
-  if (!on(k_, c.index) || !on(v_, c.index))
-    bad_value("k and v must live on the cache's " + cuda(c.index) + "; got " + k_.device().str() + " and " +
-              v_.device().str());
-  if (v_.scalar_type() != k_.scalar_type())
-    bad_type("k and v must have one dtype; got " + name(k_.scalar_type()) + " and " + name(v_.scalar_type()));
+  check_rows(c, k_, v_);
   lbfq_kv_write_params p{};
   p.dtype = dtype_code(k_.scalar_type());
   const Tensor slots = index_tensor(slots_, "slots", k_.size(0), c.index, at::kLong);
@@ -470,7 +492,63 @@ void kv_write(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Tensor
   p.slots = slots.data_ptr<int64_t>();
   c.set(p);
   check_rc(lbfq_kv_write(&p, stream(k)), "lbfq_kv_write");
-  for (const Tensor* t : {&kc, &ks, &vc, &vs}) written(*t);
+  c.written();
+}
+
+OptTensor kv_append(const OptTensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& kc, const Tensor& ks,
+                    const Tensor& vc, const Tensor& vs, const Tensor& slots_, const Tensor& cos_, const Tensor& sin_,
+                    const Tensor& positions, const std::string& pairs) {
+  const char* who = "append_kv_cache";
+  const Cache c(kc, ks, vc, vs);
+  check_rows(c, k_, v_);
+  lbfq_kv_append_params p{};
+  p.dtype = dtype_code(k_.scalar_type());
+  p.T = k_.size(0); p.Hk = c.heads; p.D = c.d;
+  if (q_) {
+    if (q_->dim() != 3 || q_->size(0) != p.T || q_->size(1) == 0 || q_->size(2) != c.d)
+      bad_value("q must be (" + std::to_string(p.T) + ", Hq, " + std::to_string(c.d) + "); got " + str(*q_));
+    if (!on(*q_, c.index)) bad_value("q must live on the cache's " + cuda(c.index) + "; got " + q_->device().str());
+    if (q_->scalar_type() != k_.scalar_type())
+      bad_type("q and k must have one dtype; got " + name(q_->scalar_type()) + " and " + name(k_.scalar_type()));
+    p.Hq = q_->size(1);
+  }
+  const Tensor slots = index_tensor(slots_, "slots", p.T, c.index, at::kLong);
+  p.halves = halves_of(pairs);
+  Tensor cos, sin;
+  set_tables(p, cos_, sin_, c.index, cos, sin);
+  if (positions.scalar_type() != at::kInt && positions.scalar_type() != at::kLong)
+    bad_type("positions must be int32 or int64; got " + name(positions.scalar_type()));
+  if (!on(positions, c.index)) bad_value("positions must live on " + cuda(c.index) + "; got " + positions.device().str());
+  if (positions.dim() != 1 || positions.size(0) != p.T)
+    bad_value("positions must have shape (" + std::to_string(p.T) + ",); got " + str(positions));
+  p.positions = positions.data_ptr();
+  p.positions_i64 = positions.scalar_type() == at::kLong;
+  p.pos_t = positions.stride(0);
+  const Tensor none;
+  if (at::GradMode::is_enabled() && ((q_ && q_->requires_grad()) || k_.requires_grad() || v_.requires_grad() ||
+                                     cos_.requires_grad() || sin_.requires_grad()))
+    refuse_grad(who);
+  c.refuse_derivatives(who);
+  refuse_tangent(who, {q_ ? &*q_ : &none, &k_, &v_, &cos_, &sin_});
+  OptTensor out;
+  On dev(k_);
+  if (q_) out = at::empty(q_->sizes(), q_->options());
+  if (p.T == 0) return out;
+  const Tensor k = aligned(k_), v = aligned(v_), q = q_ ? aligned(*q_) : none;
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.k_t = row_stride(k, 0); p.k_h = row_stride(k, 1);
+  p.v_t = row_stride(v, 0); p.v_h = row_stride(v, 1);
+  if (q_) {
+    p.q = q.data_ptr();
+    p.q_t = row_stride(q, 0); p.q_h = row_stride(q, 1);
+    p.q_out = out->data_ptr();
+  }
+  p.slots = slots.data_ptr<int64_t>();
+  c.set(p);
+  check_rc(lbfq_kv_append(&p, stream(k)), "lbfq_kv_append");
+  c.written();
+  return out;
 }
 
 std::tuple<Tensor, Tensor> kv_read(const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs,
@@ -597,6 +675,7 @@ PYBIND11_MODULE(_lbfq_torch, m) {
   });
   m.def("qk_norm_rope", &norm);
   m.def("write_kv_cache", &kv_write);
+  m.def("append_kv_cache", &kv_append);
   m.def("read_kv_cache", &kv_read);
   m.def("paged_attention", &attention);
 }

@@ -23,7 +23,14 @@ from .kmeans import (
     q_kmeans_reorder,
     v_kmeans_reorder,
 )
-from .kv_cache import PagedKVCache, empty_kv_cache, paged_attention, read_kv_cache, write_kv_cache
+from .kv_cache import (
+    PagedKVCache,
+    append_kv_cache,
+    empty_kv_cache,
+    paged_attention,
+    read_kv_cache,
+    write_kv_cache,
+)
 from .pipeline import PreparedQKV, prepare_qkv
 from .preprocess import group_mean_q, smooth_k, smooth_v_per_block
 from .qk_norm import qk_norm_rope, rotary_table
@@ -67,6 +74,7 @@ __all__ = [
     "v_kmeans_reorder",
     "reference_attention",
     "smooth_k",
+    "append_kv_cache",
     "empty_kv_cache",
     "paged_attention",
     "qk_norm_rope",

@@ -181,6 +181,24 @@ class KvWriteParams(ctypes.Structure):
         ("slots", _vp),
         ("k_codes", _vp), ("k_scale", _vp), ("v_codes", _vp), ("v_scale", _vp),
         ("num_pages", _i64), ("page_shift", _i32),
+        ("bits", _i32),
+    ]
+
+
+class KvAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("dtype", _i32),
+        ("T", _i64), ("Hq", _i64), ("Hk", _i64), ("D", _i64),
+        ("q_t", _i64), ("q_h", _i64), ("k_t", _i64), ("k_h", _i64), ("v_t", _i64), ("v_h", _i64),
+        ("cos", _vp), ("sin", _vp),
+        ("table_len", _i64), ("rot", _i32),
+        ("positions", _vp), ("positions_i64", _i32), ("pos_t", _i64),
+        ("halves", _i32),
+        ("q_out", _vp),
+        ("slots", _vp),
+        ("k_codes", _vp), ("k_scale", _vp), ("v_codes", _vp), ("v_scale", _vp),
+        ("num_pages", _i64), ("page_shift", _i32),
+        ("bits", _i32),
     ]
 
 
@@ -192,6 +210,7 @@ class KvReadParams(ctypes.Structure):
         ("block_table", _vp), ("table_stride", _i64), ("table_cols", _i64),
         ("seq_lens", _vp),
         ("k_out", _vp), ("v_out", _vp), ("dtype", _i32),
+        ("bits", _i32),
     ]
 
 
@@ -210,6 +229,7 @@ class PagedParams(ctypes.Structure):
         ("lse", _vp),
         ("fill_rest", _i32),
         ("workspace", _vp), ("workspace_bytes", _i64),
+        ("bits", _i32),
     ]
 
 
@@ -252,6 +272,7 @@ _SIGS = {
     "lbfq_qk_norm_rope_bwd_rows": (_i64, [ctypes.POINTER(QkNormParams)]),
     "lbfq_qk_norm_rope_bwd": (_i32, [ctypes.POINTER(QkNormParams), ctypes.POINTER(QkNormGrads), _vp]),
     "lbfq_kv_write": (_i32, [ctypes.POINTER(KvWriteParams), _vp]),
+    "lbfq_kv_append": (_i32, [ctypes.POINTER(KvAppendParams), _vp]),
     "lbfq_kv_read": (_i32, [ctypes.POINTER(KvReadParams), _vp]),
     "lbfq_paged_attention_workspace_bytes": (_i64, [ctypes.POINTER(PagedParams)]),
     "lbfq_paged_attention": (_i32, [ctypes.POINTER(PagedParams), _vp]),

@@ -1,9 +1,10 @@
 """A quantised paged K/V cache and attention over it, on gfx950.
 
-The cache holds K and V in the package's MXFP8 format (E4M3 codes, one E8M0
-scale per 32 columns of a row: ``quant.mxfp8_qk_quant`` bit for bit below 3e38),
-in pages that sequences take as they grow.  ``write_kv_cache`` quantises new rows into
-it, ``paged_attention`` attends over it (one token of each sequence, or a chunk),
+The cache holds K and V with one E8M0 scale per 32 columns of a row, in 8 bits
+(MXFP8, E4M3 codes: ``quant.mxfp8_qk_quant`` bit for bit below 3e38) or in 4 (MXFP4,
+E2M1 codes), in pages that sequences take as they grow.  ``write_kv_cache`` quantises
+new rows into it, ``append_kv_cache`` rotates Q and K by their positions on the way,
+``paged_attention`` attends over it (one token of each sequence, or a chunk),
 ``read_kv_cache`` gives the values back, e.g. for ``fake_quant_attention``.
 
 These are for inference: they have no derivative, backward or forward, and refuse inputs that
@@ -29,26 +30,32 @@ class PagedKVCache(NamedTuple):
     Row ``r`` of page ``p`` of head ``h`` is ``k_codes[p, h, r]``; its value is code *
     2^(scale - 127), ``k_scale[p, h, r, c]`` for columns 32 c ... 32 c + 31.  A cache
     that is not filled by ``write_kv_cache`` holds no NaN code and no scale of 255 where
-    a query looks.
+    a query looks.  In 4 bits an element of the codes holds two: the even column in its
+    low half, the odd one in its high half, 0, 1/2, 1, 3/2, 2, 3, 4, 6 as 0 ... 7 and plus
+    8 for the negative ones.  (Torch can do little with that dtype: copy pages as
+    ``k_codes.view(torch.uint8)``.)
     """
 
-    k_codes: torch.Tensor  # (pages, H, page size, D) float8_e4m3fn
+    k_codes: torch.Tensor  # (pages, H, page size, D) float8_e4m3fn, or (..., D / 2) float4_e2m1fn_x2
     k_scale: torch.Tensor  # (pages, H, page size, D / 32) uint8, E8M0
     v_codes: torch.Tensor
     v_scale: torch.Tensor
 
 
-def empty_kv_cache(num_pages: int, page_size: int, heads: int, head_dim: int, *, device="cuda") -> PagedKVCache:
-    """A cache of zeros.  page_size: 16 to 1024 tokens, a power of two."""
+def empty_kv_cache(num_pages: int, page_size: int, heads: int, head_dim: int, *, device="cuda",
+                   bits: int = 8) -> PagedKVCache:
+    """A cache of zeros.  page_size: 16 to 1024 tokens, a power of two; bits of a code: 8 or 4."""
     if head_dim not in (64, 128):
         raise ValueError(f"D must be 64 or 128; got {head_dim}")
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_size must be one of {PAGE_SIZES}; got {page_size}")
     if num_pages <= 0 or heads <= 0:
         raise ValueError(f"num_pages and heads must be positive; got {num_pages} and {heads}")
+    if bits not in (4, 8):
+        raise ValueError(f"bits must be 4 or 8; got {bits}")
     rows = (int(num_pages), int(heads), int(page_size))
-    k, v = (torch.zeros((*rows, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
-            for _ in range(2))
+    width, code = (head_dim, torch.float8_e4m3fn) if bits == 8 else (head_dim // 2, torch.float4_e2m1fn_x2)
+    k, v = (torch.zeros((*rows, width), dtype=torch.uint8, device=device).view(code) for _ in range(2))
     ks, vs = (torch.full((*rows, head_dim // BLOCK), 127, dtype=torch.uint8, device=device) for _ in range(2))
     return PagedKVCache(k, ks, v, vs)
 
@@ -65,9 +72,31 @@ def write_kv_cache(k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, slots:
     and the codes round to nearest, ties to even.  As with the package's other
     quantisers, a NaN leaves its block's scale alone and becomes -448 * scale.  An
     infinity, or anything past 448 * 2^119 = 3e38, is held as that: the cache's
-    values are finite, and what a query does not see cannot reach its result.
+    values are finite, and what a query does not see cannot reach its result.  In 4 bits
+    the same with 6 in the place of 448, and 6 * 2^125 = 2.6e38 as the largest.
     """
     _lib.torch_ops().write_kv_cache(k, v, *cache, slots)
+
+
+def append_kv_cache(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor,
+                    cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, *,
+                    pairs: str = "adjacent") -> torch.Tensor | None:
+    """Rotate new rows of Q and K by their positions, write K and V into the cache, return Q.
+
+    ``k`` and ``v`` are (T, H, D) and ``q`` (T, Hq, D) (or None: only the cache is
+    written, and None returned) in one of fp32, fp16 and bf16; views are read where
+    they are.  The first R columns are rotated in pairs as by ``qk_norm_rope``, with
+    ``cos`` and ``sin`` (P, R/2) fp32 (``rotary_table``) and ``positions`` (T,) int32
+    or int64; a negative position is not rotated.  A model that normalises Q and K
+    calls ``qk_norm_rope`` and ``write_kv_cache`` instead.  ``slots`` as in
+    ``write_kv_cache``.
+
+    The rotated values are fp32, each product and the sum rounded.  Q is rounded once
+    more, to its dtype; K goes from there into the cache, without a rounding to 16
+    bits on the way.  A token whose position lies past the tables comes out as NaN in
+    Q's rotated columns, and nothing of it is written.  Returns a new contiguous tensor.
+    """
+    return _lib.torch_ops().append_kv_cache(q, k, v, *cache, slots, cos, sin, positions, pairs)
 
 
 def read_kv_cache(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor, max_len: int, *,
@@ -115,11 +144,11 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Ten
     Scores, softmax and sums are fp32 on exact products of cached values and
     queries; P is rounded for the second product, to 11 bits or more down to 2^-21
     of the row's largest, and the result once.  A NaN in a query makes its row NaN.
-    Averages stay finite up to the cache's largest values, 448 * 2^119.
+    Averages stay finite up to the cache's largest values, 448 * 2^119 or 6 * 2^125.
     """
     out, lse = _lib.torch_ops().paged_attention(q, *cache, block_table, seq_lens, query_starts, max_query_len, sm_scale,
                                                 causal, window, out, return_lse)
     return (out, lse) if return_lse else out
 
 
-__all__ = ["PagedKVCache", "empty_kv_cache", "paged_attention", "read_kv_cache", "write_kv_cache"]
+__all__ = ["PagedKVCache", "append_kv_cache", "empty_kv_cache", "paged_attention", "read_kv_cache", "write_kv_cache"]
