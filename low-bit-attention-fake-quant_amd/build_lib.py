@@ -52,6 +52,7 @@ UNITS = {
     "lbfq_qknorm.hip": ["-ffp-contract=off"],
     "lbfq_kvcache.hip": ["-ffp-contract=off"],
     "lbfq_paged.hip": ["-ffp-contract=off"],
+    "lbfq_paged4.hip": ["-ffp-contract=off"],
 }
 
 
@@ -92,8 +93,8 @@ def _check_mfma(objs: list[str]) -> None:
     if bad:
         lines = "\n".join(f"{os.path.basename(o)}: {x}" for o, b in bad.items() for x in b[:4])
         raise RuntimeError("gfx950 code check failed (a scaled MFMA reading a scale from its own destination "
-                           "registers, an LDS DMA directly after an M0 write, or inline asm touching an MFMA's "
-                           "registers inside its hazard window):\n" + lines)
+                           "registers, an LDS DMA directly after an M0 write, inline asm touching an MFMA's "
+                           "registers inside its hazard window, or a conversion of 32 values over its own operands):\n" + lines)
 
 
 def device_asm(obj: str) -> str:

@@ -31,249 +31,22 @@
 // bf16's 8 would cost as much as the output's own rounding.  K is bf16 (exact) for bf16 queries, and for fp16 ones fp16
 // under the same rule.  4680 tokens over 32760 keys, 12 heads of 128, all seen: 1.10 ms, 855 TFLOP/s, the matrix units
 // busy 39% of the cycles at 2.1 GHz (a large library product: 1218 TFLOP/s).
-#include <algorithm>
-#include <limits>
-#include <type_traits>
-
-#include "lbfq_common.h"
-#include "../../include/lbfq.h"
+#include "lbfq_paged_common.h"
 
 using namespace lbfq;
+using namespace lbfq::paged;
 
 namespace {
-
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef float v16f __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-struct Args {
-  lbfq_paged_params p;
-  int G;          // query heads of a key head
-  int splits;     // parts of the keys
-  int least;      // key tiles of a part, at least
-  int slots;      // chunk: places for row tiles, over all sequences
-  uint32_t piece;   // chunk: neighbouring slots that go to one XCD
-  uint32_t combos;  // decode: sequences x key heads; chunk: key heads x parts
-  int64_t main;   // workgroups that attend (the others fill)
-  float sml2;     // sm_scale * log2(e)
-  float2* ml;     // (splits, T * Hq): maximum (log2 units) and sum of a part
-  float* acc;     // (splits, T * Hq, D): a part's average of the values
-};
-
-// One sequence, clamped to what the tensors hold.
-struct Seq {
-  int n, len, start;
-  bool causal;
-  int window;
-  // keys [lo, hi) of query i
-  __device__ __forceinline__ int hi(int i) const {
-    if (!causal) return len;
-    const int h = len - n + i + 1;
-    return h < 0 ? 0 : h;  // i < n: never above len
-  }
-  __device__ __forceinline__ int lo(int i) const {
-    if (!window) return 0;
-    const int l = len - n + i + 1 - window;
-    return l < 0 ? 0 : l;
-  }
-};
-
-__device__ __forceinline__ Seq sequence(const lbfq_paged_params& p, int64_t b) {
-  Seq s;
-  const int T = static_cast<int>(p.T);
-  int s0 = p.query_starts[b], s1 = p.query_starts[b + 1];
-  s0 = s0 < 0 ? 0 : s0 > T ? T : s0;
-  s1 = s1 < s0 ? s0 : s1 > T ? T : s1;
-  s.start = s0;
-  s.n = s1 - s0;
-  const int cap = static_cast<int>(p.table_cols << p.page_shift);
-  const int len = p.seq_lens[b];
-  s.len = len < 0 ? 0 : len > cap ? cap : len;
-  s.causal = p.causal != 0;
-  s.window = static_cast<int>(p.window);
-  return s;
-}
-
-// The chunk kernel's row tiles have 128 rows.  Sequence b has the slots from slot_of(b) up to slot_of(b + 1), one more
-// than its rows need at the most: where a tile belongs follows from query_starts alone, and hardly a workgroup comes
-// for nothing.
-constexpr int kChunkRows = 128;
-__device__ __forceinline__ int slot_of(const lbfq_paged_params& p, int G, int b) {
-  const int T = static_cast<int>(p.T), s0 = p.query_starts[b];
-  return (s0 < 0 ? 0 : s0 > T ? T : s0) * G / kChunkRows + b;
-}
-// The last sequence whose slots start at or before `slot`: 64 places looked at at a time.
-__device__ __forceinline__ int sequence_at(const lbfq_paged_params& p, int G, int slot) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0;
-  for (int n = static_cast<int>(p.B); n > 1;) {
-    const int step = (n + 63) / 64, i = lane * step;
-    const uint64_t before = __ballot(i < n && slot_of(p, G, lo + (i < n ? i : 0)) <= slot);
-    const int k = before ? 63 - __builtin_clzll(before) : 0;
-    lo += k * step;
-    n = step < n - k * step ? step : n - k * step;
-  }
-  return lo;
-}
-
-// Rows of the token dimension that no sequence has: zero (a new output), lse -inf.
-template <int D>
-__device__ void fill_rest(const lbfq_paged_params& p, int64_t wg, int64_t wgs) {
-  int s0 = p.query_starts[0], s1 = p.query_starts[p.B];
-  const int T = static_cast<int>(p.T);
-  s0 = s0 < 0 ? 0 : s0 > T ? T : s0;
-  s1 = s1 < s0 ? s0 : s1 > T ? T : s1;
-  const int rest = T - (s1 - s0);
-  for (int64_t k = wg; k < rest; k += wgs) {
-    const int64_t t = k < s0 ? k : k - s0 + s1;
-    for (int i = threadIdx.x; p.fill_rest && i < p.Hq * (D / 8); i += blockDim.x) {
-      const int h = i / (D / 8), d = i % (D / 8);
-      reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + t * p.out_t + h * p.out_h)[d] = make_uint4(0, 0, 0, 0);
-    }
-    if (p.lse)
-      for (int h = threadIdx.x; h < p.Hq; h += blockDim.x) p.lse[t * p.Hq + h] = -INFINITY;
-  }
-}
-
-// The larger, NaN if either is: v_maximum3_f32, three operands an instruction, where fmaxf would first quiet each
-// MFMA result with an instruction of its own
-__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-
-// v of the lanes 16 and 32 away (v_permlane16_swap / v_permlane32_swap of v with
-// itself leave it and the partner's value in the two results)
-__device__ __forceinline__ float max_x32(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float add_x32(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float max_x16(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float add_x16(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  const f32x2 v = {a, b};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-}
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  const f32x2 v = {a, b};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
-}
-template <int DT>
-__device__ __forceinline__ uint32_t pack_dt(float a, float b) {
-  if constexpr (DT == kBF16) return pack_bf16(a, b);
-  else return pack_f16(a, b);
-}
-
-// Eight fp16 values as two bf16 terms each: eight bits and the other three, exact
-__device__ __forceinline__ void split_f16(const uint4& x, uint4& hi, uint4& lo) {
-  const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-  uint32_t h[4], r[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float a = f16_bits_to_f32(static_cast<uint16_t>(in[e])), b = f16_bits_to_f32(static_cast<uint16_t>(in[e] >> 16));
-    h[e] = pack_bf16(a, b);
-    r[e] = pack_bf16(a - __uint_as_float(h[e] << 16), b - __uint_as_float(h[e] & 0xffff0000u));
-  }
-  hi = make_uint4(h[0], h[1], h[2], h[3]);
-  lo = make_uint4(r[0], r[1], r[2], r[3]);
-}
-
-// The pair I of the codes from w on (two in 16 bits, or in 8) times 2^e as 16-bit values; sc: 2^e as fp32.
-template <int BITS>
-__device__ __forceinline__ uint32_t cvt_bf16(const uint32_t* w, int i, float sc) {
-  if constexpr (BITS == 8) {
-    return __builtin_bit_cast(uint32_t, i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i >> 1], sc, true)
-                                              : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i >> 1], sc, false));
-  } else {
-    const uint32_t x = w[i >> 2];
-    switch (i & 3) {  // (known once the loops are unrolled)
-      case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 0));
-      case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 1));
-      case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 2));
-      default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 3));
-    }
-  }
-}
-template <int BITS>
-__device__ __forceinline__ uint32_t cvt_f16(const uint32_t* w, int i, float sc) {
-  if constexpr (BITS == 8) {
-    return __builtin_bit_cast(uint32_t, i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i >> 1], sc, true)
-                                              : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i >> 1], sc, false));
-  } else {
-    const uint32_t x = w[i >> 2];
-    switch (i & 3) {
-      case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 0));
-      case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 1));
-      case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 2));
-      default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 3));
-    }
-  }
-}
-
-// N bytes from p on, in words
-template <int N>
-__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
-  if constexpr (N == 16) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else if constexpr (N == 8) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x; w[1] = v.y;
-  } else if constexpr (N == 4) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  } else {
-    w[0] = *reinterpret_cast<const uint16_t*>(p);
-  }
-}
-
-__device__ __forceinline__ v4f mfma16_bf16(const uint4& a, const uint4& b, const v4f& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                  0);
-}
-__device__ __forceinline__ v16f mfma32_bf16(const uint4& a, const uint4& b, const v16f& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                  0);
-}
-__device__ __forceinline__ v16f mfma32_f16(const uint4& a, const uint4& b, const v16f& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// Whether a row's sum has anything in it (a NaN has: a row whose query holds one comes out as NaN, not as empty)
-__device__ __forceinline__ bool filled(float l) { return l != 0.0f; }
-
-
-// lse of a row (natural logarithm) from what its sum is relative to, in log2 units, and the sum
-__device__ __forceinline__ float row_lse(float m, float l) {
-  return filled(l) ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
-}
 
 // ---- decode ------------------------------------------------------------------
 
 // A wave's 32 keys in registers: key t 16 + n of K for lane (n, g) = (lane % 16,
 // lane / 16), columns 64 c + 16 g ..; rows t 16 + 4 g + i of V, columns (D/16) n ..
-template <int D, int BITS>
+template <int D>
 struct Tile {
-  static constexpr int KW = BITS / 2, VB = D / 16 * BITS / 8, VW = (VB + 3) / 4;  // words of 16 codes, bytes and words of a V row
-  uint32_t k[2][D / 64][KW];
+  uint4 k[2][D / 64];
   uint32_t ks[2];
-  uint32_t v[2][4][VW];
+  uint32_t v[2][4][D / 64];
   uint32_t vs[2][D / 32];  // the scales of its four V rows
   bool ok[2];               // the page is there
 };
@@ -287,11 +60,10 @@ __device__ __forceinline__ void load_pages(const lbfq_paged_params& p, const int
   }
 }
 
-template <int D, int BITS>
+template <int D>
 __device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int (&pages)[2], int kvh, int kb, int n,
-                                          int g, Tile<D, BITS>& x) {
-  constexpr int RB = D * BITS / 8;  // bytes of a row
-  using X = Tile<D, BITS>;
+                                          int g, Tile<D>& x) {
+  constexpr int NB = D / 16;
   int64_t row[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -299,24 +71,35 @@ __device__ __forceinline__ void load_tile(const lbfq_paged_params& p, const int 
     const int page = x.ok[t] ? pages[t] : 0;
     row[t] = (static_cast<int64_t>(page * static_cast<int>(p.Hk) + kvh) << p.page_shift) +
              ((kb + 16 * t) & ((1 << p.page_shift) - 1));
-    const uint8_t* kr = p.k_codes + row[t] * RB + (n * RB + 2 * BITS * g);
+    const uint8_t* kr = p.k_codes + row[t] * D + (n * D + 16 * g);
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) load_bytes<2 * BITS>(kr + 8 * BITS * c, x.k[t][c]);
-    load_bytes<D / 32>(p.k_scale + row[t] * (D / 32) + n * (D / 32), &x.ks[t]);
+    for (int c = 0; c < D / 64; ++c) x.k[t][c] = *reinterpret_cast<const uint4*>(kr + 64 * c);
+    const uint8_t* ks = p.k_scale + row[t] * (D / 32) + n * (D / 32);
+    if constexpr (D == 128) x.ks[t] = *reinterpret_cast<const uint32_t*>(ks);
+    else x.ks[t] = *reinterpret_cast<const uint16_t*>(ks);
   }
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const uint8_t* vr = p.v_codes + row[t] * RB + (4 * g * RB + X::VB * n);
-    load_bytes<4 * (D / 32)>(p.v_scale + row[t] * (D / 32) + 4 * g * (D / 32), x.vs[t]);
+    const uint8_t* vr = p.v_codes + row[t] * D + (4 * g * D + NB * n);
+    const uint8_t* vs = p.v_scale + row[t] * (D / 32) + 4 * g * (D / 32);
+    if constexpr (D == 128) {
+      const uint4 s = *reinterpret_cast<const uint4*>(vs);
+      x.vs[t][0] = s.x; x.vs[t][1] = s.y; x.vs[t][2] = s.z; x.vs[t][3] = s.w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_bytes<X::VB>(vr + i * RB, x.v[t][i]);
+      for (int i = 0; i < 4; ++i) {
+        const uint2 v = *reinterpret_cast<const uint2*>(vr + i * D);
+        x.v[t][i][0] = v.x; x.v[t][i][1] = v.y;
+      }
+    } else {
+      const uint2 s = *reinterpret_cast<const uint2*>(vs);
+      x.vs[t][0] = s.x; x.vs[t][1] = s.y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.v[t][i][0] = *reinterpret_cast<const uint32_t*>(vr + i * D);
+    }
   }
 }
 
-// What the decode kernel takes off a scale of V, in powers of two
-constexpr uint32_t kLess = 32;
-
-template <int DT, int D, int BITS>
+template <int DT, int D>
 __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
   constexpr int NC = D / 64, NB = D / 16, NW = 4;
   const lbfq_paged_params& p = a.p;
@@ -324,8 +107,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
     fill_rest<D>(p, blockIdx.x - a.main, gridDim.x - a.main);
     return;
   }
-  __shared__ __align__(16) float acc_s[NW][16][D + 4];
-  __shared__ float m_s[NW][16], l_s[NW][16];
+  __shared__ DecodeLds<D> join;
   // 32-bit indices: the divisions of 64-bit ones were most of this kernel's code and a fifth of a small call's time
   // The parts come last: those behind a short sequence's end then leave the XCDs (workgroups go to them in turn) and their
   // shader engines evenly loaded.
@@ -379,8 +161,8 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
     load_pages(p, table, 32 * (begin + wave), pages);
     for (int kt = begin + wave; kt < end; kt += NW) {
       const int kb = 32 * kt;
-      Tile<D, BITS> x;
-      load_tile<D, BITS>(p, pages, kvh, kb, n, g, x);
+      Tile<D> x;
+      load_tile<D>(p, pages, kvh, kb, n, g, x);
       load_pages(p, table, 32 * (kt + NW), pages);
       // S^T: lane (n, g) has query n, keys 16 t + 4 g + i
       float sc[2][4];
@@ -390,11 +172,9 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const float e = __uint_as_float(((x.ks[t] >> (16 * c + 8 * (g >> 1))) & 0xffu) << 23);
-          const uint32_t* w = x.k[t][c];
-          const uint4 k0 = make_uint4(cvt_bf16<BITS>(w, 0, e), cvt_bf16<BITS>(w, 1, e), cvt_bf16<BITS>(w, 2, e),
-                                      cvt_bf16<BITS>(w, 3, e));
-          const uint4 k1 = make_uint4(cvt_bf16<BITS>(w, 4, e), cvt_bf16<BITS>(w, 5, e), cvt_bf16<BITS>(w, 6, e),
-                                      cvt_bf16<BITS>(w, 7, e));
+          const uint32_t kw[4] = {x.k[t][c].x, x.k[t][c].y, x.k[t][c].z, x.k[t][c].w};
+          const uint4 k0 = make_uint4(cvt_bf16<8>(kw, 0, e), cvt_bf16<8>(kw, 1, e), cvt_bf16<8>(kw, 2, e), cvt_bf16<8>(kw, 3, e));
+          const uint4 k1 = make_uint4(cvt_bf16<8>(kw, 4, e), cvt_bf16<8>(kw, 5, e), cvt_bf16<8>(kw, 6, e), cvt_bf16<8>(kw, 7, e));
           d = mfma16_bf16(k0, q[c][0], d);
           d = mfma16_bf16(k1, q[c][1], d);
           if constexpr (DT == kF16) {
@@ -415,7 +195,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
             // nothing that lies in the place of a key that no row sees may reach the product
             if (!x.ok[t] || key < lo || key >= hi) {
 #pragma unroll
-              for (int c = 0; c < Tile<D, BITS>::VW; ++c) x.v[t][i][c] = 0;
+              for (int c = 0; c < NC; ++c) x.v[t][i][c] = 0;
               // (four scale bytes of the row at D = 128, two at D = 64)
               if constexpr (D == 128) x.vs[t][i] = 0x7f7f7f7fu;
               else x.vs[t][i / 2] = (x.vs[t][i / 2] & (i & 1 ? 0x0000ffffu : 0xffff0000u)) | (i & 1 ? 0x7f7f0000u : 0x7f7fu);
@@ -461,7 +241,10 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
           // times 2^-kLess: a sum of 2^30 of the largest values is then in fp32's range
           const float e = __uint_as_float(__builtin_elementwise_sub_sat(by & 0xffu, kLess) << 23);
 #pragma unroll
-          for (int c = 0; c < NB / 2; ++c) vv[4 * t + i][c] = cvt_bf16<BITS>(x.v[t][i], c, e);
+          for (int c = 0; c < NC; ++c) {
+            vv[4 * t + i][2 * c] = cvt_bf16<8>(x.v[t][i], 2 * c, e);
+            vv[4 * t + i][2 * c + 1] = cvt_bf16<8>(x.v[t][i], 2 * c + 1, e);
+          }
         }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -474,68 +257,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
         acc[nb] = mfma16_bf16(va, pc, acc[nb]);
       }
     }
-    // join the waves
-    l = add_x32(add_x16(l));
-    if (g == 0) {
-      m_s[wave][n] = m;
-      l_s[wave][n] = l;
-    }
-    __syncthreads();
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) M = vmax(M, m_s[w][n]);
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int nb = 0; nb < NB; nb += 4)
-        *reinterpret_cast<float4*>(&acc_s[wave][n][(4 * g + i) * NB + nb]) =
-            make_float4(acc[nb][i] * f, acc[nb + 1][i] * f, acc[nb + 2][i] * f, acc[nb + 3][i] * f);
-    __syncthreads();
-    {
-      const int row = threadIdx.x >> 4, part = threadIdx.x & 15;
-      float MM = -INFINITY, L = 0.0f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) MM = vmax(MM, m_s[w][row]);
-#pragma unroll
-      for (int w = 0; w < NW; ++w)
-        L += filled(l_s[w][row]) ? l_s[w][row] * __builtin_amdgcn_exp2f(m_s[w][row] - MM) : 0.0f;
-      if (r0 + row < rows) {
-        float o[NB];
-#pragma unroll
-        for (int k = 0; k < NB; k += 4) {
-          float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-          for (int w = 0; w < NW; ++w) {
-            const float4 v = *reinterpret_cast<const float4*>(&acc_s[w][row][part * NB + k]);
-            t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
-          }
-          o[k] = t.x; o[k + 1] = t.y; o[k + 2] = t.z; o[k + 3] = t.w;
-        }
-        const int qq = (r0 + row) / G, hh = kvh * G + (r0 + row - qq * G);
-        const int64_t tok = s.start + qq;
-        const float inv = filled(L) ? static_cast<float>(uint64_t{1} << kLess) / L : 0.0f;
-        if (a.splits == 1) {
-          uint32_t w[NB / 2];
-#pragma unroll
-          for (int k = 0; k < NB / 2; ++k) w[k] = pack_dt<DT>(o[2 * k] * inv, o[2 * k + 1] * inv);
-          uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + hh * p.out_h +
-                                                      part * NB);
-          if constexpr (NB == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-          else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-          if (p.lse && part == 0) p.lse[tok * p.Hq + hh] = row_lse(MM, L);
-        } else {
-          const int64_t at = split * R + tok * p.Hq + hh;
-          if (part == 0) a.ml[at] = make_float2(MM, L);
-          if (filled(L)) {
-#pragma unroll
-            for (int k = 0; k < NB; k += 4)
-              *reinterpret_cast<float4*>(a.acc + at * D + part * NB + k) =
-                  make_float4(o[k] * inv, o[k + 1] * inv, o[k + 2] * inv, o[k + 3] * inv);
-          }
-        }
-      }
-    }
+    join_waves<DT, D>(a, s, acc, m, l, join, r0, rows, split, kvh);
     __syncthreads();  // the next rows use the same LDS
   }
 }
@@ -1218,8 +940,6 @@ struct Plan {
   int64_t slots, groups, piece;  // chunk: row tiles of a head (slot_of), the pieces that they come in, row tiles of a piece
 };
 
-constexpr int kDecodeRows = 16;
-
 // Bytes of a row in each part: its average and its maximum and sum.  Parts are not made beyond a workspace of kMostBytes (a
 // token buffer may be padded; those of calls that fill it take tens of MiB), one part needs none.  That also keeps the
 // rows of a call in parts under the 2^26 waves that may join them.
@@ -1232,6 +952,13 @@ constexpr int64_t kMostBytes = (int64_t{1} << 30) - 16;
 //
 // decode: the 768 workgroups that run at a time at D = 128 (24 sequences of 2000 to 4000 keys, 8 key heads, 384 / 768 /
 // 1536: 51 / 39 / 44 us; 3 of up to 40000, 384 / 768 / 1152: 57 / 41 / 46).
+// decode in 4 bits: a workgroup alone on its CU takes 4.9 ns a key (its waves' own chain of instructions), and from about 192
+// of them on they share the memory; joining parts costs 3.5 us.  So: as many parts of 300 keys or more as give 256
+// workgroups, one for fewer than 1100 keys; and, to even out several sequences, parts of 4000 keys from 12000 on (us for 1 / 2 /
+// 3 / 4 / 6 / 8 / 16 / 32 parts, * the rule's, 8 key heads of 128: one sequence of 700 keys 9.5* / 12.8 / 11.1 / 10.9 / 11.0 /
+// 10.8; 5003 31 / 21 / 18 / 15 / 14 / 13 / 11.8* / 12.1; 40000 197 / 105 / 74 / 58 / 42 / 34 / 22 / 18.8*; 24 of 2000 to 4000
+// 25.8* / 28.0 / 27.6 / 28.5 / 29.6; 48 of 8000 to 16000 152 / 134 / 127 / 121* / 124 / 127; 8 of 4000 to 8000, 40 heads 53.6*
+// / 59.6 / 56.0 / 55.7 / 57.1 / 61.7; 12 of 1000 to 16000, 12 heads 79 / 54 / 50 / 46* / 47 / 44 / 50).
 // chunk, one sequence: the parts that take the least time by a count of tiles.  A part costs the time of 12 tiles besides
 // its own (its start, and its sums written and read again), and an XCD has two or three workgroups a CU at a time.  Row
 // tiles that see much the same keys go in whole rounds (us for 1 / 2 / 4 / 6 / 7 parts, * the rule's: 1560 tokens, 32760
@@ -1257,12 +984,16 @@ Plan plan(const lbfq_paged_params* p) {
   x.piece = (x.slots + x.groups - 1) / x.groups;
   int64_t keys = p->table_cols << p->page_shift;  // that a row tile may see
   if (p->causal && p->window) keys = std::min(keys, p->window + std::min(most, kChunkRows / G + 1));
-  const int64_t least = x.decode ? 192 : 128;
+  const bool four = p->bits == 4;
+  const int64_t least = !x.decode ? 128 : four ? 256 : 192;
   // (a lane each in the combine kernel)
   const int64_t limit = std::min({keys / least, int64_t{64}, kMostBytes / part_bytes(p)});
   const int64_t places = 32 * chunk_groups(p->dtype, p->D);  // for workgroups on an XCD
   int64_t s = 1;
-  if (x.decode) {
+  if (x.decode && four) {
+    if (keys >= 1100) s = std::min(256 / (p->B * p->Hk), keys / 300);
+    if (p->B > 1 && keys >= 12000) s = std::max(s, keys / 4000);
+  } else if (x.decode) {
     const int64_t wgs = p->B * p->Hk;
     s = (768 + wgs / 2) / wgs;
   } else if (p->B == 1) {
@@ -1280,7 +1011,7 @@ Plan plan(const lbfq_paged_params* p) {
     while (120 * (s + 1) * (s + 1) * wgs <= places * keys && s < limit) ++s;
   }
   x.splits = static_cast<int>(std::max<int64_t>(std::min(s, limit), 1));
-  x.least = static_cast<int>(least / (x.decode ? 32 : 64));
+  x.least = static_cast<int>(least / (x.decode && !four ? 32 : 64));
   return x;
 }
 
@@ -1366,17 +1097,25 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   const dim3 grid(static_cast<unsigned>(a.main + fill));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool bf = p->dtype == kBF16, d128 = p->D == 128;
-#define LBFQ_PA(KERNEL, BB)                                                                              \
-  do {                                                                                                   \
-    if (bf && d128) hipLaunchKernelGGL((KERNEL<kBF16, 128, BB>), grid, dim3(256), 0, st, a);             \
-    else if (bf) hipLaunchKernelGGL((KERNEL<kBF16, 64, BB>), grid, dim3(256), 0, st, a);                 \
-    else if (d128) hipLaunchKernelGGL((KERNEL<kF16, 128, BB>), grid, dim3(256), 0, st, a);               \
-    else hipLaunchKernelGGL((KERNEL<kF16, 64, BB>), grid, dim3(256), 0, st, a);                          \
+#define LBFQ_PA(...)                                                                                       \
+  do {                                                                                                     \
+    if (bf && d128) hipLaunchKernelGGL((LBFQ_PK(kBF16, 128, __VA_ARGS__)), grid, dim3(256), 0, st, a);     \
+    else if (bf) hipLaunchKernelGGL((LBFQ_PK(kBF16, 64, __VA_ARGS__)), grid, dim3(256), 0, st, a);         \
+    else if (d128) hipLaunchKernelGGL((LBFQ_PK(kF16, 128, __VA_ARGS__)), grid, dim3(256), 0, st, a);       \
+    else hipLaunchKernelGGL((LBFQ_PK(kF16, 64, __VA_ARGS__)), grid, dim3(256), 0, st, a);                  \
   } while (0)
-  if (x.decode && p->bits == 4) LBFQ_PA(paged_decode_kernel, 4);
-  else if (x.decode) LBFQ_PA(paged_decode_kernel, 8);
-  else if (p->bits == 4) LBFQ_PA(paged_chunk_kernel, 4);
-  else LBFQ_PA(paged_chunk_kernel, 8);
+  if (x.decode && p->bits == 4) {
+    launch_decode4(a, grid.x, st);
+  } else if (x.decode) {
+#define LBFQ_PK(DT, DD, ...) paged_decode_kernel<DT, DD>
+    LBFQ_PA();
+#undef LBFQ_PK
+  } else {
+#define LBFQ_PK(DT, DD, BB) paged_chunk_kernel<DT, DD, BB>
+    if (p->bits == 4) LBFQ_PA(4);
+    else LBFQ_PA(8);
+#undef LBFQ_PK
+  }
 #undef LBFQ_PA
   LBFQ_LAUNCH_CHECK("lbfq_paged_attention");
   if (x.splits > 1) {

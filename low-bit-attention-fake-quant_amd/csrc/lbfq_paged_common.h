@@ -1,0 +1,327 @@
+// What the kernels of attention over the paged cache share: a sequence's extent and masks, conversions and products,
+// and the end of the two decode kernels.
+#pragma once
+
+#include <algorithm>
+#include <limits>
+#include <type_traits>
+
+#include "lbfq_common.h"
+#include "../../include/lbfq.h"
+
+namespace lbfq {
+namespace paged {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct Args {
+  lbfq_paged_params p;
+  int G;          // query heads of a key head
+  int splits;     // parts of the keys
+  int least;      // key tiles of a part, at least
+  int slots;      // chunk: places for row tiles, over all sequences
+  uint32_t piece;   // chunk: neighbouring slots that go to one XCD
+  uint32_t combos;  // decode: sequences x key heads; chunk: key heads x parts
+  int64_t main;   // workgroups that attend (the others fill)
+  float sml2;     // sm_scale * log2(e)
+  float2* ml;     // (splits, T * Hq): maximum (log2 units) and sum of a part
+  float* acc;     // (splits, T * Hq, D): a part's average of the values
+};
+
+// One sequence, clamped to what the tensors hold.
+struct Seq {
+  int n, len, start;
+  bool causal;
+  int window;
+  // keys [lo, hi) of query i
+  __device__ __forceinline__ int hi(int i) const {
+    if (!causal) return len;
+    const int h = len - n + i + 1;
+    return h < 0 ? 0 : h;  // i < n: never above len
+  }
+  __device__ __forceinline__ int lo(int i) const {
+    if (!window) return 0;
+    const int l = len - n + i + 1 - window;
+    return l < 0 ? 0 : l;
+  }
+};
+
+__device__ __forceinline__ Seq sequence(const lbfq_paged_params& p, int64_t b) {
+  Seq s;
+  const int T = static_cast<int>(p.T);
+  int s0 = p.query_starts[b], s1 = p.query_starts[b + 1];
+  s0 = s0 < 0 ? 0 : s0 > T ? T : s0;
+  s1 = s1 < s0 ? s0 : s1 > T ? T : s1;
+  s.start = s0;
+  s.n = s1 - s0;
+  const int cap = static_cast<int>(p.table_cols << p.page_shift);
+  const int len = p.seq_lens[b];
+  s.len = len < 0 ? 0 : len > cap ? cap : len;
+  s.causal = p.causal != 0;
+  s.window = static_cast<int>(p.window);
+  return s;
+}
+
+// The chunk kernel's row tiles have 128 rows.  Sequence b has the slots from slot_of(b) up to slot_of(b + 1), one more
+// than its rows need at the most: where a tile belongs follows from query_starts alone, and hardly a workgroup comes
+// for nothing.
+constexpr int kChunkRows = 128;
+__device__ __forceinline__ int slot_of(const lbfq_paged_params& p, int G, int b) {
+  const int T = static_cast<int>(p.T), s0 = p.query_starts[b];
+  return (s0 < 0 ? 0 : s0 > T ? T : s0) * G / kChunkRows + b;
+}
+// The last sequence whose slots start at or before `slot`: 64 places looked at at a time.
+__device__ __forceinline__ int sequence_at(const lbfq_paged_params& p, int G, int slot) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  for (int n = static_cast<int>(p.B); n > 1;) {
+    const int step = (n + 63) / 64, i = lane * step;
+    const uint64_t before = __ballot(i < n && slot_of(p, G, lo + (i < n ? i : 0)) <= slot);
+    const int k = before ? 63 - __builtin_clzll(before) : 0;
+    lo += k * step;
+    n = step < n - k * step ? step : n - k * step;
+  }
+  return lo;
+}
+
+// Rows of the token dimension that no sequence has: zero (a new output), lse -inf.
+template <int D>
+__device__ void fill_rest(const lbfq_paged_params& p, int64_t wg, int64_t wgs) {
+  int s0 = p.query_starts[0], s1 = p.query_starts[p.B];
+  const int T = static_cast<int>(p.T);
+  s0 = s0 < 0 ? 0 : s0 > T ? T : s0;
+  s1 = s1 < s0 ? s0 : s1 > T ? T : s1;
+  const int rest = T - (s1 - s0);
+  for (int64_t k = wg; k < rest; k += wgs) {
+    const int64_t t = k < s0 ? k : k - s0 + s1;
+    for (int i = threadIdx.x; p.fill_rest && i < p.Hq * (D / 8); i += blockDim.x) {
+      const int h = i / (D / 8), d = i % (D / 8);
+      reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + t * p.out_t + h * p.out_h)[d] = make_uint4(0, 0, 0, 0);
+    }
+    if (p.lse)
+      for (int h = threadIdx.x; h < p.Hq; h += blockDim.x) p.lse[t * p.Hq + h] = -INFINITY;
+  }
+}
+
+// The larger, NaN if either is: v_maximum3_f32, three operands an instruction, where fmaxf would first quiet each
+// MFMA result with an instruction of its own
+__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// v of the lanes 16 and 32 away (v_permlane16_swap / v_permlane32_swap of v with
+// itself leave it and the partner's value in the two results)
+__device__ __forceinline__ float max_x32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_x32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float max_x16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_x16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack_dt(float a, float b) {
+  if constexpr (DT == kBF16) return pack_bf16(a, b);
+  else return pack_f16(a, b);
+}
+
+// Eight fp16 values as two bf16 terms each: eight bits and the other three, exact
+__device__ __forceinline__ void split_f16(const uint4& x, uint4& hi, uint4& lo) {
+  const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+  uint32_t h[4], r[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float a = f16_bits_to_f32(static_cast<uint16_t>(in[e])), b = f16_bits_to_f32(static_cast<uint16_t>(in[e] >> 16));
+    h[e] = pack_bf16(a, b);
+    r[e] = pack_bf16(a - __uint_as_float(h[e] << 16), b - __uint_as_float(h[e] & 0xffff0000u));
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// The pair I of the codes from w on (two in 16 bits, or in 8) times 2^e as 16-bit values; sc: 2^e as fp32.
+template <int BITS>
+__device__ __forceinline__ uint32_t cvt_bf16(const uint32_t* w, int i, float sc) {
+  if constexpr (BITS == 8) {
+    return __builtin_bit_cast(uint32_t, i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i >> 1], sc, true)
+                                              : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i >> 1], sc, false));
+  } else {
+    const uint32_t x = w[i >> 2];
+    switch (i & 3) {  // (known once the loops are unrolled)
+      case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 0));
+      case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 1));
+      case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 2));
+      default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sc, 3));
+    }
+  }
+}
+template <int BITS>
+__device__ __forceinline__ uint32_t cvt_f16(const uint32_t* w, int i, float sc) {
+  if constexpr (BITS == 8) {
+    return __builtin_bit_cast(uint32_t, i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i >> 1], sc, true)
+                                              : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i >> 1], sc, false));
+  } else {
+    const uint32_t x = w[i >> 2];
+    switch (i & 3) {
+      case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 0));
+      case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 1));
+      case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 2));
+      default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sc, 3));
+    }
+  }
+}
+
+// N bytes from p on, in words
+template <int N>
+__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 16) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (N == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else if constexpr (N == 4) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  }
+}
+
+__device__ __forceinline__ v4f mfma16_bf16(const uint4& a, const uint4& b, const v4f& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                  0);
+}
+__device__ __forceinline__ v16f mfma32_bf16(const uint4& a, const uint4& b, const v16f& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                  0);
+}
+__device__ __forceinline__ v16f mfma32_f16(const uint4& a, const uint4& b, const v16f& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Whether a row's sum has anything in it (a NaN has: a row whose query holds one comes out as NaN, not as empty)
+__device__ __forceinline__ bool filled(float l) { return l != 0.0f; }
+
+
+// lse of a row (natural logarithm) from what its sum is relative to, in log2 units, and the sum
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return filled(l) ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+}
+
+// What the decode kernels take off the scales of V, or of P, in powers of two: a sum of 2^30 of the largest values is then
+// in fp32's range
+constexpr uint32_t kLess = 32;
+
+constexpr int kDecodeRows = 16;
+
+template <int D>
+struct alignas(16) DecodeLds {
+  float acc[4][kDecodeRows][D + 4];
+  float m[4][kDecodeRows], l[4][kDecodeRows];
+};
+
+// The four waves' rows r0 .. of one part joined by their maxima: into the output, or the part's place of the workspace.
+// Lane (n, g): row n's maximum m, its own share l of the sum, and columns (D/16) (4 g + i) + nb of the average times the
+// sum and 2^-kLess.
+template <int DT, int D>
+__device__ __forceinline__ void join_waves(const Args& a, const Seq& s, const v4f (&acc)[D / 16], float m, float l,
+                                           DecodeLds<D>& x, int r0, int rows, int split, int kvh) {
+  constexpr int NB = D / 16, NW = 4;
+  const lbfq_paged_params& p = a.p;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4, G = a.G;
+  const int64_t R = p.T * p.Hq;
+  l = add_x32(add_x16(l));
+  if (g == 0) {
+    x.m[wave][n] = m;
+    x.l[wave][n] = l;
+  }
+  __syncthreads();
+  float M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) M = vmax(M, x.m[w][n]);
+  const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int nb = 0; nb < NB; nb += 4)
+      *reinterpret_cast<float4*>(&x.acc[wave][n][(4 * g + i) * NB + nb]) =
+          make_float4(acc[nb][i] * f, acc[nb + 1][i] * f, acc[nb + 2][i] * f, acc[nb + 3][i] * f);
+  __syncthreads();
+  {
+    const int row = threadIdx.x >> 4, part = threadIdx.x & 15;
+    float MM = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) MM = vmax(MM, x.m[w][row]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+      L += filled(x.l[w][row]) ? x.l[w][row] * __builtin_amdgcn_exp2f(x.m[w][row] - MM) : 0.0f;
+    if (r0 + row < rows) {
+      float o[NB];
+#pragma unroll
+      for (int k = 0; k < NB; k += 4) {
+        float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(&x.acc[w][row][part * NB + k]);
+          t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+        }
+        o[k] = t.x; o[k + 1] = t.y; o[k + 2] = t.z; o[k + 3] = t.w;
+      }
+      const int qq = (r0 + row) / G, hh = kvh * G + (r0 + row - qq * G);
+      const int64_t tok = s.start + qq;
+      const float inv = filled(L) ? static_cast<float>(uint64_t{1} << kLess) / L : 0.0f;
+      if (a.splits == 1) {
+        uint32_t w[NB / 2];
+#pragma unroll
+        for (int k = 0; k < NB / 2; ++k) w[k] = pack_dt<DT>(o[2 * k] * inv, o[2 * k + 1] * inv);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + hh * p.out_h +
+                                                    part * NB);
+        if constexpr (NB == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+        if (p.lse && part == 0) p.lse[tok * p.Hq + hh] = row_lse(MM, L);
+      } else {
+        const int64_t at = split * R + tok * p.Hq + hh;
+        if (part == 0) a.ml[at] = make_float2(MM, L);
+        if (filled(L)) {
+#pragma unroll
+          for (int k = 0; k < NB; k += 4)
+            *reinterpret_cast<float4*>(a.acc + at * D + part * NB + k) =
+                make_float4(o[k] * inv, o[k + 1] * inv, o[k + 2] * inv, o[k + 3] * inv);
+        }
+      }
+    }
+  }
+}
+
+// The decode kernel of the cache in 4 bits (lbfq_paged4.hip)
+void launch_decode4(const Args& a, unsigned grid, hipStream_t stream);
+
+}  // namespace paged
+}  // namespace lbfq

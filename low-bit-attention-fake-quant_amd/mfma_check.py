@@ -13,6 +13,10 @@
    reads the compiler's assembly output (``-save-temps``), where inline asm is
    bracketed by ``;;#ASMSTART`` / ``;;#ASMEND``.
 
+4. No conversion of 32 values (``v_cvt_scalef32_pk32_*``, ``_2xpk16_*``) may have
+   its result overlap an operand: it is written before all of those are read,
+   and the compiler's builtins allow it.
+
 When the accumulator input of a scaled MFMA is the constant 0, the compiler
 does not tie the destination to it and can allocate the destination over a
 scale register that dies at the instruction; the MFMA then reads a scale that
@@ -72,6 +76,26 @@ def scale_dst_overlaps(asm: str) -> list:
             if m and lo <= int(m.group(1)) <= hi:
                 bad.append(t.split("//")[0].strip())
                 break
+    return bad
+
+
+def _range(operand: str) -> range:
+    m = _VEC.match(operand)
+    if m:
+        return range(int(m.group(1)), int(m.group(2)) + 1)
+    m = _REG.match(operand)
+    return range(int(m.group(1)), int(m.group(1)) + 1) if m else range(0)
+
+
+def wide_conversion_overlaps(asm: str) -> list:
+    """Conversions of 32 values whose result shares a register with an operand."""
+    bad = []
+    for t in _instructions(asm):
+        if re.match(r"v_cvt_scalef32_(sr_)?(pk32|2xpk16)_", t):
+            ops = [o.strip().split()[0] for o in t.split(None, 1)[1].split(",")]
+            dst = _range(ops[0])
+            if any(r in dst for o in ops[1:] for r in _range(o)):
+                bad.append(t)
     return bad
 
 
@@ -174,7 +198,7 @@ def check_assembly(s_path: str) -> list:
 
 def check_object(obj: str) -> list:
     asm = disassemble(obj)
-    return scale_dst_overlaps(asm) + m0_lds_dma_hazards(asm)
+    return scale_dst_overlaps(asm) + m0_lds_dma_hazards(asm) + wide_conversion_overlaps(asm)
 
 
 def scratch_kernels(s_text: str, name_part: str = "attn_fwd_kernel") -> list:
