@@ -53,6 +53,7 @@ UNITS = {
     "lbfq_kvcache.hip": ["-ffp-contract=off"],
     "lbfq_paged.hip": ["-ffp-contract=off"],
     "lbfq_paged4.hip": ["-ffp-contract=off"],
+    "lbfq_paged4_chunk.hip": ["-ffp-contract=off"],
 }
 
 

@@ -272,51 +272,11 @@ struct Lds {
   static constexpr int BUF = KBYTES + D * VP;
 };
 
-// Key of K row i of a 32-key block (bits 2 and 3 of i exchanged): a lane's scores are
-// then of consecutive keys, eight at a time.
-__device__ __forceinline__ int key_of(int i) { return (i & 0x13) | ((i & 4) << 1) | ((i & 8) >> 1); }
-
-// Largest (low half) and 255 - smallest (high half) of the scale bytes so far and of word v.
-__device__ __forceinline__ uint32_t span_join(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
-}
-template <int N>  // N bytes of v
-__device__ __forceinline__ uint32_t span_add(uint32_t span, uint32_t v) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const uint32_t b = (v >> (8 * i)) & 0xffu;
-    span = span_join(span, b | ((255u - b) << 16));
-  }
-  return span;
-}
-
-// What the values of a part's K or V are multiplied by, 2^(134 - E), on their way to fp16, so that the largest
-// code lands at 57344.  The smallest one, 2^-9, with a scale 2^-22 of the largest is then fp16's smallest step: within
-// that span every value is exact.  A part whose scales are further apart is `wide`: bf16, as they are.
-//
-// (A wide part's V is taken down by a power of two where its largest scale is past kWideTop: weights of up to 2^15 times
-// 2^30 of the largest values that are left, under 2^(kWideTop - 118), add up to less than 2^127.)
-//
-// E2M1's largest code, 6, lands at 49152 with 2^(140 - E), and its smallest, 1/2, stays exact 36 powers of two below.
-constexpr int span_of(int bits) { return bits == 8 ? 22 : 36; }
-constexpr int unit_of(int bits) { return bits == 8 ? 134 : 140; }
-constexpr int kWideTop = 200;
-struct Unit {
-  int E;
-  bool wide;
-};
-
-// Workgroups of a CU: three where the registers do for that, at the price of a few that go to memory (1560 tokens over 32760
-// keys, 40 heads of 64, bf16: 818 us with two, 765 with three; fp16 queries need more of them: 745 with two, 1075).
-constexpr int chunk_groups(int dt, int64_t d) { return d == 64 && dt == kBF16 ? 3 : 2; }
-
-template <int DT, int D, int BITS>
+template <int DT, int D>
 __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(const Args a) {
   constexpr int NW = 4, QB = kChunkRows, NT = 64 * NW;
   static_assert(QB == 32 * NW, "32 rows a wave");
   constexpr int NKS = D / 16, NDB = D / 32, CH = D / 32;
-  constexpr int RB = D * BITS / 8;  // bytes of a row
-  constexpr int kUnit = unit_of(BITS);
   constexpr int KC = 64 * D / NT;  // K codes of a thread
   constexpr int KT = D / KC;       // threads of a key's row
   constexpr int VK = KC / 4;       // V keys of a thread, four columns each
@@ -353,8 +313,8 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
   const int kkey = lane / KT, kq = lane % KT;           // K: key kkey of the wave's, columns KC kq ..
   const int vkg = lane / (D / 4), vdq = lane % (D / 4);  // V: keys VK vkg .. of the wave's, columns 4 vdq ..
   static_assert(64 / KT == WKEYS && 64 / (D / 4) * VK == WKEYS, "a wave's keys");
-  const uint32_t koff = kkey * RB + KC * BITS / 8 * kq, ksoff = kkey * CH + KC * kq / 32;
-  const uint32_t voff = VK * vkg * RB + BITS / 2 * vdq, vsoff = VK * vkg * CH;
+  const uint32_t koff = kkey * D + KC * kq, ksoff = kkey * CH + KC * kq / 32;
+  const uint32_t voff = VK * vkg * D + 4 * vdq, vsoff = VK * vkg * CH;
 
   auto row_of = [&](int page, int key) -> int64_t {
     return (static_cast<int64_t>(page * Hk + kvh) << shift) + (key & pmask);
@@ -382,7 +342,7 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[db][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;
-  Unit uv{kUnit, false}, uk{kUnit, false};
+  Unit uv{134, false}, uk{134, false};
   if (begin < end) {
     uint4 q[NKS];
     {
@@ -392,24 +352,26 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
     }
     // Staging registers: codes and scales of a K tile and of a V tile.
     struct KRegs {
-      uint32_t c[KC * BITS / 32], e;
+      uint32_t c[KC / 4], e;
     } kx, ky;
     uint32_t vc[VK], vse[VK * CH / 4];
     auto load_k = [&](KRegs& x, int kt, int page) {
       const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
-      const uint8_t* ks = p.k_codes + row * RB;
+      const uint8_t* ks = p.k_codes + row * D;
       const uint8_t* kss = p.k_scale + row * CH;
-      constexpr int N = KC * BITS / 8 < 16 ? KC * BITS / 8 : 16;
 #pragma unroll
-      for (int i = 0; i < KC * BITS / 8 / N; ++i) load_bytes<N>(ks + koff + N * i, x.c + N / 4 * i);
+      for (int i = 0; i < KC / 16; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4*>(ks + koff + 16 * i);
+        x.c[4 * i] = w.x; x.c[4 * i + 1] = w.y; x.c[4 * i + 2] = w.z; x.c[4 * i + 3] = w.w;
+      }
       x.e = kss[ksoff];
     };
     auto load_v = [&](int kt, int page) {
       const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
-      const uint8_t* vs = p.v_codes + row * RB;
+      const uint8_t* vs = p.v_codes + row * D;
       const uint8_t* vss = p.v_scale + row * CH;
 #pragma unroll
-      for (int j = 0; j < VK; ++j) load_bytes<BITS / 2>(vs + voff + j * RB, vc + j);
+      for (int j = 0; j < VK; ++j) vc[j] = *reinterpret_cast<const uint32_t*>(vs + voff + j * D);
       if constexpr (D == 128) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -493,16 +455,16 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
         x = __builtin_amdgcn_readfirstlane(x);
         Unit u;
         u.E = static_cast<int>(x & 0xffu);
-        u.wide = u.E - (255 - static_cast<int>(x >> 16)) > span_of(BITS);
-        if (u.wide) u.E = u.E > wide ? kUnit + u.E - wide : kUnit;
-        if (x == 0) u.E = kUnit;
+        u.wide = u.E - (255 - static_cast<int>(x >> 16)) > span_of(8);
+        if (u.wide) u.E = u.E > wide ? 134 + u.E - wide : 134;
+        if (x == 0) u.E = 134;
         return u;
       };
       uv = unit(sv, kWideTop);
       if constexpr (DT == kF16) uk = unit(sk, 255);
     }
-    const float c = DT == kF16 ? ldexpf(a.sml2, uk.E - kUnit) : a.sml2;
-    const uint32_t kadd = static_cast<uint32_t>(kUnit - uk.E) << 23, vadd = static_cast<uint32_t>(kUnit - uv.E) << 23;
+    const float c = DT == kF16 ? ldexpf(a.sml2, uk.E - 134) : a.sml2;
+    const uint32_t kadd = static_cast<uint32_t>(134 - uk.E) << 23, vadd = static_cast<uint32_t>(134 - uv.E) << 23;
 
     // Keys that no row sees, or that are not there: nothing of them may reach a product.
     auto clear_k = [&](KRegs& x, int kt, int page) {
@@ -510,7 +472,7 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
       if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
       if (page < 0 || key0 + kkey < lo || key0 + kkey >= hi) {
 #pragma unroll
-        for (int i = 0; i < KC * BITS / 32; ++i) x.c[i] = 0;
+        for (int i = 0; i < KC / 4; ++i) x.c[i] = 0;
         x.e = static_cast<uint32_t>(uk.E);
       }
     };
@@ -534,8 +496,8 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
       if (k >= KC / 4) return;  // (D = 64 has four)
       constexpr bool f16 = DT == kF16 && !WIDE;
       const float sc = __uint_as_float((x.e << 23) + (f16 ? kadd : 0u));
-      st.k[2 * k] = f16 ? cvt_f16<BITS>(x.c, 2 * k, sc) : cvt_bf16<BITS>(x.c, 2 * k, sc);
-      st.k[2 * k + 1] = f16 ? cvt_f16<BITS>(x.c, 2 * k + 1, sc) : cvt_bf16<BITS>(x.c, 2 * k + 1, sc);
+      st.k[2 * k] = f16 ? cvt_f16<8>(x.c + k, 0, sc) : cvt_bf16<8>(x.c + k, 0, sc);
+      st.k[2 * k + 1] = f16 ? cvt_f16<8>(x.c + k, 1, sc) : cvt_bf16<8>(x.c + k, 1, sc);
       if (k & 1)
         *reinterpret_cast<uint4*>(buf + (WKEYS * wave + kkey) * L::KP + 2 * KC * kq + 8 * (k - 1)) =
             make_uint4(st.k[2 * k - 2], st.k[2 * k - 1], st.k[2 * k], st.k[2 * k + 1]);
@@ -549,8 +511,8 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
           else by = __builtin_amdgcn_ubfe(vse[j / 2], 16 * (j & 1) + 8 * (vdq / 8), 8);
           // (WIDE: far below the largest, a scale may be less than what is taken off)
           const float sc = __uint_as_float(WIDE ? __builtin_elementwise_sub_sat(by << 23, 0u - vadd) : (by << 23) + vadd);
-          st.v[j][0] = WIDE ? cvt_bf16<BITS>(vc + j, 0, sc) : cvt_f16<BITS>(vc + j, 0, sc);
-          st.v[j][1] = WIDE ? cvt_bf16<BITS>(vc + j, 1, sc) : cvt_f16<BITS>(vc + j, 1, sc);
+          st.v[j][0] = WIDE ? cvt_bf16<8>(vc + j, 0, sc) : cvt_f16<8>(vc + j, 0, sc);
+          st.v[j][1] = WIDE ? cvt_bf16<8>(vc + j, 1, sc) : cvt_f16<8>(vc + j, 1, sc);
         }
       } else {
         // column 4 dq + c is V^T row c D/4 + dq, so that neighbouring lanes write neighbouring rows
@@ -799,7 +761,7 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
   if (rw + li < rows) {
     const int64_t tok = s.start + qi;
     const bool one = a.splits == 1;
-    const float f = filled(l) ? ldexpf(1.0f, uv.E - kUnit) / l : 0.0f;
+    const float f = filled(l) ? ldexpf(1.0f, uv.E - 134) / l : 0.0f;
     const int64_t at = split * R + tok * p.Hq + h;
     if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
     if (!one && g == 0) a.ml[at] = make_float2(m, l);
@@ -988,7 +950,7 @@ Plan plan(const lbfq_paged_params* p) {
   const int64_t least = !x.decode ? 128 : four ? 256 : 192;
   // (a lane each in the combine kernel)
   const int64_t limit = std::min({keys / least, int64_t{64}, kMostBytes / part_bytes(p)});
-  const int64_t places = 32 * chunk_groups(p->dtype, p->D);  // for workgroups on an XCD
+  const int64_t places = 32 * (four ? chunk4_groups(p->D) : chunk_groups(p->dtype, p->D));  // for workgroups on an XCD
   int64_t s = 1;
   if (x.decode && four) {
     if (keys >= 1100) s = std::min(256 / (p->B * p->Hk), keys / 300);
@@ -1097,24 +1059,20 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   const dim3 grid(static_cast<unsigned>(a.main + fill));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool bf = p->dtype == kBF16, d128 = p->D == 128;
-#define LBFQ_PA(...)                                                                                       \
-  do {                                                                                                     \
-    if (bf && d128) hipLaunchKernelGGL((LBFQ_PK(kBF16, 128, __VA_ARGS__)), grid, dim3(256), 0, st, a);     \
-    else if (bf) hipLaunchKernelGGL((LBFQ_PK(kBF16, 64, __VA_ARGS__)), grid, dim3(256), 0, st, a);         \
-    else if (d128) hipLaunchKernelGGL((LBFQ_PK(kF16, 128, __VA_ARGS__)), grid, dim3(256), 0, st, a);       \
-    else hipLaunchKernelGGL((LBFQ_PK(kF16, 64, __VA_ARGS__)), grid, dim3(256), 0, st, a);                  \
+#define LBFQ_PA(KERNEL)                                                                              \
+  do {                                                                                               \
+    if (bf && d128) hipLaunchKernelGGL((KERNEL<kBF16, 128>), grid, dim3(256), 0, st, a);             \
+    else if (bf) hipLaunchKernelGGL((KERNEL<kBF16, 64>), grid, dim3(256), 0, st, a);                 \
+    else if (d128) hipLaunchKernelGGL((KERNEL<kF16, 128>), grid, dim3(256), 0, st, a);               \
+    else hipLaunchKernelGGL((KERNEL<kF16, 64>), grid, dim3(256), 0, st, a);                          \
   } while (0)
-  if (x.decode && p->bits == 4) {
-    launch_decode4(a, grid.x, st);
+  if (p->bits == 4) {
+    if (x.decode) launch_decode4(a, grid.x, st);
+    else launch_chunk4(a, grid.x, st);
   } else if (x.decode) {
-#define LBFQ_PK(DT, DD, ...) paged_decode_kernel<DT, DD>
-    LBFQ_PA();
-#undef LBFQ_PK
+    LBFQ_PA(paged_decode_kernel);
   } else {
-#define LBFQ_PK(DT, DD, BB) paged_chunk_kernel<DT, DD, BB>
-    if (p->bits == 4) LBFQ_PA(4);
-    else LBFQ_PA(8);
-#undef LBFQ_PK
+    LBFQ_PA(paged_chunk_kernel);
   }
 #undef LBFQ_PA
   LBFQ_LAUNCH_CHECK("lbfq_paged_attention");

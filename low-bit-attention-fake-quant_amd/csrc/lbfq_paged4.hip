@@ -26,11 +26,6 @@ using namespace lbfq::paged;
 
 namespace {
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x32 __attribute__((ext_vector_type(32)));
-
 constexpr int kT = 4, kKeys = 16 * kT;  // a wave's tile: 64 keys, 16 at a time
 constexpr int kBufs = 2;                // tiles of a wave in LDS: one on its way, one behind it
 
@@ -45,39 +40,8 @@ struct Ring {
   Tile t[4][kBufs];
 };
 
-// Asynchronous copies into LDS: lane i's 16 (4) bytes go to lds + 16 (4) i.  In assembly, so that the compiler does not put
-// a wait for all of them before the next LDS read (wait_for does that); an LDS copy right behind a write of M0 needs one
-// wait state.  nt: nobody reads the cache a second time (48 sequences of 8000 to 16000 keys, 135 -> 124 us).
-__device__ __forceinline__ uint32_t lds_addr(const void* p) {
-  return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
-}
-__device__ __forceinline__ void copy_to(uint32_t lds) { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" ::"s"(lds) : "memory", "m0"); }
-template <int OFF>  // of both the source and the place in LDS
-__device__ __forceinline__ void copy16(const uint8_t* base, uint32_t at) {
-  asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2 nt" ::"v"(at), "s"(base), "i"(OFF) : "memory");
-}
-__device__ __forceinline__ void copy4(const uint8_t* base, uint32_t at) {
-  asm volatile("global_load_lds_dword %0, %1 nt" ::"v"(at), "s"(base) : "memory");
-}
-__device__ __forceinline__ void copy16v(const uint8_t* at) {
-  asm volatile("global_load_lds_dwordx4 %0, off nt" ::"v"(at) : "memory");
-}
-__device__ __forceinline__ void copy4v(const uint8_t* at) {
-  asm volatile("global_load_lds_dword %0, off nt" ::"v"(at) : "memory");
-}
-// Until no more than N copies are under way (they end in their order)
-template <int N>
-__device__ __forceinline__ void wait_for() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
-}
-
-// The 16-byte piece of row r (of 16) that lies at place c of its D / 32, and the place of piece c: so that both K's reads,
-// 16 lanes one piece of 16 rows each, and V's, 64 lanes four bytes of all pieces of four rows, are on distinct banks.
-template <int D>
-__device__ __forceinline__ int piece_of(int r, int c) {
-  return D == 128 ? c ^ (r >> 2 & 3) : c ^ (r >> 3 & 1);
-}
-// Key of a row of S^T within its 16: row 4 g + i is key 4 i + g, so that the four lanes groups' rows of V are neighbours.
+// Key of a row of S^T within its 16: row 4 g + i is key 4 i + g, so that the four lane groups' rows of V are neighbours, and
+// V's reads, 64 lanes four bytes of all pieces of four rows, on distinct banks, as K's are.
 __device__ __forceinline__ int key_of(int r) { return 4 * (r & 3) + (r >> 2); }
 
 // Pages of 16 and of 32 tokens: a tile lies in four or two; of 64 and more: in one.  A tile's piece is what it has of a page.
@@ -120,19 +84,19 @@ __device__ __forceinline__ uint32_t fetch(const lbfq_paged_params& p, const Page
     const int64_t row = row_of(pages.id[0]) + (kb & ((1 << shift) - 1));
     copy_to(lds + offsetof(X, k));
     const uint8_t* k = p.k_codes + row * RB;
-    copy16<0>(k, off);
-    copy16<1024>(k, off);
-    if constexpr (D == 128) copy16<2048>(k, off), copy16<3072>(k, off);
+    copy16<0, true>(k, off);
+    copy16<1024, true>(k, off);
+    if constexpr (D == 128) copy16<2048, true>(k, off), copy16<3072, true>(k, off);
     copy_to(lds + offsetof(X, v));
     const uint8_t* v = p.v_codes + row * RB;
-    copy16<0>(v, off);
-    copy16<1024>(v, off);
-    if constexpr (D == 128) copy16<2048>(v, off), copy16<3072>(v, off);
+    copy16<0, true>(v, off);
+    copy16<1024, true>(v, off);
+    if constexpr (D == 128) copy16<2048, true>(v, off), copy16<3072, true>(v, off);
     const uint32_t so = D == 128 ? 4 * lane : 4 * (lane & 31);  // (D = 64: lanes 32 .. write what nobody reads)
     copy_to(lds + offsetof(X, ks));
-    copy4(p.k_scale + row * SB, so);
+    copy4<true>(p.k_scale + row * SB, so);
     copy_to(lds + offsetof(X, vs));
-    copy4(p.v_scale + row * SB, so);
+    copy4<true>(p.v_scale + row * SB, so);
     return static_cast<uint32_t>(pages.id[0]) < num ? 15u : 0u;
   }
   if (shift == 5) {
@@ -140,12 +104,12 @@ __device__ __forceinline__ uint32_t fetch(const lbfq_paged_params& p, const Page
     auto codes = [&](const uint8_t* base, uint32_t to) {
       copy_to(lds + to);
       const uint8_t* c = base + r0 * RB;
-      copy16<0>(c, off);
-      if constexpr (D == 128) copy16<1024>(c, off);
+      copy16<0, true>(c, off);
+      if constexpr (D == 128) copy16<1024, true>(c, off);
       copy_to(lds + to + 32 * RB);
       c = base + r1 * RB;
-      copy16<0>(c, off);
-      if constexpr (D == 128) copy16<1024>(c, off);
+      copy16<0, true>(c, off);
+      if constexpr (D == 128) copy16<1024, true>(c, off);
     };
     codes(p.k_codes, offsetof(X, k));
     codes(p.v_codes, offsetof(X, v));
@@ -174,7 +138,7 @@ __device__ __forceinline__ uint32_t fetch(const lbfq_paged_params& p, const Page
 #pragma unroll
       for (int t = 0; t < kT; ++t) {
         copy_to(to + 1024 * t);
-        copy16<0>(base + row[t] * RB, off);
+        copy16<0, true>(base + row[t] * RB, off);
       }
     } else {  // a copy reaches over two pieces
 #pragma unroll
@@ -193,21 +157,8 @@ __device__ __forceinline__ uint32_t fetch(const lbfq_paged_params& p, const Page
   return there;
 }
 
-// 32 values over 2^e to E2M3, to nearest, and back; sc: 2^e.  In assembly for the &: the instructions write their results
-// before they have read all operands, and the builtins let the compiler lay the one over the other.
-__device__ __forceinline__ u32x6 to_e2m3(const f32x16& even, const f32x16& odd, float sc) {
-  u32x6 w;
-  asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3\n\ts_nop 4" : "=&v"(w) : "v"(even), "v"(odd), "v"(sc));
-  return w;
-}
-__device__ __forceinline__ f32x32 from_e2m3(const u32x6& w, float sc) {
-  f32x32 v;
-  asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2\n\ts_nop 4" : "=&v"(v) : "v"(w), "v"(sc));
-  return v;
-}
-
 // A query's columns in four E2M3 terms: D = 128 an operand each, D = 64 two terms to an operand (lanes g < 2 the first);
-// byte i of e: the E8M0 scale of operand i, 255 (not a number) where a column is infinite or NaN.
+// byte i of e: the E8M0 scale of operand i.
 template <int D>
 struct Query {
   static constexpr int N = D / 32;
@@ -216,51 +167,19 @@ struct Query {
 };
 
 template <int DT, int D>
-__device__ __forceinline__ Query<D> split_query(const uint16_t* q, int g) {
-  f32x16 even, odd;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint4 v = reinterpret_cast<const uint4*>(q)[i];
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      even[4 * i + k] = DT == kBF16 ? __uint_as_float(w[k] << 16) : f16_bits_to_f32(static_cast<uint16_t>(w[k]));
-      odd[4 * i + k] =
-          DT == kBF16 ? __uint_as_float(w[k] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(w[k] >> 16));
-    }
-  }
-  float m = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) m = vmax(vmax(m, fabsf(even[i])), fabsf(odd[i]));
-  const uint32_t top = __float_as_uint(m) >> 23;  // m is not negative, or a NaN of either sign
-  const bool bad = (top & 0xffu) == 255u;
-  // 2^(e - 127): the largest column is in 2 ... 4 of it, what a term leaves at most 4 of the next one's, E2M3 reaches 7.5
-  const uint32_t e = bad ? 100u : (top > 18u ? top : 18u) - 1u;
-  u32x6 w[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const float sc = __uint_as_float((e - 5u * t) << 23);
-    w[t] = to_e2m3(even, odd, sc);
-    if (t < 3) {
-      const f32x32 back = from_e2m3(w[t], sc);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        even[i] -= back[2 * i];
-        odd[i] -= back[2 * i + 1];
-      }
-    }
-  }
+__device__ __forceinline__ Query<D> query(const uint16_t* q, int g) {
+  const Terms s = split_query<DT>(q);
   Query<D> x;
   if constexpr (D == 128) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) x.w[t] = w[t];
-    x.e = bad ? 0xffffffffu : e * 0x01010101u - 0x0f0a0500u;
-  } else {
+    for (int t = 0; t < 4; ++t) x.w[t] = s.w[t];
+    x.e = s.e;
+  } else {  // (bytes 0 and 2, or 1 and 3)
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 6; ++i) x.w[t][i] = g < 2 ? w[2 * t][i] : w[2 * t + 1][i];
-    x.e = bad ? 0xffffu : (g < 2 ? e : e - 5u) * 0x0101u - 0x0a00u;
+      for (int i = 0; i < 6; ++i) x.w[t][i] = g < 2 ? s.w[2 * t][i] : s.w[2 * t + 1][i];
+    x.e = __builtin_amdgcn_perm(s.e, s.e, g < 2 ? 0x0c0c0200u : 0x0c0c0301u);
   }
   return x;
 }
@@ -326,7 +245,7 @@ __global__ void __launch_bounds__(256, 2) paged_decode4_kernel(const Args a) {
     if (begin + wave < end) {
       Pages pages;
       load_pages(p, table, kKeys * (begin + wave), pages);
-      const Query<D> q = split_query<DT, D>(  // (while the page ids are on their way)
+      const Query<D> q = query<DT, D>(  // (while the page ids are on their way)
           reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 32 * (D == 128 ? g : g & 1), g);
       const int lr = lane / (D / 32);  // this lane's row and place of it in a copy
       const uint32_t off = D / 2 * lr + 16 * piece_of<D>(lr & 15, lane & (D / 32 - 1));

@@ -1,0 +1,513 @@
+// Attention of chunks of new tokens over the paged cache in 4 bits (the mathematics, the masks, the row tiles and their
+// order are those of lbfq_paged.hip's chunk kernel, and so is the order of a step: the next tile's scores and this one's P V
+// beside the softmax and the conversion of V).
+//
+// What is different is K.  It stays as it lies in memory: tiles are copied to LDS asynchronously, three of them there, and
+// multiplied by the query's four E2M3 terms with the block-scaled product (32x32x64; see lbfq_paged4.hip): as many
+// cycles as bf16's, but a quarter of the LDS reads, and no conversion.  (At 16 bits, a step's reads take as long as its
+// products: 32 KiB for 16 + 16 of 32 cycles, four waves and two workgroups a CU.)  K's scales go into the product, so no
+// span of them needs bf16.
+//
+// 4680 tokens over 32760 keys, 12 heads of 128, all seen: 947 us, 1.0 PFLOP/s (the 8-bit kernel 1067 in the same run; a
+// large library product 1.24).  214 VALU instructions a step, 32 of them exponentials, issue beside 32 products of 32
+// cycles: the two take 93% of the cycles of a full CU together.  With all codes zero it takes 10 to 17% less: power.
+#include "lbfq_paged_common.h"
+
+using namespace lbfq;
+using namespace lbfq::paged;
+
+namespace {
+
+template <int D>
+struct Lds {
+  static constexpr int VP = 2 * 64 + 16;  // pitch of a V^T row
+  // A tile's K: 16 keys of each wave that copies them, rows of D / 2 bytes, pieces exchanged (piece_of), and their scales
+  // (what a copy of 64 lanes needs; D = 64 uses half of the codes' place, and the scales take 64 or 32 bytes)
+  uint8_t k[3][4][1024], ks[3][4][256];
+  uint8_t v[2][D * VP];
+};
+
+// K (E2M1; scale in byte A of ke) times term B of the query
+template <int A, int B>
+__device__ __forceinline__ v16f product(const uint4& k, uint32_t ke, const Terms& q, const v16f& c) {
+  const i32x8 x = {static_cast<int>(k.x), static_cast<int>(k.y), static_cast<int>(k.z), static_cast<int>(k.w), 0, 0, 0, 0};
+  const u32x6& w = q.w[B];
+  const i32x8 y = {static_cast<int>(w[0]), static_cast<int>(w[1]), static_cast<int>(w[2]), static_cast<int>(w[3]),
+                   static_cast<int>(w[4]), static_cast<int>(w[5]), 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 2, A, static_cast<int>(ke), B, static_cast<int>(q.e));
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(const Args a) {
+  constexpr int NW = 4, QB = kChunkRows, NT = 64 * NW;
+  static_assert(QB == 32 * NW, "32 rows a wave");
+  constexpr int NC = D / 64, NKS = 4 * NC, NDB = D / 32, CH = D / 32, RB = D / 2;
+  constexpr int VK = D / 32;      // V keys of a thread, eight columns each
+  constexpr int WKEYS = 64 / NW;  // keys that a wave stages: of one page
+  constexpr int kUnit = unit_of(4);
+  using L = Lds<D>;
+  const lbfq_paged_params& p = a.p;
+  if (static_cast<int64_t>(blockIdx.x) >= a.main) {
+    fill_rest<D>(p, blockIdx.x - a.main, gridDim.x - a.main);
+    return;
+  }
+  __shared__ __align__(16) L lds;
+  // Workgroups go to the eight XCDs in turn.  Pieces of up to eight neighbouring row tiles are dealt to them whole, so that
+  // those that read the same keys share an L2; the pieces of all heads and parts (`combos`) with the last rows first,
+  // which take longest under a causal mask, and turned by one XCD from round to round, so that none has all of a kind.
+  // (No slots in vain: where seven of eight workgroups had nothing to do, the others shared a quarter of the chip: an
+  // XCD's four shader engines take its workgroups in turn.  1024 keys, 512 heads of 128 rows: 203 us, dense 60.)
+  const uint32_t ps = a.piece, round = blockIdx.x / (8 * ps), piece = round * 8 + (blockIdx.x + round) % 8;
+  const int slot = a.slots - 1 - static_cast<int>(piece / a.combos * ps + blockIdx.x / 8 % ps);
+  if (slot < 0) return;
+  const uint32_t rest = piece % a.combos, splits = static_cast<uint32_t>(a.splits);
+  const int split = static_cast<int>(rest % splits), kvh = static_cast<int>(rest / splits);
+  const int G = a.G, Hk = static_cast<int>(p.Hk);
+  const int b = sequence_at(p, G, slot), r0 = (slot - slot_of(p, G, b)) * QB;
+  const Seq s = sequence(p, b);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int li = lane & 31, g = lane >> 5;
+  const int32_t* table = p.block_table + b * p.table_stride;
+  const int cols = static_cast<int>(p.table_cols), num_pages = static_cast<int>(p.num_pages);
+  const int shift = p.page_shift, pmask = (1 << p.page_shift) - 1;
+  const int64_t R = p.T * p.Hq;
+  const int rows = s.n * G;  // below 2^30: the host checks T * Hq
+  if (r0 < 0 || r0 >= rows) return;
+  // Staging: wave w takes keys WKEYS w .. of a tile, which lie in one page.
+  const int vkg = lane / (D / 8), vdq = lane % (D / 8);  // V: keys VK vkg .. of the wave's, columns 8 vdq ..
+  static_assert(64 / (D / 8) * VK == WKEYS, "a wave's keys");
+  const uint32_t voff = VK * vkg * RB + 4 * vdq, vsoff = VK * vkg * CH;
+  const int lr = lane / CH & 15;  // K: row and piece of this lane's 16 bytes (D = 64: lanes 32 .. copy them again)
+  const uint32_t koff = RB * lr + 16 * piece_of<D>(lr, lane % CH), ksoff = 4 * (lane & (4 * CH - 1));
+
+  auto row_of = [&](int page, int key) -> int64_t {
+    return (static_cast<int64_t>(page * Hk + kvh) << shift) + (key & pmask);
+  };
+
+  const int rw = r0 + wave * 32;
+  const int rr = rw + li < rows ? rw + li : rows - 1;
+  const int qi = rr / G, h = kvh * G + (rr - qi * G);
+  const int lo_r = s.lo(qi), hi_r = s.hi(qi);
+  const int first = r0 / G, last = ((r0 + QB < rows ? r0 + QB : rows) - 1) / G;
+  const int lo = s.lo(first), hi = s.hi(last);  // keys that some row of the workgroup sees
+  const int wf = __builtin_amdgcn_readfirstlane((rw < rows ? rw : rows - 1) / G);
+  const int wl = __builtin_amdgcn_readfirstlane((rw + 31 < rows ? rw + 31 : rows - 1) / G);
+  const int lo_all = s.lo(wl), hi_all = s.hi(wf);            // that every row of the wave sees
+
+  const int kt0 = lo / 64, nt = hi > lo ? (hi + 63) / 64 - kt0 : 0;
+  int per = (nt + a.splits - 1) / a.splits;
+  per = per > a.least ? per : a.least;
+  const int begin = kt0 + split * per;
+  const int end = begin + per < kt0 + nt ? begin + per : kt0 + nt;
+
+  v16f acc[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[db][r] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  Unit uv{kUnit, false};
+  if (begin < end) {
+    auto upto = [&](int kt) { return kt < end ? kt : end - 1; };  // steps past the end repeat it, unused
+    // Page ids of the tiles from kt on: lane 4 i + w has that of tile kt + i's keys 16 w .., which wave w stages.  One load,
+    // so one wait; looked up where they are needed, each id cost the time of a trip to memory (4680 tokens over 32760 keys,
+    // 12 heads: 1.16 ms, so 1.10).
+    auto group_of = [&](int kt) { return (64 * upto(kt + (lane >> 2 & 3)) + 16 * (lane & 3)) >> shift; };
+    auto look = [&](int kt) {
+      const int idx = group_of(kt);
+      return table[idx < cols ? idx : cols - 1];
+    };
+    auto there = [&](int kt, int id) -> uint32_t {  // a bit per lane: the page is there
+      return static_cast<uint32_t>(__ballot(group_of(kt) < cols && id >= 0 && id < num_pages));
+    };
+    auto page_in = [&](int id, uint32_t mask, int i) {  // of tile kt + i's keys of this wave, or -1; a scalar
+      return mask >> (4 * i + wave) & 1u ? __builtin_amdgcn_readlane(id, 4 * i + wave) : -1;
+    };
+    // A tile's K into LDS (place b of three), its V into registers: of a page that is not there, page 0's
+    auto copy_k = [&](int kt, int page, int b) {
+      const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
+      // (the same in every lane, which the compiler does not always see)
+      const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(row >> 32));
+      const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(row));
+      const int64_t at = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+      copy_to(lds_addr(lds.k[b][wave]));
+      copy16<0, false>(p.k_codes + at * RB, koff);
+      copy_to(lds_addr(lds.ks[b][wave]));
+      copy4<false>(p.k_scale + at * CH, ksoff);
+    };
+    uint32_t vc[VK], vse[VK * CH / 4];
+    auto load_v = [&](int kt, int page) {
+      const int64_t row = row_of(page < 0 ? 0 : page, 64 * kt + WKEYS * wave);
+      const uint8_t* vs = p.v_codes + row * RB;
+#pragma unroll
+      for (int j = 0; j < VK; ++j) load_bytes<4>(vs + voff + j * RB, vc + j);
+      load_bytes<VK * CH>(p.v_scale + row * CH + vsoff, vse);
+    };
+    const int ids = look(begin);
+    const uint32_t mask = there(begin, ids);
+    const int page0 = page_in(ids, mask, 0), page1 = page_in(ids, mask, 1);
+    int pv = page1, pk = page_in(ids, mask, 3);
+    copy_k(begin, page0, 0);
+    copy_k(upto(begin + 1), page1, 1);
+    copy_k(upto(begin + 2), page_in(ids, mask, 2), 2);
+    load_v(begin, page0);
+    Terms q[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      q[i] = split_query<DT>(reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 64 * i + 32 * g);
+    // The span of the part's V scales, over the keys that some row sees: four keys a thread and pass.
+    {
+      uint32_t sv = 0;
+      const int k1 = 64 * end < hi ? 64 * end : hi;
+      for (int key = 64 * begin + 4 * tid; key < k1; key += 4 * NT) {
+        if (key + 4 <= lo) continue;
+        const int idx = key >> shift;
+        const int page = idx < cols ? table[idx] : -1;
+        if (page < 0 || page >= num_pages) continue;
+        const int64_t row = row_of(page, key);
+        const bool whole = key >= lo && key + 4 <= k1;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const uint32_t x = reinterpret_cast<const uint32_t*>(p.v_scale + row * CH)[c];
+          if (whole) {
+            sv = span_add<4>(sv, x);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int ki = key + (4 * c + i) / CH;
+              if (ki >= lo && ki < k1) sv = span_add<1>(sv, x >> (8 * i));
+            }
+          }
+        }
+      }
+      uint32_t* red = reinterpret_cast<uint32_t*>(lds.v[1]);
+#pragma unroll
+      for (int i = 1; i < 64; i <<= 1) sv = span_join(sv, __shfl_xor(sv, i, 64));
+      if (lane == 0) red[wave] = sv;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) sv = span_join(sv, red[w]);
+      __syncthreads();
+      sv = __builtin_amdgcn_readfirstlane(sv);
+      uv.E = static_cast<int>(sv & 0xffu);
+      uv.wide = uv.E - (255 - static_cast<int>(sv >> 16)) > span_of(4);
+      if (uv.wide) uv.E = uv.E > kWideTop ? kUnit + uv.E - kWideTop : kUnit;
+      if (sv == 0) uv.E = kUnit;
+    }
+    const float c = a.sml2;
+    const uint32_t vadd = static_cast<uint32_t>(kUnit - uv.E) << 23;
+
+    // Keys that no row sees, or that are not there: their scales may be anything (their codes are finite as they are, and
+    // what K has there ends in scores that are masked).
+    auto clear_v = [&](int kt, int page) {
+      const int key0 = 64 * kt + WKEYS * wave;
+      if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
+      const uint32_t fill = static_cast<uint32_t>(uv.E) * 0x01010101u;
+#pragma unroll
+      for (int j = 0; j < VK; ++j)
+        if (const int key = key0 + VK * vkg + j; page < 0 || key < lo || key >= hi) {
+          if constexpr (CH == 4) vse[j] = fill;
+          else vse[0] = (vse[0] & (j & 1 ? 0x0000ffffu : 0xffff0000u)) | (fill & (j & 1 ? 0xffff0000u : 0xffffu));
+        }
+    };
+    // V: registers -> LDS, as fp16 in the part's unit or (WIDE) as bf16; in eight pieces.
+    struct Staged {
+      uint32_t v[VK][4];
+    };
+    auto v_piece = [&](Staged& st, int i, uint8_t* buf, auto WIDE) {
+      if (i < 4) {  // a key, then two columns in each piece
+        if (i >= VK) return;
+        uint32_t by;
+        if constexpr (CH == 4) by = __builtin_amdgcn_ubfe(vse[i], 8 * (vdq / 4), 8);
+        else by = __builtin_amdgcn_ubfe(vse[0], 16 * i + 8 * (vdq / 4), 8);
+        // (WIDE: far below the largest, a scale may be less than what is taken off)
+        const float sc = __uint_as_float(WIDE ? __builtin_elementwise_sub_sat(by << 23, 0u - vadd) : (by << 23) + vadd);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) st.v[i][k] = WIDE ? cvt_bf16<4>(vc + i, k, sc) : cvt_f16<4>(vc + i, k, sc);
+      } else {
+        // column 8 dq + c is V^T row c D/8 + dq, so that neighbouring lanes write neighbouring rows
+        const int k = i - 4;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+          uint8_t* dst = buf + ((2 * k + e) * (D / 8) + vdq) * L::VP + 2 * (WKEYS * wave + VK * vkg);
+          const uint32_t w0 = __builtin_amdgcn_perm(st.v[1][k], st.v[0][k], sel);
+          if constexpr (VK == 4)
+            *reinterpret_cast<uint2*>(dst) = make_uint2(w0, __builtin_amdgcn_perm(st.v[3][k], st.v[2][k], sel));
+          else
+            *reinterpret_cast<uint32_t*>(dst) = w0;
+        }
+      }
+    };
+    auto store_v = [&](uint8_t* buf, auto WIDE) {
+      Staged st;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v_piece(st, i, buf, WIDE);
+    };
+    // This lane's K row of a 32-key block, as A operand: its piece 2 i + g and the bytes 2 i + g of its scales (in bytes 2 i)
+    const int kr = key_of(li), krow = RB * (kr & 15), ksrow = CH * (kr & 15);
+    auto k_operand = [&](int b, int bl, int i) {
+      return *reinterpret_cast<const uint4*>(lds.k[b][2 * bl + (kr >> 4)] + krow + 16 * piece_of<D>(kr & 15, (2 * i + g) & (CH - 1)));
+    };
+    auto k_scale = [&](int b, int bl) -> uint32_t {
+      const uint8_t* at = lds.ks[b][2 * bl + (kr >> 4)] + ksrow;
+      if constexpr (CH == 4) return *reinterpret_cast<const uint32_t*>(at) >> (8 * g);
+      else return *reinterpret_cast<const uint16_t*>(at) >> (8 * g);
+    };
+    // Product n of a block's scores: step n / 4 of the columns, term n % 4
+    auto score = [&](int n, const uint4& k, uint32_t ke, const v16f& sc) -> v16f {
+      switch (n) {  // (known once the loops are unrolled)
+        case 0: return product<0, 0>(k, ke, q[0], sc);
+        case 1: return product<0, 1>(k, ke, q[0], sc);
+        case 2: return product<0, 2>(k, ke, q[0], sc);
+        case 3: return product<0, 3>(k, ke, q[0], sc);
+        case 4: return product<2, 0>(k, ke, q[NC - 1], sc);
+        case 5: return product<2, 1>(k, ke, q[NC - 1], sc);
+        case 6: return product<2, 2>(k, ke, q[NC - 1], sc);
+        default: return product<2, 3>(k, ke, q[NC - 1], sc);
+      }
+    };
+    // (a product must not write over its own scale: it stays until the block's scores are done)
+    auto keep = [](uint32_t ke) { asm volatile("" ::"v"(ke)); };
+    // S^T of 32 keys: register r is key 32 bl + 16 (r / 8) + 8 g + r % 8 of the tile in place b
+    auto scores = [&](int b, int bl, v16f& sc) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+      const uint32_t ke = k_scale(b, bl);
+#pragma unroll
+      for (int n = 0; n < NKS; ++n) sc = score(n, k_operand(b, bl, n / 4), ke, sc);
+      keep(ke);
+    };
+    // The tile's scores masked where a row does not see the key, the row's reference m brought up to date (and with it
+    // the sums so far); returns what p is relative to.
+    auto settle = [&](int kb, uint32_t here, v16f& s0, v16f& s1) -> float {
+      if (!(kb >= lo_all && kb + 64 <= hi_all && here == 0xfu)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = kb + 16 * (r >> 3) + 8 * g + (r & 7);
+          if (key < lo_r || key >= hi_r || !((here >> (r >> 3)) & 1u)) s0[r] = -INFINITY;
+          if (key + 32 < lo_r || key + 32 >= hi_r || !((here >> (2 + (r >> 3))) & 1u)) s1[r] = -INFINITY;
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = vmax(mx, vmax(s0[r], s1[r]));
+      mx = max_x32(mx) * c;
+      // m is 7 below a maximum seen: p may grow to 2^15 before m is moved (fp16 holds 65504), and is a normal fp16 number,
+      // with all its 11 bits, down to 2^-21 of the row's largest.
+      if (__any(mx > m + 15.0f)) {
+        const float mn = vmax(m, mx - 7.0f);
+        const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= al;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] *= al;
+      }
+      return m == -INFINITY ? 0.0f : m;
+    };
+
+    if (uv.wide) {
+      // Rare (see Unit), and plain: one tile after the other.
+      wait_for<0>();  // (the first tiles' copies)
+      for (int kt = begin; kt < end; ++kt) {
+        const int id = look(kt);
+        const uint32_t here = there(kt, id);
+        const int page = page_in(id, here, 0);
+        copy_k(kt, page, 0);
+        load_v(kt, page);
+        clear_v(kt, page);
+        store_v(lds.v[0], std::true_type{});
+        wait_for<0>();
+        __syncthreads();
+        v16f sc[2];
+#pragma unroll
+        for (int bl = 0; bl < 2; ++bl) scores(0, bl, sc[bl]);
+        const float ms = settle(64 * kt, here & 0xfu, sc[0], sc[1]);
+#pragma unroll
+        for (int bl = 0; bl < 2; ++bl)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint8_t* vr = lds.v[0] + li * L::VP + 16 * g + 32 * (2 * bl + j);
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              x[k] = __builtin_amdgcn_exp2f(fmaf(sc[bl][8 * j + k], c, -ms));
+              l += x[k];
+            }
+            uint32_t w[4], w2[4];  // V is bf16 as it is: P in two bf16 terms (16 bits)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              w[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+              w2[k] = pack_bf16(x[2 * k] - __uint_as_float(w[k] << 16), x[2 * k + 1] - __uint_as_float(w[k] & 0xffff0000u));
+            }
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) {
+              const uint4 va = *reinterpret_cast<const uint4*>(vr + 32 * db * L::VP);
+              acc[db] = mfma32_bf16(va, make_uint4(w[0], w[1], w[2], w[3]), acc[db]);
+              acc[db] = mfma32_bf16(va, make_uint4(w2[0], w2[1], w2[2], w2[3]), acc[db]);
+            }
+          }
+        __syncthreads();
+      }
+    } else {
+      constexpr std::false_type kNarrow{};
+      clear_v(begin, page0);
+      store_v(lds.v[0], kNarrow);
+      load_v(upto(begin + 1), pv);
+      uint32_t here0 = mask & 0xfu, here1 = mask >> 4 & 0xfu, here2 = mask >> 8 & 0xfu, here3 = mask >> 12 & 0xfu;
+      int pn = page_in(ids, mask, 2);
+      wait_for<0>();
+      __syncthreads();
+      v16f sa, sb, sc_;
+      scores(0, 0, sa);
+      scores(0, 1, sb);
+      __syncthreads();  // the first step puts another K tile there
+      // Tile kt: its scores are in s0 and s1; the next tile's go to s2 and, when s0 is used up, s0 (three blocks for what
+      // would be four).  In LDS: K of kt + 1 (place kn) and kt + 2, V of kt (cur); place kf is free.  In the staging
+      // registers: V of kt + 1.
+      auto step = [&](int kt, uint8_t* cur, uint8_t* nxt, int kn, int kf, v16f& s0, v16f& s1, v16f& s2) {
+        // The step's products in order: of each half of the tile the next tile's scores (NKS products) and this one's
+        // two quarters of P V (NDB each).  Their LDS operands are read kAhead products ahead, and each product is
+        // followed by a piece of what the VALU has to do meanwhile: the softmax of the half beside the scores, the
+        // conversion of the staged V tile beside P V.  The order is fixed here; left to the
+        // compiler, every read was next to its product.  The further a wave is in its products, the higher its priority:
+        // the SIMD's other wave then gives way, and does its waits, masks and maxima when this one does not multiply (4680
+        // tokens over 32760 keys, 12 heads: 1028 us without, 947; products over the rest alone 954; two levels more, the same).
+        constexpr int HALF = NKS + 2 * NDB, kAhead = 5;
+        const int id = look(kt + 4);  // back by the end of the step
+        uint4 ring[kAhead], kx[NC];
+        uint32_t ke[2];
+        const uint8_t* const vr = cur + li * L::VP + 16 * g;
+        auto fetch = [&](int n) {
+          if (n >= 2 * HALF) return;
+          const int bl = n / HALF, i = n % HALF;
+          if (i < NKS) {
+            if (i == 0) ke[bl] = k_scale(kn, bl);
+            if (i % 4 == 0) kx[i / 4] = k_operand(kn, bl, i / 4);
+          } else {
+            ring[n % kAhead] = *reinterpret_cast<const uint4*>(vr + 32 * ((i - NKS) % NDB) * L::VP + 32 * (2 * bl + (i - NKS) / NDB));
+          }
+        };
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) fetch(n);
+        const float ms = settle(64 * kt, here0, s0, s1);
+        clear_v(upto(kt + 1), pv);
+        __builtin_amdgcn_s_setprio(1);
+        Staged st;
+#pragma unroll
+        for (int bl = 0; bl < 2; ++bl) {
+          uint32_t w[8];
+          if (bl == 1) __builtin_amdgcn_s_setprio(2);
+          v16f& sc = bl == 0 ? s0 : s1;
+          v16f& sn = bl == 0 ? s2 : s0;
+#pragma unroll
+          for (int i = 0; i < HALF; ++i) {
+            const int n = bl * HALF + i;
+            if (i < NKS) {
+              if (i == 0) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sn[r] = 0.0f;
+              }
+              sn = score(i, kx[i / 4], ke[bl], sn);
+              fetch(n + kAhead);
+#pragma unroll
+              for (int e = 0; e < 8 / NKS; ++e) {
+                const int k = i * (8 / NKS) + e;
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k], c, -ms));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k + 1], c, -ms));
+                l += p0 + p1;
+                asm volatile("" : "+v"(l));  // here: else all 32 are added up at the step's end, and wait in registers
+                w[k] = pack_f16(p0, p1);
+              }
+            } else {
+              const int j = (i - NKS) / NDB, db = (i - NKS) % NDB;
+              acc[db] = mfma32_f16(ring[n % kAhead], make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]), acc[db]);
+              fetch(n + kAhead);
+              if ((i - NKS) % 2 == 1) {
+#pragma unroll
+                for (int e = 0; e < 4 / NDB; ++e) v_piece(st, 4 * bl + (i - NKS) / 2 * (4 / NDB) + e, nxt, kNarrow);
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          keep(ke[bl]);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        wait_for<0>();  // K of kt + 2, asked for a step ago
+        copy_k(upto(kt + 3), pk, kf);
+        load_v(upto(kt + 2), pn);
+        pv = pn;
+        pn = pk;
+        const uint32_t mask = there(kt + 4, id);
+        pk = page_in(id, mask, 0);
+        here0 = here1;
+        here1 = here2;
+        here2 = here3;
+        here3 = mask & 0xfu;
+        __syncthreads();
+      };
+      // (two places for V, three for K and three blocks of scores: the order comes round after six steps)
+      uint8_t* const v0 = lds.v[0];
+      uint8_t* const v1 = lds.v[1];
+      for (int kt = begin; kt < end;) {
+        step(kt, v0, v1, 1, 0, sa, sb, sc_);
+        if (++kt >= end) break;
+        step(kt, v1, v0, 2, 1, sc_, sa, sb);
+        if (++kt >= end) break;
+        step(kt, v0, v1, 0, 2, sb, sc_, sa);
+        if (++kt >= end) break;
+        step(kt, v1, v0, 1, 0, sa, sb, sc_);
+        if (++kt >= end) break;
+        step(kt, v0, v1, 2, 1, sc_, sa, sb);
+        if (++kt >= end) break;
+        step(kt, v1, v0, 0, 2, sb, sc_, sa);
+        ++kt;
+      }
+      wait_for<0>();  // (no copy may come after the workgroup's end)
+    }
+    l = add_x32(l);
+  }
+  if (rw + li < rows) {
+    const int64_t tok = s.start + qi;
+    const bool one = a.splits == 1;
+    const float f = filled(l) ? ldexpf(1.0f, uv.E - kUnit) / l : 0.0f;
+    const int64_t at = split * R + tok * p.Hq + h;
+    if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
+    if (!one && g == 0) a.ml[at] = make_float2(m, l);
+    if (one || filled(l)) {
+      // Register r of acc[db] is V^T row 32 db + 8 (r / 4) + 4 g + r % 4 = c D/8 + dq, column 8 dq + c.  D = 128: dq = 8 (r / 4
+      // % 2) + 4 g + r % 4, c = 2 db + r / 8; D = 64: dq = 4 g + r % 4, c = 4 db + r / 4.  So columns 64 i + 32 g + 8 k ..:
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int col = 64 * i + 32 * g;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float o[8];
+#pragma unroll
+          for (int cc = 0; cc < 8; ++cc)
+            o[cc] = (D == 128 ? acc[cc / 2 % NDB][8 * (cc & 1) + 4 * i + k] : acc[cc / 4][4 * (cc & 3) + k]) * f;
+          if (one) {
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col + 8 * k) =
+                make_uint4(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]), pack_dt<DT>(o[4], o[5]), pack_dt<DT>(o[6], o[7]));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(a.acc + at * D + col + 8 * k);
+            dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+            dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+          }
+        }
+      }
+    }
+  }
+}
+
+}  // namespace
+
+void lbfq::paged::launch_chunk4(const Args& a, unsigned grid, hipStream_t st) {
+  const bool bf = a.p.dtype == kBF16, d128 = a.p.D == 128;
+  if (bf && d128) hipLaunchKernelGGL((paged_chunk4_kernel<kBF16, 128>), dim3(grid), dim3(256), 0, st, a);
+  else if (bf) hipLaunchKernelGGL((paged_chunk4_kernel<kBF16, 64>), dim3(grid), dim3(256), 0, st, a);
+  else if (d128) hipLaunchKernelGGL((paged_chunk4_kernel<kF16, 128>), dim3(grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((paged_chunk4_kernel<kF16, 64>), dim3(grid), dim3(256), 0, st, a);
+}

@@ -320,8 +320,150 @@ __device__ __forceinline__ void join_waves(const Args& a, const Seq& s, const v4
   }
 }
 
-// The decode kernel of the cache in 4 bits (lbfq_paged4.hip)
-void launch_decode4(const Args& a, unsigned grid, hipStream_t stream);
+// ---- the chunk kernels
+
+// Key of K row i of a 32-key block (bits 2 and 3 of i exchanged): a lane's scores are
+// then of consecutive keys, eight at a time.
+__device__ __forceinline__ int key_of(int i) { return (i & 0x13) | ((i & 4) << 1) | ((i & 8) >> 1); }
+
+// Largest (low half) and 255 - smallest (high half) of the scale bytes so far and of word v.
+__device__ __forceinline__ uint32_t span_join(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <int N>  // N bytes of v
+__device__ __forceinline__ uint32_t span_add(uint32_t span, uint32_t v) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t b = (v >> (8 * i)) & 0xffu;
+    span = span_join(span, b | ((255u - b) << 16));
+  }
+  return span;
+}
+
+// What the values of a part's K or V are multiplied by, 2^(134 - E), on their way to fp16, so that the largest
+// code lands at 57344.  The smallest one, 2^-9, with a scale 2^-22 of the largest is then fp16's smallest step: within
+// that span every value is exact.  A part whose scales are further apart is `wide`: bf16, as they are.
+//
+// (A wide part's V is taken down by a power of two where its largest scale is past kWideTop: weights of up to 2^15 times
+// 2^30 of the largest values that are left, under 2^(kWideTop - 118), add up to less than 2^127.)
+//
+// E2M1's largest code, 6, lands at 49152 with 2^(140 - E), and its smallest, 1/2, stays exact 36 powers of two below.
+constexpr int span_of(int bits) { return bits == 8 ? 22 : 36; }
+constexpr int unit_of(int bits) { return bits == 8 ? 134 : 140; }
+constexpr int kWideTop = 200;
+struct Unit {
+  int E;
+  bool wide;
+};
+
+// Workgroups of a CU: three where the registers do for that, at the price of a few that go to memory (1560 tokens over 32760
+// keys, 40 heads of 64, bf16: 818 us with two, 765 with three; fp16 queries need more of them: 745 with two, 1075).
+constexpr int chunk_groups(int dt, int64_t d) { return d == 64 && dt == kBF16 ? 3 : 2; }
+constexpr int chunk4_groups(int64_t d) { return d == 64 ? 3 : 2; }  // (the 4-bit cache's kernel: 168 registers, none in memory)
+
+// ---- the kernels of the cache in 4 bits
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x32 __attribute__((ext_vector_type(32)));
+
+// Asynchronous copies into LDS: lane i's 16 (4) bytes go to lds + 16 (4) i.  In assembly, so that the compiler does not put
+// a wait for all of them before the next LDS read (wait_for does that); an LDS copy right behind a write of M0 needs one
+// wait state.  NT, for what nobody reads a second time (one token of 48 sequences of 8000 to 16000 keys, 135 -> 124 us).
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
+}
+__device__ __forceinline__ void copy_to(uint32_t lds) { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" ::"s"(lds) : "memory", "m0"); }
+template <int OFF, bool NT>  // OFF: of both the source and the place in LDS
+__device__ __forceinline__ void copy16(const uint8_t* base, uint32_t at) {
+  if constexpr (NT) asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2 nt" ::"v"(at), "s"(base), "i"(OFF) : "memory");
+  else asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2" ::"v"(at), "s"(base), "i"(OFF) : "memory");
+}
+template <bool NT>
+__device__ __forceinline__ void copy4(const uint8_t* base, uint32_t at) {
+  if constexpr (NT) asm volatile("global_load_lds_dword %0, %1 nt" ::"v"(at), "s"(base) : "memory");
+  else asm volatile("global_load_lds_dword %0, %1" ::"v"(at), "s"(base) : "memory");
+}
+__device__ __forceinline__ void copy16v(const uint8_t* at) {
+  asm volatile("global_load_lds_dwordx4 %0, off nt" ::"v"(at) : "memory");
+}
+__device__ __forceinline__ void copy4v(const uint8_t* at) {
+  asm volatile("global_load_lds_dword %0, off nt" ::"v"(at) : "memory");
+}
+// Until no more than N copies are under way (they end in their order)
+template <int N>
+__device__ __forceinline__ void wait_for() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+
+// The 16-byte piece of row r (of 16) that lies at place c of its D / 32 in LDS, and the place of piece c: so that 16 lanes
+// that read one piece of 16 rows each are on distinct banks.
+template <int D>
+__device__ __forceinline__ int piece_of(int r, int c) {
+  return D == 128 ? c ^ (r >> 2 & 3) : c ^ (r >> 3 & 1);
+}
+
+// 32 values over 2^e to E2M3, to nearest, and back; sc: 2^e.  In assembly for the &: the instructions write their results
+// before they have read all operands, and the builtins let the compiler lay the one over the other.
+__device__ __forceinline__ u32x6 to_e2m3(const f32x16& even, const f32x16& odd, float sc) {
+  u32x6 w;
+  asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3\n\ts_nop 4" : "=&v"(w) : "v"(even), "v"(odd), "v"(sc));
+  return w;
+}
+__device__ __forceinline__ f32x32 from_e2m3(const u32x6& w, float sc) {
+  f32x32 v;
+  asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2\n\ts_nop 4" : "=&v"(v) : "v"(w), "v"(sc));
+  return v;
+}
+
+// 32 columns of a query in four E2M3 terms, and their E8M0 scales in the bytes of e: 255 (not a number) where a column is
+// infinite or NaN.
+struct Terms {
+  u32x6 w[4];
+  uint32_t e;
+};
+template <int DT>
+__device__ __forceinline__ Terms split_query(const uint16_t* q) {
+  f32x16 even, odd;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 v = reinterpret_cast<const uint4*>(q)[i];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      even[4 * i + k] = DT == kBF16 ? __uint_as_float(w[k] << 16) : f16_bits_to_f32(static_cast<uint16_t>(w[k]));
+      odd[4 * i + k] =
+          DT == kBF16 ? __uint_as_float(w[k] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(w[k] >> 16));
+    }
+  }
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = vmax(vmax(m, fabsf(even[i])), fabsf(odd[i]));
+  const uint32_t top = __float_as_uint(m) >> 23;  // m is not negative, or a NaN of either sign
+  const bool bad = (top & 0xffu) == 255u;
+  // 2^(e - 127): the largest column is in 2 ... 4 of it, what a term leaves at most 4 of the next one's, E2M3 reaches 7.5
+  const uint32_t e = bad ? 100u : (top > 18u ? top : 18u) - 1u;
+  Terms x;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const float sc = __uint_as_float((e - 5u * t) << 23);
+    x.w[t] = to_e2m3(even, odd, sc);
+    if (t < 3) {
+      const f32x32 back = from_e2m3(x.w[t], sc);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        even[i] -= back[2 * i];
+        odd[i] -= back[2 * i + 1];
+      }
+    }
+  }
+  x.e = bad ? 0xffffffffu : e * 0x01010101u - 0x0f0a0500u;
+  return x;
+}
+
+void launch_decode4(const Args& a, unsigned grid, hipStream_t stream);  // lbfq_paged4.hip
+void launch_chunk4(const Args& a, unsigned grid, hipStream_t stream);   // lbfq_paged4_chunk.hip
 
 }  // namespace paged
 }  // namespace lbfq
