@@ -216,6 +216,16 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
   const uint32_t block = blockIdx.x / a.groups;
   const int h0 = static_cast<int>(blockIdx.x - block * a.groups) * kHeads;
   const int64_t t = static_cast<int64_t>(block) * RPI + r, tok = t < p.T ? t : p.T - 1;
+  Raw<DT> raw[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int g = h0 + i < heads ? h0 + i : heads - 1;
+    const bool isq = g < Hq, isk = g < Hq + Hk;
+    raw[i] = load_raw<DT>(isq ? p.q : isk ? p.k : p.v,
+                          tok * (isq ? p.q_t : isk ? p.k_t : p.v_t) +
+                              (isq ? g * p.q_h : isk ? (g - Hq) * p.k_h : (g - Hq - Hk) * p.v_h) + d0);
+  }
+  const int64_t slot = t < p.T ? p.slots[tok] : -1;
   const int half = p.rot / 2;
   bool past = false, turned = false;
   int partner = lane;
@@ -252,18 +262,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
                             : reinterpret_cast<const int32_t*>(p.positions)[tok * p.pos_t]) >= p.table_len;
   }
   const int64_t slots = p.num_pages << p.page_shift;
-  const int64_t slot = t < p.T ? p.slots[tok] : -1;
   const bool live = slot >= 0 && slot < slots && !past;
   const int64_t page_row = (slot >> p.page_shift) * Hk, in_page = slot & ((int64_t{1} << p.page_shift) - 1);
-  Raw<DT> raw[kHeads];
-#pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int g = h0 + i < heads ? h0 + i : heads - 1;
-    const bool isq = g < Hq, isk = g < Hq + Hk;
-    raw[i] = load_raw<DT>(isq ? p.q : isk ? p.k : p.v,
-                          tok * (isq ? p.q_t : isk ? p.k_t : p.v_t) +
-                              (isq ? g * p.q_h : isk ? (g - Hq) * p.k_h : (g - Hq - Hk) * p.v_h) + d0);
-  }
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     const int g = h0 + i;

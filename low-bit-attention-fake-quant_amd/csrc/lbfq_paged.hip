@@ -935,6 +935,19 @@ constexpr int64_t kMostBytes = (int64_t{1} << 30) - 16;
 // 71 / 57* / 72 / 69 / 67 / 76; 4 of 700 and 9001, 12 heads 192 / 142 / 117 / 127 / 120* / 115 / 123; 2 of 1024 and 16000 475 /
 // 469 / 474 / 432* / 449 / 457 / 468; 2 of 300 and 5000 111 / 70 / 68 / 63* / 76 / 76 / 77; 4 of 509, fp16, window 4096 77 / 63 /
 // 53* / 52 / 58 / 58 / 66).
+//
+// In 4 bits the last round is counted as what it takes where it does not fill the chip, 0.7 of a round up to half of it (us
+// for 1 / 2 / 3 / 4 / 5 / 6 / 7 / 8 parts, * the rule's: 4680 tokens, 32760 keys, 12 heads 995 / 949* / 975 / 994; 1560 tokens, 40
+// heads 1735 / 1375 / 1265 / 1224 / 1214* / 1198 / 1207 / 1210; 700 tokens, 8000 keys, 12 heads 173 / 102 / 81 / 73 / 67 / 62* / 89); and
+// parts of several sequences that come out at a little over whole rounds are made fewer (2 of 300 and 5000 112 / 75 / 66 / 58* /
+// 79 / 76; 8 of 128 and 4000 101 / 76* / 82 / 79; 4 of 700 and 9001, 12 heads 216 / 134 / 146 / 130 / 126* / 139).
+int64_t rounds10(int64_t n, int64_t places) {
+  const int64_t whole = n / places, rest = n % places;
+  if (rest == 0) return 10 * whole;
+  if (whole == 0) return 10;
+  return 10 * whole + (2 * rest <= places ? 7 : 7 + (2 * rest - places) * 3 / places);
+}
+
 Plan plan(const lbfq_paged_params* p) {
   Plan x;
   const int64_t G = p->Hq / p->Hk;
@@ -965,12 +978,14 @@ Plan plan(const lbfq_paged_params* p) {
     for (int64_t n = 1; n <= limit; ++n) {
       const int64_t of_xcd = (x.groups * p->Hk * n + 7) / 8 * x.piece, longest = keys / n + 12 * 64;
       const int64_t cost = uneven ? std::max(of_xcd * ((keys - seeing / 2) / n + 12 * 64), 45 * longest)
-                                  : (of_xcd + places - 1) / places * places * longest;
+                                  : (four ? rounds10(of_xcd, places) * places / 10 : (of_xcd + places - 1) / places * places) * longest;
       if (cost < best) best = cost, s = n;
     }
   } else {
     const int64_t wgs = (tiles + p->B / 2) * p->Hk;
     while (120 * (s + 1) * (s + 1) * wgs <= places * keys && s < limit) ++s;
+    if (const int64_t all = 8 * places, over = wgs * s % all; four && wgs * s > all && 3 * over < all)
+      s = std::max<int64_t>((wgs * s - over) / wgs, 1);
   }
   x.splits = static_cast<int>(std::max<int64_t>(std::min(s, limit), 1));
   x.least = static_cast<int>(least / (x.decode && !four ? 32 : 64));
