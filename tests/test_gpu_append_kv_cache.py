@@ -113,6 +113,21 @@ def test_columns_that_are_not_rotated_do_not_reach_each_other(gpu):
         assert torch.equal(torch.isnan(got).sum((1, 2)).cpu(), torch.tensor([0, 1, 0, 0]))
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("pairs", ["adjacent", "halves"])
+def test_infinities_and_nan_reach_the_cache_as_by_a_write(gpu, pairs, bits):
+    from low_bit_fake_quant import append_kv_cache, empty_kv_cache, write_kv_cache
+    q, k, v, cos, sin, pos = inputs(gpu, 12, 2, 2, 128, torch.float32, 96, packed=False)
+    for i, x in enumerate((math.inf, -math.inf, math.nan, 3.4e38, -3.4e38, 1e-44)):
+        k[i, 0, 5 * i], k[i, 1, 100], v[i, :, 7 * i] = x, x, x
+    slots = torch.arange(12, device=gpu)
+    got, want = (empty_kv_cache(1, 16, 2, 128, device=gpu, bits=bits) for _ in range(2))
+    append_kv_cache(q, k, v, got, slots, cos, sin, pos, pairs=pairs)
+    write_kv_cache(turned(k, cos, sin, pos, pairs), v, want, slots)
+    for a, b in zip(bytes_of(got), bytes_of(want)):
+        assert torch.equal(a, b)
+
+
 def test_layouts_no_queries_and_strided_tables(gpu):
     from low_bit_fake_quant import append_kv_cache, empty_kv_cache
     T, hq, hk, d = 37, 4, 2, 128

@@ -52,7 +52,10 @@ def attend(q, cache, table, lens, starts, *, causal=True, window=None, sm_scale=
     """kv_reference.attend of the same values, whose bound is added to what it leaves out.  Many E2M1 values are 0, so
     what a row's large weights multiply may be nothing at all, and its result the product of a weight that fp16 holds as
     one of its smallest numbers: the chunk kernel's largest weight is 2^7 at least, so fp16's step there, 2^-24, rounds
-    the others by up to 2^-32 of it.  Added up: 2^-32 sum |V_j| over the keys that are seen (l >= 1)."""
+    the others by up to 2^-32 of it.  Added up: 2^-32 sum |V_j| over the keys that are seen (l >= 1).
+
+    And the query's terms leave up to 2^-19 of the largest of 32 columns (2^-3 2^-15 of a scale that the largest is
+    twice of at least): scores off by dq = 2^-19 sum of that |k_j| sm_scale, the result by 2 dq max |V_j|, its lse by dq."""
     if cache[0].dtype == torch.float4_e2m1fn_x2:
         cache = ref4.widen(cache)
     out, lse, tol, ltol = plain(q, cache, table, lens, starts, causal=causal, window=window, sm_scale=sm_scale)
@@ -61,7 +64,15 @@ def attend(q, cache, table, lens, starts, *, causal=True, window=None, sm_scale=
         v = torch.nan_to_num(ref.rows_of(cache[2], cache[3], table[b], int(lens[b]))).abs()
         if r1 > r0 and v.shape[0]:
             seen = ref.visible(r1 - r0, v.shape[0], causal, window, q.device).any(0)
-            tol[r0:r1] += 2.0 ** -32 * v[seen].sum(0).repeat_interleave(q.shape[1] // v.shape[1], 0)
+            k = torch.nan_to_num(ref.rows_of(cache[0], cache[1], table[b], int(lens[b]))).abs()
+            g, d = q.shape[1] // v.shape[1], q.shape[2]
+            tol[r0:r1] += 2.0 ** -32 * v[seen].sum(0).repeat_interleave(g, 0)
+            if seen.any():
+                top = torch.nan_to_num(q[r0:r1].double()).abs().unflatten(-1, (-1, 32)).amax(-1).repeat_interleave(32, -1)
+                kt = k[seen].permute(1, 2, 0).repeat_interleave(g, 0).contiguous()
+                dq = 2.0 ** -19 * torch.bmm(top.transpose(0, 1).contiguous(), kt).amax(-1).t() * (sm_scale or 1.0 / math.sqrt(d))
+                tol[r0:r1] += 2 * dq[..., None] * v[seen].amax(0).repeat_interleave(g, 0)
+                ltol[r0:r1] += dq
     return out, lse, tol, ltol
 
 
@@ -119,7 +130,7 @@ def test_scale_bytes_of_a_cache_filled_elsewhere(gpu, n, d, dtype, low, high):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("n", [1, 40])
-@pytest.mark.parametrize("kind", ["outliers", "tiny", "huge", "one"])
+@pytest.mark.parametrize("kind", ["outliers", "tiny", "huge", "one", "hidden"])
 def test_queries_of_very_different_columns(gpu, n, d, dtype, kind):
     """A few columns a thousand times the others; values next to the dtype's smallest and largest; one column."""
     q, cache, table, lens, starts = problem(gpu, lens=[150, 90], counts=[n, n], d=d, dtype=dtype, garbage=False, qscale=1.0)
@@ -133,6 +144,10 @@ def test_queries_of_very_different_columns(gpu, n, d, dtype, kind):
     elif kind == "huge":
         q.mul_(2.0 ** (13 if dtype == torch.float16 else 100))
         sm = 2.0 ** (-16 if dtype == torch.float16 else -64)
+    elif kind == "hidden":  # one column of 32 is thousands of times the others, and K is 0 there
+        q[..., ::32] *= 4000 if dtype == torch.bfloat16 else 1000
+        cache[0].view(torch.uint8)[..., ::16] &= 0xF0
+        sm = 0.1
     else:
         q[..., 1:] = 0
         sm = 1.0
