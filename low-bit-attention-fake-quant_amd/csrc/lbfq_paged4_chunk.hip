@@ -6,11 +6,12 @@
 // multiplied by the query's four E2M3 terms with the block-scaled product (32x32x64; see lbfq_paged4.hip): as many
 // cycles as bf16's, but a quarter of the LDS reads, and no conversion.  (At 16 bits, a step's reads take as long as its
 // products: 32 KiB for 16 + 16 of 32 cycles, four waves and two workgroups a CU.)  K's scales go into the product, so no
-// span of them needs bf16.
+// span of them needs bf16.  V is converted as there, but staged as rows of keys, and turned by the reads that feed the
+// products (with 16 permutations a step instead, heads of 64 took 2.5% longer, of 128 the same).
 //
-// 4680 tokens over 32760 keys, 12 heads of 128, all seen: 947 us, 1.0 PFLOP/s (the 8-bit kernel 1067 in the same run; a
-// large library product 1.24).  214 VALU instructions a step, 32 of them exponentials, issue beside 32 products of 32
-// cycles: the two take 93% of the cycles of a full CU together.  With all codes zero it takes 10 to 17% less: power.
+// 8192 tokens over 32768 keys, 8 heads of 128, all seen: 965 us, 1.14 PFLOP/s, where a large library product reaches 1.24 (with
+// all codes zero 860: power).  4680 over 32760, 12 heads: 925 us, 1.02 PFLOP/s (the 8-bit kernel 1067 where this one took
+// 947).  200 VALU instructions a step, 32 of them exponentials, issue beside 32 products of 32 cycles.  Heads of 64: 0.88.
 #include "lbfq_paged_common.h"
 
 using namespace lbfq;
@@ -20,11 +21,13 @@ namespace {
 
 template <int D>
 struct Lds {
-  static constexpr int VP = 2 * 64 + 16;  // pitch of a V^T row
+  // Pitch of a V row, one key's columns: 64 more than a multiple of 256 or of 128, so that the four rows that 32 lanes of a
+  // transposing read take 64 bytes of are on distinct banks.
+  static constexpr int VP = 2 * D + 64;
   // A tile's K: 16 keys of each wave that copies them, rows of D / 2 bytes, pieces exchanged (piece_of), and their scales
   // (what a copy of 64 lanes needs; D = 64 uses half of the codes' place, and the scales take 64 or 32 bytes)
   uint8_t k[3][4][1024], ks[3][4][256];
-  uint8_t v[2][D * VP];
+  uint8_t v[2][64 * VP];
 };
 
 // K (E2M1; scale in byte A of ke) times term B of the query
@@ -35,6 +38,17 @@ __device__ __forceinline__ v16f product(const uint4& k, uint32_t ke, const Terms
   const i32x8 y = {static_cast<int>(w[0]), static_cast<int>(w[1]), static_cast<int>(w[2]), static_cast<int>(w[3]),
                    static_cast<int>(w[4]), static_cast<int>(w[5]), 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 2, A, static_cast<int>(ke), B, static_cast<int>(q.e));
+}
+
+// V^T as A operand of a product of 32 columns and 16 keys from rows of keys: a read that transposes 4 x 16 values between 16
+// lanes gives each its column of four keys.  at: this lane's 8 bytes of the first four keys' rows.
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4* LdsRow;
+template <int VP>
+__device__ __forceinline__ uint4 v_operand(const uint8_t* at) {
+  const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(at)));
+  const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(at + 4 * VP)));
+  return make_uint4(a.x, a.y, b.x, b.y);
 }
 
 template <int DT, int D>
@@ -218,40 +232,24 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
           else vse[0] = (vse[0] & (j & 1 ? 0x0000ffffu : 0xffff0000u)) | (fill & (j & 1 ? 0xffff0000u : 0xffffu));
         }
     };
-    // V: registers -> LDS, as fp16 in the part's unit or (WIDE) as bf16; in eight pieces.
-    struct Staged {
-      uint32_t v[VK][4];
-    };
-    auto v_piece = [&](Staged& st, int i, uint8_t* buf, auto WIDE) {
-      if (i < 4) {  // a key, then two columns in each piece
-        if (i >= VK) return;
-        uint32_t by;
-        if constexpr (CH == 4) by = __builtin_amdgcn_ubfe(vse[i], 8 * (vdq / 4), 8);
-        else by = __builtin_amdgcn_ubfe(vse[0], 16 * i + 8 * (vdq / 4), 8);
-        // (WIDE: far below the largest, a scale may be less than what is taken off)
-        const float sc = __uint_as_float(WIDE ? __builtin_elementwise_sub_sat(by << 23, 0u - vadd) : (by << 23) + vadd);
+    // V's key i of this thread's VK: registers -> LDS, as fp16 in the part's unit or (WIDE) as bf16
+    auto put_v = [&](int i, uint8_t* buf, auto WIDE) {
+      uint32_t by;
+      if constexpr (CH == 4) by = __builtin_amdgcn_ubfe(vse[i], 8 * (vdq / 4), 8);
+      else by = __builtin_amdgcn_ubfe(vse[0], 16 * i + 8 * (vdq / 4), 8);
+      // (WIDE: far below the largest, a scale may be less than what is taken off)
+      const float sc = __uint_as_float(WIDE ? __builtin_elementwise_sub_sat(by << 23, 0u - vadd) : (by << 23) + vadd);
+      uint32_t w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) st.v[i][k] = WIDE ? cvt_bf16<4>(vc + i, k, sc) : cvt_f16<4>(vc + i, k, sc);
-      } else {
-        // column 8 dq + c is V^T row c D/8 + dq, so that neighbouring lanes write neighbouring rows
-        const int k = i - 4;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t sel = e ? 0x07060302u : 0x05040100u;
-          uint8_t* dst = buf + ((2 * k + e) * (D / 8) + vdq) * L::VP + 2 * (WKEYS * wave + VK * vkg);
-          const uint32_t w0 = __builtin_amdgcn_perm(st.v[1][k], st.v[0][k], sel);
-          if constexpr (VK == 4)
-            *reinterpret_cast<uint2*>(dst) = make_uint2(w0, __builtin_amdgcn_perm(st.v[3][k], st.v[2][k], sel));
-          else
-            *reinterpret_cast<uint32_t*>(dst) = w0;
-        }
-      }
+      for (int k = 0; k < 4; ++k) w[k] = WIDE ? cvt_bf16<4>(vc + i, k, sc) : cvt_f16<4>(vc + i, k, sc);
+      *reinterpret_cast<uint4*>(buf + (WKEYS * wave + VK * vkg + i) * L::VP + 16 * vdq) = make_uint4(w[0], w[1], w[2], w[3]);
     };
     auto store_v = [&](uint8_t* buf, auto WIDE) {
-      Staged st;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v_piece(st, i, buf, WIDE);
+      for (int i = 0; i < VK; ++i) put_v(i, buf, WIDE);
     };
+    // This lane's part in V's reads: keys 8 g + li % 16 / 4 (and four on), columns 16 (li / 16) + 4 (li % 4) ..
+    const int vrow = (8 * g + (li & 15) / 4) * L::VP + 32 * (li >> 4) + 8 * (li & 3);
     // This lane's K row of a 32-key block, as A operand: its piece 2 i + g and the bytes 2 i + g of its scales (in bytes 2 i)
     const int kr = key_of(li), krow = RB * (kr & 15), ksrow = CH * (kr & 15);
     auto k_operand = [&](int b, int bl, int i) {
@@ -337,7 +335,7 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
         for (int bl = 0; bl < 2; ++bl)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const uint8_t* vr = lds.v[0] + li * L::VP + 16 * g + 32 * (2 * bl + j);
+            const uint8_t* vr = lds.v[0] + vrow + 16 * (2 * bl + j) * L::VP;
             float x[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -352,7 +350,7 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
             }
 #pragma unroll
             for (int db = 0; db < NDB; ++db) {
-              const uint4 va = *reinterpret_cast<const uint4*>(vr + 32 * db * L::VP);
+              const uint4 va = v_operand<L::VP>(vr + 64 * db);
               acc[db] = mfma32_bf16(va, make_uint4(w[0], w[1], w[2], w[3]), acc[db]);
               acc[db] = mfma32_bf16(va, make_uint4(w2[0], w2[1], w2[2], w2[3]), acc[db]);
             }
@@ -387,7 +385,7 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
         const int id = look(kt + 4);  // back by the end of the step
         uint4 ring[kAhead], kx[NC];
         uint32_t ke[2];
-        const uint8_t* const vr = cur + li * L::VP + 16 * g;
+        const uint8_t* const vr = cur + vrow;
         auto fetch = [&](int n) {
           if (n >= 2 * HALF) return;
           const int bl = n / HALF, i = n % HALF;
@@ -395,7 +393,7 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
             if (i == 0) ke[bl] = k_scale(kn, bl);
             if (i % 4 == 0) kx[i / 4] = k_operand(kn, bl, i / 4);
           } else {
-            ring[n % kAhead] = *reinterpret_cast<const uint4*>(vr + 32 * ((i - NKS) % NDB) * L::VP + 32 * (2 * bl + (i - NKS) / NDB));
+            ring[n % kAhead] = v_operand<L::VP>(vr + 16 * (2 * bl + (i - NKS) / NDB) * L::VP + 64 * ((i - NKS) % NDB));
           }
         };
 #pragma unroll
@@ -403,7 +401,6 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
         const float ms = settle(64 * kt, here0, s0, s1);
         clear_v(upto(kt + 1), pv);
         __builtin_amdgcn_s_setprio(1);
-        Staged st;
 #pragma unroll
         for (int bl = 0; bl < 2; ++bl) {
           uint32_t w[8];
@@ -433,10 +430,7 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
               const int j = (i - NKS) / NDB, db = (i - NKS) % NDB;
               acc[db] = mfma32_f16(ring[n % kAhead], make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]), acc[db]);
               fetch(n + kAhead);
-              if ((i - NKS) % 2 == 1) {
-#pragma unroll
-                for (int e = 0; e < 4 / NDB; ++e) v_piece(st, 4 * bl + (i - NKS) / 2 * (4 / NDB) + e, nxt, kNarrow);
-              }
+              if ((i - NKS) % 4 == 1) put_v(bl * (VK / 2) + (i - NKS) / 4, nxt, kNarrow);
             }
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -485,27 +479,21 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
     if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
     if (!one && g == 0) a.ml[at] = make_float2(m, l);
     if (one || filled(l)) {
-      // Register r of acc[db] is V^T row 32 db + 8 (r / 4) + 4 g + r % 4 = c D/8 + dq, column 8 dq + c.  D = 128: dq = 8 (r / 4
-      // % 2) + 4 g + r % 4, c = 2 db + r / 8; D = 64: dq = 4 g + r % 4, c = 4 db + r / 4.  So columns 64 i + 32 g + 8 k ..:
+      // Register r of acc[db] is column 32 db + 8 (r / 4) + 4 g + r % 4.
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int col = 64 * i + 32 * g;
+      for (int db = 0; db < NDB; ++db)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          float o[8];
+          const int col = 32 * db + 8 * k + 4 * g;
+          float o[4];
 #pragma unroll
-          for (int cc = 0; cc < 8; ++cc)
-            o[cc] = (D == 128 ? acc[cc / 2 % NDB][8 * (cc & 1) + 4 * i + k] : acc[cc / 4][4 * (cc & 3) + k]) * f;
-          if (one) {
-            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col + 8 * k) =
-                make_uint4(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]), pack_dt<DT>(o[4], o[5]), pack_dt<DT>(o[6], o[7]));
-          } else {
-            float4* dst = reinterpret_cast<float4*>(a.acc + at * D + col + 8 * k);
-            dst[0] = make_float4(o[0], o[1], o[2], o[3]);
-            dst[1] = make_float4(o[4], o[5], o[6], o[7]);
-          }
+          for (int i = 0; i < 4; ++i) o[i] = acc[db][4 * k + i] * f;
+          if (one)
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col) =
+                make_uint2(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]));
+          else
+            *reinterpret_cast<float4*>(a.acc + at * D + col) = make_float4(o[0], o[1], o[2], o[3]);
         }
-      }
     }
   }
 }
