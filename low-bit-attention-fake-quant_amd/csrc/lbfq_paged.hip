@@ -899,6 +899,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Args a) {
 struct Plan {
   bool decode;
   int splits, least;
+  int64_t share;  // chunk in 4 bits: Args::share
   int64_t slots, groups, piece;  // chunk: row tiles of a head (slot_of), the pieces that they come in, row tiles of a piece
 };
 
@@ -950,6 +951,7 @@ int64_t rounds10(int64_t n, int64_t places) {
 
 Plan plan(const lbfq_paged_params* p) {
   Plan x;
+  x.share = 0;
   const int64_t G = p->Hq / p->Hk;
   const int64_t most = p->max_query_len > 0 && p->max_query_len < p->T ? p->max_query_len : p->T;
   x.decode = most * G <= kDecodeRows;
@@ -980,6 +982,19 @@ Plan plan(const lbfq_paged_params* p) {
       const int64_t cost = uneven ? std::max(of_xcd * ((keys - seeing / 2) / n + 12 * 64), 45 * longest)
                                   : (four ? rounds10(of_xcd, places) * places / 10 : (of_xcd + places - 1) / places * places) * longest;
       if (cost < best) best = cost, s = n;
+    }
+    // Two unequal parts (in 4 bits): row tiles that fill more than half of the chip, but not all of it, leave the last keys of
+    // each to the places that are free, where they come one after the other (4680 tokens over 32760 keys, 12 heads, one part /
+    // two equal / these: 899 / 937 / 878 us; 3800 tokens 865 / 883 / 718).  Joining them takes a tile's time for 550000 values.
+    const int64_t wgs = x.slots * p->Hk, all = 8 * places, o = 12 * 64;
+    if (four && !uneven && limit >= 2 && wgs < all && 2 * wgs > all) {
+      const int64_t turns = (wgs + all - wgs - 1) / (all - wgs);
+      const int64_t rest = (keys + o - turns * o) / (turns + 1);
+      const int64_t join = 64 * (p->T * p->Hq * p->D / 550000 + 2);
+      if (rest >= 128 && places * (keys - rest + o + join) < best) {
+        s = 2;
+        x.share = ((keys - rest) << 16) / keys;
+      }
     }
   } else {
     const int64_t wgs = (tiles + p->B / 2) * p->Hk;
@@ -1066,6 +1081,8 @@ extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t st
   LBFQ_CHECK_ARG(a.main < (1 << 24) - 8, "lbfq_paged_attention: problem too large");
   a.combos = static_cast<uint32_t>(combos);
   a.piece = static_cast<uint32_t>(x.piece);
+  a.share = static_cast<uint32_t>(x.share);
+  if (x.share) a.main = (x.slots * p->Hk + 7) / 8 * 8 * 2;
   // rows that no sequence has: the combine kernel sees every row, otherwise some workgroups more, one for 64 KiB that the
   // output holds
   const int64_t fill = (p->fill_rest || p->lse) && x.splits == 1

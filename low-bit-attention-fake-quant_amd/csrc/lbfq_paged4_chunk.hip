@@ -10,8 +10,8 @@
 // products (with 16 permutations a step instead, heads of 64 took 2.5% longer, of 128 the same).
 //
 // 8192 tokens over 32768 keys, 8 heads of 128, all seen: 965 us, 1.14 PFLOP/s, where a large library product reaches 1.24 (with
-// all codes zero 860: power).  4680 over 32760, 12 heads: 925 us, 1.02 PFLOP/s (the 8-bit kernel 1067 where this one took
-// 947).  200 VALU instructions a step, 32 of them exponentials, issue beside 32 products of 32 cycles.  Heads of 64: 0.88.
+// all codes zero 860: power).  4680 over 32760, 12 heads: 878 us, 1.07 PFLOP/s (in two equal parts 937, the 8-bit kernel
+// 1067).  200 VALU instructions a step, 32 of them exponentials, issue beside 32 products of 32 cycles.  Heads of 64: 0.88.
 #include "lbfq_paged_common.h"
 
 using namespace lbfq;
@@ -66,18 +66,28 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
     return;
   }
   __shared__ __align__(16) L lds;
-  // Workgroups go to the eight XCDs in turn.  Pieces of up to eight neighbouring row tiles are dealt to them whole, so that
-  // those that read the same keys share an L2; the pieces of all heads and parts (`combos`) with the last rows first,
-  // which take longest under a causal mask, and turned by one XCD from round to round, so that none has all of a kind.
-  // (No slots in vain: where seven of eight workgroups had nothing to do, the others shared a quarter of the chip: an
-  // XCD's four shader engines take its workgroups in turn.  1024 keys, 512 heads of 128 rows: 203 us, dense 60.)
-  const uint32_t ps = a.piece, round = blockIdx.x / (8 * ps), piece = round * 8 + (blockIdx.x + round) % 8;
-  const int slot = a.slots - 1 - static_cast<int>(piece / a.combos * ps + blockIdx.x / 8 % ps);
-  if (slot < 0) return;
-  const uint32_t rest = piece % a.combos, splits = static_cast<uint32_t>(a.splits);
-  const int split = static_cast<int>(rest % splits), kvh = static_cast<int>(rest / splits);
   const int G = a.G, Hk = static_cast<int>(p.Hk);
-  const int b = sequence_at(p, G, slot), r0 = (slot - slot_of(p, G, b)) * QB;
+  int split, kvh, slot, b = 0, r0;
+  if (a.share) {
+    // Two unequal parts of one sequence: all the longer ones first, each XCD a stretch of neighbouring row tiles.
+    const uint32_t half = static_cast<uint32_t>(a.main) / 2, all = a.slots * static_cast<uint32_t>(Hk);
+    split = blockIdx.x >= half;
+    const uint32_t i = blockIdx.x - split * half, id = i % 8 * (half / 8) + i / 8;
+    if (id >= all) return;
+    kvh = static_cast<int>(id / a.slots);
+    slot = static_cast<int>(id % a.slots);
+    r0 = slot * QB;
+  } else {
+    // (the 8-bit kernel's order: neighbouring row tiles to one XCD, the last rows first)
+    const uint32_t ps = a.piece, round = blockIdx.x / (8 * ps), piece = round * 8 + (blockIdx.x + round) % 8;
+    slot = a.slots - 1 - static_cast<int>(piece / a.combos * ps + blockIdx.x / 8 % ps);
+    if (slot < 0) return;
+    const uint32_t rest = piece % a.combos, splits = static_cast<uint32_t>(a.splits);
+    split = static_cast<int>(rest % splits);
+    kvh = static_cast<int>(rest / splits);
+    b = sequence_at(p, G, slot);
+    r0 = (slot - slot_of(p, G, b)) * QB;
+  }
   const Seq s = sequence(p, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 31, g = lane >> 5;
@@ -110,8 +120,9 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
 
   const int kt0 = lo / 64, nt = hi > lo ? (hi + 63) / 64 - kt0 : 0;
   int per = (nt + a.splits - 1) / a.splits;
+  if (a.share) per = static_cast<int>((static_cast<int64_t>(nt) * a.share + 65535) >> 16);
   per = per > a.least ? per : a.least;
-  const int begin = kt0 + split * per;
+  const int begin = kt0 + split * per;  // (unequal parts: the second is the shorter one)
   const int end = begin + per < kt0 + nt ? begin + per : kt0 + nt;
 
   v16f acc[NDB];

@@ -32,6 +32,7 @@ struct Args {
   int least;      // key tiles of a part, at least
   int slots;      // chunk: places for row tiles, over all sequences
   uint32_t piece;   // chunk: neighbouring slots that go to one XCD
+  uint32_t share;   // chunk in 4 bits: of 2^16, what the first of two unequal parts has of the keys (0: equal parts)
   uint32_t combos;  // decode: sequences x key heads; chunk: key heads x parts
   int64_t main;   // workgroups that attend (the others fill)
   float sml2;     // sm_scale * log2(e)

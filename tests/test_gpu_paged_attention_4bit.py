@@ -156,6 +156,25 @@ def test_queries_of_very_different_columns(gpu, n, d, dtype, kind):
     eight.run_and_check((q, cache, table, lens, starts), kind, hint=n, sm_scale=sm)
 
 
+@pytest.mark.parametrize("n,L,cols,hk,d,dtype,causal,before", [
+    (2200, 2500, None, 16, 128, torch.bfloat16, False, 0), (2200, 4480, None, 16, 128, torch.float16, True, 0),
+    (2200, 2500, 300, 16, 128, torch.bfloat16, False, 5), (2100, 2200, None, 24, 64, torch.float16, False, 0),
+    (2200, 30, 300, 16, 128, torch.bfloat16, False, 0)])
+def test_two_unequal_parts(gpu, n, L, cols, hk, d, dtype, causal, before):
+    """Row tiles of one sequence that fill more than half of the chip, but not all; also where the sequence is much shorter
+    than its table, and behind rows of no sequence."""
+    from low_bit_fake_quant import paged_attention
+    q, cache, table, lens, starts = problem(gpu, lens=[L], counts=[n], hq=hk, hk=hk, d=d, dtype=dtype, page=64, cols=cols,
+                                            tail=before, garbage=False)
+    q, starts = torch.roll(q, before, 0), starts + before
+    out, lse = paged_attention(q, cache, table, lens, starts, causal=causal, return_lse=True)
+    for h in range(0, hk, 8):
+        part = type(cache)(*(t.view(torch.uint8)[:, h:h + 8].contiguous().view(t.dtype) for t in cache))
+        want, wlse, tol, ltol = attend(q[:, h:h + 8].contiguous(), part, table, lens, starts, causal=causal)
+        ref.check(out[:, h:h + 8], want, tol, "out")
+        ref.check(lse[:, h:h + 8], wlse, ltol, "lse")
+
+
 @pytest.mark.parametrize("n", [1, 3, 17, 100, 700])
 def test_equals_the_8_bit_cache_of_the_same_values(gpu, n):
     from low_bit_fake_quant import paged_attention
