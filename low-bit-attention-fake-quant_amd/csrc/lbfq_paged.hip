@@ -13,7 +13,7 @@
 // output as O^T = V^T P^T: a lane's scores are of one query, and P goes into the
 // second product from the registers that the first left it in.
 //
-// Two kernels.
+// Two kernels (for the cache in 8 bits; in 4 bits those of lbfq_paged4.hip and lbfq_paged4_chunk.hip).
 //
 // decode (up to 16 rows: one token of a sequence, 16x16x32 MFMA).  Bound by reading the cache, 2 D (1 + 1/32) bytes a key
 // and head.  A wave takes 32 keys at a time straight into registers; a workgroup's four waves take turns, workgroups

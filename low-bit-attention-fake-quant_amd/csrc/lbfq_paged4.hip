@@ -1,5 +1,5 @@
 // Attention of single tokens over the paged cache in 4 bits: the decode kernel for E2M1 codes (the mathematics and the
-// masks are lbfq_paged.hip's; its chunk kernel takes both widths).
+// masks are lbfq_paged.hip's, which also joins the parts; more rows go to lbfq_paged4_chunk.hip).
 //
 // Reading the cache is half of what it is in 8 bits, so what the arithmetic costs comes to the fore.  Scores are formed
 // from the codes as they lie in memory, by the block-scaled product (16x16x128, a lane's 16 bytes and its scale byte are
@@ -86,12 +86,12 @@ __device__ __forceinline__ uint32_t fetch(const lbfq_paged_params& p, const Page
     const uint8_t* k = p.k_codes + row * RB;
     copy16<0, true>(k, off);
     copy16<1024, true>(k, off);
-    if constexpr (D == 128) copy16<2048, true>(k, off), copy16<3072, true>(k, off);
+    if constexpr (D == 128) copy16<2 * 1024, true>(k, off), copy16<3 * 1024, true>(k, off);
     copy_to(lds + offsetof(X, v));
     const uint8_t* v = p.v_codes + row * RB;
     copy16<0, true>(v, off);
     copy16<1024, true>(v, off);
-    if constexpr (D == 128) copy16<2048, true>(v, off), copy16<3072, true>(v, off);
+    if constexpr (D == 128) copy16<2 * 1024, true>(v, off), copy16<3 * 1024, true>(v, off);
     const uint32_t so = D == 128 ? 4 * lane : 4 * (lane & 31);  // (D = 64: lanes 32 .. write what nobody reads)
     copy_to(lds + offsetof(X, ks));
     copy4<true>(p.k_scale + row * SB, so);

@@ -1,5 +1,5 @@
-// What the kernels of attention over the paged cache share: a sequence's extent and masks, conversions and products,
-// and the end of the two decode kernels.
+// What the kernels of attention over the paged cache share: a sequence's extent and masks, conversions and products, the
+// end of the two decode kernels, and copies into LDS and a query's terms for the cache in 4 bits.
 #pragma once
 
 #include <algorithm>
@@ -228,7 +228,6 @@ __device__ __forceinline__ v16f mfma32_f16(const uint4& a, const uint4& b, const
 
 // Whether a row's sum has anything in it (a NaN has: a row whose query holds one comes out as NaN, not as empty)
 __device__ __forceinline__ bool filled(float l) { return l != 0.0f; }
-
 
 // lse of a row (natural logarithm) from what its sum is relative to, in log2 units, and the sum
 __device__ __forceinline__ float row_lse(float m, float l) {
