@@ -299,11 +299,16 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
     // the sums so far); returns what p is relative to.
     auto settle = [&](int kb, uint32_t here, v16f& s0, v16f& s1) -> float {
       if (!(kb >= lo_all && kb + 64 <= hi_all && here == 0xfu)) {
+        // seen: from lo_r on, fewer than `span` keys (of a page that is not there: none); one compare, and no branches
+        const uint32_t at = static_cast<uint32_t>(kb + 8 * g - lo_r), span = hi_r > lo_r ? static_cast<uint32_t>(hi_r - lo_r) : 0u;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = kb + 16 * (r >> 3) + 8 * g + (r & 7);
-          if (key < lo_r || key >= hi_r || !((here >> (r >> 3)) & 1u)) s0[r] = -INFINITY;
-          if (key + 32 < lo_r || key + 32 >= hi_r || !((here >> (2 + (r >> 3))) & 1u)) s1[r] = -INFINITY;
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t n0 = here >> t & 1u ? span : 0u, n1 = here >> (t + 2) & 1u ? span : 0u;
+#pragma unroll
+          for (int i = 8 * t; i < 8 * t + 8; ++i) {
+            s0[i] = at + (8 * t + i) < n0 ? s0[i] : -INFINITY;
+            s1[i] = at + (8 * t + i + 32) < n1 ? s1[i] : -INFINITY;
+          }
         }
       }
       float mx = -INFINITY;
@@ -449,12 +454,14 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
         }
         __builtin_amdgcn_s_setprio(0);
         wait_for<0>();  // K of kt + 2, asked for a step ago
+        // (id is looked at before the next copies: the compiler does not count those, and its wait for id would be for them too)
+        const uint32_t mask = there(kt + 4, id);
+        const int next_page = page_in(id, mask, 0);
         copy_k(upto(kt + 3), pk, kf);
         load_v(upto(kt + 2), pn);
         pv = pn;
         pn = pk;
-        const uint32_t mask = there(kt + 4, id);
-        pk = page_in(id, mask, 0);
+        pk = next_page;
         here0 = here1;
         here1 = here2;
         here2 = here3;
