@@ -451,8 +451,9 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
             __builtin_amdgcn_sched_barrier(0);
           }
           keep(ke[bl]);
-          // (else the compiler moves these products to the next step, where their results are used)
-          asm volatile("" ::"v"(sn));
+          // (else the compiler moves these products to the next step, where their results are used; heads of 64 have too few
+          // registers for them here)
+          if constexpr (D == 128) asm volatile("" ::"v"(sn));
         }
         __builtin_amdgcn_s_setprio(0);
         wait_for<0>();  // K of kt + 2, asked for a step ago
