@@ -985,7 +985,7 @@ Plan plan(const lbfq_paged_params* p) {
     }
     // Two unequal parts (in 4 bits): row tiles that fill more than half of the chip, but not all of it, leave the last keys of
     // each to the places that are free, where they come one after the other (4680 tokens over 32760 keys, 12 heads, one part /
-    // two equal / these: 899 / 937 / 878 us; 3800 tokens 865 / 883 / 718).  Joining them takes a tile's time for 550000 values.
+    // two equal / these, by an earlier state of the kernel: 899 / 937 / 878 us, now 840; 3800 tokens 865 / 883 / 718).  Joining them takes a tile's time for 550000 values.
     const int64_t wgs = x.slots * p->Hk, all = 8 * places, o = 12 * 64;
     if (four && !uneven && limit >= 2 && wgs < all && 2 * wgs > all) {
       const int64_t turns = (wgs + all - wgs - 1) / (all - wgs);

@@ -9,9 +9,10 @@
 // span of them needs bf16.  V is converted as there, but staged as rows of keys, and turned by the reads that feed the
 // products (with 16 permutations a step instead, heads of 64 took 2.5% longer, of 128 the same).
 //
-// 8192 tokens over 32768 keys, 8 heads of 128, all seen: 965 us, 1.14 PFLOP/s, where a large library product reaches 1.24 (with
-// all codes zero 860: power).  4680 over 32760, 12 heads: 878 us, 1.07 PFLOP/s (in two equal parts 937, the 8-bit kernel
-// 1067).  200 VALU instructions a step, 32 of them exponentials, issue beside 32 products of 32 cycles.  Heads of 64: 0.88.
+// 8192 tokens over 32768 keys, 8 heads of 128, all seen: 930 to 980 us, 1.12 to 1.18 PFLOP/s, where a large library product
+// reaches 1.24 (with all codes zero 756: power).  4680 over 32760, 12 heads: 840 us, 1.12 PFLOP/s, the matrix units busy 55% of
+// the cycles at 2.0 GHz (the 8-bit kernel 1034).  200 VALU instructions a step besides 32 products of 32 cycles, 32 of them
+// exponentials.  Heads of 64, twice the exponentials per product: 0.92.
 #include "lbfq_paged_common.h"
 
 using namespace lbfq;
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
         // conversion of the staged V tile beside P V.  The order is fixed here; left to the
         // compiler, every read was next to its product.  The further a wave is in its products, the higher its priority:
         // the SIMD's other wave then gives way, and does its waits, masks and maxima when this one does not multiply (4680
-        // tokens over 32760 keys, 12 heads: 1028 us without, 947; products over the rest alone 954; two levels more, the same).
+        // tokens over 32760 keys, 12 heads: 888 us without, 840; one level instead of two 865).
         constexpr int HALF = NKS + 2 * NDB, kAhead = 5;
         const int id = look(kt + 4);  // back by the end of the step
         uint4 ring[kAhead], kx[NC];
@@ -451,8 +452,8 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
             __builtin_amdgcn_sched_barrier(0);
           }
           keep(ke[bl]);
-          // (else the compiler moves these products to the next step, where their results are used; heads of 64 have too few
-          // registers for them here)
+          // (else the compiler moves these products to the next step, where their results are used: 871 us instead of 840;
+          // heads of 64 have too few registers for them here, 48 us instead of 45 on 4 chunks of 509)
           if constexpr (D == 128) asm volatile("" ::"v"(sn));
         }
         __builtin_amdgcn_s_setprio(0);
