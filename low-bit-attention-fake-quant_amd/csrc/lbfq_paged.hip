@@ -938,10 +938,10 @@ constexpr int64_t kMostBytes = (int64_t{1} << 30) - 16;
 // 53* / 52 / 58 / 58 / 66).
 //
 // In 4 bits the last round is counted as what it takes where it does not fill the chip, 0.7 of a round up to half of it (us
-// for 1 / 2 / 3 / 4 / 5 / 6 / 7 / 8 parts, * the rule's: 4680 tokens, 32760 keys, 12 heads 995 / 949* / 975 / 994; 1560 tokens, 40
-// heads 1735 / 1375 / 1265 / 1224 / 1214* / 1198 / 1207 / 1210; 700 tokens, 8000 keys, 12 heads 173 / 102 / 81 / 73 / 67 / 62* / 89); and
-// parts of several sequences that come out at a little over whole rounds are made fewer (2 of 300 and 5000 112 / 75 / 66 / 58* /
-// 79 / 76; 8 of 128 and 4000 101 / 76* / 82 / 79; 4 of 700 and 9001, 12 heads 216 / 134 / 146 / 130 / 126* / 139).
+// for 1 / 2 / 3 / 4 / 5 / 6 / 7 / 8 parts, * the rule's: 1560 tokens, 32760 keys, 40 heads 1513 / 1237 / 1155 /
+// 1141 / 1110* / 1107 / 1106 / 1112; 700 tokens, 8000 keys, 12 heads 148 / 89 / 69 / 71 / 63 / 58* / 81; 5000, 5 heads, causal 100 / 73 /
+// 62* / 68); and parts of several sequences that come out at a little over whole rounds are made fewer (2 of 300 and 5000 97 /
+// 63 / 60 / 53* / 71 / 72; 8 of 128 and 4000 84 / 67* / 75 / 73; 4 of 700 and 9001, 12 heads 175 / 119 / 132 / 124 / 116* / 129).
 int64_t rounds10(int64_t n, int64_t places) {
   const int64_t whole = n / places, rest = n % places;
   if (rest == 0) return 10 * whole;
@@ -985,7 +985,7 @@ Plan plan(const lbfq_paged_params* p) {
     }
     // Two unequal parts (in 4 bits): row tiles that fill more than half of the chip, but not all of it, leave the last keys of
     // each to the places that are free, where they come one after the other (4680 tokens over 32760 keys, 12 heads, one part /
-    // two equal / these, by an earlier state of the kernel: 899 / 937 / 878 us, now 840; 3800 tokens 865 / 883 / 718).  Joining them takes a tile's time for 550000 values.
+    // two equal / these: 861 / 885 / 838 us; 3800 tokens 787 / 777 / 693).  Joining them takes a tile's time for 550000 values.
     const int64_t wgs = x.slots * p->Hk, all = 8 * places, o = 12 * 64;
     if (four && !uneven && limit >= 2 && wgs < all && 2 * wgs > all) {
       const int64_t turns = (wgs + all - wgs - 1) / (all - wgs);
