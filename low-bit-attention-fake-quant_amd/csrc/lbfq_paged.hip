@@ -151,6 +151,8 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[nb][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    int up = kUp;
+    bool large = false;  // some block's unit is below the bytes
 
     const int kt0 = lo / 32, nt = hi > lo ? (hi + 31) / 32 - kt0 : 0;
     int per = (nt + a.splits - 1) / a.splits;
@@ -202,6 +204,26 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
             }
           }
       }
+      // this lane's block's scales of its eight keys
+      int by[8], top = 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w;
+          if constexpr (D == 128) w = x.vs[t][i] >> (8 * (n >> 2));
+          else w = x.vs[t][i / 2] >> (16 * (i & 1) + 8 * (n >> 3));
+          by[4 * t + i] = static_cast<int>(w & 0xffu);
+          top = by[4 * t + i] > top ? by[4 * t + i] : top;
+        }
+      if (__any(top + up > kTop)) {
+        lower_unit<D>(top, up, acc);
+        large = __any(up < 0);
+      }
+      if (large) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) by[j] = by[j] > -up ? by[j] : -up;
+      }
       float mx = vmax(vmax(vmax(sc[0][0], sc[0][1]), vmax(sc[0][2], sc[0][3])),
                        vmax(vmax(sc[1][0], sc[1][1]), vmax(sc[1][2], sc[1][3])));
       mx = max_x32(max_x16(mx)) * a.sml2;
@@ -235,11 +257,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          uint32_t by;
-          if constexpr (D == 128) by = x.vs[t][i] >> (8 * (n >> 2));
-          else by = x.vs[t][i / 2] >> (16 * (i & 1) + 8 * (n >> 3));
-          // times 2^-kLess: a sum of 2^30 of the largest values is then in fp32's range
-          const float e = __uint_as_float(__builtin_elementwise_sub_sat(by & 0xffu, kLess) << 23);
+          const float e = __uint_as_float(static_cast<uint32_t>(by[4 * t + i] + up) << 23);
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
             vv[4 * t + i][2 * c] = cvt_bf16<8>(x.v[t][i], 2 * c, e);
@@ -257,7 +275,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(const Args a) {
         acc[nb] = mfma16_bf16(va, pc, acc[nb]);
       }
     }
-    join_waves<DT, D>(a, s, acc, m, l, join, r0, rows, split, kvh);
+    join_waves<DT, D>(a, s, acc, m, l, up, join, r0, rows, split, kvh);
     __syncthreads();  // the next rows use the same LDS
   }
 }
@@ -343,6 +361,8 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
     for (int r = 0; r < 16; ++r) acc[db][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;
   Unit uv{134, false}, uk{134, false};
+  uint32_t vtops = 0;  // V's unit: the byte that block b's scale vtops >> 8 b comes to is vtop
+  int vtop = 134;
   if (begin < end) {
     uint4 q[NKS];
     {
@@ -451,20 +471,26 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
         sk = span_join(sk, red[NW + w]);
       }
       __syncthreads();
-      auto unit = [&](uint32_t x, int wide) {
+      auto unit = [&](uint32_t x) {
         x = __builtin_amdgcn_readfirstlane(x);
         Unit u;
         u.E = static_cast<int>(x & 0xffu);
         u.wide = u.E - (255 - static_cast<int>(x >> 16)) > span_of(8);
-        if (u.wide) u.E = u.E > wide ? 134 + u.E - wide : 134;
         if (x == 0) u.E = 134;
         return u;
       };
-      uv = unit(sv, kWideTop);
-      if constexpr (DT == kF16) uk = unit(sk, 255);
+      uv = unit(sv);
+      if constexpr (DT == kF16) {
+        uk = unit(sk);
+        if (uk.wide) uk.E = 134;
+      }
+      vtops = uv.wide ? block_tops<D, NT>(p, table, kvh, lo > 64 * begin ? lo : 64 * begin, k1, red) : uv.E * 0x01010101u;
+      if (uv.wide) vtop = wide_top(64 * (end - begin));
     }
     const float c = DT == kF16 ? ldexpf(a.sml2, uk.E - 134) : a.sml2;
-    const uint32_t kadd = static_cast<uint32_t>(134 - uk.E) << 23, vadd = static_cast<uint32_t>(134 - uv.E) << 23;
+    const uint32_t kadd = static_cast<uint32_t>(134 - uk.E) << 23;
+    // (wide: of this thread's block of columns)
+    const int vup = uv.wide ? vtop - static_cast<int>(vtops >> 8 * (vdq / 8) & 0xffu) : 134 - uv.E;
 
     // Keys that no row sees, or that are not there: nothing of them may reach a product.
     auto clear_k = [&](KRegs& x, int kt, int page) {
@@ -479,13 +505,12 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
     auto clear_v = [&](int kt, int page) {
       const int key0 = 64 * kt + WKEYS * wave;
       if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
-      const uint32_t fill = static_cast<uint32_t>(uv.E) * 0x01010101u;
 #pragma unroll
       for (int j = 0; j < VK; ++j)
         if (const int key = key0 + VK * vkg + j; page < 0 || key < lo || key >= hi) {
           vc[j] = 0;
-          if constexpr (CH == 4) vse[j] = fill;
-          else vse[j / 2] = (vse[j / 2] & (j & 1 ? 0x0000ffffu : 0xffff0000u)) | (fill & (j & 1 ? 0xffff0000u : 0xffffu));
+          if constexpr (CH == 4) vse[j] = vtops;
+          else vse[j / 2] = (vse[j / 2] & (j & 1 ? 0x0000ffffu : 0xffff0000u)) | (vtops & (j & 1 ? 0xffff0000u : 0xffffu));
         }
     };
     // Registers -> LDS, as fp16 in the part's unit or (WIDE, and K for bf16 queries) as bf16; in eight pieces each.
@@ -509,8 +534,8 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
           uint32_t by;
           if constexpr (CH == 4) by = __builtin_amdgcn_ubfe(vse[j], 8 * (vdq / 8), 8);
           else by = __builtin_amdgcn_ubfe(vse[j / 2], 16 * (j & 1) + 8 * (vdq / 8), 8);
-          // (WIDE: far below the largest, a scale may be less than what is taken off)
-          const float sc = __uint_as_float(WIDE ? __builtin_elementwise_sub_sat(by << 23, 0u - vadd) : (by << 23) + vadd);
+          const int e = static_cast<int>(by) + vup;
+          const float sc = __uint_as_float(static_cast<uint32_t>(WIDE && e < 0 ? 0 : e) << 23);
           st.v[j][0] = WIDE ? cvt_bf16<8>(vc + j, 0, sc) : cvt_f16<8>(vc + j, 0, sc);
           st.v[j][1] = WIDE ? cvt_bf16<8>(vc + j, 1, sc) : cvt_f16<8>(vc + j, 1, sc);
         }
@@ -761,7 +786,7 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
   if (rw + li < rows) {
     const int64_t tok = s.start + qi;
     const bool one = a.splits == 1;
-    const float f = filled(l) ? ldexpf(1.0f, uv.E - 134) / l : 0.0f;
+    const float f = filled(l) ? 1.0f / l : 0.0f;
     const int64_t at = split * R + tok * p.Hq + h;
     if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
     if (!one && g == 0) a.ml[at] = make_float2(m, l);
@@ -770,13 +795,13 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
       // the columns 32 i + 16 g + 4 k + c.  D = 128: c = db, r = 4 i + k; D = 64: c = 2 db + r / 8, r % 8 = 4 i + k.
 #pragma unroll
       for (int i = 0; i < NDB; ++i) {
-        const int col = 32 * i + 16 * g;
+        const int col = 32 * i + 16 * g, e = static_cast<int>(vtops >> 8 * i & 0xffu) - vtop;
         float o[16];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int cc = 0; cc < 4; ++cc)
-            o[4 * k + cc] = (D == 128 ? acc[cc % NDB][4 * i + k] : acc[cc / 2][8 * (cc & 1) + 4 * (i & 1) + k]) * f;
+            o[4 * k + cc] = ldexpf((D == 128 ? acc[cc % NDB][4 * i + k] : acc[cc / 2][8 * (cc & 1) + 4 * (i & 1) + k]) * f, e);
         if (one) {
           uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col);
           dst[0] = make_uint4(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]), pack_dt<DT>(o[4], o[5]),

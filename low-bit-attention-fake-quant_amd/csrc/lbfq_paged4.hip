@@ -242,6 +242,8 @@ __global__ void __launch_bounds__(256, 2) paged_decode4_kernel(const Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[nb][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    int up = kUp;
+    bool large = false;  // some block's unit is below the bytes
     if (begin + wave < end) {
       Pages pages;
       load_pages(p, table, kKeys * (begin + wave), pages);
@@ -313,6 +315,21 @@ __global__ void __launch_bounds__(256, 2) paged_decode4_kernel(const Args a) {
               if (!(here >> t & 1u) || key < lo || key >= hi) vs[t][i] = 127;
             }
         }
+        int top = static_cast<int>(vs[0][0]);
+#pragma unroll
+        for (int t = 0; t < kT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = static_cast<int>(vs[t][i]) > top ? static_cast<int>(vs[t][i]) : top;
+        if (__any(top + up > kTop)) {
+          lower_unit<D>(top, up, acc);
+          large = __any(up < 0);
+        }
+        if (large) {
+#pragma unroll
+          for (int t = 0; t < kT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vs[t][i] = static_cast<int>(vs[t][i]) > -up ? vs[t][i] : static_cast<uint32_t>(-up);
+        }
         float mx = vmax(vmax(sc[0][0], sc[0][1]), vmax(sc[0][2], sc[0][3]));
 #pragma unroll
         for (int t = 1; t < kT; ++t) mx = vmax(vmax(mx, vmax(sc[t][0], sc[t][1])), vmax(sc[t][2], sc[t][3]));
@@ -348,9 +365,7 @@ __global__ void __launch_bounds__(256, 2) paged_decode4_kernel(const Args a) {
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              e[4 * t + i] = __uint_as_float(__builtin_elementwise_sub_sat(vs[u + t][i], kLess) << 23);
-            }
+            for (int i = 0; i < 4; ++i) e[4 * t + i] = __uint_as_float((vs[u + t][i] + up) << 23);
 #pragma unroll
           for (int c = 0; c < NB / 2; ++c) {  // two columns of a lane
             uint32_t vv[8];
@@ -373,7 +388,7 @@ __global__ void __launch_bounds__(256, 2) paged_decode4_kernel(const Args a) {
       }
     }
     __syncthreads();  // (the ring's place)
-    join_waves<DT, D>(a, s, acc, m, l, lds.join, r0, rows, split, kvh);
+    join_waves<DT, D>(a, s, acc, m, l, up, lds.join, r0, rows, split, kvh);
     __syncthreads();  // the next rows use the same LDS
   }
 }

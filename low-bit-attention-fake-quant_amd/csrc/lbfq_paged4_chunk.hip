@@ -133,6 +133,8 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
     for (int r = 0; r < 16; ++r) acc[db][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;
   Unit uv{kUnit, false};
+  uint32_t vtops = 0;  // V's unit: the byte that block b's scale vtops >> 8 b comes to is vtop
+  int vtop = kUnit;
   if (begin < end) {
     auto upto = [&](int kt) { return kt < end ? kt : end - 1; };  // steps past the end repeat it, unused
     // Page ids of the tiles from kt on: lane 4 i + w has that of tile kt + i's keys 16 w .., which wave w stages.  One load,
@@ -225,23 +227,24 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
       sv = __builtin_amdgcn_readfirstlane(sv);
       uv.E = static_cast<int>(sv & 0xffu);
       uv.wide = uv.E - (255 - static_cast<int>(sv >> 16)) > span_of(4);
-      if (uv.wide) uv.E = uv.E > kWideTop ? kUnit + uv.E - kWideTop : kUnit;
       if (sv == 0) uv.E = kUnit;
+      vtops = uv.wide ? block_tops<D, NT>(p, table, kvh, lo > 64 * begin ? lo : 64 * begin, k1, red) : uv.E * 0x01010101u;
+      if (uv.wide) vtop = wide_top(64 * (end - begin));
     }
     const float c = a.sml2;
-    const uint32_t vadd = static_cast<uint32_t>(kUnit - uv.E) << 23;
+    // (wide: of this thread's block of columns)
+    const int vup = uv.wide ? vtop - static_cast<int>(vtops >> 8 * (vdq / 4) & 0xffu) : kUnit - uv.E;
 
     // Keys that no row sees, or that are not there: their scales may be anything (their codes are finite as they are, and
     // what K has there ends in scores that are masked).
     auto clear_v = [&](int kt, int page) {
       const int key0 = 64 * kt + WKEYS * wave;
       if (page >= 0 && key0 >= lo && key0 + WKEYS <= hi) return;
-      const uint32_t fill = static_cast<uint32_t>(uv.E) * 0x01010101u;
 #pragma unroll
       for (int j = 0; j < VK; ++j)
         if (const int key = key0 + VK * vkg + j; page < 0 || key < lo || key >= hi) {
-          if constexpr (CH == 4) vse[j] = fill;
-          else vse[0] = (vse[0] & (j & 1 ? 0x0000ffffu : 0xffff0000u)) | (fill & (j & 1 ? 0xffff0000u : 0xffffu));
+          if constexpr (CH == 4) vse[j] = vtops;
+          else vse[0] = (vse[0] & (j & 1 ? 0x0000ffffu : 0xffff0000u)) | (vtops & (j & 1 ? 0xffff0000u : 0xffffu));
         }
     };
     // V's key i of this thread's VK: registers -> LDS, as fp16 in the part's unit or (WIDE) as bf16
@@ -249,8 +252,8 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
       uint32_t by;
       if constexpr (CH == 4) by = __builtin_amdgcn_ubfe(vse[i], 8 * (vdq / 4), 8);
       else by = __builtin_amdgcn_ubfe(vse[0], 16 * i + 8 * (vdq / 4), 8);
-      // (WIDE: far below the largest, a scale may be less than what is taken off)
-      const float sc = __uint_as_float(WIDE ? __builtin_elementwise_sub_sat(by << 23, 0u - vadd) : (by << 23) + vadd);
+      const int e = static_cast<int>(by) + vup;
+      const float sc = __uint_as_float(static_cast<uint32_t>(WIDE && e < 0 ? 0 : e) << 23);
       uint32_t w[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) w[k] = WIDE ? cvt_bf16<4>(vc + i, k, sc) : cvt_f16<4>(vc + i, k, sc);
@@ -496,26 +499,28 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
   if (rw + li < rows) {
     const int64_t tok = s.start + qi;
     const bool one = a.splits == 1;
-    const float f = filled(l) ? ldexpf(1.0f, uv.E - kUnit) / l : 0.0f;
+    const float f = filled(l) ? 1.0f / l : 0.0f;
     const int64_t at = split * R + tok * p.Hq + h;
     if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
     if (!one && g == 0) a.ml[at] = make_float2(m, l);
     if (one || filled(l)) {
       // Register r of acc[db] is column 32 db + 8 (r / 4) + 4 g + r % 4.
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
+      for (int db = 0; db < NDB; ++db) {
+        const int e = static_cast<int>(vtops >> 8 * db & 0xffu) - vtop;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int col = 32 * db + 8 * k + 4 * g;
           float o[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = acc[db][4 * k + i] * f;
+          for (int i = 0; i < 4; ++i) o[i] = ldexpf(acc[db][4 * k + i] * f, e);
           if (one)
             *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col) =
                 make_uint2(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]));
           else
             *reinterpret_cast<float4*>(a.acc + at * D + col) = make_float4(o[0], o[1], o[2], o[3]);
         }
+      }
     }
   }
 }

@@ -234,9 +234,11 @@ __device__ __forceinline__ float row_lse(float m, float l) {
   return filled(l) ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
 
-// What the decode kernels take off the scales of V, or of P, in powers of two: a sum of 2^30 of the largest values is then
-// in fp32's range
-constexpr uint32_t kLess = 32;
+// The unit of V's sums in the decode kernels, for each block of 32 columns: scale bytes (E8M0) are taken up by `up`, so that
+// sums over small values keep fp32's precision down to 2^-127.  A byte may come out at kTop: 2^30 values of 448 2^(kTop - 127)
+// add up to less than 2^127.  kUp does for scales of up to 2^32; where a block's are larger, the unit follows the largest so
+// far, as a row's maximum does, and bytes that would be negative (2^-kTop of the largest) count as 0.
+constexpr int kTop = 215, kUp = 56;
 
 constexpr int kDecodeRows = 16;
 
@@ -244,13 +246,38 @@ template <int D>
 struct alignas(16) DecodeLds {
   float acc[4][kDecodeRows][D + 4];
   float m[4][kDecodeRows], l[4][kDecodeRows];
+  int up[4][D / 32];
 };
+
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }  // e: -126 .. 127
+
+// The unit brought down for scale bytes of up to `top`.  Lane (n, g) has up and top for V's columns (D/16) n .., and rows
+// 4 g + i of acc, which are columns (D/16) (4 g + i) + nb.
+template <int D>
+__device__ __forceinline__ void lower_unit(int top, int& up, v4f (&acc)[D / 16]) {
+  constexpr int NB = D / 16, PER = 16 / (D / 32);  // lanes n of a block
+  const int g = (threadIdx.x & 63) >> 4;
+  int now = kTop - top < up ? kTop - top : up;
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) {
+    if (i >= PER && i < 16) continue;
+    const int o = __shfl_xor(now, i, 64);
+    now = o < now ? o : now;
+  }
+  const int from = PER * (g * (D / 32) / 4);  // a lane that has the block of these rows of acc
+  const float f = two_to(__shfl(now, from, 64) - __shfl(up, from, 64));
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[nb][i] *= f;
+  up = now;
+}
 
 // The four waves' rows r0 .. of one part joined by their maxima: into the output, or the part's place of the workspace.
 // Lane (n, g): row n's maximum m, its own share l of the sum, and columns (D/16) (4 g + i) + nb of the average times the
-// sum and 2^-kLess.
+// sum and 2^up (its lanes' up: lower_unit).
 template <int DT, int D>
-__device__ __forceinline__ void join_waves(const Args& a, const Seq& s, const v4f (&acc)[D / 16], float m, float l,
+__device__ __forceinline__ void join_waves(const Args& a, const Seq& s, v4f (&acc)[D / 16], float m, float l, int up,
                                            DecodeLds<D>& x, int r0, int rows, int split, int kvh) {
   constexpr int NB = D / 16, NW = 4;
   const lbfq_paged_params& p = a.p;
@@ -261,8 +288,24 @@ __device__ __forceinline__ void join_waves(const Args& a, const Seq& s, const v4
   if (g == 0) {
     x.m[wave][n] = m;
     x.l[wave][n] = l;
+    if (n % (16 / (D / 32)) == 0) x.up[wave][n / (16 / (D / 32))] = up;
   }
   __syncthreads();
+  auto unit = [&](int block) {  // the least of the waves'
+    int u = x.up[0][block];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) u = x.up[w][block] < u ? x.up[w][block] : u;
+    return u;
+  };
+  {
+    const int block = g * (D / 32) / 4, less = unit(block) - x.up[wave][block];
+    if (__any(less != 0)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[nb][i] *= two_to(less);
+    }
+  }
   float M = -INFINITY;
 #pragma unroll
   for (int w = 0; w < NW; ++w) M = vmax(M, x.m[w][n]);
@@ -296,7 +339,7 @@ __device__ __forceinline__ void join_waves(const Args& a, const Seq& s, const v4
       }
       const int qq = (r0 + row) / G, hh = kvh * G + (r0 + row - qq * G);
       const int64_t tok = s.start + qq;
-      const float inv = filled(L) ? static_cast<float>(uint64_t{1} << kLess) / L : 0.0f;
+      const float inv = filled(L) ? two_to(-unit(part * NB / 32)) / L : 0.0f;
       if (a.splits == 1) {
         uint32_t w[NB / 2];
 #pragma unroll
@@ -344,17 +387,55 @@ __device__ __forceinline__ uint32_t span_add(uint32_t span, uint32_t v) {
 // code lands at 57344.  The smallest one, 2^-9, with a scale 2^-22 of the largest is then fp16's smallest step: within
 // that span every value is exact.  A part whose scales are further apart is `wide`: bf16, as they are.
 //
-// (A wide part's V is taken down by a power of two where its largest scale is past kWideTop: weights of up to 2^15 times
-// 2^30 of the largest values that are left, under 2^(kWideTop - 118), add up to less than 2^127.)
+// A wide part's V is taken to where each block's (of 32 columns) largest scale byte is wide_top: weights of up to 2^15 times
+// the part's `keys` (a power of two above them) values of up to 2^(wide_top - 118) add up to less than 2^127.  Scales 2^-wide_top
+// of the largest count as that.
 //
 // E2M1's largest code, 6, lands at 49152 with 2^(140 - E), and its smallest, 1/2, stays exact 36 powers of two below.
 constexpr int span_of(int bits) { return bits == 8 ? 22 : 36; }
 constexpr int unit_of(int bits) { return bits == 8 ? 134 : 140; }
-constexpr int kWideTop = 200;
+__device__ __forceinline__ int wide_top(int keys) { return 198 + __builtin_clz(keys); }  // 2^30 keys: 200
 struct Unit {
   int E;
   bool wide;
 };
+
+// Each block's largest scale byte of V over keys k0 .. k1 - 1 of a sequence (pages that are not there left out), for all of a
+// workgroup's threads: byte b is that of block b (D = 64: of block b & 1).  red: a word for each wave and half.
+template <int D, int NT>
+__device__ __forceinline__ uint32_t block_tops(const lbfq_paged_params& p, const int32_t* table, int kvh, int k0, int k1,
+                                               uint32_t* red) {
+  const int cols = static_cast<int>(p.table_cols);
+  uint32_t even = 0, odd = 0;
+  for (int key = k0 + static_cast<int>(threadIdx.x); key < k1; key += NT) {
+    const int idx = key >> p.page_shift, page = idx < cols ? table[idx] : -1;
+    if (page < 0 || page >= p.num_pages) continue;
+    const int64_t row = ((page * p.Hk + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+    uint32_t w;
+    load_bytes<D / 32>(p.v_scale + row * (D / 32), &w);
+    even = span_join(even, w & 0x00ff00ffu);
+    odd = span_join(odd, w >> 8 & 0x00ff00ffu);
+  }
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) {
+    even = span_join(even, __shfl_xor(even, i, 64));
+    odd = span_join(odd, __shfl_xor(odd, i, 64));
+  }
+  constexpr int NW = NT / 64;
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = even;
+    red[NW + (threadIdx.x >> 6)] = odd;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    even = span_join(even, red[w]);
+    odd = span_join(odd, red[NW + w]);
+  }
+  __syncthreads();
+  const uint32_t tops = __builtin_amdgcn_readfirstlane(even | odd << 8);
+  return D == 128 ? tops : (tops & 0xffffu) * 0x10001u;
+}
 
 // Workgroups of a CU: three where the registers do for that, at the price of a few that go to memory (1560 tokens over 32760
 // keys, 40 heads of 64, bf16: 818 us with two, 765 with three; fp16 queries need more of them: 745 with two, 1075).
