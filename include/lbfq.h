@@ -445,7 +445,9 @@ int lbfq_qk_norm_rope_bwd(const lbfq_qk_norm_params* p, const lbfq_qk_norm_grads
  * scales at most 2^119 (infinities are held as 448 * 2^119).  bits = 4 in the
  * parameters below (0 and 8 are E4M3): codes (num_pages, H, page, D / 2), two E2M1
  * values a byte, the even column in the low half; the scale is 2^ceil(log2(max(amax,
- * 1e-4) / 6)), at most 2^125.
+ * 1e-4) / 6)), at most 2^125.  (bits lies where the parameters of write, read and
+ * attention had padding: callers of those from before it need no rebuild if they clear
+ * the whole struct first, as all should.)
  * write: rows k[t], v[t] (fp32, fp16 or bf16) to slot slots[t] = page id * page
  * + row; a slot outside the cache is skipped; slots must differ. */
 typedef struct {
@@ -521,8 +523,8 @@ typedef struct {
   void* out; int64_t out_t, out_h;
   float* lse;                              /* or NULL                           */
   int fill_rest;
-  void* workspace; int64_t workspace_bytes;
   int bits;
+  void* workspace; int64_t workspace_bytes;
 } lbfq_paged_params;
 
 int64_t lbfq_paged_attention_workspace_bytes(const lbfq_paged_params* p);

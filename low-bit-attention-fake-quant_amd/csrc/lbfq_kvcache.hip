@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const lbfq_kv_read_params 
   }
 }
 
-// bits of a code: 4, or 8 (also as 0, what a struct of before has there)
+// bits of a code: 4, or 8 (also as 0, what a cleared struct of before has in that place, its padding)
 bool four(int bits) { return bits == 4; }
 
 int check_cache(const char* who, int bits, int64_t num_pages, int page_shift, int64_t H, int64_t D, const void* kc,

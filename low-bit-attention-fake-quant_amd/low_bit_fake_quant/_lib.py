@@ -228,8 +228,8 @@ class PagedParams(ctypes.Structure):
         ("out", _vp), ("out_t", _i64), ("out_h", _i64),
         ("lse", _vp),
         ("fill_rest", _i32),
-        ("workspace", _vp), ("workspace_bytes", _i64),
         ("bits", _i32),
+        ("workspace", _vp), ("workspace_bytes", _i64),
     ]
 
 
