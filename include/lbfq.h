@@ -528,6 +528,9 @@ typedef struct {
 } lbfq_paged_params;
 
 int64_t lbfq_paged_attention_workspace_bytes(const lbfq_paged_params* p);
+/* How many parts that call cuts the keys into (0: invalid parameters).  *share (or NULL):
+ * of 65536, what the first of two unequal parts has; 0 where parts are equal. */
+int lbfq_paged_attention_parts(const lbfq_paged_params* p, int* share);
 int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t stream);
 
 /* ---- measurement probe ----------------------------------------------------- */

@@ -1083,6 +1083,14 @@ extern "C" int64_t lbfq_paged_attention_workspace_bytes(const lbfq_paged_params*
   return workspace(p, plan(p));
 }
 
+extern "C" int lbfq_paged_attention_parts(const lbfq_paged_params* p, int* share) {
+  if (share) *share = 0;
+  if (check_sizes(p)) return 0;
+  const Plan x = plan(p);
+  if (share) *share = static_cast<int>(x.share);
+  return x.splits;
+}
+
 extern "C" int lbfq_paged_attention(const lbfq_paged_params* p, lbfq_stream_t stream) {
   if (int rc = check(p)) return rc;
   const Plan x = plan(p);

@@ -275,6 +275,7 @@ _SIGS = {
     "lbfq_kv_append": (_i32, [ctypes.POINTER(KvAppendParams), _vp]),
     "lbfq_kv_read": (_i32, [ctypes.POINTER(KvReadParams), _vp]),
     "lbfq_paged_attention_workspace_bytes": (_i64, [ctypes.POINTER(PagedParams)]),
+    "lbfq_paged_attention_parts": (_i32, [ctypes.POINTER(PagedParams), ctypes.POINTER(_i32)]),
     "lbfq_paged_attention": (_i32, [ctypes.POINTER(PagedParams), _vp]),
     "lbfq_hbm_stream": (_i32, [_i32, _vp, _vp, _i64, _i32, _vp, _vp]),
     "lbfq_issue_probe": (_i32, [_i32, _i32, _i32, _vp, _vp, _vp]),
