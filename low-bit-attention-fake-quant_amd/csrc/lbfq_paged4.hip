@@ -143,8 +143,10 @@ __device__ __forceinline__ uint32_t fetch(const lbfq_paged_params& p, const Page
     } else {  // a copy reaches over two pieces
 #pragma unroll
       for (int t = 0; t < kT; t += 2) {
+        // (two scalars: an array's place that goes by the lane lies in scratch memory, and each wait for that is one for all copies)
+        const int64_t r0 = row[t], r1 = row[t + 1];
         copy_to(to + 512 * t);
-        copy16v(base + (lane & 32 ? row[t + 1] : row[t]) * RB + (off & 511));
+        copy16v(base + (lane & 32 ? r1 : r0) * RB + (off & 511));
       }
     }
   }
