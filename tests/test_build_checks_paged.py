@@ -1,4 +1,5 @@
-"""The 4-bit cache's attention kernels, as built: none keeps anything in scratch memory, and both units were looked at."""
+"""The 4-bit cache's attention kernels, as built: none keeps anything in scratch memory or converts 32 values over its own
+operands, and both units were looked at."""
 
 import os
 
@@ -25,3 +26,12 @@ def test_no_scratch_memory(unit):
         text = f.read()
     assert text.count("; -- End function") >= 4  # bf16 and fp16, heads of 64 and 128
     assert mfma_check.scratch_kernels(text, "paged") == []
+
+
+@needs_build
+@pytest.mark.skipif(not mfma_check.tools_available(), reason="no LLVM tools")
+@pytest.mark.parametrize("unit", UNITS)
+def test_conversions_do_not_lie_over_their_operands(unit):
+    assert unit in BUILT, f"{unit} is not in the build directory"
+    asm = mfma_check.disassemble(BUILT[unit])
+    assert "v_cvt_scalef32_2xpk16" in asm and mfma_check.wide_conversion_overlaps(asm) == []
