@@ -946,7 +946,10 @@ constexpr int64_t kMostBytes = (int64_t{1} << 30) - 16;
 // 3 / 4 / 6 / 8 / 16 / 32 parts, * the rule's, 8 key heads of 128: one sequence of 700 keys 9.5* / 12.8 / 11.1 / 10.9 / 11.0 /
 // 10.8; 5003 31 / 21 / 18 / 15 / 14 / 13 / 11.8* / 12.1; 40000 197 / 105 / 74 / 58 / 42 / 34 / 22 / 18.8*; 24 of 2000 to 4000
 // 25.8* / 28.0 / 27.6 / 28.5 / 29.6; 48 of 8000 to 16000 152 / 134 / 127 / 121* / 124 / 127; 8 of 4000 to 8000, 40 heads 53.6*
-// / 59.6 / 56.0 / 55.7 / 57.1 / 61.7; 12 of 1000 to 16000, 12 heads 79 / 54 / 50 / 46* / 47 / 44 / 50).
+// / 59.6 / 56.0 / 55.7 / 57.1 / 61.7; 12 of 1000 to 16000, 12 heads 79 / 54 / 50 / 46* / 47 / 44 / 50).  Evening out takes
+// workgroups for at most six rounds of 512 places: where the sequences alone come to three rounds or more, it mostly costs (8
+// key heads, 6016 to 12032 keys, 1 / 2 / 3 / 4 parts: 96 sequences 182 / 169 / 168* / 174; 128 226 / 225 / 229* / 230; 192 330 /
+// 335* / 343 / 355; 256 420* / 429 / 447 / 457; 512 815* / 854 / 877 / 915; 512 of 750 to 12032 576* / 627 / 668 / 682).
 // chunk, one sequence: the parts that take the least time by a count of tiles.  A part costs the time of 12 tiles besides
 // its own (its start, and its sums written and read again), and an XCD has two or three workgroups a CU at a time.  Row
 // tiles that see much the same keys go in whole rounds (us for 1 / 2 / 4 / 6 / 7 parts, * the rule's: 1560 tokens, 32760
@@ -994,7 +997,7 @@ Plan plan(const lbfq_paged_params* p) {
   int64_t s = 1;
   if (x.decode && four) {
     if (keys >= 1100) s = std::min(256 / (p->B * p->Hk), keys / 300);
-    if (p->B > 1 && keys >= 12000) s = std::max(s, keys / 4000);
+    if (p->B > 1 && keys >= 12000) s = std::max(s, std::min(keys / 4000, 6 * 512 / (p->B * p->Hk)));
   } else if (x.decode) {
     const int64_t wgs = p->B * p->Hk;
     s = (768 + wgs / 2) / wgs;
