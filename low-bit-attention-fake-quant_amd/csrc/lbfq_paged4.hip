@@ -7,7 +7,8 @@
 // (whose products span more powers of two than its sums keep: errors of 3e-6 of a score), it adds up theirs exactly to
 // fp32's precision.  So a query goes in as four E2M3 terms with scales 2^-5 apart, relative to the largest of its 32
 // columns: bf16's eight bits are exact down to 2^-11 of that, fp16's eleven to 2^-8, and what is left is below 2^-19 of
-// it.  Four products of 16 cycles take the time of bf16's four, without converting K.
+// it.  Four products of 16 cycles take the time of bf16's four, without converting K.  (Queries whose columns lie so far apart
+// that this would be less than bf16 itself holds of them take four more: split_query.)
 //
 // V's scales change from key to key, along the sum, so V is converted to bf16 (exact).  P is two bf16 terms.
 //
@@ -168,9 +169,9 @@ struct Query {
   uint32_t e;
 };
 
-template <int DT, int D>
-__device__ __forceinline__ Query<D> query(const uint16_t* q, int g) {
-  const Terms s = split_query<DT>(q);
+template <int DT, int D, bool REST = false>
+__device__ __forceinline__ Query<D> query(const uint16_t* q, int g, bool* more = nullptr) {
+  const Terms s = split_query<DT, REST>(q, more);
   Query<D> x;
   if constexpr (D == 128) {
 #pragma unroll
@@ -203,8 +204,23 @@ __device__ __forceinline__ void products(const uint4 (&k)[kT], uint32_t ke, cons
   if constexpr (I + 1 < Query<D>::N) products<I + 1, D>(k, ke, q, sc);
 }
 
+// The same with the operands in LDS, one after the other
+template <int I, int D>
+__device__ __forceinline__ void products_of(const uint4 (&k)[kT], uint32_t ke, const uint32_t (*x)[64], int lane, v4f (&sc)[kT]) {
+  u32x6 w;
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = x[6 * I + i][lane];
+  const uint32_t e = x[6 * Query<D>::N][lane];
+  sc[0] = product<0, I>(k[0], ke, w, e, sc[0]);
+  sc[1] = product<1, I>(k[1], ke, w, e, sc[1]);
+  sc[2] = product<2, I>(k[2], ke, w, e, sc[2]);
+  sc[3] = product<3, I>(k[3], ke, w, e, sc[3]);
+  asm volatile("" ::"v"(e) : "memory");
+  if constexpr (I + 1 < Query<D>::N) products_of<I + 1, D>(k, ke, x, lane, sc);
+}
+
 template <int DT, int D>
-__global__ void __launch_bounds__(256, 2) paged_decode4_kernel(const Args a) {
+__global__ void __launch_bounds__(256, decode4_groups(D)) paged_decode4_kernel(const Args a) {
   constexpr int NB = D / 16, NW = 4;
   const lbfq_paged_params& p = a.p;
   if (static_cast<int64_t>(blockIdx.x) >= a.main) {
@@ -215,6 +231,7 @@ __global__ void __launch_bounds__(256, 2) paged_decode4_kernel(const Args a) {
     Ring<D> ring;
     DecodeLds<D> join;
   } lds;
+  __shared__ uint32_t rest_lds[Query<D>::N * 6 + 1][64];  // each lane's four more terms, where a query takes them
   const uint32_t Hk = static_cast<uint32_t>(p.Hk);
   const int split = static_cast<int>(blockIdx.x / a.combos);
   const uint32_t rest = blockIdx.x % a.combos;
@@ -249,8 +266,19 @@ __global__ void __launch_bounds__(256, 2) paged_decode4_kernel(const Args a) {
     if (begin + wave < end) {
       Pages pages;
       load_pages(p, table, kKeys * (begin + wave), pages);
-      const Query<D> q = query<DT, D>(  // (while the page ids are on their way)
-          reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 32 * (D == 128 ? g : g & 1), g);
+      const uint16_t* const qr =
+          reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 32 * (D == 128 ? g : g & 1);
+      bool more;
+      const Query<D> q = query<DT, D>(qr, g, &more);  // (while the page ids are on their way)
+      more = __any(more);
+      if (more) {  // (the same from all four waves)
+        const Query<D> rest = query<DT, D, true>(qr, g);
+#pragma unroll
+        for (int i = 0; i < Query<D>::N; ++i)
+#pragma unroll
+          for (int k = 0; k < 6; ++k) rest_lds[6 * i + k][lane] = rest.w[i][k];
+        rest_lds[6 * Query<D>::N][lane] = rest.e;
+      }
       const int lr = lane / (D / 32);  // this lane's row and place of it in a copy
       const uint32_t off = D / 2 * lr + 16 * piece_of<D>(lr & 15, lane & (D / 32 - 1));
       const uint32_t ring = lds_addr(&lds.ring.t[wave][0]);
@@ -306,6 +334,9 @@ __global__ void __launch_bounds__(256, 2) paged_decode4_kernel(const Args a) {
 #pragma unroll
         for (int t = 0; t < kT; ++t) sc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         products<0, D>(k, ke, q, sc);
+        if (more) {
+          products_of<0, D>(k, ke, rest_lds, lane, sc);
+        }
         if (!(kb >= lo_all && kb + kKeys <= hi_all && here == 15u)) {
 #pragma unroll
           for (int t = 0; t < kT; ++t)

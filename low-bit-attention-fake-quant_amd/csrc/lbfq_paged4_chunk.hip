@@ -6,7 +6,8 @@
 // multiplied by the query's four E2M3 terms with the block-scaled product (32x32x64; see lbfq_paged4.hip): as many
 // cycles as bf16's, but a quarter of the LDS reads, and no conversion.  (At 16 bits, a step's reads take as long as its
 // products: 32 KiB for 16 + 16 of 32 cycles, four waves and two workgroups a CU.)  K's scales go into the product, so no
-// span of them needs bf16.  V is converted as there, but staged as rows of keys, and turned by the reads that feed the
+// span of them needs bf16.  (Queries that take eight terms, as parts whose V scales lie far apart, go through a plain loop.)
+// P is one fp16 term, 11 bits, as in the 8-bit kernel: a second would be half as many products again.  V is converted as there, but staged as rows of keys, and turned by the reads that feed the
 // products (with 16 permutations a step instead, heads of 64 took 2.5% longer, of 128 the same).
 //
 // 8192 tokens over 32768 keys, 8 heads of 128, all seen: 930 to 980 us, 1.12 to 1.18 PFLOP/s, where a large library product
@@ -179,10 +180,18 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
     copy_k(upto(begin + 1), page1, 1);
     copy_k(upto(begin + 2), page_in(ids, mask, 2), 2);
     load_v(begin, page0);
+    auto columns = [&](int row, int i) {  // this lane's 32 of step i
+      const int query = row / G, head = kvh * G + (row - query * G);
+      return reinterpret_cast<const uint16_t*>(p.q) + (s.start + query) * p.q_t + head * p.q_h + 64 * i + 32 * g;
+    };
     Terms q[NC];
+    bool more = false;
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      q[i] = split_query<DT>(reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 64 * i + 32 * g);
+    for (int i = 0; i < NC; ++i) {
+      bool x;
+      q[i] = split_query<DT>(reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 64 * i + 32 * g, &x);
+      more |= x;
+    }
     // The span of the part's V scales, over the keys that some row sees: four keys a thread and look, eight looks on their
     // way at a time (one after the other, each is two trips to memory: 32 looks were 5% of a long part).
     {
@@ -219,14 +228,22 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
       uint32_t* red = reinterpret_cast<uint32_t*>(lds.v[1]);
 #pragma unroll
       for (int i = 1; i < 64; i <<= 1) sv = span_join(sv, __shfl_xor(sv, i, 64));
-      if (lane == 0) red[wave] = sv;
+      more = __any(more);
+      if (lane == 0) {
+        red[wave] = sv;
+        red[NW + wave] = more;
+      }
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < NW; ++w) sv = span_join(sv, red[w]);
+      for (int w = 0; w < NW; ++w) {
+        sv = span_join(sv, red[w]);
+        more |= red[NW + w] != 0;
+      }
       __syncthreads();
+      more = __builtin_amdgcn_readfirstlane(more);
       sv = __builtin_amdgcn_readfirstlane(sv);
       uv.E = static_cast<int>(sv & 0xffu);
-      uv.wide = uv.E - (255 - static_cast<int>(sv >> 16)) > span_of(4);
+      uv.wide = more || uv.E - (255 - static_cast<int>(sv >> 16)) > span_of(4);
       if (sv == 0) uv.E = kUnit;
       vtops = uv.wide ? block_tops<D, NT>(p, table, kvh, lo > 64 * begin ? lo : 64 * begin, k1, red) : uv.E * 0x01010101u;
       if (uv.wide) vtop = wide_top(64 * (end - begin));
@@ -276,7 +293,7 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
       else return *reinterpret_cast<const uint16_t*>(at) >> (8 * g);
     };
     // Product n of a block's scores: step n / 4 of the columns, term n % 4
-    auto score = [&](int n, const uint4& k, uint32_t ke, const v16f& sc) -> v16f {
+    auto score = [&](int n, const uint4& k, uint32_t ke, const v16f& sc, const Terms (&q)[NC]) -> v16f {
       switch (n) {  // (known once the loops are unrolled)
         case 0: return product<0, 0>(k, ke, q[0], sc);
         case 1: return product<0, 1>(k, ke, q[0], sc);
@@ -291,12 +308,12 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
     // (a product must not write over its own scale: it stays until the block's scores are done)
     auto keep = [](uint32_t ke) { asm volatile("" ::"v"(ke)); };
     // S^T of 32 keys: register r is key 32 bl + 16 (r / 8) + 8 g + r % 8 of the tile in place b
-    auto scores = [&](int b, int bl, v16f& sc) {
+    auto scores = [&](int b, int bl, v16f& sc, const Terms (&q)[NC], bool fresh = true) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+      for (int r = 0; r < 16; ++r) sc[r] = fresh ? 0.0f : sc[r];
       const uint32_t ke = k_scale(b, bl);
 #pragma unroll
-      for (int n = 0; n < NKS; ++n) sc = score(n, k_operand(b, bl, n / 4), ke, sc);
+      for (int n = 0; n < NKS; ++n) sc = score(n, k_operand(b, bl, n / 4), ke, sc, q);
       keep(ke);
     };
     // The tile's scores masked where a row does not see the key, the row's reference m brought up to date (and with it
@@ -335,7 +352,19 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
     };
 
     if (uv.wide) {
-      // Rare (see Unit), and plain: one tile after the other.
+      // Rare (see Unit, and split_query), and plain: one tile after the other.
+      Terms rest[NC];
+      if (more) {
+        int row = rw + li < rows ? rw + li : rows - 1;
+        asm volatile("" : "+v"(row));  // (the address formed again: it would wait in memory, there are no registers for it)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) rest[i] = split_query<DT, true>(columns(row, i));
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {  // (and these, in place of waiting meanwhile)
+          bool x;
+          q[i] = split_query<DT>(columns(row, i), &x);
+        }
+      }
       wait_for<0>();  // (the first tiles' copies)
       for (int kt = begin; kt < end; ++kt) {
         const int id = look(kt);
@@ -349,7 +378,10 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
         __syncthreads();
         v16f sc[2];
 #pragma unroll
-        for (int bl = 0; bl < 2; ++bl) scores(0, bl, sc[bl]);
+        for (int bl = 0; bl < 2; ++bl) {
+          scores(0, bl, sc[bl], q);
+          if (more) scores(0, bl, sc[bl], rest, false);
+        }
         const float ms = settle(64 * kt, here & 0xfu, sc[0], sc[1]);
 #pragma unroll
         for (int bl = 0; bl < 2; ++bl)
@@ -387,8 +419,8 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
       wait_for<0>();
       __syncthreads();
       v16f sa, sb, sc_;
-      scores(0, 0, sa);
-      scores(0, 1, sb);
+      scores(0, 0, sa, q);
+      scores(0, 1, sb, q);
       __syncthreads();  // the first step puts another K tile there
       // Tile kt: its scores are in s0 and s1; the next tile's go to s2 and, when s0 is used up, s0 (three blocks for what
       // would be four).  In LDS: K of kt + 1 (place kn) and kt + 2, V of kt (cur); place kf is free.  In the staging
@@ -435,7 +467,7 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sn[r] = 0.0f;
               }
-              sn = score(i, kx[i / 4], ke[bl], sn);
+              sn = score(i, kx[i / 4], ke[bl], sn, q);
               fetch(n + kAhead);
 #pragma unroll
               for (int e = 0; e < 8 / NKS; ++e) {
@@ -497,11 +529,14 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
     l = add_x32(l);
   }
   if (rw + li < rows) {
-    const int64_t tok = s.start + qi;
+    int row = rw + li;
+    asm volatile("" : "+v"(row));  // (formed again, so that nothing waits for this in registers)
+    const int query = row / G, head = kvh * G + (row - query * G);
+    const int64_t tok = s.start + query;
     const bool one = a.splits == 1;
     const float f = filled(l) ? 1.0f / l : 0.0f;
-    const int64_t at = split * R + tok * p.Hq + h;
-    if (one && p.lse && g == 0) p.lse[tok * p.Hq + h] = row_lse(m, l);
+    const int64_t at = split * R + tok * p.Hq + head;
+    if (one && p.lse && g == 0) p.lse[tok * p.Hq + head] = row_lse(m, l);
     if (!one && g == 0) a.ml[at] = make_float2(m, l);
     if (one || filled(l)) {
       // Register r of acc[db] is column 32 db + 8 (r / 4) + 4 g + r % 4.
@@ -515,7 +550,7 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] = ldexpf(acc[db][4 * k + i] * f, e);
           if (one)
-            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + h * p.out_h + col) =
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + tok * p.out_t + head * p.out_h + col) =
                 make_uint2(pack_dt<DT>(o[0], o[1]), pack_dt<DT>(o[2], o[3]));
           else
             *reinterpret_cast<float4*>(a.acc + at * D + col) = make_float4(o[0], o[1], o[2], o[3]);

@@ -118,6 +118,7 @@ __device__ void fill_rest(const lbfq_paged_params& p, int64_t wg, int64_t wgs) {
 // The larger, NaN if either is: v_maximum3_f32, three operands an instruction, where fmaxf would first quiet each
 // MFMA result with an instruction of its own
 __device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float vmin(float a, float b) { return __builtin_elementwise_minimum(a, b); }  // (likewise)
 
 // v of the lanes 16 and 32 away (v_permlane16_swap / v_permlane32_swap of v with
 // itself leave it and the partner's value in the two results)
@@ -318,7 +319,9 @@ __device__ __forceinline__ void join_waves(const Args& a, const Seq& s, v4f (&ac
           make_float4(acc[nb][i] * f, acc[nb + 1][i] * f, acc[nb + 2][i] * f, acc[nb + 3][i] * f);
   __syncthreads();
   {
-    const int row = threadIdx.x >> 4, part = threadIdx.x & 15;
+    int part = threadIdx.x & 15;
+    asm volatile("" : "+v"(part));  // (here: an output address formed before the loops would wait in memory)
+    const int row = threadIdx.x >> 4;
     float MM = -INFINITY, L = 0.0f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) MM = vmax(MM, x.m[w][row]);
@@ -440,6 +443,7 @@ __device__ __forceinline__ uint32_t block_tops(const lbfq_paged_params& p, const
 // Workgroups of a CU: three where the registers do for that, at the price of a few that go to memory (1560 tokens over 32760
 // keys, 40 heads of 64, bf16: 818 us with two, 765 with three; fp16 queries need more of them: 745 with two, 1075).
 constexpr int chunk_groups(int dt, int64_t d) { return d == 64 && dt == kBF16 ? 3 : 2; }
+constexpr int decode4_groups(int64_t d) { return d == 64 ? 3 : 2; }
 constexpr int chunk4_groups(int64_t d) { return d == 64 ? 3 : 2; }  // (the 4-bit cache's kernel: 168 registers, none in memory)
 
 // ---- the kernels of the cache in 4 bits
@@ -499,13 +503,19 @@ __device__ __forceinline__ f32x32 from_e2m3(const u32x6& w, float sc) {
 }
 
 // 32 columns of a query in four E2M3 terms, and their E8M0 scales in the bytes of e: 255 (not a number) where a column is
-// infinite or NaN.
+// infinite or NaN.  They hold each column to 2^-19 of the largest (2^-129, if that is less than 2^-109).
+//
+// REST: what the four terms leave in four more, down to 2^-39 of the largest (2^-130).  Calls take those where the first four
+// would keep fewer than nine bits, what bf16 has, of much of a block: *more, eight columns or more (not 0) that are below 2^-10
+// of the largest.  Random columns do not come to that; one of 1000 times the others does.  (With such queries and without, us:
+// one token of 48 sequences of 8000 to 16000 keys, 32 / 8 heads of 128, 148 and 123; a prompt of 8192, 778 and 526, in the
+// chunk kernel's plain loop.  To look for them costs 0.2 us of a call of 11, 2 of the prompt.)
 struct Terms {
   u32x6 w[4];
   uint32_t e;
 };
-template <int DT>
-__device__ __forceinline__ Terms split_query(const uint16_t* q) {
+template <int DT, bool REST = false>
+__device__ __forceinline__ Terms split_query(const uint16_t* q, bool* more = nullptr) {
   f32x16 even, odd;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -524,14 +534,35 @@ __device__ __forceinline__ Terms split_query(const uint16_t* q) {
   const uint32_t top = __float_as_uint(m) >> 23;  // m is not negative, or a NaN of either sign
   const bool bad = (top & 0xffu) == 255u;
   // 2^(e - 127): the largest column is in 2 ... 4 of it, what a term leaves at most 4 of the next one's, E2M3 reaches 7.5
-  const uint32_t e = bad ? 100u : (top > 18u ? top : 18u) - 1u;
+  uint32_t e = bad ? 100u : (top > 18u ? top : 18u) - 1u;
+  if constexpr (!REST) {
+    const float few = m * 0x1p-10f;
+    // Eight columns are of two groups of four at least: the second smallest of the groups' smallest says where to count.
+    float least = INFINITY, second = INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float x = vmin(vmin(fabsf(even[i]), fabsf(odd[i])), vmin(fabsf(even[i + 1]), fabsf(odd[i + 1])));
+      second = __builtin_amdgcn_fmed3f(least, second, x);
+      least = vmin(least, x);
+    }
+    *more = false;
+    if (__any(second < few)) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        n += (even[i] != 0.0f && fabsf(even[i]) < few) + (odd[i] != 0.0f && fabsf(odd[i]) < few);
+      *more = !bad && n >= 8;
+    }
+  }
   Terms x;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const float sc = __uint_as_float((e - 5u * t) << 23);
-    x.w[t] = to_e2m3(even, odd, sc);
+  for (int t = REST ? -4 : 0; t < 4; ++t) {
+    if (REST && t == 0) e = (e > 36u ? e : 36u) - 20u;
+    const int at = t < 0 ? t + 4 : t;
+    const float sc = __uint_as_float((e - 5u * at) << 23);
+    x.w[at] = to_e2m3(even, odd, sc);
     if (t < 3) {
-      const f32x32 back = from_e2m3(x.w[t], sc);
+      const f32x32 back = from_e2m3(x.w[at], sc);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         even[i] -= back[2 * i];

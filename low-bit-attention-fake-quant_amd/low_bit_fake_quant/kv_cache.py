@@ -143,11 +143,13 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Ten
 
     Scores, softmax and sums are fp32 on exact products of cached values and
     queries; P is rounded for the second product, to 11 bits or more down to 2^-21
-    of the row's largest, and the result once.  Over a cache in 4 bits each query
-    column is first taken to 2^-19 of the largest of its 32 (bf16 holds columns down to
-    2^-11 of that exactly, fp16 to 2^-8).  A NaN in a query makes its row NaN, in 4
+    of the row's largest (single tokens: 16 bits), and the result once.  Over a cache in
+    4 bits each query column is first taken to 2^-19 of the largest of its 32, or to
+    2^-129 (bf16 holds columns down to 2^-11 of that exactly, fp16 to 2^-8); where eight
+    or more of the 32 are below 2^-10 of the largest, to 2^-39 of it, or 2^-130, at a
+    fifth (single tokens) to a half more time.  A NaN in a query makes its row NaN, in 4
     bits an infinity too.
-    Averages stay finite up to the cache's largest values, 448 * 2^119 or 6 * 2^125.
+    Values are right down to the smallest scales, 2^-127.  Averages stay finite up to the cache's largest values, 448 * 2^119 or 6 * 2^125.
     """
     out, lse = _lib.torch_ops().paged_attention(q, *cache, block_table, seq_lens, query_starts, max_query_len, sm_scale,
                                                 causal, window, out, return_lse)
