@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
     };
     // S^T of 32 keys: register r is key 32 bl + 16 (r / 8) + 8 g + r % 8 of the tile in buf
     auto scores = [&](const uint8_t* buf, int bl, v16f& sc, auto WIDE) {
-      const uint8_t* kr = buf + (32 * bl + key_of(li)) * L::KP + 16 * g;
+      const uint8_t* kr = buf + (32 * bl + key_of_32(li)) * L::KP + 16 * g;
 #pragma unroll
       for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
 #pragma unroll
@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(256, chunk_groups(DT, D)) paged_chunk_kernel(c
         constexpr int HALF = NKS + 2 * NDB, kAhead = 5;
         const int id = look(kt + 4);  // back by the end of the step
         uint4 ring[kAhead];
-        const uint8_t* const kr = nxt + key_of(li) * L::KP + 16 * g;
+        const uint8_t* const kr = nxt + key_of_32(li) * L::KP + 16 * g;
         const uint8_t* const vr = cur + L::KBYTES + li * L::VP + 16 * g;
         auto fetch = [&](int n) {
           if (n >= 2 * HALF) return;

@@ -43,7 +43,7 @@ struct Ring {
 
 // Key of a row of S^T within its 16: row 4 g + i is key 4 i + g, so that the four lane groups' rows of V are neighbours, and
 // V's reads, 64 lanes four bytes of all pieces of four rows, on distinct banks, as K's are.
-__device__ __forceinline__ int key_of(int r) { return 4 * (r & 3) + (r >> 2); }
+__device__ __forceinline__ int key_of_16(int r) { return 4 * (r & 3) + (r >> 2); }
 
 // Pages of 16 and of 32 tokens: a tile lies in four or two; of 64 and more: in one.  A tile's piece is what it has of a page.
 __device__ __forceinline__ int pieces(const lbfq_paged_params& p) { return p.page_shift >= 6 ? 1 : 64 >> p.page_shift; }
@@ -289,9 +289,9 @@ __global__ void __launch_bounds__(256, decode4_groups(D)) paged_decode4_kernel(c
         next = fetch<D>(p, pages, kvh, kKeys * (begin + wave + NW), lane, off, ring + sizeof(typename Ring<D>::Tile));
       }
       load_pages(p, table, kKeys * (begin + wave + 2 * NW), pages);
-      // This lane's places in a tile: its piece of K row key_of(n), and columns (D/16) n .. of V rows 4 i + g, of 16 keys
+      // This lane's places in a tile: its piece of K row key_of_16(n), and columns (D/16) n .. of V rows 4 i + g, of 16 keys
       using X = typename Ring<D>::Tile;
-      const int kr = key_of(n), kpiece = D == 128 ? g : g & 1, vpiece = D == 128 ? n >> 2 : n >> 3;
+      const int kr = key_of_16(n), kpiece = D == 128 ? g : g & 1, vpiece = D == 128 ? n >> 2 : n >> 3;
       const int k_at = offsetof(X, k) + D / 2 * kr + 16 * piece_of<D>(kr, kpiece);
       const int ks_at = offsetof(X, ks) + D / 32 * kr + kpiece;
       const int vs_at = offsetof(X, vs) + D / 32 * g + vpiece;

@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
     // This lane's part in V's reads: keys 8 g + li % 16 / 4 (and four on), columns 16 (li / 16) + 4 (li % 4) ..
     const int vrow = (8 * g + (li & 15) / 4) * L::VP + 32 * (li >> 4) + 8 * (li & 3);
     // This lane's K row of a 32-key block, as A operand: its piece 2 i + g and the bytes 2 i + g of its scales (in bytes 2 i)
-    const int kr = key_of(li), krow = RB * (kr & 15), ksrow = CH * (kr & 15);
+    const int kr = key_of_32(li), krow = RB * (kr & 15), ksrow = CH * (kr & 15);
     auto k_operand = [&](int b, int bl, int i) {
       return *reinterpret_cast<const uint4*>(lds.k[b][2 * bl + (kr >> 4)] + krow + 16 * piece_of<D>(kr & 15, (2 * i + g) & (CH - 1)));
     };

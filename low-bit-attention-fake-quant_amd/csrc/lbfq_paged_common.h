@@ -370,7 +370,7 @@ __device__ __forceinline__ void join_waves(const Args& a, const Seq& s, v4f (&ac
 
 // Key of K row i of a 32-key block (bits 2 and 3 of i exchanged): a lane's scores are
 // then of consecutive keys, eight at a time.
-__device__ __forceinline__ int key_of(int i) { return (i & 0x13) | ((i & 4) << 1) | ((i & 8) >> 1); }
+__device__ __forceinline__ int key_of_32(int i) { return (i & 0x13) | ((i & 4) << 1) | ((i & 8) >> 1); }
 
 // Largest (low half) and 255 - smallest (high half) of the scale bytes so far and of word v.
 __device__ __forceinline__ uint32_t span_join(uint32_t a, uint32_t b) {
