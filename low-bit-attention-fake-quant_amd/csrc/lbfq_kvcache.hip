@@ -23,8 +23,8 @@
 // few tokens: 3.0 and 4.6 us, a launch's own time.
 //
 // Everything else goes by tokens, four heads of 16 at a time: 32760 tokens rotated and
-// appended, 40 / 40 heads of 128, to 4 bits 267 us, 5.8 TB/s, to 8 bits 287 us, 5.9; written
-// in 4 bits 158 us, 5.4; 8 sequences of up to 16384 x 8 heads read from 4 bits 97 us, 6.4.
+// appended, 40 / 40 heads of 128, to 4 bits 263 us, 5.9 TB/s, to 8 bits 285 us, 6.0; written
+// in 4 bits 149 us, 5.7; 8 sequences of up to 16384 x 8 heads read from 4 bits 97 us, 6.3.
 #include <algorithm>
 
 #include "lbfq_common.h"
@@ -55,7 +55,7 @@ __device__ __forceinline__ void load8(const void* base, int64_t i, float (&x)[8]
 }
 
 // NT: marked as not read again soon.  Where each instruction of a wave fills whole lines, that is faster (append of 32760
-// tokens, 40 / 40 heads: 295 -> 281 us with Q's, 289 with the codes'; reading them from 4 bits 148 -> 141); fp32's two stores
+// tokens, 40 / 40 heads, when each store was made so: 295 -> 281 us with Q's, 289 with the codes'; reading them from 4 bits 148 -> 141); fp32's two stores
 // a lane leave holes (8000 tokens, 8 heads: 16 -> 25).
 template <typename T, bool NT>
 __device__ __forceinline__ void put(void* at, const T& v) {
@@ -203,8 +203,8 @@ enum Rotation { kNone, kAdjacent, kHalves };
 
 // A workgroup takes four heads of 16 (D = 64: 32) tokens, the heads of Q, of K and of V being one list: a KiB of a token
 // that lies together where Q, K and V are one projection's output.  (Longer stretches of a token's heads, which read its
-// cos and sin less often, are slower: 32760 tokens, 40 / 40 heads to 4 bits, 4 / 8 / 12 / 16 / 48 / 120 heads: 274 / 277 / 291 /
-// 339 / 322 / 357 us; 32 / 8 heads 127 / 136 / 144 / 151 / 173.)  Every product and the sum are rounded, so what is
+// cos and sin less often, are slower: 32760 tokens, 40 / 40 heads to 4 bits, 4 / 8 / 12 / 16 / 48 heads: 263 / 267 / 275 / 320 /
+// 318 us; 32 / 8 heads 121 / 126 / 131 / 130 / 143.)  Every product and the sum are rounded, so what is
 // quantised is defined to the bit.  kNone: writing without a rotation, in 4 bits.
 template <int DT, int D, int BITS, Rotation ROT>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {

@@ -16,8 +16,9 @@
 // 16 bytes a lane: it never waits for a tile that it has only just asked for.  (The same kernel with a tile's loads into
 // registers took 154 us where this one takes 118, with K's loads before and V's behind the arithmetic 196.)  48
 // sequences of 8000 to 16000 keys, 32 / 8 heads of 128: 118 us, 5.3 TB/s; the same copies without softmax and P V 110, a
-// kernel that only reads 6.1 TB/s.  Heads of 64: 85 us, 3.7 TB/s: 330 VALU instructions a tile of 64 keys whatever the head
-// size, and a chain of 3000 cycles for a wave alone.
+// kernel that only reads 6.1 TB/s; in pages of 64, of 32 120, of 16 128.  Heads of 64: 77 us, 4.0 TB/s (pages of 32 and 16: 87 and
+// 84): 290 VALU instructions a tile of 64 keys, where heads of 128 have 350 for twice the bytes, and a chain of 3000 cycles for
+// a wave alone.  Pages of 16 read 18% more than they need: scales of a head and page are 32 bytes.
 #include <cstddef>
 
 #include "lbfq_paged_common.h"
