@@ -55,8 +55,8 @@ __device__ __forceinline__ void load8(const void* base, int64_t i, float (&x)[8]
 }
 
 // NT: marked as not read again soon.  Where each instruction of a wave fills whole lines, that is faster (append of 32760
-// tokens, 40 / 40 heads, when each store was made so: 295 -> 281 us with Q's, 289 with the codes'; reading them from 4 bits 148 -> 141); fp32's two stores
-// a lane leave holes (8000 tokens, 8 heads: 16 -> 25).
+// tokens, 40 / 40 heads, when each store was made so: 295 -> 281 us with Q's, 289 with the codes'; reading them from 4 bits
+// 148 -> 141); fp32's two stores a lane leave holes (8000 tokens, 8 heads: 16 -> 25).
 template <typename T, bool NT>
 __device__ __forceinline__ void put(void* at, const T& v) {
   if constexpr (NT) __builtin_nontemporal_store(v, static_cast<T*>(at));

@@ -7,13 +7,14 @@
 // cycles as bf16's, but a quarter of the LDS reads, and no conversion.  (At 16 bits, a step's reads take as long as its
 // products: 32 KiB for 16 + 16 of 32 cycles, four waves and two workgroups a CU.)  K's scales go into the product, so no
 // span of them needs bf16.  (Queries that take eight terms, as parts whose V scales lie far apart, go through a plain loop.)
-// P is one fp16 term, 11 bits, as in the 8-bit kernel: a second would be half as many products again.  V is converted as there, but staged as rows of keys, and turned by the reads that feed the
-// products (with 16 permutations a step instead, heads of 64 took 2.5% longer, of 128 the same).
+// P is one fp16 term, 11 bits, as in the 8-bit kernel: a second would be half as many products again.  V is converted as
+// there, but staged as rows of keys, and turned by the reads that feed the products (with 16 permutations a step instead,
+// heads of 64 took 2.5% longer, of 128 the same).
 //
 // 8192 tokens over 32768 keys, 8 heads of 128, all seen: 930 to 980 us, 1.12 to 1.18 PFLOP/s, where a large library product
-// reaches 1.24 (with all codes zero 756: power).  4680 over 32760, 12 heads: 840 to 850 us, 1.11 to 1.12 PFLOP/s, the matrix units busy 55% of
-// the cycles at 2.0 GHz (the 8-bit kernel 1040 to 1140).  200 VALU instructions a step besides 32 products of 32 cycles, 32 of them
-// exponentials.  Heads of 64, twice the exponentials per product: 0.92.
+// reaches 1.24 (with all codes zero 756: power).  4680 over 32760, 12 heads: 840 to 850 us, 1.11 to 1.12 PFLOP/s, the matrix
+// units busy 56% of the cycles at 2.0 GHz (the 8-bit kernel 1040 to 1140).  200 VALU instructions a step besides 32 products
+// of 32 cycles, 32 of them exponentials.  Heads of 64, twice the exponentials per product: 0.92.
 #include "lbfq_paged_common.h"
 
 using namespace lbfq;

@@ -75,3 +75,30 @@ def test_scales_that_grow_or_fall_along_the_keys(gpu, order, bits, d, n, L):
         page = table[b].long()[at.to(gpu) // 64]
         scale[page, :, at.to(gpu) % 64] = x
     run_and_check(bits, args, order, n)
+
+
+@pytest.mark.parametrize("n,L", [(1, 300), (40, 300), (200, 2500)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("causal,window", [(True, None), (True, 70), (False, 33), (False, None)])
+def test_masks_over_scales_far_apart(gpu, causal, window, bits, d, n, L):
+    """Windows, pages that are not there, shared heads, more new tokens than a sequence has, rows behind the last one; what no
+    query sees has any bytes, scales of 255 among them."""
+    from low_bit_fake_quant import paged_attention
+    lens, counts = [L, 0, 17, L // 2], [n, n, n, min(n, 5)]
+    args = (eight if bits == 8 else four).problem(gpu, lens=lens, counts=counts, hq=6, d=d, page=16, tail=3, qscale=0.3)
+    q, cache, table, sl, starts = args
+    g = torch.Generator().manual_seed(d + n)
+    table[0, 1] = -1
+    table[3, 2] = cache[0].shape[0] + 5
+    for b, length in enumerate(lens):
+        at = torch.arange(length, device=gpu)
+        page = table[b].long()[at // 16]
+        there = (page >= 0) & (page < cache[0].shape[0])
+        low = torch.tensor([0, 60, 20, 30])[:d // 32]  # a stretch of 100 scales, another for each block
+        x = (torch.randint(0, 100, (length, 2, d // 32), generator=g) + low).to(torch.uint8).to(gpu)
+        cache[3][page[there], :, at[there] % 16] = x[there]
+    out, lse = paged_attention(*args, max_query_len=n, causal=causal, window=window, return_lse=True)
+    want, wlse, tol, ltol = (ref if bits == 8 else four).attend(*args, causal=causal, window=window)
+    large_values.check(out, want, tol, "out")
+    ref.check(lse, wlse, ltol, "lse")
