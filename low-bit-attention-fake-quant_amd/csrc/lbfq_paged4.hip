@@ -171,7 +171,7 @@ struct Query {
 };
 
 template <int DT, int D, bool REST = false>
-__device__ __forceinline__ Query<D> query(const uint16_t* q, int g, bool* more = nullptr) {
+__device__ __forceinline__ Query<D> query(const Columns& q, int g, bool* more = nullptr) {
   const Terms s = split_query<DT, REST>(q, more);
   Query<D> x;
   if constexpr (D == 128) {
@@ -267,22 +267,13 @@ __global__ void __launch_bounds__(256, decode4_groups(D)) paged_decode4_kernel(c
     if (begin + wave < end) {
       Pages pages;
       load_pages(p, table, kKeys * (begin + wave), pages);
-      const uint16_t* const qr =
-          reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 32 * (D == 128 ? g : g & 1);
-      bool more;
-      const Query<D> q = query<DT, D>(qr, g, &more);  // (while the page ids are on their way)
-      more = __any(more);
-      if (more) {  // (the same from all four waves)
-        const Query<D> rest = query<DT, D, true>(qr, g);
-#pragma unroll
-        for (int i = 0; i < Query<D>::N; ++i)
-#pragma unroll
-          for (int k = 0; k < 6; ++k) rest_lds[6 * i + k][lane] = rest.w[i][k];
-        rest_lds[6 * Query<D>::N][lane] = rest.e;
-      }
+      Columns raw = load_columns(reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h +
+                                 32 * (D == 128 ? g : g & 1));
       const int lr = lane / (D / 32);  // this lane's row and place of it in a copy
       const uint32_t off = D / 2 * lr + 16 * piece_of<D>(lr & 15, lane & (D / 32 - 1));
       const uint32_t ring = lds_addr(&lds.ring.t[wave][0]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(raw.w[i]));  // (here: a wait for them later is one for the copies too)
       wait_for<0>();
       uint32_t there = fetch<D>(p, pages, kvh, kKeys * (begin + wave), lane, off, ring), next = 0;
       if (begin + wave + NW < end) {
@@ -290,6 +281,17 @@ __global__ void __launch_bounds__(256, decode4_groups(D)) paged_decode4_kernel(c
         next = fetch<D>(p, pages, kvh, kKeys * (begin + wave + NW), lane, off, ring + sizeof(typename Ring<D>::Tile));
       }
       load_pages(p, table, kKeys * (begin + wave + 2 * NW), pages);
+      bool more;
+      const Query<D> q = query<DT, D>(raw, g, &more);  // (while the tiles are on their way)
+      more = __any(more);
+      if (more) {  // (the same from all four waves)
+        const Query<D> rest = query<DT, D, true>(raw, g);
+#pragma unroll
+        for (int i = 0; i < Query<D>::N; ++i)
+#pragma unroll
+          for (int k = 0; k < 6; ++k) rest_lds[6 * i + k][lane] = rest.w[i][k];
+        rest_lds[6 * Query<D>::N][lane] = rest.e;
+      }
       // This lane's places in a tile: its piece of K row key_of_16(n), and columns (D/16) n .. of V rows 4 i + g, of 16 keys
       using X = typename Ring<D>::Tile;
       const int kr = key_of_16(n), kpiece = D == 128 ? g : g & 1, vpiece = D == 128 ? n >> 2 : n >> 3;

@@ -190,7 +190,8 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       bool x;
-      q[i] = split_query<DT>(reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 64 * i + 32 * g, &x);
+      q[i] = split_query<DT>(
+          load_columns(reinterpret_cast<const uint16_t*>(p.q) + (s.start + qi) * p.q_t + h * p.q_h + 64 * i + 32 * g), &x);
       more |= x;
     }
     // The span of the part's V scales, over the keys that some row sees: four keys a thread and look, eight looks on their
@@ -359,11 +360,11 @@ __global__ void __launch_bounds__(256, chunk4_groups(D)) paged_chunk4_kernel(con
         int row = rw + li < rows ? rw + li : rows - 1;
         asm volatile("" : "+v"(row));  // (the address formed again: it would wait in memory, there are no registers for it)
 #pragma unroll
-        for (int i = 0; i < NC; ++i) rest[i] = split_query<DT, true>(columns(row, i));
+        for (int i = 0; i < NC; ++i) rest[i] = split_query<DT, true>(load_columns(columns(row, i)));
 #pragma unroll
         for (int i = 0; i < NC; ++i) {  // (and these, in place of waiting meanwhile)
           bool x;
-          q[i] = split_query<DT>(columns(row, i), &x);
+          q[i] = split_query<DT>(load_columns(columns(row, i)), &x);
         }
       }
       wait_for<0>();  // (the first tiles' copies)

@@ -514,19 +514,22 @@ struct Terms {
   u32x6 w[4];
   uint32_t e;
 };
+struct Columns {
+  uint32_t w[16];  // as they lie in memory
+};
+__device__ __forceinline__ Columns load_columns(const uint16_t* q) {
+  Columns x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) load_bytes<16>(reinterpret_cast<const uint8_t*>(q) + 16 * i, x.w + 4 * i);
+  return x;
+}
 template <int DT, bool REST = false>
-__device__ __forceinline__ Terms split_query(const uint16_t* q, bool* more = nullptr) {
+__device__ __forceinline__ Terms split_query(const Columns& q, bool* more = nullptr) {
   f32x16 even, odd;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint4 v = reinterpret_cast<const uint4*>(q)[i];
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      even[4 * i + k] = DT == kBF16 ? __uint_as_float(w[k] << 16) : f16_bits_to_f32(static_cast<uint16_t>(w[k]));
-      odd[4 * i + k] =
-          DT == kBF16 ? __uint_as_float(w[k] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(w[k] >> 16));
-    }
+  for (int i = 0; i < 16; ++i) {
+    even[i] = DT == kBF16 ? __uint_as_float(q.w[i] << 16) : f16_bits_to_f32(static_cast<uint16_t>(q.w[i]));
+    odd[i] = DT == kBF16 ? __uint_as_float(q.w[i] & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(q.w[i] >> 16));
   }
   float m = 0.0f;
 #pragma unroll
