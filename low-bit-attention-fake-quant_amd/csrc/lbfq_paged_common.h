@@ -509,7 +509,7 @@ __device__ __forceinline__ f32x32 from_e2m3(const u32x6& w, float sc) {
 // would keep fewer than nine bits, what bf16 has, of much of a block: *more, eight columns or more (not 0) that are below 2^-10
 // of the largest.  Random columns do not come to that; one of 1000 times the others does.  (With such queries and without, us:
 // one token of 48 sequences of 8000 to 16000 keys, 32 / 8 heads of 128, 148 and 123; a prompt of 8192, 778 and 526, in the
-// chunk kernel's plain loop.  To look for them costs 0.2 us of a call of 11, 2 of the prompt.)
+// chunk kernel's plain loop.  To look for them costs 1 us of four chunks' 96, 2 of the prompt.)
 struct Terms {
   u32x6 w[4];
   uint32_t e;
